@@ -488,6 +488,107 @@ int t2i_prompt_advance(const int32_t* prompt, int32_t B, int32_t P, int32_t* tok
                        int32_t* positions, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Packed prompts: the rows of many sequences of different lengths, one after the
+ * other, each sequence with its own earlier slots (0 for a fresh prompt; one row
+ * after a context is a decode step).  Rows of sequence s follow those of s - 1; row r
+ * of a sequence has position (and cache slot) starts[s] + r in cache row
+ * cache_rows[s] (NULL: s).
+ *
+ * t2i_packed_plan (host only; every pointer is host memory): checks the batch and
+ * writes its table of int32 words, which the two calls below take on the device in
+ * the order row_pos [rows], row_cache [rows], items [n_items][8], merges
+ * [n_merges][8].  sizes receives rows, n_items, n_merges, n_parts and the table's
+ * words; table NULL: sizes only.  0 <= lengths[s], 0 <= starts[s], starts[s] +
+ * lengths[s] <= ctx_cap, distinct cache rows.  The table holds for the heads, the cache
+ * rows and the ctx_cap that it was made for.
+ *
+ * t2i_packed_qk_rope_kv: t2i_prefill_qk_rope_kv for packed rows (the same bits):
+ * q_out bf16 [rows, Hq, D], k and v written to their slots.  A row whose position or
+ * cache row lies outside the cache writes nothing.
+ *
+ * t2i_packed_attention: row r of a sequence attends its slots 0 .. starts + r (causal;
+ * fp32 scores and softmax, weights rounded to bf16 for the product with V); q bf16
+ * [rows, Hq, D], out bf16 [rows, Hq * D].  Slots that no row attends are never read.
+ * out_sums (nullable): fp32 [Hq][rows], as t2i_prefill_attention_sums.  The workspace
+ * (t2i_packed_attention_workspace_bytes, 0: none needed) is scratch: no initial
+ * value, nothing kept; calls that overlap in time must not share one.
+ * D = 128; Hq % Hkv == 0; Hq <= 1024.
+ * Replaces: the prompt pass of quantized_qwen3/model.py:453-478 for sequences of
+ *           different lengths, which the reference runs one by one
+ *           (quantized_qwen3/qwen_npu.py:309-315).
+ */
+int t2i_packed_plan(const int32_t* lengths, const int32_t* starts, const int32_t* cache_rows, int32_t n,
+                    int32_t Hq, int32_t Hkv, int32_t n_cache_rows, int32_t ctx_cap, int32_t* table,
+                    int64_t table_words, int64_t* sizes);
+int t2i_packed_qk_rope_kv(const uint16_t* qkv, int32_t rows, const int32_t* row_pos, const int32_t* row_cache,
+                          int32_t n_cache_rows, int32_t Hq, int32_t Hkv, int32_t D, const uint16_t* q_norm,
+                          const uint16_t* k_norm, float eps, const uint16_t* rope, int32_t rope_style,
+                          uint16_t* q_out, uint16_t* k_cache, uint16_t* v_cache, int32_t ctx_cap, void* stream);
+size_t t2i_packed_attention_workspace_bytes(int64_t n_parts, int32_t Hkv);
+int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32_t* items, int32_t n_items,
+                         const int32_t* merges, int32_t n_merges, int32_t n_parts, int32_t Hq, int32_t Hkv,
+                         int32_t D, const uint16_t* k_cache, const uint16_t* v_cache, int32_t n_cache_rows,
+                         int32_t ctx_cap, uint16_t* out, float* out_sums, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Trees of drafted tokens.  Sequence b (cache row b) has context_lens[b] committed
+ * slots and a tree of node_counts[b] nodes (NULL: N; at most N <= 64): node i hangs from
+ * node parents[b][i] < i (anything else makes it a root), stands in slot
+ * context + i and has position context + its depth.  Arrays of nodes are [B, N]; entries
+ * behind a sequence's count are neither read nor written.  A sequence whose context
+ * is negative or whose nodes pass ctx_cap writes no slot; its attention rows are zero.
+ *
+ * t2i_tree_qk_rope_kv: t2i_prefill_qk_rope_kv for the nodes; q_out bf16 [B, N, Hq, D].
+ * t2i_tree_attention: node i attends the slots 0 .. context - 1, the nodes above it and
+ * itself; q bf16 [B, N, Hq, D], out bf16 [B * N, Hq * D]; arithmetic and workspace
+ * (t2i_tree_attention_workspace_bytes) as t2i_packed_attention.
+ * t2i_tree_commit: the greedy walk from node 0 (the sequence's own last token, always
+ * accepted): from node n to the lowest-numbered child whose token is picks[b][n], as long
+ * as there is one.  Writes path [B, N] (the walk's nodes, then -1), path_counts [B],
+ * next_tokens [B] (the last node's pick), context_out [B] = context + count (not
+ * context_lens itself), and moves the walk's K/V rows to slots context .. context +
+ * count - 1 in all `layers` caches [layers, B, Hkv, ctx_cap, D].  A sequence without
+ * nodes, or whose nodes lie outside the cache: count 0, next token -1, context as it was.
+ * No counterpart in the reference, which decodes one token a step.
+ */
+int t2i_tree_qk_rope_kv(const uint16_t* qkv, const int32_t* parents, const int32_t* context_lens,
+                        const int32_t* node_counts, int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t D,
+                        const uint16_t* q_norm, const uint16_t* k_norm, float eps, const uint16_t* rope,
+                        int32_t rope_style, uint16_t* q_out, uint16_t* k_cache, uint16_t* v_cache,
+                        int32_t ctx_cap, void* stream);
+size_t t2i_tree_attention_workspace_bytes(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t ctx_cap);
+int t2i_tree_attention(const uint16_t* q, const int32_t* parents, const int32_t* context_lens,
+                       const int32_t* node_counts, int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t D,
+                       const uint16_t* k_cache, const uint16_t* v_cache, int32_t ctx_cap, uint16_t* out,
+                       void* workspace, size_t workspace_bytes, void* stream);
+int t2i_tree_commit(const int32_t* tokens, const int32_t* parents, const int32_t* picks,
+                    const int32_t* context_lens, const int32_t* node_counts, int32_t layers, int32_t B,
+                    int32_t N, int32_t Hkv, int32_t D, uint16_t* k_cache, uint16_t* v_cache, int32_t ctx_cap,
+                    int32_t* path, int32_t* path_counts, int32_t* next_tokens, int32_t* context_out,
+                    void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Log probabilities over M rows of V logits (fp32, bf16 or fp16, row_stride values
+ * apart, aligned to their values only), in one pass: logprobs [M] = log softmax at
+ * tokens[row] (an id outside [0, V) gives 0; tokens NULL: none), entropy [M] (nullable)
+ * of the row's distribution in nats, and its top_k (0 to 32) values' log
+ * probabilities and indices [M, top_k], best first, the lower index first among equal
+ * logits.  All arithmetic in fp32.  A logit of -inf has probability 0; a row that holds
+ * a NaN or +inf, or nothing but -inf, gives NaN (NaN ranks above every number).  The
+ * workspace (t2i_token_logprobs_workspace_bytes) is scratch as for t2i_packed_attention.
+ * No counterpart in the reference, whose host takes the argmax (qwen_npu.py:321).
+ */
+#define T2I_LOGITS_FP32 0
+#define T2I_LOGITS_BF16 1
+#define T2I_LOGITS_FP16 2
+size_t t2i_token_logprobs_workspace_bytes(int32_t M, int32_t V, int32_t top_k);
+int t2i_token_logprobs(const void* logits, int32_t logits_type, int64_t row_stride, int32_t M, int32_t V,
+                       const int32_t* tokens, int32_t top_k, float* logprobs, float* entropy,
+                       float* top_logprobs, int32_t* top_ids, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* ---------------------------------------------------------------------------
  * Measurement helper, no counterpart in the reference: the HBM read ceiling that
  * a linear's bandwidth is compared with.  Reads `bytes` (a positive multiple of
  * 16) from src with 16-byte loads, loads_per_thread (1, 2, 4 or 8) per thread in

@@ -9,7 +9,7 @@ library's ``libamdhip64.so.7`` dependency then resolves to that same runtime.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int32, c_size_t, c_void_p
+from ctypes import c_float, c_int32, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 import torch  # noqa: F401  (must precede the library load, see module docstring)
@@ -25,6 +25,9 @@ T2I_ERR_VALUE = -6
 T2I_TILES_STORE = 0
 T2I_TILES_SWIGLU = 1
 T2I_TILES_PAIRED = 2
+T2I_LOGITS_FP32 = 0
+T2I_LOGITS_BF16 = 1
+T2I_LOGITS_FP16 = 2
 
 # name -> (restype, argtypes); mirrors include/t2i_hip.h
 SIGNATURES = {
@@ -101,6 +104,27 @@ SIGNATURES = {
                                              c_void_p, c_void_p, c_void_p]),
     "t2i_greedy_advance": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     "t2i_prompt_advance": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
+    "t2i_packed_plan": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p,
+                                  c_int64, c_void_p]),
+    "t2i_packed_qk_rope_kv": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
+                                        c_void_p, c_void_p, c_float, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
+                                        c_int32, c_void_p]),
+    "t2i_packed_attention_workspace_bytes": (c_size_t, [c_int64, c_int32]),
+    "t2i_packed_attention": (c_int32, [c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_int32, c_int32, c_int32,
+                                       c_int32, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
+                                       c_void_p, c_size_t, c_void_p]),
+    "t2i_tree_qk_rope_kv": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
+                                      c_int32, c_void_p, c_void_p, c_float, c_void_p, c_int32, c_void_p, c_void_p,
+                                      c_void_p, c_int32, c_void_p]),
+    "t2i_tree_attention_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "t2i_tree_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
+                                     c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "t2i_tree_commit": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
+                                  c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
+                                  c_void_p]),
+    "t2i_token_logprobs_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "t2i_token_logprobs": (c_int32, [c_void_p, c_int32, c_int64, c_int32, c_int32, c_void_p, c_int32, c_void_p,
+                                     c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "t2i_stream_read_out_words": (ctypes.c_int64, [c_size_t, c_int32]),
     "t2i_stream_read": (c_int32, [c_void_p, c_size_t, c_int32, c_void_p, c_void_p]),
 }

@@ -1,0 +1,788 @@
+// Attention of ragged batches over the contiguous KV cache for gfx950:
+//
+//   * t2i_packed_qk_rope_kv / t2i_tree_qk_rope_kv: per-head q/k RMSNorm + RoPE and the
+//     cache write of packed prompt rows, or of the nodes of drafted trees;
+//   * t2i_packed_attention: causal GQA attention of packed rows of many sequences, each
+//     with its own length and its own earlier slots;
+//   * t2i_tree_attention: GQA attention of a tree of drafted tokens: a node attends the
+//     sequence's context, the nodes above it and itself;
+//   * t2i_tree_commit: the greedy walk down the drafted trees and the accepted path's K/V
+//     rows moved to the front, in every layer.
+//
+// Scores, softmax statistics and sums are fp32; the softmax weights enter the P . V product
+// as bf16, as in t2i_prefill_attention (quantized_qwen3/model.py:277), and each row's
+// normaliser sums those rounded weights, so that a row of equal values comes back exact.
+#include <math.h>
+
+#include <new>
+
+#include "t2i_common.h"
+#include "qk_prep.h"
+#include "ragged_plan.h"
+
+namespace t2i {
+
+constexpr int RG_D = 128;
+constexpr int RG_ROWS = t2i_host::RG_ROWS;
+constexpr int RG_KEYS = t2i_host::RG_KEYS;
+constexpr int RG_ITEM = t2i_host::RG_ITEM;
+constexpr int TREE_NODES = 64;               // nodes of a tree: one lane of a wave each
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short i16x4;
+
+// ---- trees: a wave holds one, lane i its node i ----
+
+// The parent of node `lane`, or -1 for a root (a parent outside [0, lane) makes one).
+__device__ __forceinline__ int tree_parent(const int32_t* parents, int N, int lane) {
+  const int p = parents[min(lane, N - 1)];
+  return p >= 0 && p < lane ? p : -1;
+}
+
+// Nodes above node `lane`, and their number, by doubling the steps: after k rounds a lane
+// knows the nodes up to 2^k steps above it, and the one that stands there.
+__device__ __forceinline__ unsigned long long tree_above(int p, int lane, int& depth) {
+  uint32_t lo = 0, hi = 0;
+  if (p >= 0) (p < 32 ? lo : hi) = 1u << (p & 31);
+  depth = p >= 0 ? 1 : 0;
+#pragma unroll
+  for (int k = 0; k < 6; ++k) {
+    const int at = max(p, 0);
+    const uint32_t l = __shfl(lo, at, 64), h = __shfl(hi, at, 64);
+    const int d = __shfl(depth, at, 64), q = __shfl(p, at, 64);
+    if (p >= 0) {
+      lo |= l;
+      hi |= h;
+      depth += d;
+      p = q;
+    }
+  }
+  return (unsigned long long)hi << 32 | lo;
+}
+
+// A tree's nodes and context as the kernels take them: nodes = 0 where there is nothing to
+// do; ok: the context and its nodes lie in the cache.
+struct TreeSeq {
+  int ctx, nodes;
+  bool ok;
+};
+__device__ __forceinline__ TreeSeq tree_seq(const int32_t* ctx_lens, const int32_t* counts, int b, int N, int cap) {
+  TreeSeq t;
+  t.ctx = ctx_lens[b];
+  t.nodes = counts ? max(0, min(counts[b], N)) : N;
+  t.ok = t.ctx >= 0 && t.ctx <= cap - t.nodes;
+  return t;
+}
+
+// ============================================================================
+// q/k RMSNorm + RoPE + KV-cache write of ragged rows
+// ============================================================================
+struct RaggedPrepParams {
+  const uint16_t* qkv;      // [rows, (Hq + 2 Hkv) * D]
+  const uint16_t* qn;
+  const uint16_t* kn;
+  const uint16_t* rope;     // [>= cap, D] cos even / sin odd
+  uint16_t* q;              // [rows, Hq, D]
+  uint16_t* kc;             // [cache rows, Hkv, cap, D]
+  uint16_t* vc;
+  const int32_t* row_pos;   // packed: position (and slot) of each row, its cache row
+  const int32_t* row_cache;
+  const int32_t* parents;   // trees: [B, N]; slot = context + node, position = context + depth
+  const int32_t* ctx;
+  const int32_t* counts;
+  int N, n_cache, Hq, Hkv, cap, style;
+  float eps;
+};
+
+// One workgroup (4 waves) per row, a head vector to a 16-lane row of a wave, as
+// prefill_prep_kernel (same bits): PREP_NB batches of 16 vectors in flight.  A row whose
+// position, slot or cache row lies outside the cache writes nothing.  Bound by HBM:
+// every byte is read and written once.
+constexpr int RG_PREP_NB = 2;
+
+template <bool TREE>
+__global__ __launch_bounds__(256) void ragged_prep_kernel(const RaggedPrepParams p) {
+  constexpr int D = RG_D;
+  const int row = blockIdx.x;
+  const int lane = threadIdx.x & 63;
+  int pos, dst_slot, crow;
+  if (TREE) {
+    crow = row / p.N;
+    const int node = row - crow * p.N;
+    const TreeSeq t = tree_seq(p.ctx, p.counts, crow, p.N, p.cap);
+    if (!t.ok || node >= t.nodes) return;
+    int depth;
+    tree_above(tree_parent(p.parents + (size_t)crow * p.N, p.N, lane), lane, depth);
+    dst_slot = t.ctx + node;
+    pos = t.ctx + __builtin_amdgcn_readlane(depth, node);
+  } else {
+    pos = dst_slot = p.row_pos[row];
+    crow = p.row_cache[row];
+    if (pos < 0 || pos >= p.cap || crow < 0 || crow >= p.n_cache) return;
+  }
+  const int c = lane & 15;
+  const int slot = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 4 + (lane >> 4);   // 0 .. 15
+  const int nvec = p.Hq + 2 * p.Hkv;
+  const uint16_t* src_row = p.qkv + (size_t)row * nvec * D;
+  for (int base = 0; base < nvec; base += 16 * RG_PREP_NB) {
+    u32x4 raw[RG_PREP_NB];
+#pragma unroll
+    for (int j = 0; j < RG_PREP_NB; ++j)
+      raw[j] = prep_load(src_row + (size_t)min(base + 16 * j + slot, nvec - 1) * D, c, p.style);
+    const u32x4 rp = *reinterpret_cast<const u32x4*>(p.rope + (size_t)pos * D + 8 * c);
+    const u32x4 gqv = prep_load(p.qn, c, p.style);
+    const u32x4 gkv = prep_load(p.kn, c, p.style);
+#pragma unroll
+    for (int j = 0; j < RG_PREP_NB; ++j) asm volatile("" : "+v"(raw[j]));   // every load before the first use
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < RG_PREP_NB; ++j) {
+      const int vi = base + 16 * j + slot;     // uniform over the 16-lane row
+      const bool isq = vi < p.Hq;
+      const bool normed = vi < p.Hq + p.Hkv;   // q and k: RMSNorm + RoPE; v as is
+      const u32x4 y = prep_vector(raw[j], rp, isq ? gqv : gkv, normed, p.style, p.eps);
+      if (vi >= nvec) continue;
+      uint16_t* dst;
+      if (isq) dst = p.q + ((size_t)row * p.Hq + vi) * D;
+      else if (normed) dst = p.kc + (((size_t)crow * p.Hkv + (vi - p.Hq)) * p.cap + dst_slot) * D;
+      else dst = p.vc + (((size_t)crow * p.Hkv + (vi - p.Hq - p.Hkv)) * p.cap + dst_slot) * D;
+      prep_store(dst, c, p.style, y);
+    }
+  }
+}
+
+// ============================================================================
+// attention
+// ============================================================================
+struct RaggedAttnParams {
+  const uint16_t* q;        // [rows, Hq, D]
+  const uint16_t* kc;       // [cache rows, Hkv, cap, D]
+  const uint16_t* vc;
+  uint16_t* out;            // [rows, Hq * D]
+  float* out_sums;          // NULL, or [Hq, rows]: each head's sum of its bf16 context values
+  float* part_o;            // [parts][Hkv][RG_ROWS][D] unnormalised outputs of a part of the keys
+  float2* part_ml;          // [parts][Hkv][RG_ROWS] their running maximum and sum
+  const int32_t* items;     // packed: [n_items][RG_ITEM]; merge: [n_merges][RG_ITEM]
+  const int32_t* parents;   // trees: [B, N]
+  const int32_t* ctx;
+  const int32_t* counts;
+  long long rows;
+  int n_cache, n_parts, Hq, Hkv, G, cap, N, splits, tiles;
+  float scale_log2;         // D^-1/2 * log2(e)
+};
+
+// What one workgroup does: pairs j0 .. j0 + RG_ROWS - 1 of a sequence's (row, q head of kv
+// head h) pairs over key blocks kb0 .. kb1 - 1.
+struct RaggedItem {
+  int row0, rows, start, crow, kb0, kb1, part, kend;
+  long long j0, pairs;
+};
+
+// Until every vector memory operation of this wave is done, and every wave is here.
+__device__ __forceinline__ void loads_done_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+// 16 bytes a lane from src into LDS at lds + 16 lane, left in flight: written as asm because
+// the compiler waits for every load into LDS before any read of LDS.  A wait state between
+// the move into M0 and the load; no other SGPR is read.  loads_done_barrier covers it.
+__device__ __forceinline__ void lds_load16(const uint16_t* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(lds), "v"(src) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t rg_lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+// max / sum over the two lanes (c, c + 32) of a row, in both
+__device__ __forceinline__ float pair_max(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// One workgroup (4 waves of 32 pairs, two workgroups a CU) an item and kv head.  All products
+// run transposed on the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32, h2 = lane / 32) holds
+// one pair's scores and outputs:
+//   S^T = K Q^T: A = K from LDS (lane: key 32 n + c, dims 16 ks + 8 h2 ..), B = the wave's q
+//     rows (registers); register i holds the score of key 32 n + 8 (i / 4) + 4 h2 + i % 4;
+//   the online softmax per lane: the row's maximum from its two lanes by one lane swap, the
+//     weights' sum left per lane until the end.  The reference m moves only when a maximum
+//     passes it by 8 (weights up to 2^8, the same relative precision): after the first blocks
+//     outputs are hardly ever rescaled;
+//   O^T += V^T P^T: B = P^T straight from those registers (16 keys a step, in the order they
+//     stand in), A = V^T from LDS in that order by transposing reads (ds_read_b64_tr_b16: four
+//     keys of one dim a lane out of V's own row order).
+// K and V blocks go straight from memory into LDS, two buffers, one barrier a block; a row's
+// 16-byte chunk ch stands at place ch ^ 2 (row % 8), which spreads both kinds of reads over all
+// banks (a load into LDS cannot pad rows, but each lane chooses what it loads).  Keys past the
+// last one reload it: slots that no row attends are never read.
+template <bool TREE>
+__global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
+  constexpr int D = RG_D;
+  __shared__ __align__(256) uint16_t s_kv[2][2][RG_KEYS * D];   // [buffer][K, V][key][dim]
+
+  const int h = blockIdx.x % p.Hkv;
+  const int idx = blockIdx.x / p.Hkv;
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h2 = lane >> 5;
+
+  RaggedItem it;
+  if (TREE) {
+    const int tile = idx % p.tiles, bs = idx / p.tiles;
+    const int s = bs % p.splits, b = bs / p.splits;
+    const TreeSeq t = tree_seq(p.ctx, p.counts, b, p.N, p.cap);
+    it.row0 = b * p.N;
+    it.rows = t.nodes;
+    it.start = t.ctx;
+    it.crow = b;
+    it.j0 = (long long)tile * RG_ROWS;
+    it.pairs = (long long)t.nodes * p.G;
+    it.kend = t.ctx + t.nodes;
+    const int blocks = t.ok ? (it.kend + RG_KEYS - 1) / RG_KEYS : 0;
+    it.kb0 = (int)((long long)blocks * s / p.splits);
+    it.kb1 = (int)((long long)blocks * (s + 1) / p.splits);
+    it.part = p.splits > 1 ? (b * p.tiles + tile) * p.splits + s : -1;
+    if (it.j0 >= it.pairs) return;
+  } else {
+    const int32_t* w = p.items + (size_t)idx * RG_ITEM;
+    it.row0 = w[0]; it.rows = w[1]; it.start = w[2]; it.crow = w[3];
+    it.j0 = w[4]; it.kb0 = w[5]; it.kb1 = w[6]; it.part = w[7];
+    it.pairs = (long long)it.rows * p.G;
+    // a table that does not fit the tensors is not followed
+    if (it.row0 < 0 || it.rows < 1 || it.row0 + (long long)it.rows > p.rows || it.start < 0 ||
+        it.start > p.cap - it.rows || it.crow < 0 || it.crow >= p.n_cache || it.j0 < 0 || it.j0 >= it.pairs ||
+        it.pairs > 0x7FFFFFFF - RG_ROWS || it.part >= p.n_parts)
+      return;
+    it.kend = it.start + (int)((min(it.j0 + RG_ROWS, it.pairs) - 1) / p.G) + 1;
+    it.kb0 = max(it.kb0, 0);
+    it.kb1 = min(it.kb1, (it.kend + RG_KEYS - 1) / RG_KEYS);
+  }
+
+  // ---- K / V staging: a wave's instruction moves 4 keys (1 KB); 4 each of K and V a block ----
+  const size_t cache_base = ((size_t)it.crow * p.Hkv + h) * (size_t)p.cap * D;
+  const uint16_t* const kbase = p.kc + cache_base;
+  const uint16_t* const vbase = p.vc + cache_base;
+  const int srow = lane >> 4;                              // key within the instruction's four
+  // chunk of the key that this lane loads, for even and odd instructions (rows 0-3 and 4-7 of 8)
+  const int ch0 = ((lane & 15) ^ (2 * srow)) * 8, ch1 = ((lane & 15) ^ (2 * (4 + srow))) * 8;
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rg_lds_address(s_kv) + wave * 16 * D * 2);
+  auto stage = [&](int kb, int buf) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = min(kb * RG_KEYS + wave * 16 + 4 * i + srow, it.kend - 1);
+      const size_t off = (size_t)key * D + (i & 1 ? ch1 : ch0);
+      lds_load16(kbase + off, lds0 + buf * (4 * RG_KEYS * D) + i * 4 * D * 2);
+      lds_load16(vbase + off, lds0 + buf * (4 * RG_KEYS * D) + 2 * RG_KEYS * D + i * 4 * D * 2);
+    }
+  };
+  if (it.kb0 < it.kb1) stage(it.kb0, 0);
+
+  // ---- this lane's pair, and its q row as the B operand ----
+  const long long j = it.j0 + wave * 32 + c;
+  const bool wave_on = it.j0 + wave * 32 < it.pairs;       // some pair of the wave exists
+  const int jj = (int)min(j, it.pairs - 1);
+  const int t = jj / p.G;
+  const int head = h * p.G + (jj - t * p.G);
+  const size_t qrow = (size_t)it.row0 + t;
+  u32x4 qb[8];
+  {
+    const uint16_t* src = p.q + (qrow * p.Hq + head) * D + 8 * h2;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qb[ks] = *reinterpret_cast<const u32x4*>(src + 16 * ks);
+  }
+  // positions of the wave's rows: first and last (wave-uniform), this lane's
+  const int t_first = (int)((it.j0 + wave * 32) / p.G);
+  const int t_last = (int)((min(it.j0 + wave * 32 + 32, it.pairs) - 1) / p.G);
+  const int qpos = it.start + t;
+  const int mask_from = TREE ? it.start : it.start + t_first + 1;   // keys below it are seen by every row
+  const int wave_end = TREE ? it.kend : it.start + t_last + 1;      // keys from it on by none
+  uint32_t seen_lo = 0, seen_hi = 0;                       // tree: the nodes that the lane's node attends
+  if (TREE && it.kb1 * RG_KEYS > it.start && it.kb0 < it.kb1) {
+    int depth;
+    const unsigned long long own = 1ull << lane;
+    const unsigned long long s = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane), lane, depth) | own;
+    seen_lo = __shfl((uint32_t)s, t, 64);
+    seen_hi = __shfl((uint32_t)(s >> 32), t, 64);
+  }
+
+  float m = -INFINITY, mref = 0.0f, l = 0.0f;              // mref: m, or 0 while m is -inf; l: of this lane's keys
+  f32x16 o[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
+
+  // LDS offsets (elements): K row c of a 32-key tile, V rows by transposing reads
+  const int kx = 2 * (c & 7);
+  const int vi = lane & 15, vrow = 4 * h2 + (vi >> 2);     // key of the 8 that the lane's read names
+  const int vcol = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);   // its 16-byte chunk within a 32-dim tile
+
+  for (int kb = it.kb0; kb < it.kb1; ++kb) {
+    const int buf = (kb - it.kb0) & 1;
+    loads_done_barrier();                                  // this block is here, the other buffer is free
+    if (kb + 1 < it.kb1) stage(kb + 1, buf ^ 1);
+    if (!wave_on || kb * RG_KEYS >= wave_end) continue;
+    const uint16_t* const bk = s_kv[buf][0];
+    const uint16_t* const bv = s_kv[buf][1];
+    // ---- S^T = K Q^T ----
+    f32x16 s[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        const u32x4 ka = *reinterpret_cast<const u32x4*>(bk + (32 * n + c) * D + ((2 * ks + h2) ^ kx) * 8);
+        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ka),
+                                                       __builtin_bit_cast(bf16x8, qb[ks]), s[n], 0, 0, 0);
+      }
+    }
+    // ---- masks, only on blocks that some row does not see whole ----
+    if (kb * RG_KEYS + RG_KEYS > mask_from) {
+      if (TREE) {
+        const int rel = kb * RG_KEYS - it.start;           // node of the block's first key (negative: a context slot)
+        const unsigned long long w = (unsigned long long)seen_hi << 32 | seen_lo;
+        unsigned long long bm = rel >= 64 ? 0ull : rel >= 0 ? w >> rel : (w << -rel) | ((1ull << -rel) - 1);
+        bm >>= 4 * h2;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!((uint32_t)(bm >> (32 * n)) & (1u << (8 * (i / 4) + i % 4)))) s[n][i] = -INFINITY;
+      } else {
+        const int rel = qpos - kb * RG_KEYS - 4 * h2;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * n + 8 * (i / 4) + i % 4 > rel) s[n][i] = -INFINITY;
+      }
+    }
+    // ---- online softmax (log2 domain) ----
+    float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+    mx = pair_max(mx) * p.scale_log2;
+    if (__any(mx > m + 8.0f)) {
+      const float mn = fmaxf(m, mx);
+      const float f = m > -INFINITY ? exp2_fast(m - mn) : 0.0f;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] *= f;
+      m = mn;
+      mref = mn > -INFINITY ? mn : 0.0f;
+    }
+    uint32_t pw[2][8];                                     // bf16 weights, two keys a word
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const uint32_t w = pack_bf16x2(exp2_fast(fmaf(s[n][i], p.scale_log2, -mref)),
+                                       exp2_fast(fmaf(s[n][i + 1], p.scale_log2, -mref)));
+        pw[n][i / 2] = w;
+        l = dot2_bf16(w, 0x3F803F80u, l);                  // the rounded weights
+      }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t* const w = pw[u / 2] + 4 * (u % 2);
+      const u32x4 pb = u32x4{w[0], w[1], w[2], w[3]};
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        const uint16_t* const v = bv + (16 * u + vrow) * D + ((4 * dt + vcol) ^ (2 * vrow)) * 8 + 4 * (vi & 1);
+        typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+        const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
+        const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D));
+        const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u32x4{b0.x, b0.y, b1.x, b1.y}),
+                                                        __builtin_bit_cast(bf16x8, pb), o[dt], 0, 0, 0);
+      }
+    }
+  }
+
+  // ---- outputs: register i of o[dt] is dim 32 dt + 8 (i / 4) + 4 h2 + i % 4 of the lane's pair ----
+  if (!wave_on) return;
+  l = pair_sum(l);
+  const bool live = j < it.pairs;
+  if (it.part >= 0) {
+    const size_t st = ((size_t)it.part * p.Hkv + h) * RG_ROWS + wave * 32 + c;
+    m = l != l ? INFINITY : m;                             // a row that saw a NaN stays one in the merge
+    if (live && h2 == 0) p.part_ml[st] = float2{m, l};
+    if (live && m > -INFINITY) {                           // else its outputs are not read
+      float* dst = p.part_o + st * D + 4 * h2;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+    }
+    return;
+  }
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);   // nothing attended: a zero row; NaN stays
+  uint16_t* const dst = p.out + (qrow * p.Hq + head) * D + 8 * h2;
+  float hs = 0.0f;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      uint32_t x[2], y[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        x[e] = pack_bf16x2(o[dt][4 * g + 2 * e] * inv, o[dt][4 * g + 2 * e + 1] * inv);
+        y[e] = pack_bf16x2(o[dt][4 * g + 4 + 2 * e] * inv, o[dt][4 * g + 5 + 2 * e] * inv);
+        hs += (bf16_lo(x[e]) + bf16_hi(x[e])) + (bf16_lo(y[e]) + bf16_hi(y[e]));
+      }
+      // lanes trade halves: each ends up with 8 neighbouring dims
+      const auto a = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+      const auto b = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+      if (live) *reinterpret_cast<u32x4*>(dst + 32 * dt + 8 * g) = u32x4{a[0], b[0], a[1], b[1]};
+    }
+  if (p.out_sums) {
+    hs = pair_sum(hs);
+    if (live && h2 == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
+  }
+}
+
+// The parts of a tile joined: one wave a (row, q head) pair, lane e its dims 2 e and 2 e + 1,
+// parts in their order.
+template <bool TREE>
+__global__ __launch_bounds__(256) void ragged_merge_kernel(const RaggedAttnParams p) {
+  constexpr int D = RG_D;
+  const int lane = threadIdx.x & 63;
+  const int at = blockIdx.x % (RG_ROWS / 4) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // pair of the tile
+  const int h = blockIdx.x / (RG_ROWS / 4) % p.Hkv;
+  const int idx = blockIdx.x / (RG_ROWS / 4) / p.Hkv;
+  int row0, rows, first, parts;
+  long long j0;
+  if (TREE) {
+    const int b = idx / p.tiles, tile = idx - b * p.tiles;
+    const TreeSeq t = tree_seq(p.ctx, p.counts, b, p.N, p.cap);
+    row0 = b * p.N;
+    rows = t.nodes;
+    j0 = (long long)tile * RG_ROWS;
+    first = idx * p.splits;
+    parts = p.splits;
+  } else {
+    const int32_t* w = p.items + (size_t)idx * RG_ITEM;
+    row0 = w[0]; rows = w[1]; j0 = w[2]; first = w[3]; parts = w[4];
+    if (row0 < 0 || rows < 1 || row0 + (long long)rows > p.rows || j0 < 0 || first < 0 || parts < 1 ||
+        first > p.n_parts - parts)
+      return;
+  }
+  const long long j = j0 + at;
+  if (j >= (long long)rows * p.G) return;
+  const int t = (int)(j / p.G);
+  const int head = h * p.G + (int)(j - (long long)t * p.G);
+  const size_t st0 = ((size_t)first * p.Hkv + h) * RG_ROWS + at, step = (size_t)p.Hkv * RG_ROWS;
+  float M = -INFINITY;
+  for (int s = 0; s < parts; ++s) M = fmaxf(M, p.part_ml[st0 + s * step].x);
+  float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  for (int s = 0; s < parts; ++s) {
+    const float2 ml = p.part_ml[st0 + s * step];
+    if (!(ml.x > -INFINITY)) continue;                     // uniform: the part attended nothing
+    const float f = exp2_fast(ml.x - M);
+    const float2 v = *reinterpret_cast<const float2*>(p.part_o + (st0 + s * step) * D + 2 * lane);
+    l += f * ml.y;
+    o0 += f * v.x;
+    o1 += f * v.y;
+  }
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+  const uint32_t w = pack_bf16x2(o0 * inv, o1 * inv);
+  const size_t qrow = (size_t)row0 + t;
+  *reinterpret_cast<uint32_t*>(p.out + (qrow * p.Hq + head) * D + 2 * lane) = w;
+  if (p.out_sums) {
+    const float hs = wave_sum(bf16_lo(w) + bf16_hi(w));
+    if (lane == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
+  }
+}
+
+// ============================================================================
+// the accepted path of a drafted tree
+// ============================================================================
+struct TreeCommitParams {
+  const int32_t* tokens;    // [B, N]
+  const int32_t* parents;
+  const int32_t* picks;
+  const int32_t* ctx;       // [B]
+  const int32_t* counts;    // [B] or NULL
+  uint16_t* kc;             // [layers, B, Hkv, cap, D]
+  uint16_t* vc;
+  int32_t* path;            // [B, N]
+  int32_t* n_path;          // [B]
+  int32_t* next;
+  int32_t* ctx_out;
+  int B, N, layers, Hkv, cap;
+};
+
+// A wave per (layer, sequence, kv head); lane i holds node i.  Every wave walks the tree itself
+// (a ballot a step; the walk costs less than a hand-over), then moves its head's rows: four
+// slots at a time, 16 lanes of 16 bytes each.  The path's nodes ascend, so entry e comes from a
+// slot at or behind e: a group's writes never reach a slot that a later group reads.
+__global__ __launch_bounds__(256) void tree_commit_kernel(const TreeCommitParams p) {
+  constexpr int D = RG_D;
+  const int lane = threadIdx.x & 63;
+  const long long id = (long long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (id >= (long long)p.layers * p.B * p.Hkv) return;
+  const int b = (int)(id / p.Hkv % p.B);
+  const TreeSeq t = tree_seq(p.ctx, p.counts, b, p.N, p.cap);
+  const int at = b * p.N + min(lane, p.N - 1);
+  const int token = p.tokens[at], pick = p.picks[at];
+  const int parent = tree_parent(p.parents + (size_t)b * p.N, p.N, lane);
+  int mine = -1, n = 0, cur = -1;
+  if (t.ok && t.nodes > 0) {
+    cur = 0;
+    for (;;) {                                             // at most N steps: cur ascends
+      if (lane == n) mine = cur;
+      ++n;
+      const int want = __builtin_amdgcn_readlane(pick, cur);
+      const unsigned long long right = __ballot(lane < t.nodes && parent == cur && token == want);
+      if (!right) break;
+      cur = __builtin_ctzll(right);
+    }
+  }
+  const int next = __builtin_amdgcn_readlane(pick, max(cur, 0));
+  if (id < (long long)p.B * p.Hkv && id % p.Hkv == 0) {    // layer 0, head 0: the record
+    if (lane < p.N) p.path[b * p.N + lane] = mine;
+    if (lane == 0) {
+      p.n_path[b] = n;
+      p.next[b] = n ? next : -1;
+      p.ctx_out[b] = t.ctx + n;
+    }
+  }
+  const size_t base = (size_t)id * p.cap * D + (size_t)t.ctx * D + (lane & 15) * 8;
+  for (int e0 = 0; e0 < n; e0 += 4) {
+    const int e = e0 + (lane >> 4);
+    const int from = __shfl(mine, e, 64);                  // e < 64
+    if (e < n && from != e) {
+      const u32x4 k = *reinterpret_cast<const u32x4*>(p.kc + base + (size_t)from * D);
+      const u32x4 v = *reinterpret_cast<const u32x4*>(p.vc + base + (size_t)from * D);
+      *reinterpret_cast<u32x4*>(p.kc + base + (size_t)e * D) = k;
+      *reinterpret_cast<u32x4*>(p.vc + base + (size_t)e * D) = v;
+    }
+  }
+}
+
+}  // namespace t2i
+
+// ============================================================================
+// host side
+// ============================================================================
+using t2i_host::aligned16;
+using t2i_host::fail;
+
+namespace {
+
+bool aligned4(const void* p) { return ((uintptr_t)p & 3u) == 0; }
+
+int check_heads(int32_t Hq, int32_t Hkv, int32_t D, int32_t cap) {
+  if (D != t2i::RG_D) return fail(T2I_ERR_SHAPE, "head_dim %d unsupported (only 128)", D);
+  if (Hkv < 1 || Hq < Hkv || Hq % Hkv) return fail(T2I_ERR_SHAPE, "Hq=%d Hkv=%d invalid", Hq, Hkv);
+  if (Hq > 1024) return fail(T2I_ERR_SHAPE, "Hq=%d exceeds 1024", Hq);
+  if (cap < 1) return fail(T2I_ERR_SHAPE, "ctx_cap=%d invalid", cap);
+  return T2I_OK;
+}
+
+// Pairs, parts and workgroups stay below 2^31.
+bool too_many(long long n) { return n > 0x7FFFFFFFLL; }
+
+size_t part_bytes(long long parts, int32_t Hkv) {
+  return (size_t)parts * Hkv * t2i::RG_ROWS * (t2i::RG_D * sizeof(float) + sizeof(float2));
+}
+
+// The workspace's parts: outputs first, then the (max, sum) pairs.
+void set_parts(t2i::RaggedAttnParams& p, void* ws, long long parts) {
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)parts * p.Hkv * t2i::RG_ROWS * t2i::RG_D);
+}
+
+int check_prep(const void* qkv, const void* qn, const void* kn, const void* rope, const void* q, const void* kc,
+               const void* vc, float eps, int32_t style) {
+  if (!qkv || !qn || !kn || !rope || !q || !kc || !vc) return fail(T2I_ERR_NULL, "ragged prep pointers must not be NULL");
+  if (!aligned16(qkv) || !aligned16(qn) || !aligned16(kn) || !aligned16(rope) || !aligned16(q) || !aligned16(kc) ||
+      !aligned16(vc))
+    return fail(T2I_ERR_ALIGN, "ragged prep tensors must be 16-byte aligned");
+  if (style != 0 && style != 1) return fail(T2I_ERR_VALUE, "rope_style must be 0 or 1");
+  if (!(eps > 0.0f)) return fail(T2I_ERR_VALUE, "eps must be positive");
+  return T2I_OK;
+}
+
+int check_tree(const int32_t* parents, const int32_t* ctx, const int32_t* counts, int32_t B, int32_t N, int32_t cap) {
+  if (!parents || !ctx) return fail(T2I_ERR_NULL, "parents and context_lens must not be NULL");
+  if (!aligned4(parents) || !aligned4(ctx) || !aligned4(counts))
+    return fail(T2I_ERR_ALIGN, "parents, context_lens and node_counts must be 4-byte aligned");
+  if (B < 1 || N < 1 || N > t2i::TREE_NODES || N > cap)
+    return fail(T2I_ERR_SHAPE, "B=%d N=%d invalid (1 to %d nodes, at most the cache's %d slots)", B, N, t2i::TREE_NODES, cap);
+  return T2I_OK;
+}
+
+}  // namespace
+
+extern "C" int t2i_packed_plan(const int32_t* lengths, const int32_t* starts, const int32_t* cache_rows, int32_t n,
+                               int32_t Hq, int32_t Hkv, int32_t n_cache_rows, int32_t ctx_cap, int32_t* table,
+                               int64_t table_words, int64_t* sizes) {
+  if (!lengths || !starts || !sizes) return fail(T2I_ERR_NULL, "lengths, starts and sizes must not be NULL");
+  if (int rc = check_heads(Hq, Hkv, t2i::RG_D, ctx_cap)) return rc;
+  if (n < 1 || n_cache_rows < 1 || n > n_cache_rows)
+    return fail(T2I_ERR_SHAPE, "%d sequences over %d cache rows invalid", n, n_cache_rows);
+  try {
+    std::vector<char> used(n_cache_rows, 0);
+    long long rows = 0;
+    for (int i = 0; i < n; ++i) {
+      const int crow = cache_rows ? cache_rows[i] : i;
+      if (lengths[i] < 0 || starts[i] < 0 || (long long)starts[i] + lengths[i] > ctx_cap)
+        return fail(T2I_ERR_VALUE, "sequence %d: rows %d from slot %d exceed the cache (%d)", i, lengths[i], starts[i], ctx_cap);
+      if (crow < 0 || crow >= n_cache_rows) return fail(T2I_ERR_VALUE, "sequence %d: cache row %d out of range", i, crow);
+      if (used[crow]) return fail(T2I_ERR_VALUE, "sequence %d: cache row %d is another sequence's", i, crow);
+      used[crow] = 1;
+      rows += lengths[i];
+    }
+    if (too_many(rows * Hq)) return fail(T2I_ERR_SHAPE, "%lld packed rows are too many", rows);
+    const t2i_host::PackedTable t = t2i_host::packed_table(lengths, starts, cache_rows, n, Hq / Hkv, Hkv);
+    sizes[0] = (int64_t)t.row_pos.size();
+    sizes[1] = (int64_t)t.items.size() / t2i::RG_ITEM;
+    sizes[2] = (int64_t)t.merges.size() / t2i::RG_ITEM;
+    sizes[3] = t.n_parts;
+    sizes[4] = (int64_t)(2 * t.row_pos.size() + t.items.size() + t.merges.size());
+    if (!table) return T2I_OK;
+    if (table_words < sizes[4]) return fail(T2I_ERR_WORKSPACE, "the table holds %lld words, %lld needed", (long long)table_words, (long long)sizes[4]);
+    for (const auto* v : {&t.row_pos, &t.row_cache, &t.items, &t.merges}) table = std::copy(v->begin(), v->end(), table);
+    return T2I_OK;
+  } catch (const std::bad_alloc&) {
+    return fail(T2I_ERR_WORKSPACE, "host memory for the plan ran out");
+  }
+}
+
+extern "C" int t2i_packed_qk_rope_kv(const uint16_t* qkv, int32_t rows, const int32_t* row_pos, const int32_t* row_cache,
+                                     int32_t n_cache_rows, int32_t Hq, int32_t Hkv, int32_t D, const uint16_t* q_norm,
+                                     const uint16_t* k_norm, float eps, const uint16_t* rope, int32_t rope_style,
+                                     uint16_t* q_out, uint16_t* k_cache, uint16_t* v_cache, int32_t ctx_cap, void* stream) {
+  if (int rc = check_prep(qkv, q_norm, k_norm, rope, q_out, k_cache, v_cache, eps, rope_style)) return rc;
+  if (!row_pos || !row_cache) return fail(T2I_ERR_NULL, "row_pos and row_cache must not be NULL");
+  if (!aligned4(row_pos) || !aligned4(row_cache)) return fail(T2I_ERR_ALIGN, "row_pos and row_cache must be 4-byte aligned");
+  if (int rc = check_heads(Hq, Hkv, D, ctx_cap)) return rc;
+  if (rows < 1 || n_cache_rows < 1) return fail(T2I_ERR_SHAPE, "rows=%d cache rows=%d invalid", rows, n_cache_rows);
+  t2i::RaggedPrepParams p{};
+  p.qkv = qkv; p.qn = q_norm; p.kn = k_norm; p.rope = rope; p.q = q_out; p.kc = k_cache; p.vc = v_cache;
+  p.row_pos = row_pos; p.row_cache = row_cache; p.n_cache = n_cache_rows;
+  p.Hq = Hq; p.Hkv = Hkv; p.cap = ctx_cap; p.style = rope_style; p.eps = eps;
+  hipLaunchKernelGGL(t2i::ragged_prep_kernel<false>, dim3(rows), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p);
+  return t2i_host::hip_status(hipGetLastError(), "packed prep launch");
+}
+
+extern "C" size_t t2i_packed_attention_workspace_bytes(int64_t n_parts, int32_t Hkv) {
+  return n_parts < 1 || Hkv < 1 || too_many(n_parts) ? 0 : part_bytes(n_parts, Hkv);
+}
+
+extern "C" int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32_t* items, int32_t n_items,
+                                    const int32_t* merges, int32_t n_merges, int32_t n_parts, int32_t Hq, int32_t Hkv,
+                                    int32_t D, const uint16_t* k_cache, const uint16_t* v_cache, int32_t n_cache_rows,
+                                    int32_t ctx_cap, uint16_t* out, float* out_sums, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  if (!q || !items || !k_cache || !v_cache || !out) return fail(T2I_ERR_NULL, "packed attention pointers must not be NULL");
+  if (int rc = check_heads(Hq, Hkv, D, ctx_cap)) return rc;
+  if (rows < 1 || n_cache_rows < 1 || n_items < 1 || n_merges < 0 || n_parts < 0 || (n_parts > 0 && (n_merges < 1 || !merges)))
+    return fail(T2I_ERR_SHAPE, "rows=%d items=%d merges=%d parts=%d invalid", rows, n_items, n_merges, n_parts);
+  if (too_many((long long)n_items * Hkv) || too_many((long long)n_merges * Hkv * (t2i::RG_ROWS / 4)))
+    return fail(T2I_ERR_SHAPE, "%d items of %d kv heads exceed the grid", n_items, Hkv);
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
+    return fail(T2I_ERR_ALIGN, "packed attention tensors must be 16-byte aligned");
+  if (!aligned4(items) || !aligned4(merges) || !aligned4(out_sums))
+    return fail(T2I_ERR_ALIGN, "tables and out_sums must be 4-byte aligned");
+  const size_t need = part_bytes(n_parts, Hkv);
+  if (need && (!workspace || workspace_bytes < need)) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
+  if (need && !aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
+  t2i::RaggedAttnParams p{};
+  p.q = q; p.kc = k_cache; p.vc = v_cache; p.out = out; p.out_sums = out_sums; p.items = items;
+  p.rows = rows; p.n_cache = n_cache_rows; p.n_parts = n_parts; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap;
+  p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
+  if (need) set_parts(p, workspace, n_parts);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(t2i::ragged_attention_kernel<false>, dim3(n_items * Hkv), dim3(256), 0, s, p);
+  if (int rc = t2i_host::hip_status(hipGetLastError(), "packed attention launch")) return rc;
+  if (!need) return T2I_OK;
+  p.items = merges;
+  hipLaunchKernelGGL(t2i::ragged_merge_kernel<false>, dim3(n_merges * Hkv * (t2i::RG_ROWS / 4)), dim3(256), 0, s, p);
+  return t2i_host::hip_status(hipGetLastError(), "packed attention merge launch");
+}
+
+extern "C" int t2i_tree_qk_rope_kv(const uint16_t* qkv, const int32_t* parents, const int32_t* context_lens,
+                                   const int32_t* node_counts, int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t D,
+                                   const uint16_t* q_norm, const uint16_t* k_norm, float eps, const uint16_t* rope,
+                                   int32_t rope_style, uint16_t* q_out, uint16_t* k_cache, uint16_t* v_cache,
+                                   int32_t ctx_cap, void* stream) {
+  if (int rc = check_prep(qkv, q_norm, k_norm, rope, q_out, k_cache, v_cache, eps, rope_style)) return rc;
+  if (int rc = check_heads(Hq, Hkv, D, ctx_cap)) return rc;
+  if (int rc = check_tree(parents, context_lens, node_counts, B, N, ctx_cap)) return rc;
+  if (too_many((long long)B * N)) return fail(T2I_ERR_SHAPE, "B=%d N=%d exceed the grid", B, N);
+  t2i::RaggedPrepParams p{};
+  p.qkv = qkv; p.qn = q_norm; p.kn = k_norm; p.rope = rope; p.q = q_out; p.kc = k_cache; p.vc = v_cache;
+  p.parents = parents; p.ctx = context_lens; p.counts = node_counts; p.N = N; p.n_cache = B;
+  p.Hq = Hq; p.Hkv = Hkv; p.cap = ctx_cap; p.style = rope_style; p.eps = eps;
+  hipLaunchKernelGGL(t2i::ragged_prep_kernel<true>, dim3(B * N), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p);
+  return t2i_host::hip_status(hipGetLastError(), "tree prep launch");
+}
+
+extern "C" size_t t2i_tree_attention_workspace_bytes(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t ctx_cap) {
+  if (B < 1 || N < 1 || N > t2i::TREE_NODES || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq > 1024 || ctx_cap < N) return 0;
+  const int tiles = (N * (Hq / Hkv) + t2i::RG_ROWS - 1) / t2i::RG_ROWS;
+  const int splits = t2i_host::tree_splits((long long)B * Hkv * tiles, ctx_cap);
+  return splits > 1 ? part_bytes((long long)B * tiles * splits, Hkv) : 0;
+}
+
+extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, const int32_t* context_lens,
+                                  const int32_t* node_counts, int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t D,
+                                  const uint16_t* k_cache, const uint16_t* v_cache, int32_t ctx_cap, uint16_t* out,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !k_cache || !v_cache || !out) return fail(T2I_ERR_NULL, "tree attention pointers must not be NULL");
+  if (int rc = check_heads(Hq, Hkv, D, ctx_cap)) return rc;
+  if (int rc = check_tree(parents, context_lens, node_counts, B, N, ctx_cap)) return rc;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
+    return fail(T2I_ERR_ALIGN, "tree attention tensors must be 16-byte aligned");
+  t2i::RaggedAttnParams p{};
+  p.q = q; p.kc = k_cache; p.vc = v_cache; p.out = out; p.parents = parents; p.ctx = context_lens; p.counts = node_counts;
+  p.rows = (long long)B * N; p.n_cache = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap; p.N = N;
+  p.tiles = (N * p.G + t2i::RG_ROWS - 1) / t2i::RG_ROWS;
+  p.splits = t2i_host::tree_splits((long long)B * Hkv * p.tiles, ctx_cap);
+  p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
+  if (too_many((long long)B * p.tiles * Hkv * std::max(p.splits, t2i::RG_ROWS / 4)) || too_many((long long)B * N))
+    return fail(T2I_ERR_SHAPE, "B=%d N=%d Hkv=%d exceed the grid", B, N, Hkv);
+  const size_t need = t2i_tree_attention_workspace_bytes(B, N, Hq, Hkv, ctx_cap);
+  if (need && (!workspace || workspace_bytes < need)) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
+  if (need && !aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
+  if (need) set_parts(p, workspace, (long long)B * p.tiles * p.splits);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(t2i::ragged_attention_kernel<true>, dim3(B * p.tiles * p.splits * Hkv), dim3(256), 0, s, p);
+  if (int rc = t2i_host::hip_status(hipGetLastError(), "tree attention launch")) return rc;
+  if (!need) return T2I_OK;
+  hipLaunchKernelGGL(t2i::ragged_merge_kernel<true>, dim3(B * p.tiles * Hkv * (t2i::RG_ROWS / 4)), dim3(256), 0, s, p);
+  return t2i_host::hip_status(hipGetLastError(), "tree attention merge launch");
+}
+
+extern "C" int t2i_tree_commit(const int32_t* tokens, const int32_t* parents, const int32_t* picks,
+                               const int32_t* context_lens, const int32_t* node_counts, int32_t layers, int32_t B,
+                               int32_t N, int32_t Hkv, int32_t D, uint16_t* k_cache, uint16_t* v_cache, int32_t ctx_cap,
+                               int32_t* path, int32_t* path_counts, int32_t* next_tokens, int32_t* context_out,
+                               void* stream) {
+  if (!tokens || !picks || !k_cache || !v_cache || !path || !path_counts || !next_tokens || !context_out)
+    return fail(T2I_ERR_NULL, "tree commit pointers must not be NULL");
+  if (int rc = check_heads(Hkv, Hkv, D, ctx_cap)) return rc;
+  if (int rc = check_tree(parents, context_lens, node_counts, B, N, ctx_cap)) return rc;
+  if (layers < 1 || too_many((long long)layers * B * Hkv)) return fail(T2I_ERR_SHAPE, "layers=%d invalid", layers);
+  if (!aligned4(tokens) || !aligned4(picks) || !aligned4(path) || !aligned4(path_counts) || !aligned4(next_tokens) || !aligned4(context_out))
+    return fail(T2I_ERR_ALIGN, "token and count arrays must be 4-byte aligned");
+  if (!aligned16(k_cache) || !aligned16(v_cache)) return fail(T2I_ERR_ALIGN, "caches must be 16-byte aligned");
+  if (context_out == context_lens) return fail(T2I_ERR_VALUE, "context_out must not be context_lens (every wave reads it)");
+  t2i::TreeCommitParams p{};
+  p.tokens = tokens; p.parents = parents; p.picks = picks; p.ctx = context_lens; p.counts = node_counts;
+  p.kc = k_cache; p.vc = v_cache; p.path = path; p.n_path = path_counts; p.next = next_tokens; p.ctx_out = context_out;
+  p.B = B; p.N = N; p.layers = layers; p.Hkv = Hkv; p.cap = ctx_cap;
+  const long long waves = (long long)layers * B * Hkv;
+  hipLaunchKernelGGL(t2i::tree_commit_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), p);
+  return t2i_host::hip_status(hipGetLastError(), "tree commit launch");
+}

@@ -994,6 +994,354 @@ def prompt_advance(prompt, tokens, positions):
     _lib.check(rc, "t2i_prompt_advance")
 
 
+# ---- ragged batches: packed prompts, drafted trees, token probabilities ----
+MAX_TREE_NODES = 64
+MAX_TOP_K = 32
+_LOGITS_TYPES = {torch.float32: _lib.T2I_LOGITS_FP32, torch.bfloat16: _lib.T2I_LOGITS_BF16,
+                 torch.float16: _lib.T2I_LOGITS_FP16}
+
+
+def _same_device(device, **tensors):
+    for n, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{n} is on {t.device}, not on {device}")
+
+
+def _on(device):
+    """The device made current for a launch (the library launches on the current one)."""
+    return torch.cuda.device(device)
+
+
+def _scratch(workspace: Workspace | None, key: str, nbytes: int, device):
+    """Scratch of at least ``nbytes`` (a power of two: a buffer of one size is never replaced, so
+    a captured call keeps its own).  Without a workspace each stream has its own buffers."""
+    if nbytes == 0:
+        return None
+    size = 1 << (nbytes - 1).bit_length()
+    if workspace is None:
+        return DEFAULT_WORKSPACE.get((key, size, _lib.stream_handle(device)), size, device)
+    return workspace.get((key, size), size, device)
+
+
+class PackedPlan:
+    """A batch of packed prompt rows: ``lengths[s]`` rows of sequence s (0: none), one
+    sequence after the other, at cache slots ``starts[s] ..`` (0 by default) of cache row
+    ``cache_rows[s]`` (s by default) out of ``n_cache_rows`` (``len(lengths)`` by default,
+    or one more than the largest given row).  Host integers, checked here (``ValueError``: a sequence past
+    ``ctx_cap``, two on one cache row); the table that the kernels take is made once and
+    serves every layer of the pass.
+
+    ``rows``: packed rows; ``first_rows[s]`` / ``last_rows[s]``: a sequence's first and last
+    packed row (last = first - 1 for a sequence without rows)."""
+
+    def __init__(self, lengths, n_heads: int, n_kv_heads: int, ctx_cap: int, device, starts=None, cache_rows=None,
+                 n_cache_rows: int | None = None):
+        lengths = [int(x) for x in lengths]
+        starts = [0] * len(lengths) if starts is None else [int(x) for x in starts]
+        if not lengths or len(starts) != len(lengths):
+            raise ValueError("lengths must hold at least one sequence, and starts one entry for each")
+        if cache_rows is not None:
+            cache_rows = [int(x) for x in cache_rows]
+            if len(cache_rows) != len(lengths):
+                raise ValueError("cache_rows must hold one entry for each sequence")
+        if n_cache_rows is None:
+            n_cache_rows = len(lengths) if cache_rows is None else max(len(lengths), max(cache_rows) + 1)
+        for n, v in (("lengths", lengths), ("starts", starts), ("cache_rows", cache_rows or [])):
+            if any(not -2**31 <= x < 2**31 for x in v):
+                raise ValueError(f"{n} must be 32-bit integers")
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.lengths, self.starts = lengths, starts
+        self.cache_rows = list(range(len(lengths))) if cache_rows is None else cache_rows
+        self.n_heads, self.n_kv_heads, self.ctx_cap, self.n_cache_rows = n_heads, n_kv_heads, ctx_cap, n_cache_rows
+        lib = _lib.load()
+        args = [torch.tensor(v, dtype=torch.int32) for v in (lengths, starts, self.cache_rows)]
+        sizes = torch.zeros(5, dtype=torch.int64)
+        call = (*(a.data_ptr() for a in args), len(lengths), n_heads, n_kv_heads, n_cache_rows, ctx_cap)
+        _lib.check(lib.t2i_packed_plan(*call, None, 0, sizes.data_ptr()), "t2i_packed_plan")
+        self.rows, self.n_items, self.n_merges, self.n_parts, words = sizes.tolist()
+        table = torch.empty(max(words, 1), dtype=torch.int32)
+        _lib.check(lib.t2i_packed_plan(*call, table.data_ptr(), words, sizes.data_ptr()), "t2i_packed_plan")
+        self.table = table.to(self.device)
+        base, n = self.table.data_ptr(), 4 * self.rows
+        self._row_pos, self._row_cache, self._items = base, base + n, base + 2 * n
+        self._merges = self._items + 32 * self.n_items
+        self._nbytes = lib.t2i_packed_attention_workspace_bytes(self.n_parts, n_kv_heads)
+        self.first_rows, self.last_rows, at = [], [], 0
+        for x in lengths:
+            self.first_rows.append(at)
+            at += x
+            self.last_rows.append(at - 1)
+
+    def _check(self, k_cache, v_cache, d: int | None = None):
+        _check_dev("k_cache", k_cache, BF16)
+        _check_dev("v_cache", v_cache, BF16)
+        want = (self.n_cache_rows, self.n_kv_heads, self.ctx_cap)
+        if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or tuple(k_cache.shape[:3]) != want:
+            raise ValueError(f"caches must be [{want[0]}, {want[1]}, {want[2]}, D], as the plan was made for")
+        if d is not None and k_cache.shape[3] != d:
+            raise ValueError(f"the caches' head dimension must be {d}")
+
+
+def packed_qk_rope_kv(qkv: torch.Tensor, plan: PackedPlan, q_norm: torch.Tensor, k_norm: torch.Tensor, eps: float,
+                      rope: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, rope_style: int = ROPE_HALVES,
+                      q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``prefill_qk_rope_kv`` for the packed rows of ``plan`` (the same bits): q/k RMSNorm +
+    RoPE at each row's position and the cache write at its slot.
+
+    ``qkv`` bf16 ``[rows, (Hq + 2 Hkv) * D]``; returns q bf16 ``[rows, Hq, D]``."""
+    for n, t in (("qkv", qkv), ("q_norm", q_norm), ("k_norm", k_norm), ("rope", rope)):
+        _check_dev(n, t, BF16)
+    d = q_norm.numel()
+    plan._check(k_cache, v_cache, d)
+    if k_norm.numel() != d:
+        raise ValueError("q_norm and k_norm must both hold head_dim values")
+    if qkv.numel() != plan.rows * (plan.n_heads + 2 * plan.n_kv_heads) * d:
+        raise ValueError("qkv must be [rows, (Hq + 2 Hkv) * D]")
+    if rope.dim() != 2 or rope.shape[0] < plan.ctx_cap or rope.shape[1] != d:
+        raise ValueError("rope table must be [>= ctx_cap, D]")
+    if q_out is None:
+        q_out = torch.empty(plan.rows, plan.n_heads, d, dtype=BF16, device=qkv.device)
+    _check_dev("q_out", q_out, BF16)
+    if q_out.numel() != plan.rows * plan.n_heads * d:
+        raise ValueError("q_out must be [rows, Hq, D]")
+    _same_device(plan.device, qkv=qkv, q_norm=q_norm, k_norm=k_norm, rope=rope, k_cache=k_cache, v_cache=v_cache,
+                 q_out=q_out)
+    if plan.rows == 0:
+        return q_out
+    with _on(plan.device):
+        rc = _lib.load().t2i_packed_qk_rope_kv(qkv.data_ptr(), plan.rows, plan._row_pos, plan._row_cache,
+                                               plan.n_cache_rows, plan.n_heads, plan.n_kv_heads, d, q_norm.data_ptr(),
+                                               k_norm.data_ptr(), float(eps), rope.data_ptr(), int(rope_style),
+                                               q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), plan.ctx_cap,
+                                               _lib.stream_handle(plan.device))
+    _lib.check(rc, "t2i_packed_qk_rope_kv")
+    return q_out
+
+
+def packed_attention(q: torch.Tensor, plan: PackedPlan, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                     out: torch.Tensor | None = None, out_sums: torch.Tensor | None = None,
+                     workspace: Workspace | None = None) -> torch.Tensor:
+    """Causal GQA attention of packed rows ``q [rows, Hq, D]``: each row over its own
+    sequence's cache slots ``0 .. its position``; returns bf16 ``[rows, Hq * D]``.
+    ``out_sums`` (fp32 ``[Hq, rows]``) as ``prefill_attention``.  Slots that no row attends
+    are never read."""
+    _check_dev("q", q, BF16)
+    if q.dim() != 3 or q.shape[0] != plan.rows or q.shape[1] != plan.n_heads:
+        raise ValueError(f"q must be [{plan.rows}, {plan.n_heads}, D], as the plan was made for")
+    d = q.shape[2]
+    plan._check(k_cache, v_cache, d)
+    if out is None:
+        out = torch.empty(plan.rows, plan.n_heads * d, dtype=BF16, device=q.device)
+    _check_dev("out", out, BF16)
+    if out.numel() != plan.rows * plan.n_heads * d:
+        raise ValueError("out must be [rows, Hq * D]")
+    if out_sums is not None:
+        _check_sums("out_sums", out_sums, plan.rows, plan.n_heads)
+    _same_device(plan.device, q=q, k_cache=k_cache, v_cache=v_cache, out=out, out_sums=out_sums)
+    if plan.rows == 0:
+        return out
+    ws = _scratch(workspace, "packed_attn", plan._nbytes, q.device)
+    with _on(plan.device):
+        rc = _lib.load().t2i_packed_attention(q.data_ptr(), plan.rows, plan._items, plan.n_items, plan._merges,
+                                              plan.n_merges, plan.n_parts, plan.n_heads, plan.n_kv_heads, d,
+                                              k_cache.data_ptr(), v_cache.data_ptr(), plan.n_cache_rows, plan.ctx_cap,
+                                              out.data_ptr(), _lib.ptr(out_sums), _lib.ptr(ws), plan._nbytes,
+                                              _lib.stream_handle(plan.device))
+    _lib.check(rc, "t2i_packed_attention")
+    return out
+
+
+def _check_tree(parents, context_lens, node_counts):
+    _check_dev("parents", parents, torch.int32)
+    _check_dev("context_lens", context_lens, torch.int32)
+    if parents.dim() != 2:
+        raise ValueError("parents must be [B, N]")
+    b, n = parents.shape
+    if not 1 <= n <= MAX_TREE_NODES or b < 1:
+        raise ValueError(f"a tree has 1 to {MAX_TREE_NODES} nodes, got parents {tuple(parents.shape)}")
+    if context_lens.numel() != b:
+        raise ValueError(f"context_lens must hold {b} values")
+    if node_counts is not None:
+        _check_dev("node_counts", node_counts, torch.int32)
+        if node_counts.numel() != b:
+            raise ValueError(f"node_counts must hold {b} values")
+    return b, n
+
+
+def _check_tree_caches(k_cache, v_cache, b, n_kv_heads, n):
+    _check_dev("k_cache", k_cache, BF16)
+    _check_dev("v_cache", v_cache, BF16)
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or tuple(k_cache.shape[:2]) != (b, n_kv_heads):
+        raise ValueError(f"caches must be [{b}, {n_kv_heads}, ctx_cap, D] of equal shape")
+    if k_cache.shape[2] < n:
+        raise ValueError(f"{n} nodes exceed the cache capacity {k_cache.shape[2]}")
+
+
+def tree_qk_rope_kv(qkv: torch.Tensor, parents: torch.Tensor, context_lens: torch.Tensor, n_heads: int,
+                    n_kv_heads: int, q_norm: torch.Tensor, k_norm: torch.Tensor, eps: float, rope: torch.Tensor,
+                    k_cache: torch.Tensor, v_cache: torch.Tensor, rope_style: int = ROPE_HALVES,
+                    node_counts: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """q/k RMSNorm + RoPE of drafted nodes and their cache write: node i of sequence b at
+    position ``context_lens[b] + depth`` and slot ``context_lens[b] + i``.
+
+    ``qkv`` bf16 ``[B * N, (Hq + 2 Hkv) * D]``, ``parents`` int32 ``[B, N]`` (a node's parent
+    stands before it; anything else makes it a root), ``context_lens`` int32 ``[B]``,
+    ``node_counts`` int32 ``[B]`` (all N by default; rows behind a count are left as they are).
+    A sequence whose nodes do not fit the cache writes nothing.  Returns q bf16 ``[B, N, Hq, D]``."""
+    b, n = _check_tree(parents, context_lens, node_counts)
+    for nm, t in (("qkv", qkv), ("q_norm", q_norm), ("k_norm", k_norm), ("rope", rope)):
+        _check_dev(nm, t, BF16)
+    d = q_norm.numel()
+    _check_tree_caches(k_cache, v_cache, b, n_kv_heads, n)
+    ctx_cap = k_cache.shape[2]
+    if k_norm.numel() != d or k_cache.shape[3] != d:
+        raise ValueError("q_norm, k_norm and the caches must have one head dimension")
+    if qkv.numel() != b * n * (n_heads + 2 * n_kv_heads) * d:
+        raise ValueError("qkv must be [B * N, (Hq + 2 Hkv) * D]")
+    if rope.dim() != 2 or rope.shape[0] < ctx_cap or rope.shape[1] != d:
+        raise ValueError("rope table must be [>= ctx_cap, D]")
+    if q_out is None:
+        q_out = torch.empty(b, n, n_heads, d, dtype=BF16, device=qkv.device)
+    _check_dev("q_out", q_out, BF16)
+    if q_out.numel() != b * n * n_heads * d:
+        raise ValueError("q_out must be [B, N, Hq, D]")
+    dev = qkv.device
+    _same_device(dev, parents=parents, context_lens=context_lens, node_counts=node_counts, q_norm=q_norm,
+                 k_norm=k_norm, rope=rope, k_cache=k_cache, v_cache=v_cache, q_out=q_out)
+    with _on(dev):
+        rc = _lib.load().t2i_tree_qk_rope_kv(qkv.data_ptr(), parents.data_ptr(), context_lens.data_ptr(),
+                                             _lib.ptr(node_counts), b, n, n_heads, n_kv_heads, d, q_norm.data_ptr(),
+                                             k_norm.data_ptr(), float(eps), rope.data_ptr(), int(rope_style),
+                                             q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ctx_cap,
+                                             _lib.stream_handle(dev))
+    _lib.check(rc, "t2i_tree_qk_rope_kv")
+    return q_out
+
+
+def tree_attention(q: torch.Tensor, parents: torch.Tensor, context_lens: torch.Tensor, n_kv_heads: int,
+                   k_cache: torch.Tensor, v_cache: torch.Tensor, node_counts: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None, workspace: Workspace | None = None) -> torch.Tensor:
+    """GQA attention of drafted trees: node i of sequence b attends the cache slots
+    ``0 .. context_lens[b] - 1``, the nodes above it and itself (their K/V in slots
+    ``context_lens[b] + node``, as ``tree_qk_rope_kv`` writes them).
+
+    ``q`` bf16 ``[B, N, Hq, D]``, N at most 64; the rest as ``tree_qk_rope_kv``.  Returns bf16
+    ``[B * N, Hq * D]``; rows behind a sequence's count are left as they are, and a sequence
+    whose nodes do not fit the cache gets zero rows.  Everything that varies from step to step
+    is on the device: a captured call serves every later step."""
+    _check_dev("q", q, BF16)
+    b, n = _check_tree(parents, context_lens, node_counts)
+    if q.dim() != 4 or tuple(q.shape[:2]) != (b, n):
+        raise ValueError(f"q must be [{b}, {n}, Hq, D]")
+    hq, d = q.shape[2:]
+    _check_tree_caches(k_cache, v_cache, b, n_kv_heads, n)
+    ctx_cap = k_cache.shape[2]
+    if k_cache.shape[3] != d:
+        raise ValueError(f"the caches' head dimension must be {d}")
+    if out is None:
+        out = torch.empty(b * n, hq * d, dtype=BF16, device=q.device)
+    _check_dev("out", out, BF16)
+    if out.numel() != b * n * hq * d:
+        raise ValueError("out must be [B * N, Hq * D]")
+    dev = q.device
+    _same_device(dev, parents=parents, context_lens=context_lens, node_counts=node_counts, k_cache=k_cache,
+                 v_cache=v_cache, out=out)
+    lib = _lib.load()
+    nbytes = lib.t2i_tree_attention_workspace_bytes(b, n, hq, n_kv_heads, ctx_cap)
+    ws = _scratch(workspace, "tree_attn", nbytes, dev)
+    with _on(dev):
+        rc = lib.t2i_tree_attention(q.data_ptr(), parents.data_ptr(), context_lens.data_ptr(), _lib.ptr(node_counts),
+                                    b, n, hq, n_kv_heads, d, k_cache.data_ptr(), v_cache.data_ptr(), ctx_cap,
+                                    out.data_ptr(), _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
+    _lib.check(rc, "t2i_tree_attention")
+    return out
+
+
+def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor, context_lens: torch.Tensor,
+                k_cache: torch.Tensor, v_cache: torch.Tensor, node_counts: torch.Tensor | None = None):
+    """The greedy walk down each drafted tree, and its K/V rows moved to the front of the tree's
+    slots in every layer's cache (in place).
+
+    ``tokens`` int32 ``[B, N]``: the nodes' tokens (node 0: the sequence's own last token, always
+    accepted); ``picks`` int32 ``[B, N]``: the model's token after each node.  From a node the
+    walk goes to its lowest-numbered child whose token is the node's pick.  Caches bf16
+    ``[layers, B, Hkv, ctx_cap, D]`` (or one layer's, four-dimensional).
+
+    Returns int32 ``(path [B, N]: the walk's nodes, then -1; counts [B]; next_tokens [B]: the last
+    node's pick; context_lens [B] after the walk)``."""
+    b, n = _check_tree(parents, context_lens, node_counts)
+    for nm, t in (("tokens", tokens), ("picks", picks)):
+        _check_dev(nm, t, torch.int32)
+        if t.numel() != b * n:
+            raise ValueError(f"{nm} must be [{b}, {n}]")
+    if k_cache.dim() == 4 and v_cache.dim() == 4:
+        k_cache, v_cache = k_cache.unsqueeze(0), v_cache.unsqueeze(0)
+    if k_cache.dim() != 5 or k_cache.shape != v_cache.shape or k_cache.shape[0] < 1:
+        raise ValueError("caches must be [layers, B, Hkv, ctx_cap, D] of equal shape")
+    layers, _, hkv, ctx_cap, d = k_cache.shape
+    _check_dev("k_cache", k_cache, BF16)
+    _check_dev("v_cache", v_cache, BF16)
+    if k_cache.shape[1] != b or ctx_cap < n:
+        raise ValueError(f"caches must be [layers, {b}, Hkv, >= {n}, D]")
+    dev = tokens.device
+    _same_device(dev, parents=parents, picks=picks, context_lens=context_lens, node_counts=node_counts,
+                 k_cache=k_cache, v_cache=v_cache)
+    rec = torch.empty(b * (n + 3), dtype=torch.int32, device=dev)   # one allocation for the four
+    path, counts, nxt, context = rec[:b * n].view(b, n), rec[b * n:b * n + b], rec[-2 * b:-b], rec[-b:]
+    with _on(dev):
+        rc = _lib.load().t2i_tree_commit(tokens.data_ptr(), parents.data_ptr(), picks.data_ptr(),
+                                         context_lens.data_ptr(), _lib.ptr(node_counts), layers, b, n, hkv, d,
+                                         k_cache.data_ptr(), v_cache.data_ptr(), ctx_cap, path.data_ptr(),
+                                         counts.data_ptr(), nxt.data_ptr(), context.data_ptr(),
+                                         _lib.stream_handle(dev))
+    _lib.check(rc, "t2i_tree_commit")
+    return path, counts, nxt, context
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, workspace: Workspace | None = None):
+    """Log probabilities of ``tokens`` (int32 ``[M]``) under the rows of ``logits`` (fp32, bf16 or
+    fp16 ``[M, V]``; rows may be strided), each row's entropy (nats), and its ``top_k`` (0 to 32)
+    best alternatives, in one pass over the logits and fp32 arithmetic.
+
+    Returns ``(logprobs [M], entropy [M], top_logprobs [M, top_k], top_ids [M, top_k])``, fp32 and
+    int32; alternatives best first, the lower index first among equal logits.  A token outside
+    ``[0, V)`` (padding) gives 0.  Logits of -inf have probability 0; a row with a NaN, a +inf
+    or nothing but -inf gives NaN."""
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise ValueError("logits must be a GPU tensor (the W4A16 path has no CPU fallback)")
+    if logits.dtype not in _LOGITS_TYPES:
+        raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("logits must be [M, V]")
+    m, v = logits.shape
+    stride = logits.stride(0) if m > 1 else v
+    if (v > 1 and logits.stride(1) != 1) or stride < v:
+        raise ValueError("logits rows must be contiguous and must not overlap")
+    _check_dev("tokens", tokens, torch.int32)
+    if tokens.numel() != m:
+        raise ValueError(f"tokens must hold {m} ids")
+    if not 0 <= top_k <= min(MAX_TOP_K, v):
+        raise ValueError(f"top_k must be 0 to {min(MAX_TOP_K, v)}, got {top_k}")
+    dev = logits.device
+    _same_device(dev, tokens=tokens)
+    buf = torch.empty(2 * m + m * top_k, dtype=torch.float32, device=dev)
+    ids = torch.empty(m, top_k, dtype=torch.int32, device=dev)
+    lp, entropy, top = buf[:m], buf[m:2 * m], buf[2 * m:].view(m, top_k)
+    if m == 0:
+        return lp, entropy, top, ids
+    lib = _lib.load()
+    nbytes = lib.t2i_token_logprobs_workspace_bytes(m, v, top_k)
+    ws = _scratch(workspace, "logprobs", nbytes, dev)
+    with _on(dev):
+        rc = lib.t2i_token_logprobs(logits.data_ptr(), _LOGITS_TYPES[logits.dtype], stride, m, v, tokens.data_ptr(),
+                                    top_k, lp.data_ptr(), entropy.data_ptr(), top.data_ptr() if top_k else None,
+                                    ids.data_ptr() if top_k else None, _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
+    _lib.check(rc, "t2i_token_logprobs")
+    return lp, entropy, top, ids
+
+
 def stream_read(src, nbytes: int | None = None, offset: int = 0, loads_per_thread: int = 4, out=None):
     """Read ``nbytes`` of ``src`` from byte ``offset`` with the HBM read-ceiling
     kernel (``t2i_stream_read``) and return the per-wave XOR words (uint32 bit
