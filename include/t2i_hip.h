@@ -497,8 +497,8 @@ int t2i_prompt_advance(const int32_t* prompt, int32_t B, int32_t P, int32_t* tok
  * t2i_packed_plan (host only; every pointer is host memory): checks the batch and
  * writes its table of int32 words, which the two calls below take on the device in
  * the order row_pos [rows], row_cache [rows], items [n_items][8], merges
- * [n_merges][8].  sizes receives rows, n_items, n_merges, n_parts and the table's
- * words; table NULL: sizes only.  0 <= lengths[s], 0 <= starts[s], starts[s] +
+ * [n_merges][8], bins [n_bins + 1].  sizes (6) receives rows, n_items, n_merges, n_parts,
+ * n_bins and the table's words; table NULL: sizes only.  0 <= lengths[s], 0 <= starts[s], starts[s] +
  * lengths[s] <= ctx_cap, distinct cache rows.  The table holds for the heads, the cache
  * rows and the ctx_cap that it was made for.
  *
@@ -526,10 +526,10 @@ int t2i_packed_qk_rope_kv(const uint16_t* qkv, int32_t rows, const int32_t* row_
                           uint16_t* q_out, uint16_t* k_cache, uint16_t* v_cache, int32_t ctx_cap, void* stream);
 size_t t2i_packed_attention_workspace_bytes(int64_t n_parts, int32_t Hkv);
 int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32_t* items, int32_t n_items,
-                         const int32_t* merges, int32_t n_merges, int32_t n_parts, int32_t Hq, int32_t Hkv,
-                         int32_t D, const uint16_t* k_cache, const uint16_t* v_cache, int32_t n_cache_rows,
-                         int32_t ctx_cap, uint16_t* out, float* out_sums, void* workspace,
-                         size_t workspace_bytes, void* stream);
+                         const int32_t* merges, int32_t n_merges, int32_t n_parts, const int32_t* bins,
+                         int32_t n_bins, int32_t Hq, int32_t Hkv, int32_t D, const uint16_t* k_cache,
+                         const uint16_t* v_cache, int32_t n_cache_rows, int32_t ctx_cap, uint16_t* out,
+                         float* out_sums, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Trees of drafted tokens.  Sequence b (cache row b) has context_lens[b] committed

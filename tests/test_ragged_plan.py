@@ -18,8 +18,9 @@ def _tables(plan):
     t, n = plan.table, plan.rows
     items = t[2 * n:2 * n + 8 * plan.n_items].view(-1, 8).tolist()
     at = 2 * n + 8 * plan.n_items
-    merges = t[at:at + 8 * plan.n_merges].view(-1, 8).tolist()
-    return t[:n].tolist(), t[n:2 * n].tolist(), items, merges
+    end = at + 8 * plan.n_merges
+    assert t.numel() == end + plan.n_bins + 1
+    return t[:n].tolist(), t[n:2 * n].tolist(), items, t[at:end].view(-1, 8).tolist(), t[end:].tolist()
 
 
 def _batches():
@@ -41,10 +42,10 @@ def _batches():
 
 @pytest.mark.parametrize("lengths,starts,rows,hq,hkv,cap", list(_batches()))
 def test_plan_covers_every_pair_once(lengths, starts, rows, hq, hkv, cap):
-    """Every (row, head) pair and every key block it attends is in exactly one item; split tiles have one merge
-    over their own parts; rows go to their slots."""
+    """Every (row, head) pair and every key block it attends is in exactly one item, every item in one bin; cut
+    tiles have one merge over their own parts; rows go to their slots; cut plans have even bins."""
     plan = ops.PackedPlan(lengths, hq, hkv, cap, "cpu", starts=starts, cache_rows=rows)
-    pos, crow, items, merges = _tables(plan)
+    pos, crow, items, merges, bins = _tables(plan)
     g, at, want = hq // hkv, 0, {}
     for s, (n, start) in enumerate(zip(lengths, starts)):
         c = s if rows is None else rows[s]
@@ -68,13 +69,20 @@ def test_plan_covers_every_pair_once(lengths, starts, rows, hq, hkv, cap):
             assert ranges[0][2] == -1
         else:
             parts[(key[0], key[1], key[4])] = [p for _, _, p in ranges]
-    assert len(merges) == len(parts)
-    for row0, n, j0, first, count, *_ in merges:
-        assert parts.pop((row0, n, j0)) == list(range(first, first + count))
+    joined = {}
+    for row0, n, j0, first, count, e, *_ in merges:
+        assert parts[row0, n, j0] == list(range(first, first + count))
+        joined.setdefault((row0, n, j0), []).append(e)
+    assert joined == {k: list(range(0, min(k[1] * g - k[2], ROWS), 8)) for k in parts}
     used = [i[7] for i in items if i[7] >= 0]
     assert sorted(used) == list(range(plan.n_parts))
-    lens = [i[6] - i[5] for i in items]
-    assert lens == sorted(lens, reverse=True)
+    assert bins[0] == 0 and bins[-1] == len(items) and all(a < b for a, b in zip(bins, bins[1:]))
+    if plan.n_parts:          # even shares: about one round of workgroups
+        assert plan.n_bins * hkv <= 512 + hkv
+        loads = [sum(i[6] - i[5] for i in items[a:b]) for a, b in zip(bins, bins[1:])]
+        assert max(loads) <= 2 * (sum(loads) / len(loads)) + 3
+    else:                     # a workgroup a tile
+        assert bins == list(range(len(items) + 1))
 
 
 def test_plan_splits_few_rows_over_a_long_context_only():
@@ -99,10 +107,10 @@ def test_plan_entry_point_checks_its_table():
     lib = _lib.load()
     n = torch.tensor([300], dtype=torch.int32)
     s = torch.zeros(1, dtype=torch.int32)
-    sizes = torch.zeros(5, dtype=torch.int64)
+    sizes = torch.zeros(6, dtype=torch.int64)
     call = (n.data_ptr(), s.data_ptr(), None, 1, 16, 8, 1, 512)
     assert lib.t2i_packed_plan(*call, None, 0, sizes.data_ptr()) == 0
-    words = int(sizes[4])
+    words = int(sizes[5])
     table = torch.full((words + 1,), -7, dtype=torch.int32)
     assert lib.t2i_packed_plan(*call, table.data_ptr(), words - 1, sizes.data_ptr()) == E.T2I_ERR_WORKSPACE
     assert (table == -7).all()
@@ -123,9 +131,9 @@ def test_packed_entry_points_refuse():
                      (dict(eps=0.0), E.T2I_ERR_VALUE), (dict(style=2), E.T2I_ERR_VALUE), (dict(kc=ODD), E.T2I_ERR_ALIGN)):
         assert prep(**kw) == code, kw
 
-    def attn(q=FAKE, rows=5, items=FAKE, n_items=3, merges=None, n_merges=0, parts=0, hq=16, hkv=8, d=128, cache=2, cap=64,
+    def attn(q=FAKE, rows=5, items=FAKE, n_items=3, merges=None, n_merges=0, parts=0, bins=FAKE, n_bins=3, hq=16, hkv=8, d=128, cache=2, cap=64,
              out=FAKE, sums=None, ws=None, nbytes=0):
-        return lib.t2i_packed_attention(q, rows, items, n_items, merges, n_merges, parts, hq, hkv, d, FAKE, FAKE, cache, cap, out,
+        return lib.t2i_packed_attention(q, rows, items, n_items, merges, n_merges, parts, bins, n_bins, hq, hkv, d, FAKE, FAKE, cache, cap, out,
                                         sums, ws, nbytes, None)
 
     need = lib.t2i_packed_attention_workspace_bytes(2, 8)
@@ -134,7 +142,8 @@ def test_packed_entry_points_refuse():
     for kw, code in ((dict(q=None), E.T2I_ERR_NULL), (dict(out=ODD), E.T2I_ERR_ALIGN), (dict(items=ODD), E.T2I_ERR_ALIGN),
                      (dict(sums=ODD), E.T2I_ERR_ALIGN), (dict(rows=0), E.T2I_ERR_SHAPE), (dict(n_items=0), E.T2I_ERR_SHAPE),
                      (dict(parts=2), E.T2I_ERR_SHAPE), (dict(hq=15), E.T2I_ERR_SHAPE), (dict(hq=2048), E.T2I_ERR_SHAPE),
-                     (dict(d=256), E.T2I_ERR_SHAPE), (dict(n_items=2**29), E.T2I_ERR_SHAPE), (split, E.T2I_ERR_WORKSPACE),
+                     (dict(d=256), E.T2I_ERR_SHAPE), (dict(n_bins=2**29), E.T2I_ERR_SHAPE), (dict(n_bins=0), E.T2I_ERR_SHAPE),
+                     (dict(bins=None), E.T2I_ERR_NULL), (dict(bins=ODD), E.T2I_ERR_ALIGN), (dict(cap=2**23 + 1), E.T2I_ERR_SHAPE), (split, E.T2I_ERR_WORKSPACE),
                      (dict(**split, ws=FAKE, nbytes=need - 1), E.T2I_ERR_WORKSPACE),
                      (dict(**split, ws=FAKE + 8, nbytes=need), E.T2I_ERR_ALIGN)):
         assert attn(**kw) == code, kw

@@ -110,9 +110,9 @@ SIGNATURES = {
                                         c_void_p, c_void_p, c_float, c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
                                         c_int32, c_void_p]),
     "t2i_packed_attention_workspace_bytes": (c_size_t, [c_int64, c_int32]),
-    "t2i_packed_attention": (c_int32, [c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_int32, c_int32, c_int32,
-                                       c_int32, c_int32, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
-                                       c_void_p, c_size_t, c_void_p]),
+    "t2i_packed_attention": (c_int32, [c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_int32, c_int32, c_void_p,
+                                       c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_int32,
+                                       c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "t2i_tree_qk_rope_kv": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32,
                                       c_int32, c_void_p, c_void_p, c_float, c_void_p, c_int32, c_void_p, c_void_p,
                                       c_void_p, c_int32, c_void_p]),

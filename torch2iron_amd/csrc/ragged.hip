@@ -15,6 +15,7 @@
 #include <math.h>
 
 #include <new>
+#include <type_traits>
 
 #include "t2i_common.h"
 #include "qk_prep.h"
@@ -160,14 +161,16 @@ struct RaggedAttnParams {
   const uint16_t* vc;
   uint16_t* out;            // [rows, Hq * D]
   float* out_sums;          // NULL, or [Hq, rows]: each head's sum of its bf16 context values
-  float* part_o;            // [parts][Hkv][RG_ROWS][D] unnormalised outputs of a part of the keys
-  float2* part_ml;          // [parts][Hkv][RG_ROWS] their running maximum and sum
+  float* part_o;            // [parts][Hkv][part_rows][D] unnormalised outputs of a part of the keys
+  float2* part_ml;          // [parts][Hkv][part_rows] their running maximum and sum
+  int2* cuts;               // trees: [B] first slot and last run of a cut sequence ({-1, }: it is in one piece)
   const int32_t* items;     // packed: [n_items][RG_ITEM]; merge: [n_merges][RG_ITEM]
+  const int32_t* bins;      // packed: [n_bins + 1] each workgroup's first item
   const int32_t* parents;   // trees: [B, N]
   const int32_t* ctx;
   const int32_t* counts;
   long long rows;
-  int n_cache, n_parts, Hq, Hkv, G, cap, N, splits, tiles;
+  int n_cache, n_items, n_bins, n_parts, part_rows, Hq, Hkv, G, cap, B, N, tiles;
   float scale_log2;         // D^-1/2 * log2(e)
 };
 
@@ -178,16 +181,118 @@ struct RaggedItem {
   long long j0, pairs;
 };
 
+// The even shares of a batch of trees: the key blocks of all sequences in a row, cut into `n`
+// equal runs.  A workgroup takes a run for one tile of pairs of one kv head; the tiles of a
+// sequence stand beside each other on one XCD and read the same K and V at the same time, so
+// memory gives them once (8 trees of 64 nodes over 32k slots, 2 tiles: TILE_FIGURES).  A sequence
+// that is cut leaves a part in each of its runs: slot 2 bin where it is the run's first piece,
+// 2 bin + 1 where it is the last of several.
+struct TreeWalk {
+  int n, total, b, blocks, kb;         // n: runs; the next piece starts at block kb of sequence b
+  TreeSeq seq;
+
+  // Key blocks of a sequence; one for zero rows (nodes that do not fit the cache).
+  __device__ __forceinline__ int blocks_of(const TreeSeq& t) const {
+    return t.nodes == 0 ? 0 : t.ok ? (t.ctx + t.nodes + RG_KEYS - 1) / RG_KEYS : 1;
+  }
+  __device__ __forceinline__ int run_start(int i) const { return (int)((long long)total * i / n); }
+  // the run that holds block x
+  __device__ __forceinline__ int run_of(int x) const { return (int)(((long long)(x + 1) * n - 1) / total); }
+
+  // Sums of 64 sequences' blocks at a time; false where there is no such run.
+  __device__ __forceinline__ bool begin(const RaggedAttnParams& p, int bin, int lane, int& at, int& end) {
+    const auto scan = [&](int base) {          // blocks of sequences base .. base + lane
+      int v = base + lane < p.B ? blocks_of(tree_seq(p.ctx, p.counts, base + lane, p.N, p.cap)) : 0;
+#pragma unroll
+      for (int s = 1; s < 64; s <<= 1) {
+        const int u = __shfl_up(v, s, 64);
+        if (lane >= s) v += u;
+      }
+      return v;
+    };
+    total = 0;
+    for (int base = 0; base < p.B; base += 64) total += __builtin_amdgcn_readlane(scan(base), 63);
+    n = max(1, min(p.n_bins, total / 2));
+    if (bin >= n || total == 0) return false;
+    at = run_start(bin);
+    end = run_start(bin + 1);
+    int before = 0;
+    for (int base = 0;; base += 64) {          // ends: at < total
+      const int v = scan(base), sum = __builtin_amdgcn_readlane(v, 63);
+      if (before + sum > at) {
+        const int first = __builtin_ctzll(__ballot(before + v > at));
+        b = base + first;
+        if (first) before += __builtin_amdgcn_readlane(v, first - 1);
+        break;
+      }
+      before += sum;
+    }
+    seq = tree_seq(p.ctx, p.counts, b, p.N, p.cap);
+    blocks = blocks_of(seq);
+    kb = at - before;
+    return true;
+  }
+
+  // The next piece of the run for a tile, and where it ends.
+  __device__ __forceinline__ int next(const RaggedAttnParams& p, int bin, int tile, int h, int at0, int at, int end, RaggedItem& it) {
+    while (kb == blocks) {                     // ends: blocks are left
+      seq = tree_seq(p.ctx, p.counts, ++b, p.N, p.cap);
+      blocks = blocks_of(seq);
+      kb = 0;
+    }
+    const int take = min(blocks - kb, end - at);
+    const bool whole = take == blocks;
+    it.row0 = b * p.N;
+    it.rows = seq.nodes;
+    it.start = seq.ctx;
+    it.crow = b;
+    it.j0 = (long long)tile * RG_ROWS;
+    it.pairs = (long long)seq.nodes * p.G;
+    it.kend = seq.ctx + seq.nodes;
+    it.kb0 = kb;
+    it.kb1 = seq.ok ? kb + take : kb;
+    it.part = whole ? -1 : (2 * bin + (at != at0)) * p.tiles + tile;
+    if (h == 0 && tile == 0 && threadIdx.x == 0 && kb + take == blocks) {   // the sequence's last piece: what its merge reads
+      const int first = at - kb, run = run_of(first);
+      p.cuts[b] = int2{whole ? -1 : 2 * run + (run_start(run) != first), bin};
+    }
+    kb += take;
+    return at + take;
+  }
+};
+
+typedef __attribute__((ext_vector_type(4))) int i32x4;
+
 // Until every vector memory operation of this wave is done, and every wave is here.
 __device__ __forceinline__ void loads_done_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
-// 16 bytes a lane from src into LDS at lds + 16 lane, left in flight: written as asm because
-// the compiler waits for every load into LDS before any read of LDS.  A wait state between
-// the move into M0 and the load; no other SGPR is read.  loads_done_barrier covers it.
+// Loads straight into LDS are written as asm, left in flight, because the compiler waits for
+// every one of them before any read of LDS; loads_done_barrier covers them.  The compiler does
+// not look into asm for hazards: M0 is written a wait state before the load that reads it, and
+// an SGPR that a VALU instruction wrote is five wait states away from a load.
+//
+// 16 bytes a lane from src into LDS at lds + 16 lane.
 __device__ __forceinline__ void lds_load16(const uint16_t* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(lds), "v"(src) : "memory", "m0");
+}
+// Four KB from a buffer: 16 keys, four an instruction, the lane's chunk of instruction i's at
+// byte at[i] (from soff on, less 1024 i).  An instruction's offset counts for the memory address
+// and for the LDS address.
+__device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[4], uint32_t soff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+               "buffer_load_dwordx4 %1, %5, %6 offen lds\n\t"
+               "buffer_load_dwordx4 %2, %5, %6 offen offset:1024 lds\n\t"
+               "buffer_load_dwordx4 %3, %5, %6 offen offset:2048 lds\n\t"
+               "buffer_load_dwordx4 %4, %5, %6 offen offset:3072 lds"
+               :: "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(rsrc), "s"(soff) : "memory", "m0");
+}
+// A buffer over everything from p on (every offset used is inside the cache: checked or clamped).
+__device__ __forceinline__ i32x4 keys_rsrc(const void* p) {
+  const uint64_t a = (uint64_t)(uintptr_t)p;
+  return i32x4{(int)__builtin_amdgcn_readfirstlane((uint32_t)a),
+               (int)(__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32)) & 0xFFFF), -1, 0x00027000};
 }
 __device__ __forceinline__ uint32_t rg_lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
@@ -215,8 +320,9 @@ __device__ __forceinline__ float pair_sum(float v) {
 //     stand in), A = V^T from LDS in that order by transposing reads (ds_read_b64_tr_b16: four
 //     keys of one dim a lane out of V's own row order).
 // K and V blocks go straight from memory into LDS, two buffers, one barrier a block; a row's
-// 16-byte chunk ch stands at place ch ^ 2 (row % 8), which spreads both kinds of reads over all
-// banks (a load into LDS cannot pad rows, but each lane chooses what it loads).  Keys past the
+// 16-byte chunk ch stands at place ch ^ (row % 16) (K) or ch ^ 4 (row % 4) (V): 16 neighbouring
+// lanes of a K read, 32 of a transposing read cover all banks (a load into LDS cannot pad rows,
+// but each lane chooses what it loads).  Keys past the
 // last one reload it: slots that no row attends are never read.
 template <bool TREE>
 __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
@@ -224,31 +330,30 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
   __shared__ __align__(256) uint16_t s_kv[2][2][RG_KEYS * D];   // [buffer][K, V][key][dim]
 
   const int h = blockIdx.x % p.Hkv;
-  const int idx = blockIdx.x / p.Hkv;
+  const int tile = TREE ? blockIdx.x / p.Hkv % p.tiles : 0;
+  const int bin = blockIdx.x / p.Hkv / (TREE ? p.tiles : 1);
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c = lane & 31, h2 = lane >> 5;
 
+  int at = 0, end = 0;          // packed: items; trees: key blocks of the whole batch
+  TreeWalk walk;
+  if (TREE) {
+    if (!walk.begin(p, bin, lane, at, end)) return;
+  } else {
+    at = max(p.bins[bin], 0);
+    end = min(p.bins[bin + 1], p.n_items);
+  }
+  const int at0 = at;
+  for (; at < end;) {
   RaggedItem it;
   if (TREE) {
-    const int tile = idx % p.tiles, bs = idx / p.tiles;
-    const int s = bs % p.splits, b = bs / p.splits;
-    const TreeSeq t = tree_seq(p.ctx, p.counts, b, p.N, p.cap);
-    it.row0 = b * p.N;
-    it.rows = t.nodes;
-    it.start = t.ctx;
-    it.crow = b;
-    it.j0 = (long long)tile * RG_ROWS;
-    it.pairs = (long long)t.nodes * p.G;
-    it.kend = t.ctx + t.nodes;
-    const int blocks = t.ok ? (it.kend + RG_KEYS - 1) / RG_KEYS : 0;
-    it.kb0 = (int)((long long)blocks * s / p.splits);
-    it.kb1 = (int)((long long)blocks * (s + 1) / p.splits);
-    it.part = p.splits > 1 ? (b * p.tiles + tile) * p.splits + s : -1;
-    if (it.j0 >= it.pairs) return;
+    at = walk.next(p, bin, tile, h, at0, at, end, it);
+    if (it.j0 >= it.pairs) continue;                       // this sequence has fewer tiles
   } else {
-    const int32_t* w = p.items + (size_t)idx * RG_ITEM;
+    const int32_t* w = p.items + (size_t)at * RG_ITEM;
+    ++at;
     it.row0 = w[0]; it.rows = w[1]; it.start = w[2]; it.crow = w[3];
     it.j0 = w[4]; it.kb0 = w[5]; it.kb1 = w[6]; it.part = w[7];
     it.pairs = (long long)it.rows * p.G;
@@ -256,7 +361,7 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
     if (it.row0 < 0 || it.rows < 1 || it.row0 + (long long)it.rows > p.rows || it.start < 0 ||
         it.start > p.cap - it.rows || it.crow < 0 || it.crow >= p.n_cache || it.j0 < 0 || it.j0 >= it.pairs ||
         it.pairs > 0x7FFFFFFF - RG_ROWS || it.part >= p.n_parts)
-      return;
+      continue;
     it.kend = it.start + (int)((min(it.j0 + RG_ROWS, it.pairs) - 1) / p.G) + 1;
     it.kb0 = max(it.kb0, 0);
     it.kb1 = min(it.kb1, (it.kend + RG_KEYS - 1) / RG_KEYS);
@@ -267,19 +372,32 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
   const uint16_t* const kbase = p.kc + cache_base;
   const uint16_t* const vbase = p.vc + cache_base;
   const int srow = lane >> 4;                              // key within the instruction's four
-  // chunk of the key that this lane loads, for even and odd instructions (rows 0-3 and 4-7 of 8)
-  const int ch0 = ((lane & 15) ^ (2 * srow)) * 8, ch1 = ((lane & 15) ^ (2 * (4 + srow))) * 8;
+  const int place = lane & 15;                             // where the lane's 16 bytes go in the key's row
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rg_lds_address(s_kv) + wave * 16 * D * 2);
-  auto stage = [&](int kb, int buf) {
+  uint32_t kat[4], vat[4];                                 // what the lane loads: byte in the block, less 1024 i
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = min(kb * RG_KEYS + wave * 16 + 4 * i + srow, it.kend - 1);
-      const size_t off = (size_t)key * D + (i & 1 ? ch1 : ch0);
-      lds_load16(kbase + off, lds0 + buf * (4 * RG_KEYS * D) + i * 4 * D * 2);
-      lds_load16(vbase + off, lds0 + buf * (4 * RG_KEYS * D) + 2 * RG_KEYS * D + i * 4 * D * 2);
+  for (int i = 0; i < 4; ++i) {
+    kat[i] = (wave * 16 + srow) * (D * 2) + 16 * (place ^ (4 * i + srow));
+    vat[i] = (wave * 16 + srow) * (D * 2) + 16 * (place ^ (4 * srow));
+  }
+  const i32x4 krsrc = keys_rsrc(kbase), vrsrc = keys_rsrc(vbase);
+  // K (which = 0) or V (1) block kb into its buffer
+  auto stage = [&](int which, int kb) __attribute__((always_inline)) {
+    const uint32_t lds = lds0 + ((kb - it.kb0) & 1) * (4 * RG_KEYS * D) + which * (2 * RG_KEYS * D);
+    if ((kb + 1) * RG_KEYS <= it.kend) {
+      lds_load_keys(which ? vrsrc : krsrc, which ? vat : kat, (uint32_t)kb * (RG_KEYS * D * 2), lds);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = min(kb * RG_KEYS + wave * 16 + 4 * i + srow, it.kend - 1);
+        lds_load16((which ? vbase : kbase) + (size_t)key * D + 8 * (place ^ (which ? 4 * srow : 4 * i + srow)), lds + i * 4 * D * 2);
+      }
     }
   };
-  if (it.kb0 < it.kb1) stage(it.kb0, 0);
+  if (it.kb0 < it.kb1) {
+    stage(0, it.kb0);
+    stage(1, it.kb0);
+  }
 
   // ---- this lane's pair, and its q row as the B operand ----
   const long long j = it.j0 + wave * 32 + c;
@@ -317,14 +435,14 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
 
   // LDS offsets (elements): K row c of a 32-key tile, V rows by transposing reads
-  const int kx = 2 * (c & 7);
+  const int kx = c & 15;
   const int vi = lane & 15, vrow = 4 * h2 + (vi >> 2);     // key of the 8 that the lane's read names
   const int vcol = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);   // its 16-byte chunk within a 32-dim tile
 
   for (int kb = it.kb0; kb < it.kb1; ++kb) {
     const int buf = (kb - it.kb0) & 1;
     loads_done_barrier();                                  // this block is here, the other buffer is free
-    if (kb + 1 < it.kb1) stage(kb + 1, buf ^ 1);
+    if (kb + 1 < it.kb1) { stage(0, kb + 1); stage(1, kb + 1); }
     if (!wave_on || kb * RG_KEYS >= wave_end) continue;
     const uint16_t* const bk = s_kv[buf][0];
     const uint16_t* const bv = s_kv[buf][1];
@@ -395,7 +513,7 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
       const u32x4 pb = u32x4{w[0], w[1], w[2], w[3]};
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) {
-        const uint16_t* const v = bv + (16 * u + vrow) * D + ((4 * dt + vcol) ^ (2 * vrow)) * 8 + 4 * (vi & 1);
+        const uint16_t* const v = bv + (16 * u + vrow) * D + ((4 * dt + vcol) ^ (4 * (vi >> 2))) * 8 + 4 * (vi & 1);
         typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
         const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
         const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D));
@@ -406,12 +524,14 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
     }
   }
 
+  // the buffers are free for the next item
+  if (at < end) loads_done_barrier();
   // ---- outputs: register i of o[dt] is dim 32 dt + 8 (i / 4) + 4 h2 + i % 4 of the lane's pair ----
-  if (!wave_on) return;
+  if (!wave_on) continue;
   l = pair_sum(l);
   const bool live = j < it.pairs;
   if (it.part >= 0) {
-    const size_t st = ((size_t)it.part * p.Hkv + h) * RG_ROWS + wave * 32 + c;
+    const size_t st = ((size_t)it.part * p.Hkv + h) * p.part_rows + wave * 32 + c;
     m = l != l ? INFINITY : m;                             // a row that saw a NaN stays one in the merge
     if (live && h2 == 0) p.part_ml[st] = float2{m, l};
     if (live && m > -INFINITY) {                           // else its outputs are not read
@@ -422,7 +542,7 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
     }
-    return;
+    continue;
   }
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);   // nothing attended: a zero row; NaN stays
   uint16_t* const dst = p.out + (qrow * p.Hq + head) * D + 8 * h2;
@@ -447,57 +567,84 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
     hs = pair_sum(hs);
     if (live && h2 == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
   }
+  }
 }
 
-// The parts of a tile joined: one wave a (row, q head) pair, lane e its dims 2 e and 2 e + 1,
-// parts in their order.
+// The parts of a tile joined: 32 lanes a (row, q head) pair, four dims each, eight pairs a
+// workgroup; parts in their order, MERGE_AHEAD of them in flight.
+constexpr int MERGE_AHEAD = 4;
+constexpr int MERGE_PAIRS = t2i_host::RG_MERGE;
+
 template <bool TREE>
 __global__ __launch_bounds__(256) void ragged_merge_kernel(const RaggedAttnParams p) {
   constexpr int D = RG_D;
-  const int lane = threadIdx.x & 63;
-  const int at = blockIdx.x % (RG_ROWS / 4) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // pair of the tile
-  const int h = blockIdx.x / (RG_ROWS / 4) % p.Hkv;
-  const int idx = blockIdx.x / (RG_ROWS / 4) / p.Hkv;
-  int row0, rows, first, parts;
-  long long j0;
+  const int lane = threadIdx.x & 31;
+  const int h = blockIdx.x % p.Hkv;
+  const int idx = blockIdx.x / p.Hkv;
+  int row0, rows, first, parts, second, step, j0, at = threadIdx.x >> 5;   // parts: first, then second, second + step, ...
   if (TREE) {
-    const int b = idx / p.tiles, tile = idx - b * p.tiles;
-    const TreeSeq t = tree_seq(p.ctx, p.counts, b, p.N, p.cap);
+    const int groups = p.part_rows / MERGE_PAIRS, group = idx % groups;
+    const int tile = idx / groups % p.tiles, b = idx / groups / p.tiles;
     row0 = b * p.N;
-    rows = t.nodes;
-    j0 = (long long)tile * RG_ROWS;
-    first = idx * p.splits;
-    parts = p.splits;
+    rows = tree_seq(p.ctx, p.counts, b, p.N, p.cap).nodes;
+    at += group * MERGE_PAIRS;
+    j0 = tile * RG_ROWS;
+    if (j0 + group * MERGE_PAIRS >= rows * p.G) return;   // nothing was written for it
+    const int2 w = p.cuts[b];
+    if (w.x < 0) return;                       // one piece: its rows are written
+    first = w.x * p.tiles + tile;
+    parts = w.y - w.x / 2 + 1;
+    second = (w.x / 2 + 1) * 2 * p.tiles + tile;
+    step = 2 * p.tiles;
   } else {
     const int32_t* w = p.items + (size_t)idx * RG_ITEM;
     row0 = w[0]; rows = w[1]; j0 = w[2]; first = w[3]; parts = w[4];
-    if (row0 < 0 || rows < 1 || row0 + (long long)rows > p.rows || j0 < 0 || first < 0 || parts < 1 ||
-        first > p.n_parts - parts)
+    at += w[5];
+    second = first + 1;
+    step = 1;
+    if (row0 < 0 || rows < 1 || row0 + (long long)rows > p.rows || j0 < 0 || j0 > 0x7FFFFFFF - RG_ROWS || first < 0 ||
+        parts < 1 || first > p.n_parts - parts || w[5] < 0 || w[5] > RG_ROWS - MERGE_PAIRS)
       return;
   }
-  const long long j = j0 + at;
-  if (j >= (long long)rows * p.G) return;
-  const int t = (int)(j / p.G);
-  const int head = h * p.G + (int)(j - (long long)t * p.G);
-  const size_t st0 = ((size_t)first * p.Hkv + h) * RG_ROWS + at, step = (size_t)p.Hkv * RG_ROWS;
-  float M = -INFINITY;
-  for (int s = 0; s < parts; ++s) M = fmaxf(M, p.part_ml[st0 + s * step].x);
-  float l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int s = 0; s < parts; ++s) {
-    const float2 ml = p.part_ml[st0 + s * step];
-    if (!(ml.x > -INFINITY)) continue;                     // uniform: the part attended nothing
-    const float f = exp2_fast(ml.x - M);
-    const float2 v = *reinterpret_cast<const float2*>(p.part_o + (st0 + s * step) * D + 2 * lane);
-    l += f * ml.y;
-    o0 += f * v.x;
-    o1 += f * v.y;
+  const int j = j0 + at;
+  if (j >= (long long)rows * p.G) return;      // 32 lanes together
+  const int t = j / p.G;
+  const int head = h * p.G + (j - t * p.G);
+  float M = -INFINITY, l = 0.0f;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < parts; s0 += MERGE_AHEAD) {
+    float2 ml[MERGE_AHEAD];
+    f32x4 v[MERGE_AHEAD];
+#pragma unroll
+    for (int u = 0; u < MERGE_AHEAD; ++u) {
+      const int s = min(s0 + u, parts - 1), part = s == 0 ? first : second + (s - 1) * step;
+      const size_t st = ((size_t)part * p.Hkv + h) * p.part_rows + at;
+      ml[u] = p.part_ml[st];
+      v[u] = *reinterpret_cast<const f32x4*>(p.part_o + st * D + 4 * lane);
+    }
+    float mn = M;
+#pragma unroll
+    for (int u = 0; u < MERGE_AHEAD; ++u) mn = fmaxf(mn, ml[u].x);
+    const float f = state_weight(M, mn);
+    l *= f;
+    o *= f;
+    M = mn;
+#pragma unroll
+    for (int u = 0; u < MERGE_AHEAD; ++u) {
+      const bool some = s0 + u < parts && ml[u].x > -INFINITY;   // else nothing was attended, nor written
+      const float g = exp2_fast(ml[u].x - M);
+      l += some ? g * ml[u].y : 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += some ? g * v[u][e] : 0.0f;
+    }
   }
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-  const uint32_t w = pack_bf16x2(o0 * inv, o1 * inv);
+  const u32x2 w = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
   const size_t qrow = (size_t)row0 + t;
-  *reinterpret_cast<uint32_t*>(p.out + (qrow * p.Hq + head) * D + 2 * lane) = w;
+  *reinterpret_cast<u32x2*>(p.out + (qrow * p.Hq + head) * D + 4 * lane) = w;
   if (p.out_sums) {
-    const float hs = wave_sum(bf16_lo(w) + bf16_hi(w));
+    float hs = row_sum16((bf16_lo(w.x) + bf16_hi(w.x)) + (bf16_lo(w.y) + bf16_hi(w.y)));
+    hs += __shfl_xor(hs, 16, 32);
     if (lane == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
   }
 }
@@ -584,21 +731,39 @@ int check_heads(int32_t Hq, int32_t Hkv, int32_t D, int32_t cap) {
   if (D != t2i::RG_D) return fail(T2I_ERR_SHAPE, "head_dim %d unsupported (only 128)", D);
   if (Hkv < 1 || Hq < Hkv || Hq % Hkv) return fail(T2I_ERR_SHAPE, "Hq=%d Hkv=%d invalid", Hq, Hkv);
   if (Hq > 1024) return fail(T2I_ERR_SHAPE, "Hq=%d exceeds 1024", Hq);
-  if (cap < 1) return fail(T2I_ERR_SHAPE, "ctx_cap=%d invalid", cap);
+  // a kv head's rows of the cache are addressed with 32-bit byte offsets
+  if (cap < 1 || cap > (1 << 23)) return fail(T2I_ERR_SHAPE, "ctx_cap=%d must be 1 to 8388608", cap);
   return T2I_OK;
 }
 
 // Pairs, parts and workgroups stay below 2^31.
 bool too_many(long long n) { return n > 0x7FFFFFFFLL; }
 
-size_t part_bytes(long long parts, int32_t Hkv) {
-  return (size_t)parts * Hkv * t2i::RG_ROWS * (t2i::RG_D * sizeof(float) + sizeof(float2));
+size_t part_bytes(long long parts, int32_t Hkv, int32_t rows) {
+  return (size_t)parts * Hkv * rows * (t2i::RG_D * sizeof(float) + sizeof(float2));
 }
 
-// The workspace's parts: outputs first, then the (max, sum) pairs.
-void set_parts(t2i::RaggedAttnParams& p, void* ws, long long parts) {
+// The workspace's parts: outputs first, then the (max, sum) pairs; returns what follows them.
+void* set_parts(t2i::RaggedAttnParams& p, void* ws, long long parts, int32_t rows) {
+  p.part_rows = rows;
   p.part_o = reinterpret_cast<float*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)parts * p.Hkv * t2i::RG_ROWS * t2i::RG_D);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)parts * p.Hkv * rows * t2i::RG_D);
+  return p.part_ml + (size_t)parts * p.Hkv * rows;
+}
+
+// A tree call's launch: tiles of a sequence, workgroups of a kv head, rows of a part's tile.
+struct TreePlan {
+  int tiles, bins, rows;
+  size_t bytes;
+};
+TreePlan tree_plan(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t cap) {
+  TreePlan t;
+  const int pairs = N * (Hq / Hkv);
+  t.tiles = (pairs + t2i::RG_ROWS - 1) / t2i::RG_ROWS;
+  t.bins = t2i_host::tree_bins(B, t.tiles * Hkv, cap);
+  t.rows = std::min(t2i::RG_ROWS, (pairs + 31) / 32 * 32);
+  t.bytes = part_bytes(2LL * t.bins * t.tiles, Hkv, t.rows) + (size_t)B * sizeof(int2);
+  return t;
 }
 
 int check_prep(const void* qkv, const void* qn, const void* kn, const void* rope, const void* q, const void* kc,
@@ -648,10 +813,11 @@ extern "C" int t2i_packed_plan(const int32_t* lengths, const int32_t* starts, co
     sizes[1] = (int64_t)t.items.size() / t2i::RG_ITEM;
     sizes[2] = (int64_t)t.merges.size() / t2i::RG_ITEM;
     sizes[3] = t.n_parts;
-    sizes[4] = (int64_t)(2 * t.row_pos.size() + t.items.size() + t.merges.size());
+    sizes[4] = (int64_t)t.bins.size() - 1;
+    sizes[5] = (int64_t)(2 * t.row_pos.size() + t.items.size() + t.merges.size() + t.bins.size());
     if (!table) return T2I_OK;
-    if (table_words < sizes[4]) return fail(T2I_ERR_WORKSPACE, "the table holds %lld words, %lld needed", (long long)table_words, (long long)sizes[4]);
-    for (const auto* v : {&t.row_pos, &t.row_cache, &t.items, &t.merges}) table = std::copy(v->begin(), v->end(), table);
+    if (table_words < sizes[5]) return fail(T2I_ERR_WORKSPACE, "the table holds %lld words, %lld needed", (long long)table_words, (long long)sizes[5]);
+    for (const auto* v : {&t.row_pos, &t.row_cache, &t.items, &t.merges, &t.bins}) table = std::copy(v->begin(), v->end(), table);
     return T2I_OK;
   } catch (const std::bad_alloc&) {
     return fail(T2I_ERR_WORKSPACE, "host memory for the plan ran out");
@@ -676,38 +842,40 @@ extern "C" int t2i_packed_qk_rope_kv(const uint16_t* qkv, int32_t rows, const in
 }
 
 extern "C" size_t t2i_packed_attention_workspace_bytes(int64_t n_parts, int32_t Hkv) {
-  return n_parts < 1 || Hkv < 1 || too_many(n_parts) ? 0 : part_bytes(n_parts, Hkv);
+  return n_parts < 1 || Hkv < 1 || too_many(n_parts) ? 0 : part_bytes(n_parts, Hkv, t2i::RG_ROWS);
 }
 
 extern "C" int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32_t* items, int32_t n_items,
-                                    const int32_t* merges, int32_t n_merges, int32_t n_parts, int32_t Hq, int32_t Hkv,
-                                    int32_t D, const uint16_t* k_cache, const uint16_t* v_cache, int32_t n_cache_rows,
-                                    int32_t ctx_cap, uint16_t* out, float* out_sums, void* workspace,
-                                    size_t workspace_bytes, void* stream) {
-  if (!q || !items || !k_cache || !v_cache || !out) return fail(T2I_ERR_NULL, "packed attention pointers must not be NULL");
+                                    const int32_t* merges, int32_t n_merges, int32_t n_parts, const int32_t* bins,
+                                    int32_t n_bins, int32_t Hq, int32_t Hkv, int32_t D, const uint16_t* k_cache,
+                                    const uint16_t* v_cache, int32_t n_cache_rows, int32_t ctx_cap, uint16_t* out,
+                                    float* out_sums, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !items || !bins || !k_cache || !v_cache || !out) return fail(T2I_ERR_NULL, "packed attention pointers must not be NULL");
   if (int rc = check_heads(Hq, Hkv, D, ctx_cap)) return rc;
-  if (rows < 1 || n_cache_rows < 1 || n_items < 1 || n_merges < 0 || n_parts < 0 || (n_parts > 0 && (n_merges < 1 || !merges)))
-    return fail(T2I_ERR_SHAPE, "rows=%d items=%d merges=%d parts=%d invalid", rows, n_items, n_merges, n_parts);
-  if (too_many((long long)n_items * Hkv) || too_many((long long)n_merges * Hkv * (t2i::RG_ROWS / 4)))
-    return fail(T2I_ERR_SHAPE, "%d items of %d kv heads exceed the grid", n_items, Hkv);
+  if (rows < 1 || n_cache_rows < 1 || n_items < 1 || n_bins < 1 || n_merges < 0 || n_parts < 0 ||
+      (n_parts > 0 && (n_merges < 1 || !merges)))
+    return fail(T2I_ERR_SHAPE, "rows=%d items=%d bins=%d merges=%d parts=%d invalid", rows, n_items, n_bins, n_merges, n_parts);
+  if (too_many((long long)n_bins * Hkv) || too_many((long long)n_merges * Hkv))
+    return fail(T2I_ERR_SHAPE, "%d bins of %d kv heads exceed the grid", n_bins, Hkv);
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
     return fail(T2I_ERR_ALIGN, "packed attention tensors must be 16-byte aligned");
-  if (!aligned4(items) || !aligned4(merges) || !aligned4(out_sums))
+  if (!aligned4(items) || !aligned4(merges) || !aligned4(bins) || !aligned4(out_sums))
     return fail(T2I_ERR_ALIGN, "tables and out_sums must be 4-byte aligned");
-  const size_t need = part_bytes(n_parts, Hkv);
+  const size_t need = part_bytes(n_parts, Hkv, t2i::RG_ROWS);
   if (need && (!workspace || workspace_bytes < need)) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
   if (need && !aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
   t2i::RaggedAttnParams p{};
-  p.q = q; p.kc = k_cache; p.vc = v_cache; p.out = out; p.out_sums = out_sums; p.items = items;
-  p.rows = rows; p.n_cache = n_cache_rows; p.n_parts = n_parts; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap;
+  p.q = q; p.kc = k_cache; p.vc = v_cache; p.out = out; p.out_sums = out_sums; p.items = items; p.bins = bins;
+  p.rows = rows; p.n_cache = n_cache_rows; p.n_items = n_items; p.n_bins = n_bins; p.n_parts = n_parts;
+  p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
-  if (need) set_parts(p, workspace, n_parts);
+  if (need) set_parts(p, workspace, n_parts, t2i::RG_ROWS);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(t2i::ragged_attention_kernel<false>, dim3(n_items * Hkv), dim3(256), 0, s, p);
+  hipLaunchKernelGGL(t2i::ragged_attention_kernel<false>, dim3(n_bins * Hkv), dim3(256), 0, s, p);
   if (int rc = t2i_host::hip_status(hipGetLastError(), "packed attention launch")) return rc;
   if (!need) return T2I_OK;
   p.items = merges;
-  hipLaunchKernelGGL(t2i::ragged_merge_kernel<false>, dim3(n_merges * Hkv * (t2i::RG_ROWS / 4)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL(t2i::ragged_merge_kernel<false>, dim3(n_merges * Hkv), dim3(256), 0, s, p);
   return t2i_host::hip_status(hipGetLastError(), "packed attention merge launch");
 }
 
@@ -730,9 +898,7 @@ extern "C" int t2i_tree_qk_rope_kv(const uint16_t* qkv, const int32_t* parents, 
 
 extern "C" size_t t2i_tree_attention_workspace_bytes(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t ctx_cap) {
   if (B < 1 || N < 1 || N > t2i::TREE_NODES || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq > 1024 || ctx_cap < N) return 0;
-  const int tiles = (N * (Hq / Hkv) + t2i::RG_ROWS - 1) / t2i::RG_ROWS;
-  const int splits = t2i_host::tree_splits((long long)B * Hkv * tiles, ctx_cap);
-  return splits > 1 ? part_bytes((long long)B * tiles * splits, Hkv) : 0;
+  return tree_plan(B, N, Hq, Hkv, ctx_cap).bytes;
 }
 
 extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, const int32_t* context_lens,
@@ -746,21 +912,21 @@ extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, con
     return fail(T2I_ERR_ALIGN, "tree attention tensors must be 16-byte aligned");
   t2i::RaggedAttnParams p{};
   p.q = q; p.kc = k_cache; p.vc = v_cache; p.out = out; p.parents = parents; p.ctx = context_lens; p.counts = node_counts;
-  p.rows = (long long)B * N; p.n_cache = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap; p.N = N;
-  p.tiles = (N * p.G + t2i::RG_ROWS - 1) / t2i::RG_ROWS;
-  p.splits = t2i_host::tree_splits((long long)B * Hkv * p.tiles, ctx_cap);
+  const TreePlan t = tree_plan(B, N, Hq, Hkv, ctx_cap);
+  p.rows = (long long)B * N; p.n_cache = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap; p.B = B; p.N = N;
+  p.tiles = t.tiles;
+  p.n_bins = t.bins;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
-  if (too_many((long long)B * p.tiles * Hkv * std::max(p.splits, t2i::RG_ROWS / 4)) || too_many((long long)B * N))
-    return fail(T2I_ERR_SHAPE, "B=%d N=%d Hkv=%d exceed the grid", B, N, Hkv);
-  const size_t need = t2i_tree_attention_workspace_bytes(B, N, Hq, Hkv, ctx_cap);
-  if (need && (!workspace || workspace_bytes < need)) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
-  if (need && !aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
-  if (need) set_parts(p, workspace, (long long)B * p.tiles * p.splits);
+  if (too_many((long long)B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS)) || too_many((long long)B * N) ||
+      too_many((long long)B * ((ctx_cap + t2i::RG_KEYS - 1) / t2i::RG_KEYS)))
+    return fail(T2I_ERR_SHAPE, "B=%d N=%d Hkv=%d over %d slots are too many", B, N, Hkv, ctx_cap);
+  if (!workspace || workspace_bytes < t.bytes) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, t.bytes);
+  if (!aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
+  p.cuts = reinterpret_cast<int2*>(set_parts(p, workspace, 2LL * t.bins * t.tiles, t.rows));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(t2i::ragged_attention_kernel<true>, dim3(B * p.tiles * p.splits * Hkv), dim3(256), 0, s, p);
+  hipLaunchKernelGGL(t2i::ragged_attention_kernel<true>, dim3(t.bins * t.tiles * Hkv), dim3(256), 0, s, p);
   if (int rc = t2i_host::hip_status(hipGetLastError(), "tree attention launch")) return rc;
-  if (!need) return T2I_OK;
-  hipLaunchKernelGGL(t2i::ragged_merge_kernel<true>, dim3(B * p.tiles * Hkv * (t2i::RG_ROWS / 4)), dim3(256), 0, s, p);
+  hipLaunchKernelGGL(t2i::ragged_merge_kernel<true>, dim3(B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS)), dim3(256), 0, s, p);
   return t2i_host::hip_status(hipGetLastError(), "tree attention merge launch");
 }
 

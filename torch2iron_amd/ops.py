@@ -1057,16 +1057,17 @@ class PackedPlan:
         self.n_heads, self.n_kv_heads, self.ctx_cap, self.n_cache_rows = n_heads, n_kv_heads, ctx_cap, n_cache_rows
         lib = _lib.load()
         args = [torch.tensor(v, dtype=torch.int32) for v in (lengths, starts, self.cache_rows)]
-        sizes = torch.zeros(5, dtype=torch.int64)
+        sizes = torch.zeros(6, dtype=torch.int64)
         call = (*(a.data_ptr() for a in args), len(lengths), n_heads, n_kv_heads, n_cache_rows, ctx_cap)
         _lib.check(lib.t2i_packed_plan(*call, None, 0, sizes.data_ptr()), "t2i_packed_plan")
-        self.rows, self.n_items, self.n_merges, self.n_parts, words = sizes.tolist()
-        table = torch.empty(max(words, 1), dtype=torch.int32)
+        self.rows, self.n_items, self.n_merges, self.n_parts, self.n_bins, words = sizes.tolist()
+        table = torch.empty(words, dtype=torch.int32)
         _lib.check(lib.t2i_packed_plan(*call, table.data_ptr(), words, sizes.data_ptr()), "t2i_packed_plan")
         self.table = table.to(self.device)
         base, n = self.table.data_ptr(), 4 * self.rows
         self._row_pos, self._row_cache, self._items = base, base + n, base + 2 * n
         self._merges = self._items + 32 * self.n_items
+        self._bins = self._merges + 32 * self.n_merges
         self._nbytes = lib.t2i_packed_attention_workspace_bytes(self.n_parts, n_kv_heads)
         self.first_rows, self.last_rows, at = [], [], 0
         for x in lengths:
@@ -1145,10 +1146,10 @@ def packed_attention(q: torch.Tensor, plan: PackedPlan, k_cache: torch.Tensor, v
     ws = _scratch(workspace, "packed_attn", plan._nbytes, q.device)
     with _on(plan.device):
         rc = _lib.load().t2i_packed_attention(q.data_ptr(), plan.rows, plan._items, plan.n_items, plan._merges,
-                                              plan.n_merges, plan.n_parts, plan.n_heads, plan.n_kv_heads, d,
-                                              k_cache.data_ptr(), v_cache.data_ptr(), plan.n_cache_rows, plan.ctx_cap,
-                                              out.data_ptr(), _lib.ptr(out_sums), _lib.ptr(ws), plan._nbytes,
-                                              _lib.stream_handle(plan.device))
+                                              plan.n_merges, plan.n_parts, plan._bins, plan.n_bins, plan.n_heads,
+                                              plan.n_kv_heads, d, k_cache.data_ptr(), v_cache.data_ptr(),
+                                              plan.n_cache_rows, plan.ctx_cap, out.data_ptr(), _lib.ptr(out_sums),
+                                              _lib.ptr(ws), plan._nbytes, _lib.stream_handle(plan.device))
     _lib.check(rc, "t2i_packed_attention")
     return out
 
