@@ -67,16 +67,21 @@ def test_strided_rows_from_any_address(gpu, dtype, offset):
     _check(ops.token_logprobs(x, t, top_k=k), _reference(x, t, k))
 
 
-@pytest.mark.parametrize("v", [40, 3000, 20011])
-def test_order_of_equal_values(gpu, v):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v,k", [(40, 32), (3000, 32), (20011, 32), (70003, 7), (9000, 1)])
+def test_order_of_equal_values(gpu, v, k, dtype):
     """Equal logits rank by index, both zeros alike, whichever lane, wave or part holds them."""
-    x = torch.randint(-2, 3, (4, v), device=gpu, generator=torch.Generator(device=gpu).manual_seed(v)).float()
+    x = torch.randint(-2, 3, (40, v), device=gpu, generator=torch.Generator(device=gpu).manual_seed(v)).to(dtype)
+    x[8:24] = torch.randn(16, v, device=gpu, generator=torch.Generator(device=gpu).manual_seed(v)).to(torch.bfloat16)
     x[1] = 0.0
     x[1, 1::2] = -0.0
     x[2] = torch.arange(v, device=gpu).float()
     x[3] = -torch.arange(v, device=gpu).float()
-    t = torch.zeros(4, dtype=torch.int32, device=gpu)
-    _check(ops.token_logprobs(x, t, top_k=32), _reference(x, t, 32))
+    t = torch.zeros(40, dtype=torch.int32, device=gpu)
+    _check(ops.token_logprobs(x, t, top_k=k), _reference(x, t, k))
+    many = x.repeat(40, 1)                                     # rows in one piece each
+    got = ops.token_logprobs(many, t.repeat(40), top_k=k)
+    _check([a[-40:] for a in got], _reference(x, t, k))
 
 
 @pytest.mark.parametrize("v", [50, 9001])
@@ -100,6 +105,23 @@ def test_infinite_and_nan_logits(gpu, v):
     assert lp[1] == -INF and (ent[2], ent[6]) == (0.0, 0.0)
     assert lp[3:6].isnan().all() and ent[3:6].isnan().all() and top[3:6].isnan().all()
     assert ids[3].tolist() == [0, 1, 2, 3] and ids[4, 0] == 7 and ids[5, 0] == v - 2
+
+
+def test_masks_of_the_lowest_value(gpu):
+    """Rows masked with the type's lowest finite value, some and all of them, and rows at its highest."""
+    for dtype in (torch.float32, torch.bfloat16):
+        lo, hi = torch.finfo(dtype).min, torch.finfo(dtype).max
+        x = torch.full((4, 5000), lo, device=gpu, dtype=dtype)
+        x[1, 77:90] = torch.randn(13, device=gpu, generator=torch.Generator(device=gpu).manual_seed(2)).to(dtype)
+        x[2] = hi
+        x[3, ::2] = hi
+        t = torch.tensor([7, 80, 4999, 1], dtype=torch.int32, device=gpu)
+        lp, ent, top, ids = ops.token_logprobs(x, t, top_k=5)
+        ref = _reference(x[:3], t[:3], 5)
+        _check((lp[:3], ent[:3], top[:3], ids[:3]), ref)
+        # a difference past fp32's range is a probability of 0
+        assert lp[3] == -INF and ids[3].tolist() == [0, 2, 4, 6, 8]
+        assert abs(float(ent[3]) - math.log(2500)) < 2e-5 * 9 and (top[3] + math.log(2500)).abs().max() < 2e-5 * 9
 
 
 def test_large_shift(gpu):

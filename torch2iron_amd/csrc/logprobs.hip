@@ -1,10 +1,11 @@
 // Log probabilities of given tokens over rows of logits for gfx950, with each row's entropy
 // and its top alternatives, in one pass over the logits (t2i_token_logprobs).
 //
-// With m the row's maximum, Z = sum e^(x - m) and T = sum e^(x - m) (x - m):
-//   log p(t) = x_t - m - log Z,   entropy = log Z - T / Z.
-// m, Z and T are kept as the pass goes: when the maximum grows by d, Z and T (Z e^-d and
-// (T - d Z) e^-d) follow it.  fp32 throughout, exponents in log2 units.
+// With m the row's largest logit and y = (x - m) log2 e:
+//   Z = sum 2^y,  T = sum 2^y y,  log p(t) = x_t - m - ln Z,  entropy = ln Z - (T / Z) ln 2.
+// m, Z and T are kept as the pass goes: when y's reference falls by d (a larger m), Z and T follow
+// it as Z 2^d and (T + d Z) 2^d.  fp32 throughout; the difference is taken before it is scaled, so
+// that logits of any size (the type's lowest value as a mask among them) keep their places.
 #include <math.h>
 
 #include <algorithm>
@@ -22,7 +23,7 @@ constexpr float LN2 = 0.6931471805599453f;
 
 typedef unsigned long long u64;
 
-// What a part of a row leaves: maximum (natural units), Z, T (log2 units).
+// What a part of a row leaves.
 struct LpState {
   float m, z, t;
 };
@@ -56,14 +57,30 @@ __device__ __forceinline__ u64 lane_key(u64 v, int lane) {
          (uint32_t)__builtin_amdgcn_readlane((uint32_t)v, lane);
 }
 
-// A wave's best keys, descending, one a lane (0: none yet).
+// A wave's best keys, descending, one a lane.  Keys below 2^32 stand for no value.
 struct LpTop {
   u64 list = 0, last = 0;                    // last: the k-th key (uniform)
+  float floor = __uint_as_float(0x7FC00000u);   // its value; NaN, which no comparison passes, while there is none
+  __device__ __forceinline__ void set_last(int k) {
+    last = lane_key(list, k - 1);
+    floor = lp_value(last);
+  }
+  // The list from one key a lane, each in the place of its rank (all different).
+  __device__ __forceinline__ void fill(u64 key, int k) {
+    int rank = 0;
+#pragma unroll 8
+    for (int i = 0; i < 64; ++i) rank += lane_key(key, i) > key;
+    list = (u64)(uint32_t)__builtin_amdgcn_ds_permute(4 * rank, (int)(key >> 32)) << 32 |
+           (uint32_t)__builtin_amdgcn_ds_permute(4 * rank, (int)key);
+    set_last(k);
+  }
   __device__ __forceinline__ void insert(u64 x, int k, int lane) {
     const int pos = __builtin_popcountll(__ballot(list > x));
-    const u64 up = (u64)(uint32_t)__shfl_up((uint32_t)(list >> 32), 1, 64) << 32 | (uint32_t)__shfl_up((uint32_t)list, 1, 64);
+    // every lane's neighbour below (wave_shr:1)
+    const u64 up = (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(list >> 32), 0x138, 0xF, 0xF, false) << 32 |
+                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)list, 0x138, 0xF, 0xF, false);
     list = lane < pos ? list : lane == pos ? x : up;
-    last = lane_key(list, k - 1);
+    set_last(k);
   }
   // every lane's key that belongs here (0: none)
   __device__ __forceinline__ void take(u64 key, int k, int lane) {
@@ -141,8 +158,10 @@ __device__ __forceinline__ void lp_finish(const LpParams& p, int row, LpState st
 }
 
 // One workgroup a (row, part of the row); waves take 16-byte pieces in turn, LP_UNROLL of them a
-// lane in flight, and keep their own state and best list; both meet in LDS.  A wave looks at
-// its values' order only when one passes its k-th best: a ballot a batch otherwise.
+// lane in flight, and keep their own state and best list; both meet in LDS.  A wave's list
+// starts as its lanes' largest values of the first pieces, in order; after that it looks at a
+// piece's order only where a lane's largest value passes the k-th best of its own list and of
+// the other waves' (which only grow, so an older one of them is as good).
 template <typename T>
 __global__ __launch_bounds__(LP_THREADS) void token_logprobs_kernel(const LpParams p) {
   using Ty = LpType<T>;
@@ -161,31 +180,67 @@ __global__ __launch_bounds__(LP_THREADS) void token_logprobs_kernel(const LpPara
 
   LpState st{-INFINITY, 0.0f, 0.0f};
   LpTop top;
-  // values v[0 .. n) of this lane (unused ones -inf, whose weight is 0)
+  // values v[0 .. n) of this lane (unused ones -inf, whose weight is 0); returns their maximum,
+  // NaN where one is NaN
   auto add = [&](const float* v, int n) __attribute__((always_inline)) {
     float mx = v[0];
-    for (int i = 1; i < n; ++i) mx = fmaxf(mx, v[i]);
-    if (mx > st.m) {
-      const float d = st.m > -INFINITY ? (st.m - mx) * LOG2E : -1e30f;   // z and t are 0 at first
+    for (int i = 1; i < n; ++i) mx = __builtin_elementwise_maximum(mx, v[i]);
+    if (!(mx <= st.m)) {
+      const float d = st.m > -INFINITY ? (st.m - mx) * LOG2E : mx != mx ? mx : -1e30f;   // z and t are 0 at first
       const float f = exp2_fast(d);
-      st.t = (st.t + d * st.z) * f;
+      st.t = (st.t + fmaxf(d, -1e30f) * st.z) * f;
       st.z *= f;
       st.m = mx;
     }
     const float ms = st.m > -INFINITY ? st.m : 0.0f;
     for (int i = 0; i < n; ++i) {
-      const float y = (v[i] - ms) * LOG2E;   // not one fma: m LOG2E rounded would shift log Z by its error
+      const float y = fmaxf((v[i] - ms) * LOG2E, -200.0f);   // 2^-200 is 0: a finite number times no weight
       const float e = exp2_fast(y);
       st.z += e;
-      st.t = fmaf(e, fmaxf(y, -1e30f), st.t);   // a weight of 0 times any finite number is 0
+      st.t = fmaf(e, y, st.t);
     }
+    return mx;
   };
+  __shared__ float s_floor[LP_WAVES];
+  if (lane == 0) s_floor[wave] = -INFINITY;
+  __syncthreads();
   const int first = p0 + wave * 64 * LP_UNROLL;
+  u32x4 ahead[LP_UNROLL];                      // the next pieces, on their way
+  const auto load = [&](int q) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < LP_UNROLL; ++u)
+      ahead[u] = *reinterpret_cast<const u32x4*>(src + (size_t)min(q + 64 * u + lane, p1 - 1) * 16);
+  };
+  if (first < p1) load(first);
   for (int q = first; q < p1; q += LP_WAVES * 64 * LP_UNROLL) {
     u32x4 raw[LP_UNROLL];
 #pragma unroll
-    for (int u = 0; u < LP_UNROLL; ++u)
-      raw[u] = *reinterpret_cast<const u32x4*>(src + (size_t)min(q + 64 * u + lane, p1 - 1) * 16);
+    for (int u = 0; u < LP_UNROLL; ++u) raw[u] = ahead[u];
+    if (q + LP_WAVES * 64 * LP_UNROLL < p1) load(q + LP_WAVES * 64 * LP_UNROLL);
+    u64 start = 0;                             // the lane's key that the list started with
+    if (p.k && q == first) {
+      float mx = -INFINITY;
+      int at = -1;
+#pragma unroll
+      for (int u = 0; u < LP_UNROLL; ++u) {
+        const int piece = q + 64 * u + lane;
+        float v[PER];
+        Ty::get(raw[u], v);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (piece < p1 && (at < 0 || v[i] > mx || (v[i] != v[i] && mx == mx))) {
+            mx = v[i];
+            at = head + piece * PER + i;
+          }
+      }
+      start = at < 0 ? (u64)(64 - lane) : lp_key(mx, at);
+      top.fill(start, p.k);
+    }
+    float others = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < LP_WAVES; ++w)
+      others = fmaxf(others, __hip_atomic_load(&s_floor[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
+    const float floor0 = top.floor;
 #pragma unroll
     for (int u = 0; u < LP_UNROLL; ++u) {
       const int piece = q + 64 * u + lane;
@@ -195,18 +250,20 @@ __global__ __launch_bounds__(LP_THREADS) void token_logprobs_kernel(const LpPara
 #pragma unroll
         for (int i = 0; i < PER; ++i) v[i] = -INFINITY;
       }
-      add(v, PER);
-      if (p.k) {
-        bool any = false;
-        const float last = top.last ? lp_value(top.last) : -INFINITY;
+      const float mx = add(v, PER);
+      // a NaN passes; a value equal to the k-th best counts only beside values that the list
+      // already holds from this piece, or at the start from later ones: others stand behind it
+      if (p.k && __ballot(piece < p1 && !(mx < top.floor || (mx == top.floor && !start) || mx < others))) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) any |= !(v[i] <= last);             // a NaN passes
-        if (__ballot(piece < p1 && (any || !top.last))) {
-#pragma unroll
-          for (int i = 0; i < PER; ++i) top.take(piece < p1 ? lp_key(v[i], head + piece * PER + i) : 0, p.k, lane);
-        }
+        for (int i = 0; i < PER; ++i)
+          if (__ballot(piece < p1 && !(v[i] < top.floor || v[i] < others))) {
+            const u64 key = lp_key(v[i], head + piece * PER + i);
+            top.take(piece < p1 && key != start ? key : 0, p.k, lane);
+          }
       }
     }
+    if (p.k && lane == 0 && top.floor != floor0 && top.floor == top.floor)
+      __hip_atomic_store(&s_floor[wave], top.floor, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
   }
   // the values outside the pieces: the first part's, by the first wave
   if (part == 0 && wave == 0) {
@@ -214,7 +271,7 @@ __global__ __launch_bounds__(LP_THREADS) void token_logprobs_kernel(const LpPara
     const int i = lane < 32 ? lane : tail + lane - 32;
     const bool in = lane < 32 ? lane < head : i < p.V;
     const float v = in ? Ty::one(base, i) : -INFINITY;
-    add(&v, 1);
+    (void)add(&v, 1);
     if (p.k) top.take(in ? lp_key(v, i) : 0, p.k, lane);
   }
 
@@ -255,8 +312,11 @@ __global__ __launch_bounds__(64) void token_logprobs_merge_kernel(const LpParams
   const u64* keys = p.part_top + (size_t)row * p.splits * p.k;
   // entry i of every part's list before entry i + 1 of any: the best come first
   for (int i = 0; i < p.k; ++i)
-    for (int s0 = 0; s0 < p.splits; s0 += 64)
-      top.take(s0 + lane < p.splits ? keys[(size_t)(s0 + lane) * p.k + i] : 0, p.k, lane);
+    for (int s0 = 0; s0 < p.splits; s0 += 64) {
+      const u64 key = s0 + lane < p.splits ? keys[(size_t)(s0 + lane) * p.k + i] : 0;
+      if (i == 0 && s0 == 0) top.fill(key >> 32 ? key : (u64)(64 - lane), p.k);
+      else top.take(key, p.k, lane);
+    }
   const char* const base = reinterpret_cast<const char*>(p.logits) + (size_t)row * p.stride * (16 / Ty::PER);
   const int t = p.tokens ? p.tokens[row] : -1;
   const bool in = t >= 0 && t < p.V;

@@ -14,6 +14,7 @@
 // normaliser sums those rounded weights, so that a row of equal values comes back exact.
 #include <math.h>
 
+#include <mutex>
 #include <new>
 #include <type_traits>
 
@@ -24,7 +25,6 @@
 namespace t2i {
 
 constexpr int RG_D = 128;
-constexpr int RG_ROWS = t2i_host::RG_ROWS;
 constexpr int RG_KEYS = t2i_host::RG_KEYS;
 constexpr int RG_ITEM = t2i_host::RG_ITEM;
 constexpr int TREE_NODES = 64;               // nodes of a tree: one lane of a wave each
@@ -170,7 +170,7 @@ struct RaggedAttnParams {
   const int32_t* ctx;
   const int32_t* counts;
   long long rows;
-  int n_cache, n_items, n_bins, n_parts, part_rows, Hq, Hkv, G, cap, B, N, tiles;
+  int n_cache, n_items, n_bins, n_parts, part_rows, tile_rows, Hq, Hkv, G, cap, B, N, tiles;
   float scale_log2;         // D^-1/2 * log2(e)
 };
 
@@ -246,7 +246,7 @@ struct TreeWalk {
     it.rows = seq.nodes;
     it.start = seq.ctx;
     it.crow = b;
-    it.j0 = (long long)tile * RG_ROWS;
+    it.j0 = (long long)tile * p.tile_rows;
     it.pairs = (long long)seq.nodes * p.G;
     it.kend = seq.ctx + seq.nodes;
     it.kb0 = kb;
@@ -263,6 +263,11 @@ struct TreeWalk {
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 
+// Until at most N of this wave's loads into LDS are in flight, and every wave is here.
+template <int N>
+__device__ __forceinline__ void loads_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
+}
 // Until every vector memory operation of this wave is done, and every wave is here.
 __device__ __forceinline__ void loads_done_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -277,16 +282,24 @@ __device__ __forceinline__ void lds_load16(const uint16_t* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(lds), "v"(src) : "memory", "m0");
 }
-// Four KB from a buffer: 16 keys, four an instruction, the lane's chunk of instruction i's at
-// byte at[i] (from soff on, less 1024 i).  An instruction's offset counts for the memory address
-// and for the LDS address.
-__device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[4], uint32_t soff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
-               "buffer_load_dwordx4 %1, %5, %6 offen lds\n\t"
-               "buffer_load_dwordx4 %2, %5, %6 offen offset:1024 lds\n\t"
-               "buffer_load_dwordx4 %3, %5, %6 offen offset:2048 lds\n\t"
-               "buffer_load_dwordx4 %4, %5, %6 offen offset:3072 lds"
-               :: "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(rsrc), "s"(soff) : "memory", "m0");
+// 4 N keys from a buffer, four an instruction, the lane's chunk of instruction i's at byte at[i]
+// (from soff on, less 1024 i).  An instruction's offset counts for the memory address and for
+// the LDS address.
+template <int N>
+__device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[N], uint32_t soff, uint32_t lds) {
+  static_assert(N == 2 || N == 4, "keys of a wave");
+  if constexpr (N == 4)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+                 "buffer_load_dwordx4 %1, %5, %6 offen lds\n\t"
+                 "buffer_load_dwordx4 %2, %5, %6 offen offset:1024 lds\n\t"
+                 "buffer_load_dwordx4 %3, %5, %6 offen offset:2048 lds\n\t"
+                 "buffer_load_dwordx4 %4, %5, %6 offen offset:3072 lds"
+                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(rsrc), "s"(soff) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+                 "buffer_load_dwordx4 %1, %3, %4 offen lds\n\t"
+                 "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 lds"
+                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "s"(rsrc), "s"(soff) : "memory", "m0");
 }
 // A buffer over everything from p on (every offset used is inside the cache: checked or clamped).
 __device__ __forceinline__ i32x4 keys_rsrc(const void* p) {
@@ -324,10 +337,12 @@ __device__ __forceinline__ float pair_sum(float v) {
 // lanes of a K read, 32 of a transposing read cover all banks (a load into LDS cannot pad rows,
 // but each lane chooses what it loads).  Keys past the
 // last one reload it: slots that no row attends are never read.
-template <bool TREE>
-__global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
+template <bool TREE, int WAVES, int RING>
+__global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
   constexpr int D = RG_D;
-  __shared__ __align__(256) uint16_t s_kv[2][2][RG_KEYS * D];   // [buffer][K, V][key][dim]
+  constexpr int ROWS = 32 * WAVES;             // pairs of a tile
+  constexpr int WKEYS = RG_KEYS / WAVES;       // keys of a block that a wave loads
+  extern __shared__ __align__(256) uint16_t s_kv[];   // [RING][K, V][key][dim]
 
   const int h = blockIdx.x % p.Hkv;
   const int tile = TREE ? blockIdx.x / p.Hkv % p.tiles : 0;
@@ -360,9 +375,9 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
     // a table that does not fit the tensors is not followed
     if (it.row0 < 0 || it.rows < 1 || it.row0 + (long long)it.rows > p.rows || it.start < 0 ||
         it.start > p.cap - it.rows || it.crow < 0 || it.crow >= p.n_cache || it.j0 < 0 || it.j0 >= it.pairs ||
-        it.pairs > 0x7FFFFFFF - RG_ROWS || it.part >= p.n_parts)
+        it.pairs > 0x7FFFFFFF - ROWS || it.part >= p.n_parts)
       continue;
-    it.kend = it.start + (int)((min(it.j0 + RG_ROWS, it.pairs) - 1) / p.G) + 1;
+    it.kend = it.start + (int)((min(it.j0 + ROWS, it.pairs) - 1) / p.G) + 1;
     it.kb0 = max(it.kb0, 0);
     it.kb1 = min(it.kb1, (it.kend + RG_KEYS - 1) / RG_KEYS);
   }
@@ -373,31 +388,34 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
   const uint16_t* const vbase = p.vc + cache_base;
   const int srow = lane >> 4;                              // key within the instruction's four
   const int place = lane & 15;                             // where the lane's 16 bytes go in the key's row
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rg_lds_address(s_kv) + wave * 16 * D * 2);
-  uint32_t kat[4], vat[4];                                 // what the lane loads: byte in the block, less 1024 i
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rg_lds_address(s_kv) + wave * WKEYS * D * 2);
+  constexpr int LOADS = WKEYS / 4;                         // instructions of a wave for K, and for V
+  uint32_t kat[LOADS], vat[LOADS];                         // what the lane loads: byte in the block, less 1024 i
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    kat[i] = (wave * 16 + srow) * (D * 2) + 16 * (place ^ (4 * i + srow));
-    vat[i] = (wave * 16 + srow) * (D * 2) + 16 * (place ^ (4 * srow));
+  for (int i = 0; i < LOADS; ++i) {
+    kat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ ((wave * WKEYS + 4 * i + srow) & 15));
+    vat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ (4 * srow));
   }
   const i32x4 krsrc = keys_rsrc(kbase), vrsrc = keys_rsrc(vbase);
-  // K (which = 0) or V (1) block kb into its buffer
-  auto stage = [&](int which, int kb) __attribute__((always_inline)) {
-    const uint32_t lds = lds0 + ((kb - it.kb0) & 1) * (4 * RG_KEYS * D) + which * (2 * RG_KEYS * D);
+  // K and V block kb into its buffer
+  auto stage = [&](int kb) __attribute__((always_inline)) {
+    const uint32_t lds = lds0 + ((kb - it.kb0) & (RING - 1)) * (4 * RG_KEYS * D);
     if ((kb + 1) * RG_KEYS <= it.kend) {
-      lds_load_keys(which ? vrsrc : krsrc, which ? vat : kat, (uint32_t)kb * (RG_KEYS * D * 2), lds);
+      lds_load_keys(krsrc, kat, (uint32_t)kb * (RG_KEYS * D * 2), lds);
+      lds_load_keys(vrsrc, vat, (uint32_t)kb * (RG_KEYS * D * 2), lds + 2 * RG_KEYS * D);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = min(kb * RG_KEYS + wave * 16 + 4 * i + srow, it.kend - 1);
-        lds_load16((which ? vbase : kbase) + (size_t)key * D + 8 * (place ^ (which ? 4 * srow : 4 * i + srow)), lds + i * 4 * D * 2);
+      for (int i = 0; i < LOADS; ++i) {
+        const int at = wave * WKEYS + 4 * i + srow;
+        const size_t key = min(kb * RG_KEYS + at, it.kend - 1);
+        lds_load16(kbase + key * D + 8 * (place ^ (at & 15)), lds + i * 4 * D * 2);
+        lds_load16(vbase + key * D + 8 * (place ^ (4 * srow)), lds + 2 * RG_KEYS * D + i * 4 * D * 2);
       }
     }
   };
-  if (it.kb0 < it.kb1) {
-    stage(0, it.kb0);
-    stage(1, it.kb0);
-  }
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s)
+    if (it.kb0 + s < it.kb1) stage(it.kb0 + s);
 
   // ---- this lane's pair, and its q row as the B operand ----
   const long long j = it.j0 + wave * 32 + c;
@@ -440,12 +458,17 @@ __global__ __launch_bounds__(256, 2) void ragged_attention_kernel(const RaggedAt
   const int vcol = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);   // its 16-byte chunk within a 32-dim tile
 
   for (int kb = it.kb0; kb < it.kb1; ++kb) {
-    const int buf = (kb - it.kb0) & 1;
-    loads_done_barrier();                                  // this block is here, the other buffer is free
-    if (kb + 1 < it.kb1) { stage(0, kb + 1); stage(1, kb + 1); }
+    // this block is here (2 LOADS of each later one may be on their way; the first wait of an
+    // item, behind other kinds of memory operations, is for everything), and the buffer of the
+    // block before it is free
+    const int later = min(RING - 2, it.kb1 - 1 - kb);
+    if (RING > 3 && later == 2 && kb > it.kb0) loads_barrier<4 * LOADS>();
+    else if (RING > 2 && later == 1 && kb > it.kb0) loads_barrier<2 * LOADS>();
+    else loads_done_barrier();
+    if (kb + RING - 1 < it.kb1) stage(kb + RING - 1);
     if (!wave_on || kb * RG_KEYS >= wave_end) continue;
-    const uint16_t* const bk = s_kv[buf][0];
-    const uint16_t* const bv = s_kv[buf][1];
+    const uint16_t* const bk = s_kv + ((kb - it.kb0) & (RING - 1)) * (2 * RG_KEYS * D);
+    const uint16_t* const bv = bk + RG_KEYS * D;
     // ---- S^T = K Q^T ----
     f32x16 s[2];
 #pragma unroll
@@ -588,7 +611,7 @@ __global__ __launch_bounds__(256) void ragged_merge_kernel(const RaggedAttnParam
     row0 = b * p.N;
     rows = tree_seq(p.ctx, p.counts, b, p.N, p.cap).nodes;
     at += group * MERGE_PAIRS;
-    j0 = tile * RG_ROWS;
+    j0 = tile * p.tile_rows;
     if (j0 + group * MERGE_PAIRS >= rows * p.G) return;   // nothing was written for it
     const int2 w = p.cuts[b];
     if (w.x < 0) return;                       // one piece: its rows are written
@@ -602,8 +625,8 @@ __global__ __launch_bounds__(256) void ragged_merge_kernel(const RaggedAttnParam
     at += w[5];
     second = first + 1;
     step = 1;
-    if (row0 < 0 || rows < 1 || row0 + (long long)rows > p.rows || j0 < 0 || j0 > 0x7FFFFFFF - RG_ROWS || first < 0 ||
-        parts < 1 || first > p.n_parts - parts || w[5] < 0 || w[5] > RG_ROWS - MERGE_PAIRS)
+    if (row0 < 0 || rows < 1 || row0 + (long long)rows > p.rows || j0 < 0 || j0 > 0x7FFFFFFF - p.part_rows || first < 0 ||
+        parts < 1 || first > p.n_parts - parts || w[5] < 0 || w[5] > p.part_rows - MERGE_PAIRS)
       return;
   }
   const int j = j0 + at;
@@ -751,17 +774,45 @@ void* set_parts(t2i::RaggedAttnParams& p, void* ws, long long parts, int32_t row
   return p.part_ml + (size_t)parts * p.Hkv * rows;
 }
 
+// The kernel's forms: 4 waves (128 pairs a tile, two workgroups a CU, the next block on its
+// way) and 8 waves (256 pairs, one workgroup a CU, three blocks on their way).
+constexpr int lds_bytes(int ring) { return ring * 2 * t2i::RG_KEYS * t2i::RG_D * 2; }
+
+template <bool TREE>
+int launch_attention(const t2i::RaggedAttnParams& p, long long groups, hipStream_t s) {
+  if (p.tile_rows == 128) {
+    hipLaunchKernelGGL((t2i::ragged_attention_kernel<TREE, 4, 2>), dim3(groups), dim3(256), lds_bytes(2), s, p);
+  } else {
+    // more than 64 KB of LDS: asked for once a device
+    static std::mutex mu;
+    static std::vector<bool> done;
+    int dev = 0;
+    if (int rc = t2i_host::hip_status(hipGetDevice(&dev), "device query")) return rc;
+    std::lock_guard<std::mutex> lock(mu);
+    if ((int)done.size() <= dev) done.resize(dev + 1, false);
+    if (!done[dev]) {
+      if (int rc = t2i_host::hip_status(hipFuncSetAttribute(reinterpret_cast<const void*>(&t2i::ragged_attention_kernel<TREE, 8, 4>),
+                                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes(4)), "LDS attribute"))
+        return rc;
+      done[dev] = true;
+    }
+    hipLaunchKernelGGL((t2i::ragged_attention_kernel<TREE, 8, 4>), dim3(groups), dim3(512), lds_bytes(4), s, p);
+  }
+  return t2i_host::hip_status(hipGetLastError(), "ragged attention launch");
+}
+
 // A tree call's launch: tiles of a sequence, workgroups of a kv head, rows of a part's tile.
 struct TreePlan {
-  int tiles, bins, rows;
+  int tiles, bins, rows, tile_rows;
   size_t bytes;
 };
 TreePlan tree_plan(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t cap) {
   TreePlan t;
   const int pairs = N * (Hq / Hkv);
-  t.tiles = (pairs + t2i::RG_ROWS - 1) / t2i::RG_ROWS;
-  t.bins = t2i_host::tree_bins(B, t.tiles * Hkv, cap);
-  t.rows = std::min(t2i::RG_ROWS, (pairs + 31) / 32 * 32);
+  t.tile_rows = pairs > 128 ? 256 : 128;
+  t.tiles = (pairs + t.tile_rows - 1) / t.tile_rows;
+  t.bins = t2i_host::tree_bins(B, t.tiles * Hkv, cap, t.tile_rows);
+  t.rows = std::min(t.tile_rows, (pairs + 31) / 32 * 32);
   t.bytes = part_bytes(2LL * t.bins * t.tiles, Hkv, t.rows) + (size_t)B * sizeof(int2);
   return t;
 }
@@ -842,7 +893,7 @@ extern "C" int t2i_packed_qk_rope_kv(const uint16_t* qkv, int32_t rows, const in
 }
 
 extern "C" size_t t2i_packed_attention_workspace_bytes(int64_t n_parts, int32_t Hkv) {
-  return n_parts < 1 || Hkv < 1 || too_many(n_parts) ? 0 : part_bytes(n_parts, Hkv, t2i::RG_ROWS);
+  return n_parts < 1 || Hkv < 1 || too_many(n_parts) ? 0 : part_bytes(n_parts, Hkv, t2i_host::RG_ROWS);
 }
 
 extern "C" int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32_t* items, int32_t n_items,
@@ -861,18 +912,19 @@ extern "C" int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32
     return fail(T2I_ERR_ALIGN, "packed attention tensors must be 16-byte aligned");
   if (!aligned4(items) || !aligned4(merges) || !aligned4(bins) || !aligned4(out_sums))
     return fail(T2I_ERR_ALIGN, "tables and out_sums must be 4-byte aligned");
-  const size_t need = part_bytes(n_parts, Hkv, t2i::RG_ROWS);
+  const size_t need = part_bytes(n_parts, Hkv, t2i_host::RG_ROWS);
+  const int tile_rows = t2i_host::RG_ROWS;
   if (need && (!workspace || workspace_bytes < need)) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
   if (need && !aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
   t2i::RaggedAttnParams p{};
   p.q = q; p.kc = k_cache; p.vc = v_cache; p.out = out; p.out_sums = out_sums; p.items = items; p.bins = bins;
+  p.tile_rows = tile_rows;
   p.rows = rows; p.n_cache = n_cache_rows; p.n_items = n_items; p.n_bins = n_bins; p.n_parts = n_parts;
   p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
-  if (need) set_parts(p, workspace, n_parts, t2i::RG_ROWS);
+  if (need) set_parts(p, workspace, n_parts, t2i_host::RG_ROWS);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(t2i::ragged_attention_kernel<false>, dim3(n_bins * Hkv), dim3(256), 0, s, p);
-  if (int rc = t2i_host::hip_status(hipGetLastError(), "packed attention launch")) return rc;
+  if (int rc = launch_attention<false>(p, (long long)n_bins * Hkv, s)) return rc;
   if (!need) return T2I_OK;
   p.items = merges;
   hipLaunchKernelGGL(t2i::ragged_merge_kernel<false>, dim3(n_merges * Hkv), dim3(256), 0, s, p);
@@ -915,6 +967,7 @@ extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, con
   const TreePlan t = tree_plan(B, N, Hq, Hkv, ctx_cap);
   p.rows = (long long)B * N; p.n_cache = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap; p.B = B; p.N = N;
   p.tiles = t.tiles;
+  p.tile_rows = t.tile_rows;
   p.n_bins = t.bins;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
   if (too_many((long long)B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS)) || too_many((long long)B * N) ||
@@ -924,8 +977,7 @@ extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, con
   if (!aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
   p.cuts = reinterpret_cast<int2*>(set_parts(p, workspace, 2LL * t.bins * t.tiles, t.rows));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(t2i::ragged_attention_kernel<true>, dim3(t.bins * t.tiles * Hkv), dim3(256), 0, s, p);
-  if (int rc = t2i_host::hip_status(hipGetLastError(), "tree attention launch")) return rc;
+  if (int rc = launch_attention<true>(p, (long long)t.bins * t.tiles * Hkv, s)) return rc;
   hipLaunchKernelGGL(t2i::ragged_merge_kernel<true>, dim3(B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS)), dim3(256), 0, s, p);
   return t2i_host::hip_status(hipGetLastError(), "tree attention merge launch");
 }

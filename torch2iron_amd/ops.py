@@ -1007,9 +1007,17 @@ def _same_device(device, **tensors):
             raise ValueError(f"{n} is on {t.device}, not on {device}")
 
 
-def _on(device):
-    """The device made current for a launch (the library launches on the current one)."""
-    return torch.cuda.device(device)
+def _launch(device, name: str, *args):
+    """A library call on torch's current stream of ``device``, with that device current (the
+    library launches on the current one)."""
+    fn = getattr(_lib.load(), name)
+    if torch.cuda.current_device() == device.index:
+        rc = fn(*args, _lib.stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, _lib.stream_handle(device))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _scratch(workspace: Workspace | None, key: str, nbytes: int, device):
@@ -1111,13 +1119,10 @@ def packed_qk_rope_kv(qkv: torch.Tensor, plan: PackedPlan, q_norm: torch.Tensor,
                  q_out=q_out)
     if plan.rows == 0:
         return q_out
-    with _on(plan.device):
-        rc = _lib.load().t2i_packed_qk_rope_kv(qkv.data_ptr(), plan.rows, plan._row_pos, plan._row_cache,
-                                               plan.n_cache_rows, plan.n_heads, plan.n_kv_heads, d, q_norm.data_ptr(),
-                                               k_norm.data_ptr(), float(eps), rope.data_ptr(), int(rope_style),
-                                               q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), plan.ctx_cap,
-                                               _lib.stream_handle(plan.device))
-    _lib.check(rc, "t2i_packed_qk_rope_kv")
+    _launch(plan.device, "t2i_packed_qk_rope_kv",
+            qkv.data_ptr(), plan.rows, plan._row_pos, plan._row_cache, plan.n_cache_rows, plan.n_heads, plan.n_kv_heads,
+            d, q_norm.data_ptr(), k_norm.data_ptr(), float(eps), rope.data_ptr(), int(rope_style), q_out.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), plan.ctx_cap)
     return q_out
 
 
@@ -1144,13 +1149,10 @@ def packed_attention(q: torch.Tensor, plan: PackedPlan, k_cache: torch.Tensor, v
     if plan.rows == 0:
         return out
     ws = _scratch(workspace, "packed_attn", plan._nbytes, q.device)
-    with _on(plan.device):
-        rc = _lib.load().t2i_packed_attention(q.data_ptr(), plan.rows, plan._items, plan.n_items, plan._merges,
-                                              plan.n_merges, plan.n_parts, plan._bins, plan.n_bins, plan.n_heads,
-                                              plan.n_kv_heads, d, k_cache.data_ptr(), v_cache.data_ptr(),
-                                              plan.n_cache_rows, plan.ctx_cap, out.data_ptr(), _lib.ptr(out_sums),
-                                              _lib.ptr(ws), plan._nbytes, _lib.stream_handle(plan.device))
-    _lib.check(rc, "t2i_packed_attention")
+    _launch(plan.device, "t2i_packed_attention",
+            q.data_ptr(), plan.rows, plan._items, plan.n_items, plan._merges, plan.n_merges, plan.n_parts, plan._bins,
+            plan.n_bins, plan.n_heads, plan.n_kv_heads, d, k_cache.data_ptr(), v_cache.data_ptr(), plan.n_cache_rows,
+            plan.ctx_cap, out.data_ptr(), _lib.ptr(out_sums), _lib.ptr(ws), plan._nbytes)
     return out
 
 
@@ -1211,13 +1213,10 @@ def tree_qk_rope_kv(qkv: torch.Tensor, parents: torch.Tensor, context_lens: torc
     dev = qkv.device
     _same_device(dev, parents=parents, context_lens=context_lens, node_counts=node_counts, q_norm=q_norm,
                  k_norm=k_norm, rope=rope, k_cache=k_cache, v_cache=v_cache, q_out=q_out)
-    with _on(dev):
-        rc = _lib.load().t2i_tree_qk_rope_kv(qkv.data_ptr(), parents.data_ptr(), context_lens.data_ptr(),
-                                             _lib.ptr(node_counts), b, n, n_heads, n_kv_heads, d, q_norm.data_ptr(),
-                                             k_norm.data_ptr(), float(eps), rope.data_ptr(), int(rope_style),
-                                             q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ctx_cap,
-                                             _lib.stream_handle(dev))
-    _lib.check(rc, "t2i_tree_qk_rope_kv")
+    _launch(dev, "t2i_tree_qk_rope_kv",
+            qkv.data_ptr(), parents.data_ptr(), context_lens.data_ptr(), _lib.ptr(node_counts), b, n, n_heads,
+            n_kv_heads, d, q_norm.data_ptr(), k_norm.data_ptr(), float(eps), rope.data_ptr(), int(rope_style),
+            q_out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), ctx_cap)
     return q_out
 
 
@@ -1252,11 +1251,9 @@ def tree_attention(q: torch.Tensor, parents: torch.Tensor, context_lens: torch.T
     lib = _lib.load()
     nbytes = lib.t2i_tree_attention_workspace_bytes(b, n, hq, n_kv_heads, ctx_cap)
     ws = _scratch(workspace, "tree_attn", nbytes, dev)
-    with _on(dev):
-        rc = lib.t2i_tree_attention(q.data_ptr(), parents.data_ptr(), context_lens.data_ptr(), _lib.ptr(node_counts),
-                                    b, n, hq, n_kv_heads, d, k_cache.data_ptr(), v_cache.data_ptr(), ctx_cap,
-                                    out.data_ptr(), _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
-    _lib.check(rc, "t2i_tree_attention")
+    _launch(dev, "t2i_tree_attention",
+            q.data_ptr(), parents.data_ptr(), context_lens.data_ptr(), _lib.ptr(node_counts), b, n, hq, n_kv_heads, d,
+            k_cache.data_ptr(), v_cache.data_ptr(), ctx_cap, out.data_ptr(), _lib.ptr(ws), nbytes)
     return out
 
 
@@ -1290,15 +1287,12 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     _same_device(dev, parents=parents, picks=picks, context_lens=context_lens, node_counts=node_counts,
                  k_cache=k_cache, v_cache=v_cache)
     rec = torch.empty(b * (n + 3), dtype=torch.int32, device=dev)   # one allocation for the four
-    path, counts, nxt, context = rec[:b * n].view(b, n), rec[b * n:b * n + b], rec[-2 * b:-b], rec[-b:]
-    with _on(dev):
-        rc = _lib.load().t2i_tree_commit(tokens.data_ptr(), parents.data_ptr(), picks.data_ptr(),
-                                         context_lens.data_ptr(), _lib.ptr(node_counts), layers, b, n, hkv, d,
-                                         k_cache.data_ptr(), v_cache.data_ptr(), ctx_cap, path.data_ptr(),
-                                         counts.data_ptr(), nxt.data_ptr(), context.data_ptr(),
-                                         _lib.stream_handle(dev))
-    _lib.check(rc, "t2i_tree_commit")
-    return path, counts, nxt, context
+    path, counts, nxt, context = rec.split((b * n, b, b, b))
+    _launch(dev, "t2i_tree_commit",
+            tokens.data_ptr(), parents.data_ptr(), picks.data_ptr(), context_lens.data_ptr(), _lib.ptr(node_counts),
+            layers, b, n, hkv, d, k_cache.data_ptr(), v_cache.data_ptr(), ctx_cap, path.data_ptr(), counts.data_ptr(),
+            nxt.data_ptr(), context.data_ptr())
+    return path.view(b, n), counts, nxt, context
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, workspace: Workspace | None = None):
@@ -1329,17 +1323,17 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, w
     _same_device(dev, tokens=tokens)
     buf = torch.empty(2 * m + m * top_k, dtype=torch.float32, device=dev)
     ids = torch.empty(m, top_k, dtype=torch.int32, device=dev)
-    lp, entropy, top = buf[:m], buf[m:2 * m], buf[2 * m:].view(m, top_k)
+    lp, entropy, top = buf.split((m, m, m * top_k))
+    top = top.view(m, top_k)
     if m == 0:
         return lp, entropy, top, ids
     lib = _lib.load()
     nbytes = lib.t2i_token_logprobs_workspace_bytes(m, v, top_k)
     ws = _scratch(workspace, "logprobs", nbytes, dev)
-    with _on(dev):
-        rc = lib.t2i_token_logprobs(logits.data_ptr(), _LOGITS_TYPES[logits.dtype], stride, m, v, tokens.data_ptr(),
-                                    top_k, lp.data_ptr(), entropy.data_ptr(), top.data_ptr() if top_k else None,
-                                    ids.data_ptr() if top_k else None, _lib.ptr(ws), nbytes, _lib.stream_handle(dev))
-    _lib.check(rc, "t2i_token_logprobs")
+    _launch(dev, "t2i_token_logprobs",
+            logits.data_ptr(), _LOGITS_TYPES[logits.dtype], stride, m, v, tokens.data_ptr(), top_k, lp.data_ptr(),
+            entropy.data_ptr(), top.data_ptr() if top_k else None, ids.data_ptr() if top_k else None, _lib.ptr(ws),
+            nbytes)
     return lp, entropy, top, ids
 
 
