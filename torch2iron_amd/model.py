@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import numpy as np
 import torch
@@ -274,6 +275,15 @@ class Qwen3DecodeLayer:
     def __call__(self, buf: DecodeBuffers, positions, k_cache, v_cache, normed: bool = False):
         self.attention_half(buf, positions, k_cache, v_cache, normed)
         self.mlp_half(buf)
+
+
+class PromptScore(NamedTuple):
+    """What ``Qwen3Model.score`` says of one prompt of n tokens (device tensors)."""
+
+    logprobs: torch.Tensor       # [n - 1] log p(token i + 1 | tokens 0 .. i)
+    entropy: torch.Tensor        # [n] of the distribution after each token, in nats
+    top_logprobs: torch.Tensor   # [n, top_k]
+    top_ids: torch.Tensor        # [n, top_k]
 
 
 class _Micro:
@@ -618,6 +628,156 @@ class Qwen3Model:
         ops.greedy_advance(self.keys, self.tokens, self.positions, self.history, self.step)
         return logits.clone() if want_logits else None
 
+    # ---- prompts of different lengths, scoring, drafted trees ----
+    def _rows_pass(self, tokens: torch.Tensor, prep, attend) -> torch.Tensor:
+        """Every layer over ``len(tokens)`` rows of any sequences; returns the residual rows.
+        ``prep(i, qkv)`` does layer i's q/k norm, RoPE and cache write and returns q;
+        ``attend(i, q, out, out_sums)`` its attention, and returns ``out_sums`` where it gave them."""
+        c, r, dev = self.cfg, tokens.numel(), self.device
+        empty = lambda *shape, dtype=BF16: torch.empty(*shape, dtype=dtype, device=dev)  # noqa: E731
+        x, xn, qkv = empty(r, c.hidden), empty(r, c.hidden), empty(r, c.qkv_dim)
+        ctx, h = empty(r, c.n_heads * c.head_dim), empty(r, c.intermediate)
+        xs_n = xs_ctx = xs_h = None
+        if self._prefill_sums(r):       # as the prompt pass: each GEMM's input comes with its row group sums
+            xs_n, xs_ctx, xs_h = (empty(n, r, dtype=torch.float32) for n in
+                                  (c.hidden // 128, c.n_heads, c.intermediate // 64))
+        ops.rmsnorm(self.embed, self.layers[0].w.ln1, c.eps, out=xn, tokens=tokens, x_out=x, out_sums=xs_n)
+        for i, layer in enumerate(self.layers):
+            w = layer.w
+            if i > 0 and r <= 64:       # decode-sized: the norm inside the linear
+                ops.rmsnorm_linear(x, w.ln1, c.eps, w.qkv, out=qkv)
+            else:
+                if i > 0:
+                    ops.rmsnorm(x, w.ln1, c.eps, out=xn, out_sums=xs_n)
+                ops.linear(xn, w.qkv, out=qkv, x_sums=xs_n)
+            sums = attend(i, prep(i, qkv), ctx, xs_ctx)
+            ops.linear(ctx, w.o, residual=x, out=x, x_sums=sums)
+            if r <= 64:
+                ops.rmsnorm_gate_up(x, w.ln2, c.eps, w.gate_up, swiglu=True, out=h)
+            else:
+                ops.rmsnorm(x, w.ln2, c.eps, out=xn, out_sums=xs_n)
+                ops.gate_up(xn, w.gate_up, swiglu=True, out=h, x_sums=xs_n, out_sums=xs_h)
+            ops.linear(h, w.down, residual=x, out=x, x_sums=xs_h, sum_parts=2)
+        return x
+
+    def _prompt_list(self, prompts) -> list:
+        """Prompts of any lengths as 1-D host tensors, one for each sequence, checked."""
+        prompts = [torch.as_tensor(p).cpu() for p in prompts]
+        if len(prompts) != self.batch:
+            raise ValueError("prompt batch does not match the model batch size")
+        for p in prompts:
+            if p.dim() != 1 or p.numel() < 1:
+                raise ValueError("every prompt must be a non-empty row of token ids")
+            if p.numel() > self.ctx_cap:
+                raise ValueError(f"a prompt of {p.numel()} tokens exceeds the cache capacity {self.ctx_cap}")
+            if int(p.min()) < 0 or int(p.max()) >= self.cfg.vocab:
+                raise ValueError("prompt token id out of range")
+        return [p.to(torch.int32) for p in prompts]
+
+    def _packed_pass(self, prompts: list):
+        """The packed prompt pass from slot 0 of every cache row: ``(residual rows, plan)``."""
+        c = self.cfg
+        plan = ops.PackedPlan([p.numel() for p in prompts], c.n_heads, c.n_kv_heads, self.ctx_cap, self.device)
+        ws = self.micro[0].buf.workspace
+
+        def prep(i, qkv):
+            layer = self.layers[i]
+            return ops.packed_qk_rope_kv(qkv, plan, layer.w.q_norm, layer.w.k_norm, c.eps, self.rope, self.k_cache[i],
+                                         self.v_cache[i], rope_style=layer.rope_style)
+
+        def attend(i, q, out, out_sums):
+            ops.packed_attention(q, plan, self.k_cache[i], self.v_cache[i], out=out, out_sums=out_sums, workspace=ws)
+            return out_sums
+
+        return self._rows_pass(torch.cat(prompts).to(self.device), prep, attend), plan
+
+    def prefill_packed(self, prompts, want_logits: bool = False):
+        """``prefill`` for prompts of different lengths (one row of token ids for each sequence of the
+        batch) without padding: one pass over their rows packed one after the other.  Afterwards
+        ``tokens`` holds each sequence's first new token, ``positions`` its prompt's length and
+        ``history[:, 0]`` the token.  Returns the fp32 logits of the last prompt rows when
+        ``want_logits`` (else None).  The reference consumes such prompts one sequence at a
+        time (``quantized_qwen3/qwen_npu.py:309-315``)."""
+        x, plan = self._packed_pass(self._prompt_list(prompts))
+        last = torch.tensor(plan.last_rows, dtype=torch.int32).to(self.device)
+        ops.rmsnorm(x, self.norm, self.cfg.eps, out=self.xn, tokens=last, x_out=self.x, argmax_keys=self.keys)
+        logits = self._logits_out(want_logits)
+        ops.lm_head_argmax(self.xn, self.lm_head, self.keys, logits=logits)
+        self.positions.copy_(torch.tensor(plan.lengths, dtype=torch.int32) - 1)
+        self.step.zero_()
+        ops.greedy_advance(self.keys, self.tokens, self.positions, self.history, self.step)
+        return logits.clone() if want_logits else None
+
+    # rows of logits that ``score`` holds at a time (Qwen3-0.6B: 156 MB)
+    SCORE_ROWS = 256
+
+    def score(self, prompts, top_k: int = 0) -> list:
+        """Log probabilities of the tokens of ``prompts`` (as ``prefill_packed``; the cache rows are
+        overwritten from slot 0): for each prompt of n tokens a ``PromptScore`` of ``logprobs [n - 1]``
+        (token i + 1 after the tokens before it), ``entropy [n]`` (nats), ``top_logprobs`` and ``top_ids
+        [n, top_k]`` of what may follow each token."""
+        prompts = self._prompt_list(prompts)
+        x, plan = self._packed_pass(prompts)
+        target = torch.cat([torch.cat((p[1:], p.new_full((1,), -1))) for p in prompts]).to(self.device)
+        xn = ops.rmsnorm(x, self.norm, self.cfg.eps)
+        chunk = min(self.SCORE_ROWS, plan.rows)
+        logits = torch.empty(chunk, self.cfg.vocab, dtype=torch.float32, device=self.device)
+        parts = []
+        for a in range(0, plan.rows, chunk):
+            n = min(chunk, plan.rows - a)
+            keys = torch.zeros(n, dtype=torch.int64, device=self.device)
+            ops.lm_head_argmax(xn[a:a + n], self.lm_head, keys, logits=logits[:n])
+            parts.append(ops.token_logprobs(logits[:n], target[a:a + n], top_k=top_k,
+                                            workspace=self.micro[0].buf.workspace))
+        lp, entropy, top, ids = (torch.cat(v) for v in zip(*parts))
+        return [PromptScore(lp[a:b], entropy[a:b + 1], top[a:b + 1], ids[a:b + 1])
+                for a, b in zip(plan.first_rows, plan.last_rows)]
+
+    def verify_tree(self, tokens: torch.Tensor, parents: torch.Tensor, node_counts: torch.Tensor | None = None):
+        """One step over drafted trees: every node of ``tokens`` int32 ``[B, N]`` (N at most 64; ``parents``
+        and ``node_counts`` as ``ops.tree_attention``) in one pass over the cache, the greedy
+        walk down each tree, and the accepted path's K/V rows left in their places.  Node 0
+        stands for the sequence's pending token (``self.tokens``, put there by this call).
+
+        The state moves on as by as many decode steps: ``positions`` by the accepted nodes, ``tokens`` to
+        the token after the last of them.  Returns device int32 ``(new_tokens [B, N], counts [B])``: the
+        tokens that the step found, padded with -1 (the accepted drafted ones, then the one after
+        them: what greedy decode emits), and how many.  A sequence without nodes or without
+        room for them in the cache stays as it is, with count 0.  Nothing is read back: the
+        call can be captured once its workspaces exist."""
+        c = self.cfg
+        b, n = ops.check_tree(parents, self.positions, node_counts)
+        if tuple(tokens.shape) != (b, n) or b != self.batch:
+            raise ValueError(f"tokens and parents must be [{self.batch}, N]")
+        if tokens.dtype != torch.int32:
+            raise ValueError(f"tokens must be int32, got {tokens.dtype}")
+        ctx, ws = self.positions, self.micro[0].buf.workspace
+        nodes = torch.cat((self.tokens[:, None], tokens[:, 1:]), 1)
+
+        def prep(i, qkv):
+            layer = self.layers[i]
+            return ops.tree_qk_rope_kv(qkv, parents, ctx, c.n_heads, c.n_kv_heads, layer.w.q_norm, layer.w.k_norm, c.eps,
+                                       self.rope, self.k_cache[i], self.v_cache[i], rope_style=layer.rope_style,
+                                       node_counts=node_counts)
+
+        def attend(i, q, out, out_sums):
+            ops.tree_attention(q, parents, ctx, c.n_kv_heads, self.k_cache[i], self.v_cache[i], node_counts=node_counts,
+                               out=out, workspace=ws)
+
+        x = self._rows_pass(nodes.view(-1), prep, attend)
+        keys = torch.empty(b * n, dtype=torch.int64, device=self.device)
+        xn = ops.rmsnorm(x, self.norm, c.eps, argmax_keys=keys)
+        ops.lm_head_argmax(xn, self.lm_head, keys)
+        picks = ops.keys_to_tokens(keys).to(torch.int32).view(b, n)
+        path, counts, nxt, after = ops.tree_commit(nodes, parents, picks, ctx, self.k_cache, self.v_cache,
+                                                   node_counts=node_counts)
+        at = torch.arange(n, dtype=torch.int32, device=self.device)
+        took = nodes.gather(1, path.clamp(min=0).long().roll(-1, 1))     # the tokens of the walk behind node 0
+        new = torch.where(at < counts[:, None] - 1, took, torch.where(at == counts[:, None] - 1, nxt[:, None], -1))
+        self.tokens.copy_(torch.where(counts > 0, nxt, self.tokens))
+        self.positions.copy_(after)
+        return new, counts
+
     # ---- graph-captured greedy generation ----
     def _capture_graph(self, stream, fn):
         stream.wait_stream(torch.cuda.current_stream(self.device))
@@ -696,10 +856,22 @@ class Qwen3Model:
         ``prompt_mode="prefill"``: the prompt goes through one prefill pass
         (``prefill``).  ``"decode"``: it is consumed one position at a time
         through the decode step (teacher forcing), as the NPU runner does.
+        ``prompt`` may also be a list of prompts of different lengths, one for each sequence
+        (``prompt_mode="prefill"``: one packed pass, ``prefill_packed``).
         Returns int64 ``[B, new_tokens]`` on the host.
         """
         if prompt_mode not in ("prefill", "decode"):
             raise ValueError("prompt_mode must be 'prefill' or 'decode'")
+        ragged = None
+        if isinstance(prompt, (list, tuple)) and all(hasattr(p, "__len__") for p in prompt) and len(set(map(len, prompt))) > 1:
+            if prompt_mode != "prefill":
+                raise ValueError("prompts of different lengths need prompt_mode 'prefill'")
+            ragged = self._prompt_list(prompt)
+            b, plen = len(ragged), max(p.numel() for p in ragged)
+            prompt = torch.zeros(b, plen, dtype=torch.int32)   # a first token each, for the eager step before a capture
+            prompt[:, 0] = torch.stack([p[0] for p in ragged])
+        elif isinstance(prompt, (list, tuple)) and all(isinstance(p, torch.Tensor) for p in prompt):
+            prompt = torch.stack(list(prompt))
         prompt = torch.as_tensor(prompt)
         b, plen = prompt.shape
         if b != self.batch:
@@ -736,7 +908,9 @@ class Qwen3Model:
             self.step.zero_()
             torch.cuda.synchronize(self.device)
         ev[0].record()
-        if prompt_mode == "prefill":
+        if ragged is not None:
+            self.prefill_packed(ragged)
+        elif prompt_mode == "prefill":
             self.prefill(self.prompt)      # the device copy: no host transfer inside the pass
         elif use_graph:
             for _ in range(plen - 1):

@@ -1156,7 +1156,8 @@ def packed_attention(q: torch.Tensor, plan: PackedPlan, k_cache: torch.Tensor, v
     return out
 
 
-def _check_tree(parents, context_lens, node_counts):
+def check_tree(parents, context_lens, node_counts):
+    """The checks that every tree call makes of its topology; returns ``(B, N)``."""
     _check_dev("parents", parents, torch.int32)
     _check_dev("context_lens", context_lens, torch.int32)
     if parents.dim() != 2:
@@ -1193,7 +1194,7 @@ def tree_qk_rope_kv(qkv: torch.Tensor, parents: torch.Tensor, context_lens: torc
     stands before it; anything else makes it a root), ``context_lens`` int32 ``[B]``,
     ``node_counts`` int32 ``[B]`` (all N by default; rows behind a count are left as they are).
     A sequence whose nodes do not fit the cache writes nothing.  Returns q bf16 ``[B, N, Hq, D]``."""
-    b, n = _check_tree(parents, context_lens, node_counts)
+    b, n = check_tree(parents, context_lens, node_counts)
     for nm, t in (("qkv", qkv), ("q_norm", q_norm), ("k_norm", k_norm), ("rope", rope)):
         _check_dev(nm, t, BF16)
     d = q_norm.numel()
@@ -1232,7 +1233,7 @@ def tree_attention(q: torch.Tensor, parents: torch.Tensor, context_lens: torch.T
     whose nodes do not fit the cache gets zero rows.  Everything that varies from step to step
     is on the device: a captured call serves every later step."""
     _check_dev("q", q, BF16)
-    b, n = _check_tree(parents, context_lens, node_counts)
+    b, n = check_tree(parents, context_lens, node_counts)
     if q.dim() != 4 or tuple(q.shape[:2]) != (b, n):
         raise ValueError(f"q must be [{b}, {n}, Hq, D]")
     hq, d = q.shape[2:]
@@ -1269,7 +1270,7 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
 
     Returns int32 ``(path [B, N]: the walk's nodes, then -1; counts [B]; next_tokens [B]: the last
     node's pick; context_lens [B] after the walk)``."""
-    b, n = _check_tree(parents, context_lens, node_counts)
+    b, n = check_tree(parents, context_lens, node_counts)
     for nm, t in (("tokens", tokens), ("picks", picks)):
         _check_dev(nm, t, torch.int32)
         if t.numel() != b * n:
