@@ -110,7 +110,7 @@ def test_packed_attention(gpu, hq, hkv, cap, lengths, starts, cache_rows, n_cach
 def test_packed_attention_splits_and_merges(gpu):
     """The batches above whose plans split keys really do."""
     plans = [ops.PackedPlan(c[3], c[0], c[1], c[2], gpu, starts=c[4], cache_rows=c[5], n_cache_rows=c[6]) for c in PACKED]
-    assert sum(p.n_parts > 0 for p in plans) >= 2 and sum(p.n_parts == 0 for p in plans) >= 6
+    assert sum(p.n_parts > 0 for p in plans) >= 5 and sum(p.n_parts == 0 for p in plans) >= 5
 
 
 def test_packed_equal_lengths_agree_with_the_batch_form(gpu):

@@ -285,9 +285,23 @@ __device__ __forceinline__ void lds_load16(const uint16_t* src, uint32_t lds) {
 // 4 N keys from a buffer, four an instruction, the lane's chunk of instruction i's at byte at[i]
 // (from soff on, less 1024 i).  An instruction's offset counts for the memory address and for
 // the LDS address.
-template <int N>
+template <int N, bool ONCE>
 __device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[N], uint32_t soff, uint32_t lds) {
   static_assert(N == 2 || N == 4, "keys of a wave");
+  if constexpr (ONCE) {
+  if constexpr (N == 4)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+                 "buffer_load_dwordx4 %1, %5, %6 offen nt lds\n\t"
+                 "buffer_load_dwordx4 %2, %5, %6 offen offset:1024 nt lds\n\t"
+                 "buffer_load_dwordx4 %3, %5, %6 offen offset:2048 nt lds\n\t"
+                 "buffer_load_dwordx4 %4, %5, %6 offen offset:3072 nt lds"
+                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(rsrc), "s"(soff) : "memory", "m0");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+                 "buffer_load_dwordx4 %1, %3, %4 offen nt lds\n\t"
+                 "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 nt lds"
+                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "s"(rsrc), "s"(soff) : "memory", "m0");
+  } else {
   if constexpr (N == 4)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
                  "buffer_load_dwordx4 %1, %5, %6 offen lds\n\t"
@@ -300,6 +314,7 @@ __device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[N
                  "buffer_load_dwordx4 %1, %3, %4 offen lds\n\t"
                  "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 lds"
                  :: "s"(lds), "v"(at[0]), "v"(at[1]), "s"(rsrc), "s"(soff) : "memory", "m0");
+  }
 }
 // A buffer over everything from p on (every offset used is inside the cache: checked or clamped).
 __device__ __forceinline__ i32x4 keys_rsrc(const void* p) {
@@ -401,8 +416,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
   auto stage = [&](int kb) __attribute__((always_inline)) {
     const uint32_t lds = lds0 + ((kb - it.kb0) & (RING - 1)) * (4 * RG_KEYS * D);
     if ((kb + 1) * RG_KEYS <= it.kend) {
-      lds_load_keys(krsrc, kat, (uint32_t)kb * (RG_KEYS * D * 2), lds);
-      lds_load_keys(vrsrc, vat, (uint32_t)kb * (RG_KEYS * D * 2), lds + 2 * RG_KEYS * D);
+      const uint32_t at = (uint32_t)kb * (RG_KEYS * D * 2);
+      if (it.pairs <= ROWS) {                              // the sequence's only tile: its keys are read once
+        lds_load_keys<LOADS, true>(krsrc, kat, at, lds);
+        lds_load_keys<LOADS, true>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
+      } else {
+        lds_load_keys<LOADS, false>(krsrc, kat, at, lds);
+        lds_load_keys<LOADS, false>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {

@@ -6,7 +6,6 @@
 #include <stdint.h>
 
 #include <algorithm>
-#include <queue>
 #include <vector>
 
 namespace t2i_host {
@@ -34,98 +33,108 @@ inline int tile_blocks(int64_t j0, int64_t pairs, int G, int start) {
   return (int)((start + last / G + RG_KEYS) / RG_KEYS);
 }
 
-// Time of a key block of a tile, in twelfths of a full tile's: with fewer than 128 pairs some of
-// the four waves have nothing to multiply, but the block's loads take nearly as long.
-inline int64_t block_cost(int64_t pairs) { return pairs > 32 ? 12 : 11; }
-constexpr int64_t TILE_COST = 3 * 12;     // first loads and outputs of an item
-constexpr int64_t MERGE_COST = 8 * 12;    // a second launch that joins parts
+// Times in us that the choice below goes by, fitted to graph-launched calls (1 to 64 sequences, 1 to
+// 4000 rows, 0 to 6000 slots before them, 8 kv heads of 2 and 4 q heads): a key block of a
+// workgroup that has its CU alone, and its share of a CU that two workgroups fill; tiles of up
+// to 32 pairs (one wave of four multiplies) wait for their loads longer.
+struct BlockTime { double alone, shared; };
+inline BlockTime block_time(int64_t pairs) { return pairs > 32 ? BlockTime{1.35, 1.1} : BlockTime{1.75, 1.35}; }
+constexpr double RG_CUS = 256, ITEM_TIME = 2.5;       // ITEM_TIME: first loads and outputs
+constexpr double CALL_TIME = 4, MERGE_TIME = 5;       // MERGE_TIME: a second launch
+constexpr double PART_BYTES_PER_US = 1e7;             // parts written and read again
 
-// Two ways to hand the tiles out, whichever a count of their costs says ends sooner:
+inline PackedTable packed_items(const int32_t* lengths, const int32_t* starts, const int32_t* cache_rows, int n, int G,
+                                int Hkv);
+
+// Two ways to hand the tiles out, whichever the times above say ends sooner:
 //   whole: a workgroup a tile, longest first (the chip takes the next as slots come free);
 //   even:  RG_SLOTS workgroups with equal shares of the tiles' key blocks, cut where a share
 //          ends; the parts of a cut tile are joined by a second launch.
+// Measured (us, whole / even; taken): 1999 rows from 6001, 32 / 8 heads 237 / 258 (whole); 1000 rows
+// from 6001 151 / 132 (even); 32 x 500 rows 129 / 213 (whole); 2000 rows from 0, 16 / 8 47 / 42
+// (even); 16 single rows from 4000 113 / 47, 4 of them 108 / 19 (even); 4 x 300 rows 11.4 / 16.5 (whole).
 inline PackedTable packed_table(const int32_t* lengths, const int32_t* starts, const int32_t* cache_rows, int n, int G,
                                 int Hkv) {
-  PackedTable t;
-  struct Tile { int32_t seq, row0; int64_t j0; int32_t blocks; int64_t cost; };
-  std::vector<Tile> tiles;
-  int64_t row0 = 0, work = 0;
-  for (int i = 0; i < n; ++i) {
-    const int64_t pairs = (int64_t)lengths[i] * G;
-    for (int64_t j0 = 0; j0 < pairs; j0 += RG_ROWS) {
-      const int b = tile_blocks(j0, pairs, G, starts[i]);
-      tiles.push_back({i, (int32_t)row0, j0, b, block_cost(std::min<int64_t>(pairs - j0, RG_ROWS))});
-      work += b * tiles.back().cost;
-    }
+  PackedTable t = packed_items(lengths, starts, cache_rows, n, G, Hkv);
+  for (int i = 0; i < n; ++i)
     for (int32_t r = 0; r < lengths[i]; ++r) {
       t.row_pos.push_back(starts[i] + r);
       t.row_cache.push_back(cache_rows ? cache_rows[i] : i);
     }
+  return t;
+}
+
+inline PackedTable packed_items(const int32_t* lengths, const int32_t* starts, const int32_t* cache_rows, int n, int G,
+                                int Hkv) {
+  struct Tile { int32_t seq, row0; int64_t j0, live; int32_t blocks; BlockTime time; };
+  std::vector<Tile> tiles;
+  int64_t row0 = 0;
+  double work = 0, longest = 0;                        // a kv head's, and one tile's
+  for (int i = 0; i < n; ++i) {
+    const int64_t pairs = (int64_t)lengths[i] * G;
+    for (int64_t j0 = 0; j0 < pairs; j0 += RG_ROWS) {
+      const int64_t live = std::min<int64_t>(pairs - j0, RG_ROWS);
+      tiles.push_back({i, (int32_t)row0, j0, live, tile_blocks(j0, pairs, G, starts[i]), block_time(live)});
+      work += tiles.back().blocks * tiles.back().time.shared;
+      longest = std::max(longest, tiles.back().blocks * tiles.back().time.alone);
+    }
     row0 += lengths[i];
   }
-  const auto item = [&](const Tile& a, int k0, int k1, int part) {
+  std::stable_sort(tiles.begin(), tiles.end(),
+                   [](const Tile& a, const Tile& b) { return a.blocks * a.time.alone > b.blocks * b.time.alone; });
+  const auto item = [&](PackedTable& t, const Tile& a, int k0, int k1, int part) {
     const int32_t w[RG_ITEM] = {a.row0, lengths[a.seq], starts[a.seq], cache_rows ? cache_rows[a.seq] : a.seq,
                                 (int32_t)a.j0, k0, k1, part};
     t.items.insert(t.items.end(), w, w + RG_ITEM);
   };
-  std::stable_sort(tiles.begin(), tiles.end(),
-                   [](const Tile& a, const Tile& b) { return a.blocks * a.cost > b.blocks * b.cost; });
-  const int64_t slots = std::max(1, RG_SLOTS / Hkv);   // a kv head's
-  int64_t whole = 0;                                   // when the last slot is done
-  {
-    std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>> free_at;
-    for (const Tile& a : tiles) {
-      int64_t at = 0;
-      if ((int64_t)free_at.size() >= slots) {
-        at = free_at.top();
-        free_at.pop();
-      }
-      free_at.push(at + a.blocks * a.cost + TILE_COST);
-      whole = std::max(whole, at + a.blocks * a.cost + TILE_COST);
-    }
-  }
-  // a share is at least two full key blocks
-  const int64_t n_even = std::max<int64_t>(1, std::min<int64_t>(slots, work / (2 * 12)));
-  const int64_t share = (work + n_even - 1) / n_even;
-  const int64_t even = share + 2 * TILE_COST + MERGE_COST;
-  t.bins.push_back(0);
-  if (whole <= even) {
-    for (const Tile& a : tiles) {
-      item(a, 0, a.blocks, -1);
-      t.bins.push_back((int32_t)(t.items.size() / RG_ITEM));
-    }
-    return t;
-  }
-  int64_t room = share;                                // of the open bin
+  const auto close_bin = [](PackedTable& t) { t.bins.push_back((int32_t)(t.items.size() / RG_ITEM)); };
+  PackedTable whole;
+  whole.bins.push_back(0);
   for (const Tile& a : tiles) {
-    std::vector<int> cuts{0};
+    item(whole, a, 0, a.blocks, -1);
+    close_bin(whole);
+  }
+  const double heads = Hkv / RG_CUS;
+  const double whole_time = CALL_TIME + std::max(longest + 1, work * heads + tiles.size() * heads * ITEM_TIME);
+  // (no cut can end before the tiles' own work)
+  if (whole_time <= CALL_TIME + MERGE_TIME + work * heads + tiles.size() * heads * ITEM_TIME) return whole;
+
+  const int64_t slots = std::max(1, RG_SLOTS / Hkv);   // a kv head's
+  // a share is at least two key blocks
+  const int64_t n_even = std::max<int64_t>(1, std::min<int64_t>(slots, (int64_t)(work / (2 * 1.1))));
+  const double share = work / n_even;
+  PackedTable even;
+  even.bins.push_back(0);
+  double room = share, merged = 0;                     // of the open bin; pairs of all parts
+  for (const Tile& a : tiles) {
     std::vector<size_t> at;                            // items of the tile
-    while (cuts.back() < a.blocks) {
-      const int left = a.blocks - cuts.back();
-      int take = (int)std::min<int64_t>(left, std::max<int64_t>(1, (room + a.cost / 2) / a.cost));
+    for (int k0 = 0; k0 < a.blocks;) {
+      const int left = a.blocks - k0;
+      int take = (int)std::min<double>(left, std::max(1.0, room / a.time.shared + 0.5));
       if (left - take == 1) take = left;               // no part of a single block
-      at.push_back(t.items.size());
-      item(a, cuts.back(), cuts.back() + take, -1);
-      cuts.push_back(cuts.back() + take);
-      room -= take * a.cost;
-      if (room < a.cost) {                             // the share is used up
-        t.bins.push_back((int32_t)(t.items.size() / RG_ITEM));
-        room += share;
-        if (room < a.cost) room = a.cost;
+      at.push_back(even.items.size());
+      item(even, a, k0, k0 + take, -1);
+      k0 += take;
+      room -= take * a.time.shared;
+      if (room < a.time.shared) {                      // the share is used up
+        close_bin(even);
+        room = std::max(room + share, a.time.shared);
       }
     }
     if (at.size() > 1) {
-      for (size_t s = 0; s < at.size(); ++s) t.items[at[s] + 7] = t.n_parts + (int32_t)s;
-      const int64_t live = std::min<int64_t>((int64_t)lengths[a.seq] * G - a.j0, RG_ROWS);
-      for (int32_t e = 0; e < live; e += RG_MERGE) {
-        const int32_t m[RG_ITEM] = {a.row0, lengths[a.seq], (int32_t)a.j0, t.n_parts, (int32_t)at.size(), e, 0, 0};
-        t.merges.insert(t.merges.end(), m, m + RG_ITEM);
+      for (size_t s = 0; s < at.size(); ++s) even.items[at[s] + 7] = even.n_parts + (int32_t)s;
+      for (int32_t e = 0; e < a.live; e += RG_MERGE) {
+        const int32_t m[RG_ITEM] = {a.row0, lengths[a.seq], (int32_t)a.j0, even.n_parts, (int32_t)at.size(), e, 0, 0};
+        even.merges.insert(even.merges.end(), m, m + RG_ITEM);
       }
-      t.n_parts += (int32_t)at.size();
+      even.n_parts += (int32_t)at.size();
+      merged += (double)a.live * at.size();
     }
   }
-  if (t.bins.back() != (int32_t)(t.items.size() / RG_ITEM)) t.bins.push_back((int32_t)(t.items.size() / RG_ITEM));
-  return t;
+  if (even.bins.back() != (int32_t)(even.items.size() / RG_ITEM)) close_bin(even);
+  const double even_time = CALL_TIME + MERGE_TIME + std::max(share * 1.3, work * heads) +
+                           even.items.size() / RG_ITEM * heads * ITEM_TIME + merged * Hkv * 1024 / PART_BYTES_PER_US;
+  return whole_time <= even_time ? whole : even;
 }
 
 // A tree's attention: its contexts are on the device, where every workgroup finds its own even
