@@ -159,6 +159,64 @@ def test_packed_nan_stays_in_its_rows(gpu):
         assert torch.equal(out.view_as(clean), clean)
 
 
+@pytest.mark.parametrize("cap,lengths,starts", [(300, [150, 20], [0, 3]), (6000, [40], [5900]), (700, [3, 300], [600, 100])])
+def test_what_a_mask_hides_stays_hidden(gpu, cap, lengths, starts):
+    """Infinities and NaN in K and V of later rows of the same tile, also over split keys: rows that do
+    not attend them are as without them, rows that do are what the definition gives."""
+    hq, hkv = 8, 2
+    plan, q, kc, vc = _packed_case(gpu, hq, hkv, cap, lengths, starts, None, len(lengths))
+    clean, mag = _packed_reference(plan, q, kc, vc)
+    sums = torch.zeros(hq, plan.rows, device=gpu)
+    hit = torch.zeros(plan.rows, hq, dtype=torch.bool, device=gpu)
+    for s, (n, start) in enumerate(zip(lengths, starts)):
+        row = max(1, 2 * n // 3)
+        kc[s, 0, start + row, 5] = NAN
+        vc[s, 0, start + row - 1, 9] = float("inf")
+        vc[s, 1, start + n - 1] = NAN
+        a = plan.first_rows[s]
+        hit[a + row - 1:a + n, :4] = True
+        hit[a + n - 1, 4:] = True
+    out = ops.packed_attention(q, plan, kc, vc, out_sums=sums).view(plan.rows, hq, D)
+    ref, m = clean.view(plan.rows, hq, D), mag.view(plan.rows, hq, D)
+    assert torch.isfinite(out[~hit].float()).all()
+    _check(out[~hit], ref[~hit], m[~hit])
+    for s, (n, start) in enumerate(zip(lengths, starts)):
+        a, row = plan.first_rows[s], max(1, 2 * n // 3)
+        assert (out[a + row - 1, :4, 9] == float("inf")).all() and out[a + row:a + n, :4].isnan().all()
+        assert out[a + n - 1, 4:].isnan().all()
+        rest = [d for d in range(D) if d != 9]
+        _check(out[a + row - 1, :4][:, rest], ref[a + row - 1, :4][:, rest], m[a + row - 1, :4][:, rest])
+    fine = ~hit
+    want = out.double().sum(-1)
+    bound = 128 * 2.0 ** -24 * out.double().abs().sum(-1)
+    assert ((sums.T.double() - want).abs()[fine] <= bound[fine] + 1e-30).all()
+
+
+@pytest.mark.parametrize("cap,ctx,n", [(200, [70, 3], 30), (4000, [3900], 64), (300, [200], 64)])
+def test_a_sibling_s_infinity_stays_its_own(gpu, cap, ctx, n):
+    """An infinity in one node's V and a NaN in another's K reach the nodes below them alone."""
+    hq, hkv = (8, 2) if cap != 300 else (32, 4)
+    q, parents, ctx_t, _, kc, vc, counts = _tree_case(gpu, hq, hkv, cap, ctx, n, None, "random")
+    ref, mag = _tree_reference(q, parents, ctx, counts, kc, vc, cap)
+    inf_node, nan_node = n // 2, n // 3
+    for i, c in enumerate(ctx):
+        vc[i, :, c + inf_node, 3] = float("inf")
+        kc[i, :, c + nan_node, 7] = NAN
+    out = ops.tree_attention(q, parents, ctx_t, hkv, kc, vc).view(len(ctx), n, hq, D)
+    for i in range(len(ctx)):
+        for node, path in enumerate(_paths(parents[i].tolist())):
+            o = out[i, node]
+            if nan_node in path:
+                assert o.isnan().all()
+                continue
+            if inf_node in path:
+                assert (o[:, 3] == float("inf")).all()
+                o = torch.cat((o[:, :3], o[:, 4:]), 1)
+                _check(o, *(torch.cat((x[i, node][:, :3], x[i, node][:, 4:]), 1) for x in (ref, mag)))
+                continue
+            _check(o, ref[i, node], mag[i, node], f"sequence {i} node {node}")
+
+
 @pytest.mark.parametrize("style", [ops.ROPE_HALVES, ops.ROPE_INTERLEAVED])
 def test_packed_prep_has_the_bits_of_the_batch_form(gpu, style):
     hq, hkv, cap = 12, 4, 300

@@ -14,8 +14,8 @@
 // normaliser sums those rounded weights, so that a row of equal values comes back exact.
 #include <math.h>
 
-#include <mutex>
-#include <new>
+#include <atomic>
+#include <exception>
 #include <type_traits>
 
 #include "t2i_common.h"
@@ -177,14 +177,14 @@ struct RaggedAttnParams {
 // What one workgroup does: pairs j0 .. j0 + RG_ROWS - 1 of a sequence's (row, q head of kv
 // head h) pairs over key blocks kb0 .. kb1 - 1.
 struct RaggedItem {
-  int row0, rows, start, crow, kb0, kb1, part, kend;
-  long long j0, pairs;
+  int row0, rows, start, crow, kb0, kb1, part, kend, j0, pairs;
 };
 
 // The even shares of a batch of trees: the key blocks of all sequences in a row, cut into `n`
 // equal runs.  A workgroup takes a run for one tile of pairs of one kv head; the tiles of a
 // sequence stand beside each other on one XCD and read the same K and V at the same time, so
-// memory gives them once (8 trees of 64 nodes over 32k slots, 2 tiles: TILE_FIGURES).  A sequence
+// memory gives them once (8 trees of two tiles over 32k slots: 307 us one tile after the other, 260
+// side by side).  A sequence
 // that is cut leaves a part in each of its runs: slot 2 bin where it is the run's first piece,
 // 2 bin + 1 where it is the last of several.
 struct TreeWalk {
@@ -246,8 +246,8 @@ struct TreeWalk {
     it.rows = seq.nodes;
     it.start = seq.ctx;
     it.crow = b;
-    it.j0 = (long long)tile * p.tile_rows;
-    it.pairs = (long long)seq.nodes * p.G;
+    it.j0 = tile * p.tile_rows;
+    it.pairs = seq.nodes * p.G;
     it.kend = seq.ctx + seq.nodes;
     it.kb0 = kb;
     it.kb1 = seq.ok ? kb + take : kb;
@@ -277,10 +277,10 @@ __device__ __forceinline__ void loads_done_barrier() {
 // not look into asm for hazards: M0 is written a wait state before the load that reads it, and
 // an SGPR that a VALU instruction wrote is five wait states away from a load.
 //
-// 16 bytes a lane from src into LDS at lds + 16 lane.
-__device__ __forceinline__ void lds_load16(const uint16_t* src, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 1\n\tglobal_load_lds_dwordx4 %1, off"
-               :: "s"(lds), "v"(src) : "memory", "m0");
+// 16 bytes a lane from byte `at` of a buffer into LDS at lds + 16 lane.
+__device__ __forceinline__ void lds_load16(i32x4 rsrc, uint32_t at, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"(lds), "v"(at), "s"(rsrc) : "memory", "m0");
 }
 // 4 N keys from a buffer, four an instruction, the lane's chunk of instruction i's at byte at[i]
 // (from soff on, less 1024 i).  An instruction's offset counts for the memory address and for
@@ -335,6 +335,62 @@ __device__ __forceinline__ float pair_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// Which keys row t of a sequence attends; the tree's nodes above its own as a mask.
+template <bool TREE>
+__device__ __forceinline__ bool attends(const RaggedItem& it, int t, unsigned long long seen, int key) {
+  if (!TREE) return key <= it.start + t;
+  return key < it.start || (seen >> (key - it.start) & 1);
+}
+
+// The item's outputs for the pairs j0 + bit of `rows`, a wave a pair after the other, lane e dims
+// 2 e and 2 e + 1: the definition key by key, for rows that hold infinities or NaN.
+template <bool TREE>
+__device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const RaggedItem& it, int h, int j0, uint32_t rows,
+                                                     int lane) {
+  constexpr int D = RG_D;
+  const size_t base = ((size_t)it.crow * p.Hkv + h) * (size_t)p.cap * D + 2 * lane;
+  unsigned long long all = 0;
+  if (TREE) {
+    int depth;
+    all = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane), lane, depth) | 1ull << lane;
+  }
+  for (; rows; rows &= rows - 1) {
+    const int j = j0 + __builtin_ctz(rows);
+    if (j >= it.pairs) break;
+    const int t = j / p.G, head = h * p.G + (j - t * p.G);
+    const size_t qrow = (size_t)it.row0 + t;
+    const unsigned long long seen = TREE ? (unsigned long long)(uint32_t)__shfl((uint32_t)(all >> 32), t, 64) << 32 |
+                                               (uint32_t)__shfl((uint32_t)all, t, 64) : 0;
+    const uint32_t q = *reinterpret_cast<const uint32_t*>(p.q + (qrow * p.Hq + head) * D + 2 * lane);
+    float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+    for (int key = it.kb0 * RG_KEYS; key < min(it.kb1 * RG_KEYS, it.kend); ++key) {
+      if (!attends<TREE>(it, t, seen, key)) continue;       // uniform
+      const uint32_t k = *reinterpret_cast<const uint32_t*>(p.kc + base + (size_t)key * D);
+      const uint32_t v = *reinterpret_cast<const uint32_t*>(p.vc + base + (size_t)key * D);
+      const float s = wave_sum(bf16_lo(q) * bf16_lo(k) + bf16_hi(q) * bf16_hi(k)) * p.scale_log2;
+      const float mn = fmaxf(m, s), f = state_weight(m, mn);
+      const float w = round_bf16(exp2_fast(s - (mn > -INFINITY ? mn : 0.0f)));
+      l = l * f + w;
+      o0 = o0 * f + w * bf16_lo(v);
+      o1 = o1 * f + w * bf16_hi(v);
+      m = mn;
+    }
+    if (it.part >= 0) {
+      const size_t st = ((size_t)it.part * p.Hkv + h) * p.part_rows + (j - it.j0);
+      if (lane == 0) p.part_ml[st] = float2{l != l ? INFINITY : m, l};
+      *reinterpret_cast<float2*>(p.part_o + st * D + 2 * lane) = float2{o0, o1};
+    } else {
+      const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+      const uint32_t w = pack_bf16x2(o0 * inv, o1 * inv);
+      *reinterpret_cast<uint32_t*>(p.out + (qrow * p.Hq + head) * D + 2 * lane) = w;
+      if (p.out_sums) {
+        const float hs = wave_sum(bf16_lo(w) + bf16_hi(w));
+        if (lane == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
+      }
+    }
+  }
+}
+
 // One workgroup (4 waves of 32 pairs, two workgroups a CU) an item and kv head.  All products
 // run transposed on the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32, h2 = lane / 32) holds
 // one pair's scores and outputs:
@@ -386,21 +442,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
     ++at;
     it.row0 = w[0]; it.rows = w[1]; it.start = w[2]; it.crow = w[3];
     it.j0 = w[4]; it.kb0 = w[5]; it.kb1 = w[6]; it.part = w[7];
-    it.pairs = (long long)it.rows * p.G;
+    it.pairs = (int)((uint32_t)it.rows * (uint32_t)p.G);   // checked below
     // a table that does not fit the tensors is not followed
     if (it.row0 < 0 || it.rows < 1 || it.row0 + (long long)it.rows > p.rows || it.start < 0 ||
-        it.start > p.cap - it.rows || it.crow < 0 || it.crow >= p.n_cache || it.j0 < 0 || it.j0 >= it.pairs ||
-        it.pairs > 0x7FFFFFFF - ROWS || it.part >= p.n_parts)
+        it.start > p.cap - it.rows || it.crow < 0 || it.crow >= p.n_cache || it.j0 < 0 ||
+        (long long)it.rows * p.G > 0x7FFFFFFF - ROWS || it.j0 >= it.pairs || it.part >= p.n_parts)
       continue;
-    it.kend = it.start + (int)((min(it.j0 + ROWS, it.pairs) - 1) / p.G) + 1;
+    it.kend = it.start + (min(it.j0 + ROWS, it.pairs) - 1) / p.G + 1;
     it.kb0 = max(it.kb0, 0);
     it.kb1 = min(it.kb1, (it.kend + RG_KEYS - 1) / RG_KEYS);
   }
 
   // ---- K / V staging: a wave's instruction moves 4 keys (1 KB); 4 each of K and V a block ----
   const size_t cache_base = ((size_t)it.crow * p.Hkv + h) * (size_t)p.cap * D;
-  const uint16_t* const kbase = p.kc + cache_base;
-  const uint16_t* const vbase = p.vc + cache_base;
   const int srow = lane >> 4;                              // key within the instruction's four
   const int place = lane & 15;                             // where the lane's 16 bytes go in the key's row
   const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rg_lds_address(s_kv) + wave * WKEYS * D * 2);
@@ -411,7 +465,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
     kat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ ((wave * WKEYS + 4 * i + srow) & 15));
     vat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ (4 * srow));
   }
-  const i32x4 krsrc = keys_rsrc(kbase), vrsrc = keys_rsrc(vbase);
+  const i32x4 krsrc = keys_rsrc(p.kc + cache_base), vrsrc = keys_rsrc(p.vc + cache_base);
   // K and V block kb into its buffer
   auto stage = [&](int kb) __attribute__((always_inline)) {
     const uint32_t lds = lds0 + ((kb - it.kb0) & (RING - 1)) * (4 * RG_KEYS * D);
@@ -428,9 +482,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int at = wave * WKEYS + 4 * i + srow;
-        const size_t key = min(kb * RG_KEYS + at, it.kend - 1);
-        lds_load16(kbase + key * D + 8 * (place ^ (at & 15)), lds + i * 4 * D * 2);
-        lds_load16(vbase + key * D + 8 * (place ^ (4 * srow)), lds + 2 * RG_KEYS * D + i * 4 * D * 2);
+        const uint32_t key = (uint32_t)min(kb * RG_KEYS + at, it.kend - 1) * (D * 2);
+        lds_load16(krsrc, key + 16 * (place ^ (at & 15)), lds + i * 4 * D * 2);
+        lds_load16(vrsrc, key + 16 * (place ^ (4 * srow)), lds + 2 * RG_KEYS * D + i * 4 * D * 2);
       }
     }
   };
@@ -439,9 +493,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
     if (it.kb0 + s < it.kb1) stage(it.kb0 + s);
 
   // ---- this lane's pair, and its q row as the B operand ----
-  const long long j = it.j0 + wave * 32 + c;
+  const int j = it.j0 + wave * 32 + c;
   const bool wave_on = it.j0 + wave * 32 < it.pairs;       // some pair of the wave exists
-  const int jj = (int)min(j, it.pairs - 1);
+  const int jj = min(j, it.pairs - 1);
   const int t = jj / p.G;
   const int head = h * p.G + (jj - t * p.G);
   const size_t qrow = (size_t)it.row0 + t;
@@ -452,8 +506,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
     for (int ks = 0; ks < 8; ++ks) qb[ks] = *reinterpret_cast<const u32x4*>(src + 16 * ks);
   }
   // positions of the wave's rows: first and last (wave-uniform), this lane's
-  const int t_first = (int)((it.j0 + wave * 32) / p.G);
-  const int t_last = (int)((min(it.j0 + wave * 32 + 32, it.pairs) - 1) / p.G);
+  const int t_first = (it.j0 + wave * 32) / p.G;
+  const int t_last = (min(it.j0 + wave * 32 + 32, it.pairs) - 1) / p.G;
   const int qpos = it.start + t;
   const int mask_from = TREE ? it.start : it.start + t_first + 1;   // keys below it are seen by every row
   const int wave_end = TREE ? it.kend : it.start + t_last + 1;      // keys from it on by none
@@ -573,7 +627,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
   // ---- outputs: register i of o[dt] is dim 32 dt + 8 (i / 4) + 4 h2 + i % 4 of the lane's pair ----
   if (!wave_on) continue;
   l = pair_sum(l);
-  const bool live = j < it.pairs;
+  // A weight of 0 times an infinity or a NaN in V is a NaN: a row whose sums are not finite is
+  // formed again from the keys that it attends alone, so that what a mask hides stays hidden.
+  float finite = 0.0f * l;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) finite = fmaf(0.0f, o[dt][i], finite);
+  const unsigned long long odd = __ballot(finite != finite);
+  const uint32_t again = (uint32_t)(odd | odd >> 32);       // bit c: the pair of lanes c and c + 32
+  if (again) exact_rows<TREE>(p, it, h, it.j0 + wave * 32, again, lane);
+  const bool live = j < it.pairs && !(again >> c & 1);
   if (it.part >= 0) {
     const size_t st = ((size_t)it.part * p.Hkv + h) * p.part_rows + wave * 32 + c;
     m = l != l ? INFINITY : m;                             // a row that saw a NaN stays one in the merge
@@ -804,18 +868,15 @@ int launch_attention(const t2i::RaggedAttnParams& p, long long groups, hipStream
   if (p.tile_rows == 128) {
     hipLaunchKernelGGL((t2i::ragged_attention_kernel<TREE, 4, 2>), dim3(groups), dim3(256), lds_bytes(2), s, p);
   } else {
-    // more than 64 KB of LDS: asked for once a device
-    static std::mutex mu;
-    static std::vector<bool> done;
+    // more than 64 KB of LDS: asked for once a device (twice does no harm)
+    static std::atomic<bool> done[64];
     int dev = 0;
     if (int rc = t2i_host::hip_status(hipGetDevice(&dev), "device query")) return rc;
-    std::lock_guard<std::mutex> lock(mu);
-    if ((int)done.size() <= dev) done.resize(dev + 1, false);
-    if (!done[dev]) {
+    if (dev < 0 || dev >= 64 || !done[dev]) {
       if (int rc = t2i_host::hip_status(hipFuncSetAttribute(reinterpret_cast<const void*>(&t2i::ragged_attention_kernel<TREE, 8, 4>),
                                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes(4)), "LDS attribute"))
         return rc;
-      done[dev] = true;
+      if (dev >= 0 && dev < 64) done[dev] = true;
     }
     hipLaunchKernelGGL((t2i::ragged_attention_kernel<TREE, 8, 4>), dim3(groups), dim3(512), lds_bytes(4), s, p);
   }
@@ -891,8 +952,8 @@ extern "C" int t2i_packed_plan(const int32_t* lengths, const int32_t* starts, co
     if (table_words < sizes[5]) return fail(T2I_ERR_WORKSPACE, "the table holds %lld words, %lld needed", (long long)table_words, (long long)sizes[5]);
     for (const auto* v : {&t.row_pos, &t.row_cache, &t.items, &t.merges, &t.bins}) table = std::copy(v->begin(), v->end(), table);
     return T2I_OK;
-  } catch (const std::bad_alloc&) {
-    return fail(T2I_ERR_WORKSPACE, "host memory for the plan ran out");
+  } catch (const std::exception& e) {
+    return fail(T2I_ERR_WORKSPACE, "host memory for the plan: %s", e.what());
   }
 }
 

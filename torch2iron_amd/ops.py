@@ -1021,13 +1021,14 @@ def _launch(device, name: str, *args):
 
 
 def _scratch(workspace: Workspace | None, key: str, nbytes: int, device):
-    """Scratch of at least ``nbytes`` (a power of two: a buffer of one size is never replaced, so
-    a captured call keeps its own).  Without a workspace each stream has its own buffers."""
+    """Scratch of at least ``nbytes``, of no value before a call and none after it: without a
+    workspace torch's own, returned behind the call (a captured one keeps it in its graph); with
+    one a buffer of a power of two, which is never replaced, so that captured calls keep theirs."""
     if nbytes == 0:
         return None
-    size = 1 << (nbytes - 1).bit_length()
     if workspace is None:
-        return DEFAULT_WORKSPACE.get((key, size, _lib.stream_handle(device)), size, device)
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    size = 1 << (nbytes - 1).bit_length()
     return workspace.get((key, size), size, device)
 
 
@@ -1039,6 +1040,7 @@ class PackedPlan:
     ``ctx_cap``, two on one cache row); the table that the kernels take is made once and
     serves every layer of the pass.
 
+    The table stays with the plan: keep the plan as long as a captured call may be replayed.
     ``rows``: packed rows; ``first_rows[s]`` / ``last_rows[s]``: a sequence's first and last
     packed row (last = first - 1 for a sequence without rows)."""
 
@@ -1072,6 +1074,7 @@ class PackedPlan:
         table = torch.empty(words, dtype=torch.int32)
         _lib.check(lib.t2i_packed_plan(*call, table.data_ptr(), words, sizes.data_ptr()), "t2i_packed_plan")
         self.table = table.to(self.device)
+        self._stream = _lib.stream_handle(self.device) if self.device.type == "cuda" else None
         base, n = self.table.data_ptr(), 4 * self.rows
         self._row_pos, self._row_cache, self._items = base, base + n, base + 2 * n
         self._merges = self._items + 32 * self.n_items
@@ -1082,6 +1085,11 @@ class PackedPlan:
             self.first_rows.append(at)
             at += x
             self.last_rows.append(at - 1)
+
+    def _use(self):
+        """The table's memory waits for the current stream before it is given to another tensor."""
+        if _lib.stream_handle(self.device) != self._stream:
+            self.table.record_stream(torch.cuda.current_stream(self.device))
 
     def _check(self, k_cache, v_cache, d: int | None = None):
         _check_dev("k_cache", k_cache, BF16)
@@ -1119,6 +1127,7 @@ def packed_qk_rope_kv(qkv: torch.Tensor, plan: PackedPlan, q_norm: torch.Tensor,
                  q_out=q_out)
     if plan.rows == 0:
         return q_out
+    plan._use()
     _launch(plan.device, "t2i_packed_qk_rope_kv",
             qkv.data_ptr(), plan.rows, plan._row_pos, plan._row_cache, plan.n_cache_rows, plan.n_heads, plan.n_kv_heads,
             d, q_norm.data_ptr(), k_norm.data_ptr(), float(eps), rope.data_ptr(), int(rope_style), q_out.data_ptr(),
@@ -1149,6 +1158,7 @@ def packed_attention(q: torch.Tensor, plan: PackedPlan, k_cache: torch.Tensor, v
     if plan.rows == 0:
         return out
     ws = _scratch(workspace, "packed_attn", plan._nbytes, q.device)
+    plan._use()
     _launch(plan.device, "t2i_packed_attention",
             q.data_ptr(), plan.rows, plan._items, plan.n_items, plan._merges, plan.n_merges, plan.n_parts, plan._bins,
             plan.n_bins, plan.n_heads, plan.n_kv_heads, d, k_cache.data_ptr(), v_cache.data_ptr(), plan.n_cache_rows,
