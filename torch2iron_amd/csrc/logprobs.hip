@@ -310,13 +310,22 @@ __global__ __launch_bounds__(64) void token_logprobs_merge_kernel(const LpParams
   for (int s = 32; s; s >>= 1) st = lp_join(st, LpState{__shfl_xor(st.m, s, 64), __shfl_xor(st.z, s, 64), __shfl_xor(st.t, s, 64)});
   LpTop top;
   const u64* keys = p.part_top + (size_t)row * p.splits * p.k;
-  // entry i of every part's list before entry i + 1 of any: the best come first
-  for (int i = 0; i < p.k; ++i)
+  // entry i of every part's list before entry i + 1 of any: the best come first, and where no
+  // list's entry i belongs here none behind it does
+  for (int i = 0; i < p.k; ++i) {
+    bool some = false;
     for (int s0 = 0; s0 < p.splits; s0 += 64) {
       const u64 key = s0 + lane < p.splits ? keys[(size_t)(s0 + lane) * p.k + i] : 0;
-      if (i == 0 && s0 == 0) top.fill(key >> 32 ? key : (u64)(64 - lane), p.k);
-      else top.take(key, p.k, lane);
+      if (i == 0 && s0 == 0) {
+        top.fill(key >> 32 ? key : (u64)(64 - lane), p.k);
+        some = true;
+      } else if (__ballot(key > top.last)) {
+        top.take(key, p.k, lane);
+        some = true;
+      }
     }
+    if (!some) break;
+  }
   const char* const base = reinterpret_cast<const char*>(p.logits) + (size_t)row * p.stride * (16 / Ty::PER);
   const int t = p.tokens ? p.tokens[row] : -1;
   const bool in = t >= 0 && t < p.V;

@@ -195,9 +195,10 @@ struct TreeWalk {
   __device__ __forceinline__ int blocks_of(const TreeSeq& t) const {
     return t.nodes == 0 ? 0 : t.ok ? (t.ctx + t.nodes + RG_KEYS - 1) / RG_KEYS : 1;
   }
-  __device__ __forceinline__ int run_start(int i) const { return (int)((long long)total * i / n); }
+  // (32-bit products: the host keeps total below 2^23, n below 2^9)
+  __device__ __forceinline__ int run_start(int i) const { return (int)((uint32_t)total * (uint32_t)i / (uint32_t)n); }
   // the run that holds block x
-  __device__ __forceinline__ int run_of(int x) const { return (int)(((long long)(x + 1) * n - 1) / total); }
+  __device__ __forceinline__ int run_of(int x) const { return (int)(((uint32_t)(x + 1) * (uint32_t)n - 1) / (uint32_t)total); }
 
   // Sums of 64 sequences' blocks at a time; false where there is no such run.
   __device__ __forceinline__ bool begin(const RaggedAttnParams& p, int bin, int lane, int& at, int& end) {
@@ -1053,7 +1054,7 @@ extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, con
   p.n_bins = t.bins;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
   if (too_many((long long)B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS)) || too_many((long long)B * N) ||
-      too_many((long long)B * ((ctx_cap + t2i::RG_KEYS - 1) / t2i::RG_KEYS)))
+      (long long)B * ((ctx_cap + t2i::RG_KEYS - 1) / t2i::RG_KEYS) >= 1 << 23)
     return fail(T2I_ERR_SHAPE, "B=%d N=%d Hkv=%d over %d slots are too many", B, N, Hkv, ctx_cap);
   if (!workspace || workspace_bytes < t.bytes) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, t.bytes);
   if (!aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
