@@ -1,10 +1,12 @@
 // Log probabilities of given tokens over rows of logits for gfx950, with each row's entropy
 // and its top alternatives, in one pass over the logits (t2i_token_logprobs).
 //
-// With m the row's largest logit and y = (x - m) log2 e:
+// With a reference m near the row's largest logit and y = (x - m) log2 e:
 //   Z = sum 2^y,  T = sum 2^y y,  log p(t) = x_t - m - ln Z,  entropy = ln Z - (T / Z) ln 2.
 // m, Z and T are kept as the pass goes: when y's reference falls by d (a larger m), Z and T follow
-// it as Z 2^d and (T + d Z) 2^d.  fp32 throughout; the difference is taken before it is scaled, so
+// it as Z 2^d and (T + d Z) 2^d.  A lane's m moves only when a logit passes it by LP_SLACK: weights
+// up to e^LP_SLACK have the same relative precision, and after its first values a lane hardly
+// ever stops for it.  fp32 throughout; the difference is taken before it is scaled, so
 // that logits of any size (the type's lowest value as a mask among them) keep their places.
 #include <math.h>
 
@@ -18,6 +20,7 @@ constexpr int LP_WAVES = 4;
 constexpr int LP_THREADS = 64 * LP_WAVES;
 constexpr int LP_TOP = 32;                   // alternatives of a row: one lane of a wave each
 constexpr int LP_UNROLL = 4;                 // 16-byte loads of a lane in flight
+constexpr float LP_SLACK = 6.0f;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -94,6 +97,12 @@ struct LpTop {
   }
 };
 
+// Word i (modulo 4) of a 16-byte piece.
+__device__ __forceinline__ uint32_t word_of(u32x4 v, int i) {
+  const uint32_t a = i & 1 ? v.y : v.x, b = i & 1 ? v.w : v.z;
+  return i & 2 ? b : a;
+}
+
 template <typename T>
 struct LpType;
 template <>
@@ -103,6 +112,8 @@ struct LpType<float> {
     f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
   }
   static __device__ __forceinline__ float one(const void* p, size_t i) { return reinterpret_cast<const float*>(p)[i]; }
+  // value i of a piece
+  static __device__ __forceinline__ float pick(u32x4 v, int i) { return __uint_as_float(word_of(v, i)); }
 };
 struct LpBf16 {};
 template <>
@@ -115,6 +126,10 @@ struct LpType<LpBf16> {
     for (int i = 0; i < 8; ++i) f[i] = g[i];
   }
   static __device__ __forceinline__ float one(const void* p, size_t i) { return bf16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]); }
+  static __device__ __forceinline__ float pick(u32x4 v, int i) {
+    const uint32_t w = word_of(v, i >> 1);
+    return i & 1 ? bf16_hi(w) : bf16_lo(w);
+  }
 };
 struct LpF16 {};
 template <>
@@ -129,6 +144,10 @@ struct LpType<LpF16> {
     }
   }
   static __device__ __forceinline__ float one(const void* p, size_t i) { return f16_to_f32(reinterpret_cast<const uint16_t*>(p)[i]); }
+  static __device__ __forceinline__ float pick(u32x4 v, int i) {
+    const uint32_t w = word_of(v, i >> 1);
+    return f16_to_f32(i & 1 ? w >> 16 : w & 0xFFFFu);
+  }
 };
 
 struct LpParams {
@@ -185,7 +204,7 @@ __global__ __launch_bounds__(LP_THREADS) void token_logprobs_kernel(const LpPara
   auto add = [&](const float* v, int n) __attribute__((always_inline)) {
     float mx = v[0];
     for (int i = 1; i < n; ++i) mx = __builtin_elementwise_maximum(mx, v[i]);
-    if (!(mx <= st.m)) {
+    if (!(mx <= st.m + LP_SLACK)) {
       const float d = st.m > -INFINITY ? (st.m - mx) * LOG2E : mx != mx ? mx : -1e30f;   // z and t are 0 at first
       const float f = exp2_fast(d);
       st.t = (st.t + fmaxf(d, -1e30f) * st.z) * f;
@@ -241,25 +260,36 @@ __global__ __launch_bounds__(LP_THREADS) void token_logprobs_kernel(const LpPara
     for (int w = 0; w < LP_WAVES; ++w)
       others = fmaxf(others, __hip_atomic_load(&s_floor[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP));
     const float floor0 = top.floor;
+    const bool full = q + 64 * LP_UNROLL <= p1;
 #pragma unroll
     for (int u = 0; u < LP_UNROLL; ++u) {
       const int piece = q + 64 * u + lane;
       float v[PER];
       Ty::get(raw[u], v);
-      if (piece >= p1) {
+      if (!full) {                             // uniform
 #pragma unroll
-        for (int i = 0; i < PER; ++i) v[i] = -INFINITY;
+        for (int i = 0; i < PER; ++i) v[i] = piece < p1 ? v[i] : -INFINITY;
       }
       const float mx = add(v, PER);
       // a NaN passes; a value equal to the k-th best counts only beside values that the list
       // already holds from this piece, or at the start from later ones: others stand behind it
-      if (p.k && __ballot(piece < p1 && !(mx < top.floor || (mx == top.floor && !start) || mx < others))) {
+      if (p.k) {
+        u64 hit = __ballot(piece < p1 && !(mx < top.floor || (mx == top.floor && !start) || mx < others));
+        if (hit && q == first) {               // many lanes, at the start: value by value over all of them
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (__ballot(piece < p1 && !(v[i] < top.floor || v[i] < others))) {
-            const u64 key = lp_key(v[i], head + piece * PER + i);
-            top.take(piece < p1 && key != start ? key : 0, p.k, lane);
-          }
+          for (int i = 0; i < PER; ++i)
+            if (__ballot(piece < p1 && !(v[i] < top.floor))) {
+              const u64 key = lp_key(v[i], head + piece * PER + i);
+              top.take(piece < p1 && key != start ? key : 0, p.k, lane);   // start is in the list
+            }
+          hit = 0;
+        }
+        for (; hit; hit &= hit - 1) {          // lane by lane: the values of its piece, one a lane
+          const int from = __builtin_ctzll(hit);
+          const u32x4 w = u32x4{(uint32_t)__builtin_amdgcn_readlane(raw[u].x, from), (uint32_t)__builtin_amdgcn_readlane(raw[u].y, from),
+                                (uint32_t)__builtin_amdgcn_readlane(raw[u].z, from), (uint32_t)__builtin_amdgcn_readlane(raw[u].w, from)};
+          top.take(lane < PER ? lp_key(Ty::pick(w, lane), head + (q + 64 * u + from) * PER + lane) : 0, p.k, lane);
+        }
       }
     }
     if (p.k && lane == 0 && top.floor != floor0 && top.floor == top.floor)
