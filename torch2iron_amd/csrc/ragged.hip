@@ -112,10 +112,10 @@ __global__ __launch_bounds__(256) void ragged_prep_kernel(const RaggedPrepParams
     const int node = row - crow * p.N;
     const TreeSeq t = tree_seq(p.ctx, p.counts, crow, p.N, p.cap);
     if (!t.ok || node >= t.nodes) return;
-    int depth;
-    tree_above(tree_parent(p.parents + (size_t)crow * p.N, p.N, lane), lane, depth);
     dst_slot = t.ctx + node;
-    pos = t.ctx + __builtin_amdgcn_readlane(depth, node);
+    pos = t.ctx;
+    const int parent = tree_parent(p.parents + (size_t)crow * p.N, p.N, lane);
+    for (int up = node; (up = __builtin_amdgcn_readlane(parent, up)) >= 0;) ++pos;   // a parent stands before its node
   } else {
     pos = dst_slot = p.row_pos[row];
     crow = p.row_cache[row];
