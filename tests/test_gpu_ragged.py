@@ -468,6 +468,42 @@ def test_tree_calls_replayed_from_a_graph(gpu):
         assert all(torch.equal(x, y) for x, y in zip(cache, twin))
 
 
+def test_wrappers_refuse(gpu):
+    """Shapes, types and plans that do not fit raise before anything is launched."""
+    plan, q, kc, vc = _packed_case(gpu, 4, 2, 32, [3, 5], [0, 1], None, 2)
+    tq, parents, ctx, _, tk, tv, _ = _tree_case(gpu, 4, 2, 32, [5, 6], 4, None, "random")
+    qkv, one = torch.zeros(8, 8 * D, dtype=BF16, device=gpu), torch.ones(D, dtype=BF16, device=gpu)
+    rope = gm.rope_table(D, 32, 1e6, gpu)
+    i8 = torch.zeros(2, 4, dtype=torch.int32, device=gpu)
+    x, t = torch.zeros(2, 9, device=gpu), torch.zeros(2, dtype=torch.int32, device=gpu)
+    for call in (
+            lambda: ops.packed_attention(q[:7].contiguous(), plan, kc, vc), lambda: ops.packed_attention(q.float(), plan, kc, vc),
+            lambda: ops.packed_attention(q[:, :2].contiguous(), plan, kc, vc),
+            lambda: ops.packed_attention(q, plan, kc[:, :, :31].contiguous(), vc[:, :, :31].contiguous()),
+            lambda: ops.packed_attention(q, plan, kc[:1], vc[:1]), lambda: ops.packed_attention(q, plan, kc, vc, out=q[:2]),
+            lambda: ops.packed_attention(q, plan, kc, vc, out_sums=torch.zeros(3, device=gpu)),
+            lambda: ops.packed_attention(q.transpose(1, 2), plan, kc, vc),
+            lambda: ops.packed_qk_rope_kv(qkv[:7], plan, one, one, 1e-6, rope, kc, vc),
+            lambda: ops.packed_qk_rope_kv(qkv, plan, one, one, 1e-6, rope[:31], kc, vc),
+            lambda: ops.packed_qk_rope_kv(qkv, plan, one, one[:64], 1e-6, rope, kc, vc),
+            lambda: ops.packed_qk_rope_kv(qkv, plan, one, one, 0.0, rope, kc, vc),
+            lambda: ops.tree_attention(tq, parents.long(), ctx, 2, tk, tv), lambda: ops.tree_attention(tq, parents, ctx[:1], 2, tk, tv),
+            lambda: ops.tree_attention(tq, parents[:, :3].contiguous(), ctx, 2, tk, tv), lambda: ops.tree_attention(tq, parents, ctx, 3, tk, tv),
+            lambda: ops.tree_attention(tq, parents, ctx, 2, tk[:, :, :3].contiguous(), tv[:, :, :3].contiguous()),
+            lambda: ops.tree_attention(tq, parents, ctx, 2, tk, tv, node_counts=ctx[:1]),
+            lambda: ops.tree_attention(tq, parents.view(-1), ctx, 2, tk, tv),
+            lambda: ops.tree_qk_rope_kv(qkv[:7], parents, ctx, 4, 2, one, one, 1e-6, rope, tk, tv),
+            lambda: ops.tree_qk_rope_kv(qkv, parents, ctx, 4, 2, one, one, 1e-6, rope[:9], tk, tv),
+            lambda: ops.tree_commit(i8, parents, i8[:1], ctx, tk, tv), lambda: ops.tree_commit(i8, parents, i8, ctx, tk, tv[:, :1]),
+            lambda: ops.tree_commit(i8, parents, i8, ctx, tk[:1], tv[:1]), lambda: ops.tree_commit(i8.float(), parents, i8, ctx, tk, tv),
+            lambda: ops.token_logprobs(x.double(), t), lambda: ops.token_logprobs(x, t[:1]), lambda: ops.token_logprobs(x, t.long()),
+            lambda: ops.token_logprobs(x, t, top_k=10), lambda: ops.token_logprobs(x, t, top_k=-1),
+            lambda: ops.token_logprobs(x[0], t), lambda: ops.token_logprobs(x.T, torch.zeros(9, dtype=torch.int32, device=gpu)),
+            lambda: ops.token_logprobs(x[:1].expand(2, 9), t), lambda: ops.token_logprobs(torch.zeros(2, 99, device=gpu), t, top_k=33)):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_calls_on_another_stream(gpu):
     """Packed and tree attention on two streams at once, without a workspace of the caller's."""
     plan, q, kc, vc = _packed_case(gpu, 4, 1, 6000, [3], [5900], None, 1)

@@ -180,7 +180,12 @@ __device__ __forceinline__ void lp_finish(const LpParams& p, int row, LpState st
 // lane in flight, and keep their own state and best list; both meet in LDS.  A wave's list
 // starts as its lanes' largest values of the first pieces, in order; after that it looks at a
 // piece's order only where a lane's largest value passes the k-th best of its own list and of
-// the other waves' (which only grow, so an older one of them is as good).
+// the other waves' (which only grow, so an older one of them is as good).  2043 rows of 151936
+// fp32 logits, 20 best: 225-235 us, 5.3-5.5 TB/s (a large copy reaches 5.15): memory.  416 bf16 rows:
+// 34.5 us without best lists, 52 with 8: VALU instructions, 88 % of a SIMD's cycles (in the sums 7.5
+// an element, an exponential among them; the lists' first orders and insertions the rest).
+// Measured and dropped: twice the pieces on their way (1-14 % slower), lists of the waves joined by
+// rank (2 %), fewer and longer parts (3-10 %).
 template <typename T>
 __global__ __launch_bounds__(LP_THREADS) void token_logprobs_kernel(const LpParams p) {
   using Ty = LpType<T>;

@@ -96,9 +96,9 @@ struct RaggedPrepParams {
 };
 
 // One workgroup (4 waves) per row, a head vector to a 16-lane row of a wave, as
-// prefill_prep_kernel (same bits): PREP_NB batches of 16 vectors in flight.  A row whose
-// position, slot or cache row lies outside the cache writes nothing.  Bound by HBM:
-// every byte is read and written once.
+// prefill_prep_kernel (same bits): RG_PREP_NB batches of 16 vectors in flight.  A row whose
+// position, slot or cache row lies outside the cache writes nothing.  Bound by HBM: every byte
+// is read and written once (4997 rows, 16 / 8 heads: 20.8 us, 3.9 TB/s; 416 nodes: 4.9 us).
 constexpr int RG_PREP_NB = 2;
 
 template <bool TREE>
@@ -174,8 +174,8 @@ struct RaggedAttnParams {
   float scale_log2;         // D^-1/2 * log2(e)
 };
 
-// What one workgroup does: pairs j0 .. j0 + RG_ROWS - 1 of a sequence's (row, q head of kv
-// head h) pairs over key blocks kb0 .. kb1 - 1.
+// A piece of work: the tile of a sequence's (row, q head of a kv head) pairs from j0 on, over key
+// blocks kb0 .. kb1 - 1; keys from kend on are seen by none of its rows.
 struct RaggedItem {
   int row0, rows, start, crow, kb0, kb1, part, kend, j0, pairs;
 };
@@ -184,9 +184,8 @@ struct RaggedItem {
 // equal runs.  A workgroup takes a run for one tile of pairs of one kv head; the tiles of a
 // sequence stand beside each other on one XCD and read the same K and V at the same time, so
 // memory gives them once (8 trees of two tiles over 32k slots: 307 us one tile after the other, 260
-// side by side).  A sequence
-// that is cut leaves a part in each of its runs: slot 2 bin where it is the run's first piece,
-// 2 bin + 1 where it is the last of several.
+// side by side).  A sequence that is cut leaves a part in each of its runs: slot 2 bin where it
+// is the run's first piece, 2 bin + 1 where it is the last of several.
 struct TreeWalk {
   int n, total, b, blocks, kb;         // n: runs; the next piece starts at block kb of sequence b
   TreeSeq seq;
@@ -286,37 +285,30 @@ __device__ __forceinline__ void lds_load16(i32x4 rsrc, uint32_t at, uint32_t lds
 // 4 N keys from a buffer, four an instruction, the lane's chunk of instruction i's at byte at[i]
 // (from soff on, less 1024 i).  An instruction's offset counts for the memory address and for
 // the LDS address.
-template <int N, bool ONCE>
+// ONCE: past the caches' own order (nt), for keys that no other workgroup reads.
+#define T2I_KEYS(mod)                                                                                             \
+  if constexpr (N == 4)                                                                                           \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"                                                                \
+                 "buffer_load_dwordx4 %1, %5, %6 offen" mod " lds\n\t"                                            \
+                 "buffer_load_dwordx4 %2, %5, %6 offen offset:1024" mod " lds\n\t"                                \
+                 "buffer_load_dwordx4 %3, %5, %6 offen offset:2048" mod " lds\n\t"                                \
+                 "buffer_load_dwordx4 %4, %5, %6 offen offset:3072" mod " lds"                                    \
+                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(rsrc), "s"(soff) : "memory", "m0"); \
+  else                                                                                                            \
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"                                                                \
+                 "buffer_load_dwordx4 %1, %3, %4 offen" mod " lds\n\t"                                            \
+                 "buffer_load_dwordx4 %2, %3, %4 offen offset:1024" mod " lds"                                    \
+                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "s"(rsrc), "s"(soff) : "memory", "m0")
+template <bool ONCE, int N>
 __device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[N], uint32_t soff, uint32_t lds) {
-  static_assert(N == 2 || N == 4, "keys of a wave");
+  static_assert(N == 2 || N == 4, "instructions of a wave");
   if constexpr (ONCE) {
-  if constexpr (N == 4)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
-                 "buffer_load_dwordx4 %1, %5, %6 offen nt lds\n\t"
-                 "buffer_load_dwordx4 %2, %5, %6 offen offset:1024 nt lds\n\t"
-                 "buffer_load_dwordx4 %3, %5, %6 offen offset:2048 nt lds\n\t"
-                 "buffer_load_dwordx4 %4, %5, %6 offen offset:3072 nt lds"
-                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(rsrc), "s"(soff) : "memory", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
-                 "buffer_load_dwordx4 %1, %3, %4 offen nt lds\n\t"
-                 "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 nt lds"
-                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "s"(rsrc), "s"(soff) : "memory", "m0");
+    T2I_KEYS(" nt");
   } else {
-  if constexpr (N == 4)
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
-                 "buffer_load_dwordx4 %1, %5, %6 offen lds\n\t"
-                 "buffer_load_dwordx4 %2, %5, %6 offen offset:1024 lds\n\t"
-                 "buffer_load_dwordx4 %3, %5, %6 offen offset:2048 lds\n\t"
-                 "buffer_load_dwordx4 %4, %5, %6 offen offset:3072 lds"
-                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(rsrc), "s"(soff) : "memory", "m0");
-  else
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
-                 "buffer_load_dwordx4 %1, %3, %4 offen lds\n\t"
-                 "buffer_load_dwordx4 %2, %3, %4 offen offset:1024 lds"
-                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "s"(rsrc), "s"(soff) : "memory", "m0");
+    T2I_KEYS("");
   }
 }
+#undef T2I_KEYS
 // A buffer over everything from p on (every offset used is inside the cache: checked or clamped).
 __device__ __forceinline__ i32x4 keys_rsrc(const void* p) {
   const uint64_t a = (uint64_t)(uintptr_t)p;
@@ -347,7 +339,7 @@ __device__ __forceinline__ bool attends(const RaggedItem& it, int t, unsigned lo
 // 2 e and 2 e + 1: the definition key by key, for rows that hold infinities or NaN.
 template <bool TREE>
 __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const RaggedItem& it, int h, int j0, uint32_t rows,
-                                                     int lane) {
+                                           int lane) {
   constexpr int D = RG_D;
   const size_t base = ((size_t)it.crow * p.Hkv + h) * (size_t)p.cap * D + 2 * lane;
   unsigned long long all = 0;
@@ -392,23 +384,37 @@ __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const Ragg
   }
 }
 
-// One workgroup (4 waves of 32 pairs, two workgroups a CU) an item and kv head.  All products
-// run transposed on the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32, h2 = lane / 32) holds
-// one pair's scores and outputs:
+// One workgroup (WAVES waves of 32 pairs) takes a bin's items for one kv head, one after the
+// other.  All products run transposed on the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32,
+// h2 = lane / 32) holds one pair's scores and outputs:
 //   S^T = K Q^T: A = K from LDS (lane: key 32 n + c, dims 16 ks + 8 h2 ..), B = the wave's q
 //     rows (registers); register i holds the score of key 32 n + 8 (i / 4) + 4 h2 + i % 4;
 //   the online softmax per lane: the row's maximum from its two lanes by one lane swap, the
 //     weights' sum left per lane until the end.  The reference m moves only when a maximum
 //     passes it by 8 (weights up to 2^8, the same relative precision): after the first blocks
 //     outputs are hardly ever rescaled;
-//   O^T += V^T P^T: B = P^T straight from those registers (16 keys a step, in the order they
-//     stand in), A = V^T from LDS in that order by transposing reads (ds_read_b64_tr_b16: four
-//     keys of one dim a lane out of V's own row order).
-// K and V blocks go straight from memory into LDS, two buffers, one barrier a block; a row's
+//   O^T += V^T P^T: B = P^T straight from those registers, rounded to bf16 (16 keys a step, in
+//     the order they stand in), A = V^T from LDS in that order by transposing reads
+//     (ds_read_b64_tr_b16: four keys of one dim a lane out of V's own row order).
+// K and V blocks go straight from memory into LDS, RING buffers, one barrier a block; a row's
 // 16-byte chunk ch stands at place ch ^ (row % 16) (K) or ch ^ 4 (row % 4) (V): 16 neighbouring
 // lanes of a K read, 32 of a transposing read cover all banks (a load into LDS cannot pad rows,
-// but each lane chooses what it loads).  Keys past the
-// last one reload it: slots that no row attends are never read.
+// but each lane chooses what it loads; with ch ^ 2 (row % 8) for both, half of the cycles of
+// LDS were bank conflicts).  Keys past the last one reload it: slots that no row attends are
+// never read.
+//   4 waves, 2 buffers (64 KB, two workgroups a CU): every packed call, and trees of up to 128
+//     pairs.  8 waves, 4 buffers (128 KB, one a CU): wider trees, whose K and V then come once
+//     for 256 pairs (8 x 64 nodes, 4 q heads a kv head, 32k slots: 264 -> 258 us; packed prompts
+//     are no faster for it, and 16 short ones 31 -> 38 us).
+// What bounds it (one MI355X; a large copy reaches 5.15 TB/s, an 8192^3 product 1.21 PFLOP/s):
+//   8001 rows from 0, 32 / 8 heads: 500-530 us, 0.98-1.05 PFLOP/s.  MFMAs take 54 % of a SIMD's
+//     cycles and VALU instructions as many beside them, at the 1.8-1.9 GHz that the card holds
+//     under this load; LDS 26 % of a CU's, no bank conflicts.
+//   16 x 26 nodes over 901 to 4001 slots, 16 / 8 heads: 46-48 us, 3.6 TB/s with the merge: memory.
+//   16 prompts of 37 to 1021 rows: 31 us: first loads and outputs of items of up to 16 blocks.
+// Measured and dropped: one half's softmax beside the other half's products (8 % slower), priorities
+// around the products (1-3 %), scheduling groups and iglp (0-4 %), two waves sharing the blocks of a
+// tile of up to 32 pairs (single rows 5 % faster, everything else 3-8 % slower: registers).
 template <bool TREE, int WAVES, int RING>
 __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
   constexpr int D = RG_D;
@@ -434,253 +440,254 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
   }
   const int at0 = at;
   for (; at < end;) {
-  RaggedItem it;
-  if (TREE) {
-    at = walk.next(p, bin, tile, h, at0, at, end, it);
-    if (it.j0 >= it.pairs) continue;                       // this sequence has fewer tiles
-  } else {
-    const int32_t* w = p.items + (size_t)at * RG_ITEM;
-    ++at;
-    it.row0 = w[0]; it.rows = w[1]; it.start = w[2]; it.crow = w[3];
-    it.j0 = w[4]; it.kb0 = w[5]; it.kb1 = w[6]; it.part = w[7];
-    it.pairs = (int)((uint32_t)it.rows * (uint32_t)p.G);   // checked below
-    // a table that does not fit the tensors is not followed
-    if (it.row0 < 0 || it.rows < 1 || it.row0 + (long long)it.rows > p.rows || it.start < 0 ||
-        it.start > p.cap - it.rows || it.crow < 0 || it.crow >= p.n_cache || it.j0 < 0 ||
-        (long long)it.rows * p.G > 0x7FFFFFFF - ROWS || it.j0 >= it.pairs || it.part >= p.n_parts)
-      continue;
-    it.kend = it.start + (min(it.j0 + ROWS, it.pairs) - 1) / p.G + 1;
-    it.kb0 = max(it.kb0, 0);
-    it.kb1 = min(it.kb1, (it.kend + RG_KEYS - 1) / RG_KEYS);
-  }
-
-  // ---- K / V staging: a wave's instruction moves 4 keys (1 KB); 4 each of K and V a block ----
-  const size_t cache_base = ((size_t)it.crow * p.Hkv + h) * (size_t)p.cap * D;
-  const int srow = lane >> 4;                              // key within the instruction's four
-  const int place = lane & 15;                             // where the lane's 16 bytes go in the key's row
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rg_lds_address(s_kv) + wave * WKEYS * D * 2);
-  constexpr int LOADS = WKEYS / 4;                         // instructions of a wave for K, and for V
-  uint32_t kat[LOADS], vat[LOADS];                         // what the lane loads: byte in the block, less 1024 i
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    kat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ ((wave * WKEYS + 4 * i + srow) & 15));
-    vat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ (4 * srow));
-  }
-  const i32x4 krsrc = keys_rsrc(p.kc + cache_base), vrsrc = keys_rsrc(p.vc + cache_base);
-  // K and V block kb into its buffer
-  auto stage = [&](int kb) __attribute__((always_inline)) {
-    const uint32_t lds = lds0 + ((kb - it.kb0) & (RING - 1)) * (4 * RG_KEYS * D);
-    if ((kb + 1) * RG_KEYS <= it.kend) {
-      const uint32_t at = (uint32_t)kb * (RG_KEYS * D * 2);
-      if (it.pairs <= ROWS) {                              // the sequence's only tile: its keys are read once
-        lds_load_keys<LOADS, true>(krsrc, kat, at, lds);
-        lds_load_keys<LOADS, true>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
-      } else {
-        lds_load_keys<LOADS, false>(krsrc, kat, at, lds);
-        lds_load_keys<LOADS, false>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
-      }
+    RaggedItem it;
+    if (TREE) {
+      at = walk.next(p, bin, tile, h, at0, at, end, it);
+      if (it.j0 >= it.pairs) continue;                       // this sequence has fewer tiles
     } else {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int at = wave * WKEYS + 4 * i + srow;
-        const uint32_t key = (uint32_t)min(kb * RG_KEYS + at, it.kend - 1) * (D * 2);
-        lds_load16(krsrc, key + 16 * (place ^ (at & 15)), lds + i * 4 * D * 2);
-        lds_load16(vrsrc, key + 16 * (place ^ (4 * srow)), lds + 2 * RG_KEYS * D + i * 4 * D * 2);
-      }
+      const int32_t* w = p.items + (size_t)at * RG_ITEM;
+      ++at;
+      it.row0 = w[0]; it.rows = w[1]; it.start = w[2]; it.crow = w[3];
+      it.j0 = w[4]; it.kb0 = w[5]; it.kb1 = w[6]; it.part = w[7];
+      it.pairs = (int)((uint32_t)it.rows * (uint32_t)p.G);   // checked below
+      // a table that does not fit the tensors is not followed
+      if (it.row0 < 0 || it.rows < 1 || it.row0 + (long long)it.rows > p.rows || it.start < 0 ||
+          it.start > p.cap - it.rows || it.crow < 0 || it.crow >= p.n_cache || it.j0 < 0 ||
+          (long long)it.rows * p.G > 0x7FFFFFFF - ROWS || it.j0 >= it.pairs || it.part >= p.n_parts)
+        continue;
+      it.kend = it.start + (min(it.j0 + ROWS, it.pairs) - 1) / p.G + 1;
+      it.kb0 = max(it.kb0, 0);
+      it.kb1 = min(it.kb1, (it.kend + RG_KEYS - 1) / RG_KEYS);
     }
-  };
-#pragma unroll
-  for (int s = 0; s < RING - 1; ++s)
-    if (it.kb0 + s < it.kb1) stage(it.kb0 + s);
 
-  // ---- this lane's pair, and its q row as the B operand ----
-  const int j = it.j0 + wave * 32 + c;
-  const bool wave_on = it.j0 + wave * 32 < it.pairs;       // some pair of the wave exists
-  const int jj = min(j, it.pairs - 1);
-  const int t = jj / p.G;
-  const int head = h * p.G + (jj - t * p.G);
-  const size_t qrow = (size_t)it.row0 + t;
-  u32x4 qb[8];
-  {
-    const uint16_t* src = p.q + (qrow * p.Hq + head) * D + 8 * h2;
+    // ---- K / V staging: a wave's instruction moves 4 keys (1 KB); 4 each of K and V a block ----
+    const size_t cache_base = ((size_t)it.crow * p.Hkv + h) * (size_t)p.cap * D;
+    const int srow = lane >> 4;                              // key within the instruction's four
+    const int place = lane & 15;                             // where the lane's 16 bytes go in the key's row
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rg_lds_address(s_kv) + wave * WKEYS * D * 2);
+    constexpr int LOADS = WKEYS / 4;                         // instructions of a wave for K, and for V
+    uint32_t kat[LOADS], vat[LOADS];                         // what the lane loads: byte in the block, less 1024 i
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) qb[ks] = *reinterpret_cast<const u32x4*>(src + 16 * ks);
-  }
-  // positions of the wave's rows: first and last (wave-uniform), this lane's
-  const int t_first = (it.j0 + wave * 32) / p.G;
-  const int t_last = (min(it.j0 + wave * 32 + 32, it.pairs) - 1) / p.G;
-  const int qpos = it.start + t;
-  const int mask_from = TREE ? it.start : it.start + t_first + 1;   // keys below it are seen by every row
-  const int wave_end = TREE ? it.kend : it.start + t_last + 1;      // keys from it on by none
-  uint32_t seen_lo = 0, seen_hi = 0;                       // tree: the nodes that the lane's node attends
-  if (TREE && it.kb1 * RG_KEYS > it.start && it.kb0 < it.kb1) {
-    int depth;
-    const unsigned long long own = 1ull << lane;
-    const unsigned long long s = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane), lane, depth) | own;
-    seen_lo = __shfl((uint32_t)s, t, 64);
-    seen_hi = __shfl((uint32_t)(s >> 32), t, 64);
-  }
-
-  float m = -INFINITY, mref = 0.0f, l = 0.0f;              // mref: m, or 0 while m is -inf; l: of this lane's keys
-  f32x16 o[4];
-#pragma unroll
-  for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
-
-  // LDS offsets (elements): K row c of a 32-key tile, V rows by transposing reads
-  const int kx = c & 15;
-  const int vi = lane & 15, vrow = 4 * h2 + (vi >> 2);     // key of the 8 that the lane's read names
-  const int vcol = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);   // its 16-byte chunk within a 32-dim tile
-
-  for (int kb = it.kb0; kb < it.kb1; ++kb) {
-    // this block is here (2 LOADS of each later one may be on their way; the first wait of an
-    // item, behind other kinds of memory operations, is for everything), and the buffer of the
-    // block before it is free
-    const int later = min(RING - 2, it.kb1 - 1 - kb);
-    if (RING > 3 && later == 2 && kb > it.kb0) loads_barrier<4 * LOADS>();
-    else if (RING > 2 && later == 1 && kb > it.kb0) loads_barrier<2 * LOADS>();
-    else loads_done_barrier();
-    if (kb + RING - 1 < it.kb1) stage(kb + RING - 1);
-    if (!wave_on || kb * RG_KEYS >= wave_end) continue;
-    const uint16_t* const bk = s_kv + ((kb - it.kb0) & (RING - 1)) * (2 * RG_KEYS * D);
-    const uint16_t* const bv = bk + RG_KEYS * D;
-    // ---- S^T = K Q^T ----
-    f32x16 s[2];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        const u32x4 ka = *reinterpret_cast<const u32x4*>(bk + (32 * n + c) * D + ((2 * ks + h2) ^ kx) * 8);
-        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ka),
-                                                       __builtin_bit_cast(bf16x8, qb[ks]), s[n], 0, 0, 0);
-      }
+    for (int i = 0; i < LOADS; ++i) {
+      kat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ ((wave * WKEYS + 4 * i + srow) & 15));
+      vat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ (4 * srow));
     }
-    // ---- masks, only on blocks that some row does not see whole ----
-    if (kb * RG_KEYS + RG_KEYS > mask_from) {
-      if (TREE) {
-        const int rel = kb * RG_KEYS - it.start;           // node of the block's first key (negative: a context slot)
-        const unsigned long long w = (unsigned long long)seen_hi << 32 | seen_lo;
-        unsigned long long bm = rel >= 64 ? 0ull : rel >= 0 ? w >> rel : (w << -rel) | ((1ull << -rel) - 1);
-        bm >>= 4 * h2;
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!((uint32_t)(bm >> (32 * n)) & (1u << (8 * (i / 4) + i % 4)))) s[n][i] = -INFINITY;
+    const i32x4 krsrc = keys_rsrc(p.kc + cache_base), vrsrc = keys_rsrc(p.vc + cache_base);
+    // K and V block kb into its buffer
+    auto stage = [&](int kb) __attribute__((always_inline)) {
+      const uint32_t lds = lds0 + ((kb - it.kb0) & (RING - 1)) * (4 * RG_KEYS * D);
+      if ((kb + 1) * RG_KEYS <= it.kend) {
+        const uint32_t at = (uint32_t)kb * (RG_KEYS * D * 2);
+        if (it.pairs <= ROWS) {                              // the sequence's only tile: its keys are read once
+          lds_load_keys<true>(krsrc, kat, at, lds);
+          lds_load_keys<true>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
+        } else {
+          lds_load_keys<false>(krsrc, kat, at, lds);
+          lds_load_keys<false>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
+        }
       } else {
-        const int rel = qpos - kb * RG_KEYS - 4 * h2;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (32 * n + 8 * (i / 4) + i % 4 > rel) s[n][i] = -INFINITY;
+        for (int i = 0; i < LOADS; ++i) {
+          const int at = wave * WKEYS + 4 * i + srow;
+          const uint32_t key = (uint32_t)min(kb * RG_KEYS + at, it.kend - 1) * (D * 2);
+          lds_load16(krsrc, key + 16 * (place ^ (at & 15)), lds + i * 4 * D * 2);
+          lds_load16(vrsrc, key + 16 * (place ^ (4 * srow)), lds + 2 * RG_KEYS * D + i * 4 * D * 2);
+        }
       }
-    }
-    // ---- online softmax (log2 domain) ----
-    float mx = fmaxf(s[0][0], s[1][0]);
+    };
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
-    mx = pair_max(mx) * p.scale_log2;
-    if (__any(mx > m + 8.0f)) {
-      const float mn = fmaxf(m, mx);
-      const float f = m > -INFINITY ? exp2_fast(m - mn) : 0.0f;
-      l *= f;
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[dt][i] *= f;
-      m = mn;
-      mref = mn > -INFINITY ? mn : 0.0f;
-    }
-    uint32_t pw[2][8];                                     // bf16 weights, two keys a word
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const uint32_t w = pack_bf16x2(exp2_fast(fmaf(s[n][i], p.scale_log2, -mref)),
-                                       exp2_fast(fmaf(s[n][i + 1], p.scale_log2, -mref)));
-        pw[n][i / 2] = w;
-        l = dot2_bf16(w, 0x3F803F80u, l);                  // the rounded weights
-      }
-    // ---- O^T += V^T P^T ----
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t* const w = pw[u / 2] + 4 * (u % 2);
-      const u32x4 pb = u32x4{w[0], w[1], w[2], w[3]};
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt) {
-        const uint16_t* const v = bv + (16 * u + vrow) * D + ((4 * dt + vcol) ^ (4 * (vi >> 2))) * 8 + 4 * (vi & 1);
-        typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-        const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
-        const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D));
-        const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
-        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u32x4{b0.x, b0.y, b1.x, b1.y}),
-                                                        __builtin_bit_cast(bf16x8, pb), o[dt], 0, 0, 0);
-      }
-    }
-  }
+    for (int s = 0; s < RING - 1; ++s)
+      if (it.kb0 + s < it.kb1) stage(it.kb0 + s);
 
-  // the buffers are free for the next item
-  if (at < end) loads_done_barrier();
-  // ---- outputs: register i of o[dt] is dim 32 dt + 8 (i / 4) + 4 h2 + i % 4 of the lane's pair ----
-  if (!wave_on) continue;
-  l = pair_sum(l);
-  // A weight of 0 times an infinity or a NaN in V is a NaN: a row whose sums are not finite is
-  // formed again from the keys that it attends alone, so that what a mask hides stays hidden.
-  float finite = 0.0f * l;
+    // ---- this lane's pair, and its q row as the B operand ----
+    const int j = it.j0 + wave * 32 + c;
+    const bool wave_on = it.j0 + wave * 32 < it.pairs;       // some pair of the wave exists
+    const int jj = min(j, it.pairs - 1);
+    const int t = jj / p.G;
+    const int head = h * p.G + (jj - t * p.G);
+    const size_t qrow = (size_t)it.row0 + t;
+    u32x4 qb[8];
+    {
+      const uint16_t* src = p.q + (qrow * p.Hq + head) * D + 8 * h2;
 #pragma unroll
-  for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) finite = fmaf(0.0f, o[dt][i], finite);
-  const unsigned long long odd = __ballot(finite != finite);
-  const uint32_t again = (uint32_t)(odd | odd >> 32);       // bit c: the pair of lanes c and c + 32
-  if (again) exact_rows<TREE>(p, it, h, it.j0 + wave * 32, again, lane);
-  const bool live = j < it.pairs && !(again >> c & 1);
-  if (it.part >= 0) {
-    const size_t st = ((size_t)it.part * p.Hkv + h) * p.part_rows + wave * 32 + c;
-    m = l != l ? INFINITY : m;                             // a row that saw a NaN stays one in the merge
-    if (live && h2 == 0) p.part_ml[st] = float2{m, l};
-    if (live && m > -INFINITY) {                           // else its outputs are not read
-      float* dst = p.part_o + st * D + 4 * h2;
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+      for (int ks = 0; ks < 8; ++ks) qb[ks] = *reinterpret_cast<const u32x4*>(src + 16 * ks);
     }
-    continue;
-  }
-  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);   // nothing attended: a zero row; NaN stays
-  uint16_t* const dst = p.out + (qrow * p.Hq + head) * D + 8 * h2;
-  float hs = 0.0f;
+    // positions of the wave's rows: first and last (wave-uniform), this lane's
+    const int t_first = (it.j0 + wave * 32) / p.G;
+    const int t_last = (min(it.j0 + wave * 32 + 32, it.pairs) - 1) / p.G;
+    const int qpos = it.start + t;
+    const int mask_from = TREE ? it.start : it.start + t_first + 1;   // keys below it are seen by every row
+    const int wave_end = TREE ? it.kend : it.start + t_last + 1;      // keys from it on by none
+    uint32_t seen_lo = 0, seen_hi = 0;                       // tree: the nodes that the lane's node attends
+    if (TREE && it.kb1 * RG_KEYS > it.start && it.kb0 < it.kb1) {
+      int depth;
+      const unsigned long long own = 1ull << lane;
+      const unsigned long long s = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane), lane, depth) | own;
+      seen_lo = __shfl((uint32_t)s, t, 64);
+      seen_hi = __shfl((uint32_t)(s >> 32), t, 64);
+    }
+
+    float m = -INFINITY, mref = 0.0f, l = 0.0f;              // mref: m, or 0 while m is -inf; l: of this lane's keys
+    f32x16 o[4];
 #pragma unroll
-  for (int dt = 0; dt < 4; ++dt)
+    for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; g += 2) {
-      uint32_t x[2], y[2];
+      for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
+
+    // LDS offsets (elements): K row c of a 32-key tile, V rows by transposing reads
+    const int kx = c & 15;
+    const int vi = lane & 15, vrow = 4 * h2 + (vi >> 2);     // key of the 8 that the lane's read names
+    const int vcol = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);   // its 16-byte chunk within a 32-dim tile
+
+    for (int kb = it.kb0; kb < it.kb1; ++kb) {
+      // this block is here (2 LOADS of each later one may be on their way; the first wait of an
+      // item, behind other kinds of memory operations, is for everything), and the buffer of the
+      // block before it is free
+      const int later = min(RING - 2, it.kb1 - 1 - kb);
+      if (RING > 3 && later == 2 && kb > it.kb0) loads_barrier<4 * LOADS>();
+      else if (RING > 2 && later == 1 && kb > it.kb0) loads_barrier<2 * LOADS>();
+      else loads_done_barrier();
+      if (kb + RING - 1 < it.kb1) stage(kb + RING - 1);
+      if (!wave_on || kb * RG_KEYS >= wave_end) continue;
+      const uint16_t* const bk = s_kv + ((kb - it.kb0) & (RING - 1)) * (2 * RG_KEYS * D);
+      const uint16_t* const bv = bk + RG_KEYS * D;
+      // ---- S^T = K Q^T ----
+      f32x16 s[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        x[e] = pack_bf16x2(o[dt][4 * g + 2 * e] * inv, o[dt][4 * g + 2 * e + 1] * inv);
-        y[e] = pack_bf16x2(o[dt][4 * g + 4 + 2 * e] * inv, o[dt][4 * g + 5 + 2 * e] * inv);
-        hs += (bf16_lo(x[e]) + bf16_hi(x[e])) + (bf16_lo(y[e]) + bf16_hi(y[e]));
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const u32x4 ka = *reinterpret_cast<const u32x4*>(bk + (32 * n + c) * D + ((2 * ks + h2) ^ kx) * 8);
+          s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ka),
+                                                         __builtin_bit_cast(bf16x8, qb[ks]), s[n], 0, 0, 0);
+        }
       }
-      // lanes trade halves: each ends up with 8 neighbouring dims
-      const auto a = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
-      const auto b = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
-      if (live) *reinterpret_cast<u32x4*>(dst + 32 * dt + 8 * g) = u32x4{a[0], b[0], a[1], b[1]};
+      // ---- masks, only on blocks that some row does not see whole ----
+      if (kb * RG_KEYS + RG_KEYS > mask_from) {
+        if (TREE) {
+          const int rel = kb * RG_KEYS - it.start;           // node of the block's first key (negative: a context slot)
+          const unsigned long long w = (unsigned long long)seen_hi << 32 | seen_lo;
+          unsigned long long bm = rel >= 64 ? 0ull : rel >= 0 ? w >> rel : (w << -rel) | ((1ull << -rel) - 1);
+          bm >>= 4 * h2;
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (!((uint32_t)(bm >> (32 * n)) & (1u << (8 * (i / 4) + i % 4)))) s[n][i] = -INFINITY;
+        } else {
+          const int rel = qpos - kb * RG_KEYS - 4 * h2;
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (32 * n + 8 * (i / 4) + i % 4 > rel) s[n][i] = -INFINITY;
+        }
+      }
+      // ---- online softmax (log2 domain) ----
+      float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+      mx = pair_max(mx) * p.scale_log2;
+      if (__any(mx > m + 8.0f)) {
+        const float mn = fmaxf(m, mx);
+        const float f = m > -INFINITY ? exp2_fast(m - mn) : 0.0f;
+        l *= f;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[dt][i] *= f;
+        m = mn;
+        mref = mn > -INFINITY ? mn : 0.0f;
+      }
+      uint32_t pw[2][8];                                     // bf16 weights, two keys a word
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const uint32_t w = pack_bf16x2(exp2_fast(fmaf(s[n][i], p.scale_log2, -mref)),
+                                         exp2_fast(fmaf(s[n][i + 1], p.scale_log2, -mref)));
+          pw[n][i / 2] = w;
+          l = dot2_bf16(w, 0x3F803F80u, l);                  // the rounded weights
+        }
+      // ---- O^T += V^T P^T ----
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t* const w = pw[u / 2] + 4 * (u % 2);
+        const u32x4 pb = u32x4{w[0], w[1], w[2], w[3]};
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) {
+          const uint16_t* const v = bv + (16 * u + vrow) * D + ((4 * dt + vcol) ^ (4 * (vi >> 2))) * 8 + 4 * (vi & 1);
+          typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+          const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
+          const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D));
+          const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u32x4{b0.x, b0.y, b1.x, b1.y}),
+                                                          __builtin_bit_cast(bf16x8, pb), o[dt], 0, 0, 0);
+        }
+      }
     }
-  if (p.out_sums) {
-    hs = pair_sum(hs);
-    if (live && h2 == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
-  }
+
+    // the buffers are free for the next item
+    if (at < end) loads_done_barrier();
+    // ---- outputs: register i of o[dt] is dim 32 dt + 8 (i / 4) + 4 h2 + i % 4 of the lane's pair ----
+    if (!wave_on) continue;
+    l = pair_sum(l);
+    // A weight of 0 times an infinity or a NaN in V is a NaN: a row whose sums are not finite is
+    // formed again from the keys that it attends alone, so that what a mask hides stays hidden.
+    float finite = 0.0f * l;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) finite = fmaf(0.0f, o[dt][i], finite);
+    const unsigned long long odd = __ballot(finite != finite);
+    const uint32_t again = (uint32_t)(odd | odd >> 32);       // bit c: the pair of lanes c and c + 32
+    if (again) exact_rows<TREE>(p, it, h, it.j0 + wave * 32, again, lane);
+    const bool live = j < it.pairs && !(again >> c & 1);
+    if (it.part >= 0) {
+      const size_t st = ((size_t)it.part * p.Hkv + h) * p.part_rows + wave * 32 + c;
+      m = l != l ? INFINITY : m;                             // a row that saw a NaN stays one in the merge
+      if (live && h2 == 0) p.part_ml[st] = float2{m, l};
+      if (live && m > -INFINITY) {                           // else its outputs are not read
+        float* dst = p.part_o + st * D + 4 * h2;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+      }
+      continue;
+    }
+    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);   // nothing attended: a zero row; NaN stays
+    uint16_t* const dst = p.out + (qrow * p.Hq + head) * D + 8 * h2;
+    float hs = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; g += 2) {
+        uint32_t x[2], y[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          x[e] = pack_bf16x2(o[dt][4 * g + 2 * e] * inv, o[dt][4 * g + 2 * e + 1] * inv);
+          y[e] = pack_bf16x2(o[dt][4 * g + 4 + 2 * e] * inv, o[dt][4 * g + 5 + 2 * e] * inv);
+          hs += (bf16_lo(x[e]) + bf16_hi(x[e])) + (bf16_lo(y[e]) + bf16_hi(y[e]));
+        }
+        // lanes trade halves: each ends up with 8 neighbouring dims
+        const auto a = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+        const auto b = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+        if (live) *reinterpret_cast<u32x4*>(dst + 32 * dt + 8 * g) = u32x4{a[0], b[0], a[1], b[1]};
+      }
+    if (p.out_sums) {
+      hs = pair_sum(hs);
+      if (live && h2 == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
+    }
   }
 }
 
 // The parts of a tile joined: 32 lanes a (row, q head) pair, four dims each, eight pairs a
-// workgroup; parts in their order, MERGE_AHEAD of them in flight.
+// workgroup; parts in their order, MERGE_AHEAD of them in flight, with a running maximum.  Bound
+// by its loads' latency (16 trees of 26 nodes: 5.5-6 us, 9.6 with a wave a pair and two passes).
 constexpr int MERGE_AHEAD = 4;
 constexpr int MERGE_PAIRS = t2i_host::RG_MERGE;
 
@@ -779,7 +786,9 @@ struct TreeCommitParams {
 // A wave per (layer, sequence, kv head); lane i holds node i.  Every wave walks the tree itself
 // (a ballot a step; the walk costs less than a hand-over), then moves its head's rows: four
 // slots at a time, 16 lanes of 16 bytes each.  The path's nodes ascend, so entry e comes from a
-// slot at or behind e: a group's writes never reach a slot that a later group reads.
+// slot at or behind e: a group's writes never reach a slot that a later group reads.  Bound by the
+// latency of its chain (nodes, walk, rows): 28 layers x 8 heads, 8 nodes 3.0 us, 32 sequences of 26
+// nodes 6.3 us.
 __global__ __launch_bounds__(256) void tree_commit_kernel(const TreeCommitParams p) {
   constexpr int D = RG_D;
   const int lane = threadIdx.x & 63;
