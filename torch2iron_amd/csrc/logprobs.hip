@@ -181,9 +181,9 @@ __device__ __forceinline__ void lp_finish(const LpParams& p, int row, LpState st
 // starts as its lanes' largest values of the first pieces, in order; after that it looks at a
 // piece's order only where a lane's largest value passes the k-th best of its own list and of
 // the other waves' (which only grow, so an older one of them is as good).  2043 rows of 151936
-// fp32 logits, 20 best: 225-235 us, 5.3-5.5 TB/s (a large copy reaches 5.15): memory.  416 bf16 rows:
-// 34.5 us without best lists, 52 with 8: VALU instructions, 88 % of a SIMD's cycles (in the sums 7.5
-// an element, an exponential among them; the lists' first orders and insertions the rest).
+// fp32 logits, 20 best: 227-238 us, 5.2-5.5 TB/s (a large copy reaches 5.15), 228-230 without lists: memory,
+// with VALU instructions in 84 % of a SIMD's cycles beside it.  416 bf16 rows: 32 us without best lists,
+// 51-54 with 8 (7 of them the merge): VALU instructions, 83 % of a SIMD's cycles.
 // Measured and dropped: twice the pieces on their way (1-14 % slower), lists of the waves joined by
 // rank (2 %), fewer and longer parts (3-10 %).
 template <typename T>

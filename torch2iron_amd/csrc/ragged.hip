@@ -407,11 +407,12 @@ __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const Ragg
 //     for 256 pairs (8 x 64 nodes, 4 q heads a kv head, 32k slots: 264 -> 258 us; packed prompts
 //     are no faster for it, and 16 short ones 31 -> 38 us).
 // What bounds it (one MI355X; a large copy reaches 5.15 TB/s, an 8192^3 product 1.21 PFLOP/s):
-//   8001 rows from 0, 32 / 8 heads: 500-530 us, 0.98-1.05 PFLOP/s.  MFMAs take 54 % of a SIMD's
+//   8001 rows from 0, 32 / 8 heads: 500-516 us, 1.02-1.05 PFLOP/s.  MFMAs take 54 % of a SIMD's
 //     cycles and VALU instructions as many beside them, at the 1.8-1.9 GHz that the card holds
 //     under this load; LDS 26 % of a CU's, no bank conflicts.
-//   16 x 26 nodes over 901 to 4001 slots, 16 / 8 heads: 46-48 us, 3.6 TB/s with the merge: memory.
-//   16 prompts of 37 to 1021 rows: 31 us: first loads and outputs of items of up to 16 blocks.
+//   16 x 26 nodes over 901 to 4001 slots, 16 / 8 heads: 46-49 us with the merge; 41 without, in which
+//     157 MB come from memory (3.8 TB/s) and waves wait 70 % of their time.
+//   16 prompts of 37 to 1021 rows: 29-32 us: first loads and outputs of items of up to 16 blocks.
 // Measured and dropped: one half's softmax beside the other half's products (8 % slower), priorities
 // around the products (1-3 %), scheduling groups and iglp (0-4 %), two waves sharing the blocks of a
 // tile of up to 32 pairs (single rows 5 % faster, everything else 3-8 % slower: registers).
@@ -788,7 +789,7 @@ struct TreeCommitParams {
 // slots at a time, 16 lanes of 16 bytes each.  The path's nodes ascend, so entry e comes from a
 // slot at or behind e: a group's writes never reach a slot that a later group reads.  Bound by the
 // latency of its chain (nodes, walk, rows): 28 layers x 8 heads, 8 nodes 3.0 us, 32 sequences of 26
-// nodes 6.3 us.
+// nodes 6.6-6.8 us.
 __global__ __launch_bounds__(256) void tree_commit_kernel(const TreeCommitParams p) {
   constexpr int D = RG_D;
   const int lane = threadIdx.x & 63;
