@@ -209,3 +209,17 @@ def test_ops_refuse_host_tensors():
               lambda: ops.token_logprobs(x[0].float(), i[0])):
         with pytest.raises(ValueError, match="GPU tensor"):
             f()
+
+
+@pytest.mark.parametrize("bad", [[1.5, 2.0], [True, False]], ids=["float", "bool"])
+def test_prompts_that_are_no_integers_are_refused(bad):
+    """They are not rounded to token ids; lists and tensors of integers pass."""
+    from types import SimpleNamespace
+
+    from torch2iron_amd.model import Qwen3Model
+    m = SimpleNamespace(batch=2, ctx_cap=8, cfg=SimpleNamespace(vocab=16))
+    for p in (bad, torch.tensor(bad)):
+        with pytest.raises(ValueError, match="integers"):
+            Qwen3Model._prompt_list(m, [[1, 2], p])
+    got = Qwen3Model._prompt_list(m, [[1, 2], torch.tensor([3], dtype=torch.int64)])
+    assert [p.tolist() for p in got] == [[1, 2], [3]] and all(p.dtype == torch.int32 for p in got)

@@ -668,6 +668,8 @@ class Qwen3Model:
         for p in prompts:
             if p.dim() != 1 or p.numel() < 1:
                 raise ValueError("every prompt must be a non-empty row of token ids")
+            if p.dtype == torch.bool or p.is_floating_point() or p.is_complex():
+                raise ValueError(f"token ids must be integers, got {p.dtype}")
             if p.numel() > self.ctx_cap:
                 raise ValueError(f"a prompt of {p.numel()} tokens exceeds the cache capacity {self.ctx_cap}")
             if int(p.min()) < 0 or int(p.max()) >= self.cfg.vocab:
