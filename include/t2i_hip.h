@@ -507,8 +507,8 @@ int t2i_prompt_advance(const int32_t* prompt, int32_t B, int32_t P, int32_t* tok
  * cache row lies outside the cache writes nothing.
  *
  * t2i_packed_attention: row r of a sequence attends its slots 0 .. starts + r (causal;
- * fp32 scores and softmax, weights rounded to bf16 for the product with V); q bf16
- * [rows, Hq, D], out bf16 [rows, Hq * D].  Slots that no row attends are never read.
+ * fp32 scores and softmax, weights rounded to bf16 for the product with V, those of a
+ * sequence of one row to 16 bits); q bf16 [rows, Hq, D], out bf16 [rows, Hq * D].  Slots that no row attends are never read.
  * out_sums (nullable): fp32 [Hq][rows], as t2i_prefill_attention_sums.  The workspace
  * (t2i_packed_attention_workspace_bytes, 0: none needed) is scratch: no initial
  * value, nothing kept; calls that overlap in time must not share one.
@@ -541,8 +541,8 @@ int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32_t* items, 
  *
  * t2i_tree_qk_rope_kv: t2i_prefill_qk_rope_kv for the nodes; q_out bf16 [B, N, Hq, D].
  * t2i_tree_attention: node i attends the slots 0 .. context - 1, the nodes above it and
- * itself; q bf16 [B, N, Hq, D], out bf16 [B * N, Hq * D]; arithmetic and workspace
- * (t2i_tree_attention_workspace_bytes) as t2i_packed_attention.
+ * itself; q bf16 [B, N, Hq, D], out bf16 [B * N, Hq * D]; arithmetic as t2i_packed_attention's
+ * for a sequence of one row, workspace (t2i_tree_attention_workspace_bytes) as its.
  * t2i_tree_commit: the greedy walk from node 0 (the sequence's own last token, always
  * accepted): from node n to the lowest-numbered child whose token is picks[b][n], as long
  * as there is one.  Writes path [B, N] (the walk's nodes, then -1), path_counts [B],

@@ -9,9 +9,10 @@
 //   * t2i_tree_commit: the greedy walk down the drafted trees and the accepted path's K/V
 //     rows moved to the front, in every layer.
 //
-// Scores, softmax statistics and sums are fp32; the softmax weights enter the P . V product
-// as bf16, as in t2i_prefill_attention (quantized_qwen3/model.py:277), and each row's
-// normaliser sums those rounded weights, so that a row of equal values comes back exact.
+// Scores, softmax statistics and sums are fp32.  The softmax weights of prompt rows enter the P . V
+// product as bf16, as in t2i_prefill_attention (quantized_qwen3/model.py:277), and each row's
+// normaliser sums those rounded weights, so that a row of equal values comes back exact; trees and
+// sequences of one row, which stand in for decode steps, multiply by weights of 16 bits.
 #include <math.h>
 
 #include <atomic>
@@ -337,7 +338,7 @@ __device__ __forceinline__ bool attends(const RaggedItem& it, int t, unsigned lo
 
 // The item's outputs for the pairs j0 + bit of `rows`, a wave a pair after the other, lane e dims
 // 2 e and 2 e + 1: the definition key by key, for rows that hold infinities or NaN.
-template <bool TREE>
+template <bool TREE, bool FINE>
 __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const RaggedItem& it, int h, int j0, uint32_t rows,
                                            int lane) {
   constexpr int D = RG_D;
@@ -362,7 +363,7 @@ __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const Ragg
       const uint32_t v = *reinterpret_cast<const uint32_t*>(p.vc + base + (size_t)key * D);
       const float s = wave_sum(bf16_lo(q) * bf16_lo(k) + bf16_hi(q) * bf16_hi(k)) * p.scale_log2;
       const float mn = fmaxf(m, s), f = state_weight(m, mn);
-      const float w = round_bf16(exp2_fast(s - (mn > -INFINITY ? mn : 0.0f)));
+      const float e = exp2_fast(s - (mn > -INFINITY ? mn : 0.0f)), w = FINE ? e : round_bf16(e);
       l = l * f + w;
       o0 = o0 * f + w * bf16_lo(v);
       o1 = o1 * f + w * bf16_hi(v);
@@ -384,9 +385,9 @@ __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const Ragg
   }
 }
 
-// One workgroup (WAVES waves of 32 pairs) takes a bin's items for one kv head, one after the
-// other.  All products run transposed on the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32,
-// h2 = lane / 32) holds one pair's scores and outputs:
+// An item of a workgroup of WAVES waves of 32 pairs, for one kv head.  All products run transposed
+// on the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32, h2 = lane / 32) holds one pair's scores
+// and outputs:
 //   S^T = K Q^T: A = K from LDS (lane: key 32 n + c, dims 16 ks + 8 h2 ..), B = the wave's q
 //     rows (registers); register i holds the score of key 32 n + 8 (i / 4) + 4 h2 + i % 4;
 //   the online softmax per lane: the row's maximum from its two lanes by one lane swap, the
@@ -396,6 +397,12 @@ __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const Ragg
 //   O^T += V^T P^T: B = P^T straight from those registers, rounded to bf16 (16 keys a step, in
 //     the order they stand in), A = V^T from LDS in that order by transposing reads
 //     (ds_read_b64_tr_b16: four keys of one dim a lane out of V's own row order).
+// FINE: what the rounding of the weights left is a second bf16 word and V is multiplied by both:
+// weights of 16 bits, whose error the output's own rounding hides, normalised by their fp32 sum.  Trees
+// and sequences of one row take it, since they stand in for decode steps, whose weights are fp32
+// (16 x 26 nodes 47.2 -> 49.8 us, 8 x 64 nodes over 32k slots 265 -> 323, 16 single rows 33.1 -> 34.2); prompt
+// rows round their weights once, as the batch form of the prompt pass does (8001 rows: 517 us,
+// with FINE 713).
 // K and V blocks go straight from memory into LDS, RING buffers, one barrier a block; a row's
 // 16-byte chunk ch stands at place ch ^ (row % 16) (K) or ch ^ 4 (row % 4) (V): 16 neighbouring
 // lanes of a K read, 32 of a transposing read cover all banks (a load into LDS cannot pad rows,
@@ -416,11 +423,253 @@ __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const Ragg
 // Measured and dropped: one half's softmax beside the other half's products (8 % slower), priorities
 // around the products (1-3 %), scheduling groups and iglp (0-4 %), two waves sharing the blocks of a
 // tile of up to 32 pairs (single rows 5 % faster, everything else 3-8 % slower: registers).
-template <bool TREE, int WAVES, int RING>
-__global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
+template <bool TREE, int WAVES, int RING, bool FINE>
+__device__ __forceinline__ void attend_item(const RaggedAttnParams& p, const RaggedItem& it, int h, uint16_t* s_kv, int lane,
+                                            int wave, bool more) {
   constexpr int D = RG_D;
   constexpr int ROWS = 32 * WAVES;             // pairs of a tile
   constexpr int WKEYS = RG_KEYS / WAVES;       // keys of a block that a wave loads
+  const int c = lane & 31, h2 = lane >> 5;
+
+  // ---- K / V staging: a wave's instruction moves 4 keys (1 KB); 4 each of K and V a block ----
+  const size_t cache_base = ((size_t)it.crow * p.Hkv + h) * (size_t)p.cap * D;
+  const int srow = lane >> 4;                              // key within the instruction's four
+  const int place = lane & 15;                             // where the lane's 16 bytes go in the key's row
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rg_lds_address(s_kv) + wave * WKEYS * D * 2);
+  constexpr int LOADS = WKEYS / 4;                         // instructions of a wave for K, and for V
+  uint32_t kat[LOADS], vat[LOADS];                         // what the lane loads: byte in the block, less 1024 i
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    kat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ ((wave * WKEYS + 4 * i + srow) & 15));
+    vat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ (4 * srow));
+  }
+  const i32x4 krsrc = keys_rsrc(p.kc + cache_base), vrsrc = keys_rsrc(p.vc + cache_base);
+  // K and V block kb into its buffer
+  auto stage = [&](int kb) __attribute__((always_inline)) {
+    const uint32_t lds = lds0 + ((kb - it.kb0) & (RING - 1)) * (4 * RG_KEYS * D);
+    if ((kb + 1) * RG_KEYS <= it.kend) {
+      const uint32_t at = (uint32_t)kb * (RG_KEYS * D * 2);
+      if (it.pairs <= ROWS) {                              // the sequence's only tile: its keys are read once
+        lds_load_keys<true>(krsrc, kat, at, lds);
+        lds_load_keys<true>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
+      } else {
+        lds_load_keys<false>(krsrc, kat, at, lds);
+        lds_load_keys<false>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int at = wave * WKEYS + 4 * i + srow;
+        const uint32_t key = (uint32_t)min(kb * RG_KEYS + at, it.kend - 1) * (D * 2);
+        lds_load16(krsrc, key + 16 * (place ^ (at & 15)), lds + i * 4 * D * 2);
+        lds_load16(vrsrc, key + 16 * (place ^ (4 * srow)), lds + 2 * RG_KEYS * D + i * 4 * D * 2);
+      }
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < RING - 1; ++s)
+    if (it.kb0 + s < it.kb1) stage(it.kb0 + s);
+
+  // ---- this lane's pair, and its q row as the B operand ----
+  const int j = it.j0 + wave * 32 + c;
+  const bool wave_on = it.j0 + wave * 32 < it.pairs;       // some pair of the wave exists
+  const int jj = min(j, it.pairs - 1);
+  const int t = jj / p.G;
+  const int head = h * p.G + (jj - t * p.G);
+  const size_t qrow = (size_t)it.row0 + t;
+  u32x4 qb[8];
+  {
+    const uint16_t* src = p.q + (qrow * p.Hq + head) * D + 8 * h2;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qb[ks] = *reinterpret_cast<const u32x4*>(src + 16 * ks);
+  }
+  // positions of the wave's rows: first and last (wave-uniform), this lane's
+  const int t_first = (it.j0 + wave * 32) / p.G;
+  const int t_last = (min(it.j0 + wave * 32 + 32, it.pairs) - 1) / p.G;
+  const int qpos = it.start + t;
+  const int mask_from = TREE ? it.start : it.start + t_first + 1;   // keys below it are seen by every row
+  const int wave_end = TREE ? it.kend : it.start + t_last + 1;      // keys from it on by none
+  uint32_t seen_lo = 0, seen_hi = 0;                       // tree: the nodes that the lane's node attends
+  if (TREE && it.kb1 * RG_KEYS > it.start && it.kb0 < it.kb1) {
+    int depth;
+    const unsigned long long own = 1ull << lane;
+    const unsigned long long s = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane), lane, depth) | own;
+    seen_lo = __shfl((uint32_t)s, t, 64);
+    seen_hi = __shfl((uint32_t)(s >> 32), t, 64);
+  }
+
+  float m = -INFINITY, mref = 0.0f, l = 0.0f;              // mref: m, or 0 while m is -inf; l: of this lane's keys
+  f32x16 o[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
+
+  // LDS offsets (elements): K row c of a 32-key tile, V rows by transposing reads
+  const int kx = c & 15;
+  const int vi = lane & 15, vrow = 4 * h2 + (vi >> 2);     // key of the 8 that the lane's read names
+  const int vcol = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);   // its 16-byte chunk within a 32-dim tile
+
+  for (int kb = it.kb0; kb < it.kb1; ++kb) {
+    // this block is here (2 LOADS of each later one may be on their way; the first wait of an
+    // item, behind other kinds of memory operations, is for everything), and the buffer of the
+    // block before it is free
+    const int later = min(RING - 2, it.kb1 - 1 - kb);
+    if (RING > 3 && later == 2 && kb > it.kb0) loads_barrier<4 * LOADS>();
+    else if (RING > 2 && later == 1 && kb > it.kb0) loads_barrier<2 * LOADS>();
+    else loads_done_barrier();
+    if (kb + RING - 1 < it.kb1) stage(kb + RING - 1);
+    if (!wave_on || kb * RG_KEYS >= wave_end) continue;
+    const uint16_t* const bk = s_kv + ((kb - it.kb0) & (RING - 1)) * (2 * RG_KEYS * D);
+    const uint16_t* const bv = bk + RG_KEYS * D;
+    // ---- S^T = K Q^T ----
+    f32x16 s[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        const u32x4 ka = *reinterpret_cast<const u32x4*>(bk + (32 * n + c) * D + ((2 * ks + h2) ^ kx) * 8);
+        s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ka),
+                                                       __builtin_bit_cast(bf16x8, qb[ks]), s[n], 0, 0, 0);
+      }
+    }
+    // ---- masks, only on blocks that some row does not see whole ----
+    if (kb * RG_KEYS + RG_KEYS > mask_from) {
+      if (TREE) {
+        const int rel = kb * RG_KEYS - it.start;           // node of the block's first key (negative: a context slot)
+        const unsigned long long w = (unsigned long long)seen_hi << 32 | seen_lo;
+        unsigned long long bm = rel >= 64 ? 0ull : rel >= 0 ? w >> rel : (w << -rel) | ((1ull << -rel) - 1);
+        bm >>= 4 * h2;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!((uint32_t)(bm >> (32 * n)) & (1u << (8 * (i / 4) + i % 4)))) s[n][i] = -INFINITY;
+      } else {
+        const int rel = qpos - kb * RG_KEYS - 4 * h2;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (32 * n + 8 * (i / 4) + i % 4 > rel) s[n][i] = -INFINITY;
+      }
+    }
+    // ---- online softmax (log2 domain) ----
+    float mx = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+    mx = pair_max(mx) * p.scale_log2;
+    if (__any(mx > m + 8.0f)) {
+      const float mn = fmaxf(m, mx);
+      const float f = m > -INFINITY ? exp2_fast(m - mn) : 0.0f;
+      l *= f;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] *= f;
+      m = mn;
+      mref = mn > -INFINITY ? mn : 0.0f;
+    }
+    uint32_t pw[2][8], pr[2][8];                           // bf16 weights, two keys a word; what their rounding left
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float e0 = exp2_fast(fmaf(s[n][i], p.scale_log2, -mref)), e1 = exp2_fast(fmaf(s[n][i + 1], p.scale_log2, -mref));
+        const uint32_t w = pack_bf16x2(e0, e1);
+        pw[n][i / 2] = w;
+        if constexpr (FINE) {
+          pr[n][i / 2] = pack_bf16x2(e0 - bf16_lo(w), e1 - bf16_hi(w));
+          l += e0 + e1;
+        } else {
+          l = dot2_bf16(w, 0x3F803F80u, l);                // the rounded weights
+        }
+      }
+    // ---- O^T += V^T P^T ----
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t* const w = pw[u / 2] + 4 * (u % 2);
+      const uint32_t* const r = pr[u / 2] + 4 * (u % 2);
+      bf16x8 va[4];
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        const uint16_t* const v = bv + (16 * u + vrow) * D + ((4 * dt + vcol) ^ (4 * (vi >> 2))) * 8 + 4 * (vi & 1);
+        typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+        const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
+        const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D));
+        const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
+        va[dt] = __builtin_bit_cast(bf16x8, u32x4{b0.x, b0.y, b1.x, b1.y});
+        o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[dt], __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]}), o[dt], 0, 0, 0);
+      }
+      if constexpr (FINE) {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[dt], __builtin_bit_cast(bf16x8, u32x4{r[0], r[1], r[2], r[3]}), o[dt], 0, 0, 0);
+      }
+    }
+  }
+
+  // the buffers are free for the next item
+  if (more) loads_done_barrier();
+  // ---- outputs: register i of o[dt] is dim 32 dt + 8 (i / 4) + 4 h2 + i % 4 of the lane's pair ----
+  if (!wave_on) return;
+  l = pair_sum(l);
+  // A weight of 0 times an infinity or a NaN in V is a NaN: a row whose sums are not finite is
+  // formed again from the keys that it attends alone, so that what a mask hides stays hidden.
+  float finite = 0.0f * l;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) finite = fmaf(0.0f, o[dt][i], finite);
+  const unsigned long long odd = __ballot(finite != finite);
+  const uint32_t again = (uint32_t)(odd | odd >> 32);       // bit c: the pair of lanes c and c + 32
+  if (again) exact_rows<TREE, FINE>(p, it, h, it.j0 + wave * 32, again, lane);
+  const bool live = j < it.pairs && !(again >> c & 1);
+  if (it.part >= 0) {
+    const size_t st = ((size_t)it.part * p.Hkv + h) * p.part_rows + wave * 32 + c;
+    m = l != l ? INFINITY : m;                             // a row that saw a NaN stays one in the merge
+    if (live && h2 == 0) p.part_ml[st] = float2{m, l};
+    if (live && m > -INFINITY) {                           // else its outputs are not read
+      float* dst = p.part_o + st * D + 4 * h2;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+    }
+    return;
+  }
+  const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);   // nothing attended: a zero row; NaN stays
+  uint16_t* const dst = p.out + (qrow * p.Hq + head) * D + 8 * h2;
+  float hs = 0.0f;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; g += 2) {
+      uint32_t x[2], y[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        x[e] = pack_bf16x2(o[dt][4 * g + 2 * e] * inv, o[dt][4 * g + 2 * e + 1] * inv);
+        y[e] = pack_bf16x2(o[dt][4 * g + 4 + 2 * e] * inv, o[dt][4 * g + 5 + 2 * e] * inv);
+        hs += (bf16_lo(x[e]) + bf16_hi(x[e])) + (bf16_lo(y[e]) + bf16_hi(y[e]));
+      }
+      // lanes trade halves: each ends up with 8 neighbouring dims
+      const auto a = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
+      const auto b = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
+      if (live) *reinterpret_cast<u32x4*>(dst + 32 * dt + 8 * g) = u32x4{a[0], b[0], a[1], b[1]};
+    }
+  if (p.out_sums) {
+    hs = pair_sum(hs);
+    if (live && h2 == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
+  }
+}
+
+// A workgroup takes a bin's items for one kv head, one after the other.
+template <bool TREE, int WAVES, int RING>
+__global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
+  constexpr int ROWS = 32 * WAVES;             // pairs of a tile
   extern __shared__ __align__(256) uint16_t s_kv[];   // [RING][K, V][key][dim]
 
   const int h = blockIdx.x % p.Hkv;
@@ -429,7 +678,6 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 31, h2 = lane >> 5;
 
   int at = 0, end = 0;          // packed: items; trees: key blocks of the whole batch
   TreeWalk walk;
@@ -461,228 +709,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
       it.kb1 = min(it.kb1, (it.kend + RG_KEYS - 1) / RG_KEYS);
     }
 
-    // ---- K / V staging: a wave's instruction moves 4 keys (1 KB); 4 each of K and V a block ----
-    const size_t cache_base = ((size_t)it.crow * p.Hkv + h) * (size_t)p.cap * D;
-    const int srow = lane >> 4;                              // key within the instruction's four
-    const int place = lane & 15;                             // where the lane's 16 bytes go in the key's row
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(rg_lds_address(s_kv) + wave * WKEYS * D * 2);
-    constexpr int LOADS = WKEYS / 4;                         // instructions of a wave for K, and for V
-    uint32_t kat[LOADS], vat[LOADS];                         // what the lane loads: byte in the block, less 1024 i
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      kat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ ((wave * WKEYS + 4 * i + srow) & 15));
-      vat[i] = (wave * WKEYS + srow) * (D * 2) + 16 * (place ^ (4 * srow));
-    }
-    const i32x4 krsrc = keys_rsrc(p.kc + cache_base), vrsrc = keys_rsrc(p.vc + cache_base);
-    // K and V block kb into its buffer
-    auto stage = [&](int kb) __attribute__((always_inline)) {
-      const uint32_t lds = lds0 + ((kb - it.kb0) & (RING - 1)) * (4 * RG_KEYS * D);
-      if ((kb + 1) * RG_KEYS <= it.kend) {
-        const uint32_t at = (uint32_t)kb * (RG_KEYS * D * 2);
-        if (it.pairs <= ROWS) {                              // the sequence's only tile: its keys are read once
-          lds_load_keys<true>(krsrc, kat, at, lds);
-          lds_load_keys<true>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
-        } else {
-          lds_load_keys<false>(krsrc, kat, at, lds);
-          lds_load_keys<false>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-          const int at = wave * WKEYS + 4 * i + srow;
-          const uint32_t key = (uint32_t)min(kb * RG_KEYS + at, it.kend - 1) * (D * 2);
-          lds_load16(krsrc, key + 16 * (place ^ (at & 15)), lds + i * 4 * D * 2);
-          lds_load16(vrsrc, key + 16 * (place ^ (4 * srow)), lds + 2 * RG_KEYS * D + i * 4 * D * 2);
-        }
-      }
-    };
-#pragma unroll
-    for (int s = 0; s < RING - 1; ++s)
-      if (it.kb0 + s < it.kb1) stage(it.kb0 + s);
-
-    // ---- this lane's pair, and its q row as the B operand ----
-    const int j = it.j0 + wave * 32 + c;
-    const bool wave_on = it.j0 + wave * 32 < it.pairs;       // some pair of the wave exists
-    const int jj = min(j, it.pairs - 1);
-    const int t = jj / p.G;
-    const int head = h * p.G + (jj - t * p.G);
-    const size_t qrow = (size_t)it.row0 + t;
-    u32x4 qb[8];
-    {
-      const uint16_t* src = p.q + (qrow * p.Hq + head) * D + 8 * h2;
-#pragma unroll
-      for (int ks = 0; ks < 8; ++ks) qb[ks] = *reinterpret_cast<const u32x4*>(src + 16 * ks);
-    }
-    // positions of the wave's rows: first and last (wave-uniform), this lane's
-    const int t_first = (it.j0 + wave * 32) / p.G;
-    const int t_last = (min(it.j0 + wave * 32 + 32, it.pairs) - 1) / p.G;
-    const int qpos = it.start + t;
-    const int mask_from = TREE ? it.start : it.start + t_first + 1;   // keys below it are seen by every row
-    const int wave_end = TREE ? it.kend : it.start + t_last + 1;      // keys from it on by none
-    uint32_t seen_lo = 0, seen_hi = 0;                       // tree: the nodes that the lane's node attends
-    if (TREE && it.kb1 * RG_KEYS > it.start && it.kb0 < it.kb1) {
-      int depth;
-      const unsigned long long own = 1ull << lane;
-      const unsigned long long s = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane), lane, depth) | own;
-      seen_lo = __shfl((uint32_t)s, t, 64);
-      seen_hi = __shfl((uint32_t)(s >> 32), t, 64);
-    }
-
-    float m = -INFINITY, mref = 0.0f, l = 0.0f;              // mref: m, or 0 while m is -inf; l: of this lane's keys
-    f32x16 o[4];
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
-
-    // LDS offsets (elements): K row c of a 32-key tile, V rows by transposing reads
-    const int kx = c & 15;
-    const int vi = lane & 15, vrow = 4 * h2 + (vi >> 2);     // key of the 8 that the lane's read names
-    const int vcol = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);   // its 16-byte chunk within a 32-dim tile
-
-    for (int kb = it.kb0; kb < it.kb1; ++kb) {
-      // this block is here (2 LOADS of each later one may be on their way; the first wait of an
-      // item, behind other kinds of memory operations, is for everything), and the buffer of the
-      // block before it is free
-      const int later = min(RING - 2, it.kb1 - 1 - kb);
-      if (RING > 3 && later == 2 && kb > it.kb0) loads_barrier<4 * LOADS>();
-      else if (RING > 2 && later == 1 && kb > it.kb0) loads_barrier<2 * LOADS>();
-      else loads_done_barrier();
-      if (kb + RING - 1 < it.kb1) stage(kb + RING - 1);
-      if (!wave_on || kb * RG_KEYS >= wave_end) continue;
-      const uint16_t* const bk = s_kv + ((kb - it.kb0) & (RING - 1)) * (2 * RG_KEYS * D);
-      const uint16_t* const bv = bk + RG_KEYS * D;
-      // ---- S^T = K Q^T ----
-      f32x16 s[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const u32x4 ka = *reinterpret_cast<const u32x4*>(bk + (32 * n + c) * D + ((2 * ks + h2) ^ kx) * 8);
-          s[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ka),
-                                                         __builtin_bit_cast(bf16x8, qb[ks]), s[n], 0, 0, 0);
-        }
-      }
-      // ---- masks, only on blocks that some row does not see whole ----
-      if (kb * RG_KEYS + RG_KEYS > mask_from) {
-        if (TREE) {
-          const int rel = kb * RG_KEYS - it.start;           // node of the block's first key (negative: a context slot)
-          const unsigned long long w = (unsigned long long)seen_hi << 32 | seen_lo;
-          unsigned long long bm = rel >= 64 ? 0ull : rel >= 0 ? w >> rel : (w << -rel) | ((1ull << -rel) - 1);
-          bm >>= 4 * h2;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (!((uint32_t)(bm >> (32 * n)) & (1u << (8 * (i / 4) + i % 4)))) s[n][i] = -INFINITY;
-        } else {
-          const int rel = qpos - kb * RG_KEYS - 4 * h2;
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (32 * n + 8 * (i / 4) + i % 4 > rel) s[n][i] = -INFINITY;
-        }
-      }
-      // ---- online softmax (log2 domain) ----
-      float mx = fmaxf(s[0][0], s[1][0]);
-#pragma unroll
-      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
-      mx = pair_max(mx) * p.scale_log2;
-      if (__any(mx > m + 8.0f)) {
-        const float mn = fmaxf(m, mx);
-        const float f = m > -INFINITY ? exp2_fast(m - mn) : 0.0f;
-        l *= f;
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[dt][i] *= f;
-        m = mn;
-        mref = mn > -INFINITY ? mn : 0.0f;
-      }
-      uint32_t pw[2][8];                                     // bf16 weights, two keys a word
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          const uint32_t w = pack_bf16x2(exp2_fast(fmaf(s[n][i], p.scale_log2, -mref)),
-                                         exp2_fast(fmaf(s[n][i + 1], p.scale_log2, -mref)));
-          pw[n][i / 2] = w;
-          l = dot2_bf16(w, 0x3F803F80u, l);                  // the rounded weights
-        }
-      // ---- O^T += V^T P^T ----
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const uint32_t* const w = pw[u / 2] + 4 * (u % 2);
-        const u32x4 pb = u32x4{w[0], w[1], w[2], w[3]};
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
-          const uint16_t* const v = bv + (16 * u + vrow) * D + ((4 * dt + vcol) ^ (4 * (vi >> 2))) * 8 + 4 * (vi & 1);
-          typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
-          const i16x4 a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v));
-          const i16x4 a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(v + 8 * D));
-          const u32x2 b0 = __builtin_bit_cast(u32x2, a0), b1 = __builtin_bit_cast(u32x2, a1);
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, u32x4{b0.x, b0.y, b1.x, b1.y}),
-                                                          __builtin_bit_cast(bf16x8, pb), o[dt], 0, 0, 0);
-        }
-      }
-    }
-
-    // the buffers are free for the next item
-    if (at < end) loads_done_barrier();
-    // ---- outputs: register i of o[dt] is dim 32 dt + 8 (i / 4) + 4 h2 + i % 4 of the lane's pair ----
-    if (!wave_on) continue;
-    l = pair_sum(l);
-    // A weight of 0 times an infinity or a NaN in V is a NaN: a row whose sums are not finite is
-    // formed again from the keys that it attends alone, so that what a mask hides stays hidden.
-    float finite = 0.0f * l;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) finite = fmaf(0.0f, o[dt][i], finite);
-    const unsigned long long odd = __ballot(finite != finite);
-    const uint32_t again = (uint32_t)(odd | odd >> 32);       // bit c: the pair of lanes c and c + 32
-    if (again) exact_rows<TREE>(p, it, h, it.j0 + wave * 32, again, lane);
-    const bool live = j < it.pairs && !(again >> c & 1);
-    if (it.part >= 0) {
-      const size_t st = ((size_t)it.part * p.Hkv + h) * p.part_rows + wave * 32 + c;
-      m = l != l ? INFINITY : m;                             // a row that saw a NaN stays one in the merge
-      if (live && h2 == 0) p.part_ml[st] = float2{m, l};
-      if (live && m > -INFINITY) {                           // else its outputs are not read
-        float* dst = p.part_o + st * D + 4 * h2;
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
-      }
-      continue;
-    }
-    const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);   // nothing attended: a zero row; NaN stays
-    uint16_t* const dst = p.out + (qrow * p.Hq + head) * D + 8 * h2;
-    float hs = 0.0f;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
-#pragma unroll
-      for (int g = 0; g < 4; g += 2) {
-        uint32_t x[2], y[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          x[e] = pack_bf16x2(o[dt][4 * g + 2 * e] * inv, o[dt][4 * g + 2 * e + 1] * inv);
-          y[e] = pack_bf16x2(o[dt][4 * g + 4 + 2 * e] * inv, o[dt][4 * g + 5 + 2 * e] * inv);
-          hs += (bf16_lo(x[e]) + bf16_hi(x[e])) + (bf16_lo(y[e]) + bf16_hi(y[e]));
-        }
-        // lanes trade halves: each ends up with 8 neighbouring dims
-        const auto a = __builtin_amdgcn_permlane32_swap(x[0], y[0], false, false);
-        const auto b = __builtin_amdgcn_permlane32_swap(x[1], y[1], false, false);
-        if (live) *reinterpret_cast<u32x4*>(dst + 32 * dt + 8 * g) = u32x4{a[0], b[0], a[1], b[1]};
-      }
-    if (p.out_sums) {
-      hs = pair_sum(hs);
-      if (live && h2 == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
-    }
+    if (TREE || it.rows == 1) attend_item<TREE, WAVES, RING, true>(p, it, h, s_kv, lane, wave, at < end);
+    else attend_item<TREE, WAVES, RING, false>(p, it, h, s_kv, lane, wave, at < end);
   }
 }
 

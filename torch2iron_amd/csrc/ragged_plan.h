@@ -36,9 +36,12 @@ inline int tile_blocks(int64_t j0, int64_t pairs, int G, int start) {
 // Times in us that the choice below goes by, fitted to graph-launched calls (1 to 64 sequences, 1 to
 // 4000 rows, 0 to 6000 slots before them, 8 kv heads of 2 and 4 q heads): a key block of a
 // workgroup that has its CU alone, and its share of a CU that two workgroups fill; tiles of up
-// to 32 pairs (one wave of four multiplies) wait for their loads longer.
+// to 32 pairs (one wave of four multiplies) wait for their loads longer, and the single row of a
+// sequence takes half as many products again.
 struct BlockTime { double alone, shared; };
-inline BlockTime block_time(int64_t pairs) { return pairs > 32 ? BlockTime{1.35, 1.1} : BlockTime{1.75, 1.35}; }
+inline BlockTime block_time(int64_t pairs, bool single_row) {
+  return pairs > 32 ? BlockTime{1.35, 1.1} : single_row ? BlockTime{1.95, 1.45} : BlockTime{1.75, 1.35};
+}
 constexpr double RG_CUS = 256, ITEM_TIME = 2.5;       // ITEM_TIME: first loads and outputs
 constexpr double CALL_TIME = 4, MERGE_TIME = 5;       // MERGE_TIME: a second launch
 constexpr double PART_BYTES_PER_US = 1e7;             // parts written and read again
@@ -74,7 +77,7 @@ inline PackedTable packed_items(const int32_t* lengths, const int32_t* starts, c
     const int64_t pairs = (int64_t)lengths[i] * G;
     for (int64_t j0 = 0; j0 < pairs; j0 += RG_ROWS) {
       const int64_t live = std::min<int64_t>(pairs - j0, RG_ROWS);
-      tiles.push_back({i, (int32_t)row0, j0, live, tile_blocks(j0, pairs, G, starts[i]), block_time(live)});
+      tiles.push_back({i, (int32_t)row0, j0, live, tile_blocks(j0, pairs, G, starts[i]), block_time(live, lengths[i] == 1)});
       work += tiles.back().blocks * tiles.back().time.shared;
       longest = std::max(longest, tiles.back().blocks * tiles.back().time.alone);
     }
