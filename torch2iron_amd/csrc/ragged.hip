@@ -269,6 +269,10 @@ template <int N>
 __device__ __forceinline__ void loads_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
 }
+// Until every LDS operation of this wave is done, and every wave is here.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 // Until every vector memory operation of this wave is done, and every wave is here.
 __device__ __forceinline__ void loads_done_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -329,62 +333,6 @@ __device__ __forceinline__ float pair_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
-// Which keys row t of a sequence attends; the tree's nodes above its own as a mask.
-template <bool TREE>
-__device__ __forceinline__ bool attends(const RaggedItem& it, int t, unsigned long long seen, int key) {
-  if (!TREE) return key <= it.start + t;
-  return key < it.start || (seen >> (key - it.start) & 1);
-}
-
-// The item's outputs for the pairs j0 + bit of `rows`, a wave a pair after the other, lane e dims
-// 2 e and 2 e + 1: the definition key by key, for rows that hold infinities or NaN.
-template <bool TREE, bool FINE>
-__device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const RaggedItem& it, int h, int j0, uint32_t rows,
-                                           int lane) {
-  constexpr int D = RG_D;
-  const size_t base = ((size_t)it.crow * p.Hkv + h) * (size_t)p.cap * D + 2 * lane;
-  unsigned long long all = 0;
-  if (TREE) {
-    int depth;
-    all = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane), lane, depth) | 1ull << lane;
-  }
-  for (; rows; rows &= rows - 1) {
-    const int j = j0 + __builtin_ctz(rows);
-    if (j >= it.pairs) break;
-    const int t = j / p.G, head = h * p.G + (j - t * p.G);
-    const size_t qrow = (size_t)it.row0 + t;
-    const unsigned long long seen = TREE ? (unsigned long long)(uint32_t)__shfl((uint32_t)(all >> 32), t, 64) << 32 |
-                                               (uint32_t)__shfl((uint32_t)all, t, 64) : 0;
-    const uint32_t q = *reinterpret_cast<const uint32_t*>(p.q + (qrow * p.Hq + head) * D + 2 * lane);
-    float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-    for (int key = it.kb0 * RG_KEYS; key < min(it.kb1 * RG_KEYS, it.kend); ++key) {
-      if (!attends<TREE>(it, t, seen, key)) continue;       // uniform
-      const uint32_t k = *reinterpret_cast<const uint32_t*>(p.kc + base + (size_t)key * D);
-      const uint32_t v = *reinterpret_cast<const uint32_t*>(p.vc + base + (size_t)key * D);
-      const float s = wave_sum(bf16_lo(q) * bf16_lo(k) + bf16_hi(q) * bf16_hi(k)) * p.scale_log2;
-      const float mn = fmaxf(m, s), f = state_weight(m, mn);
-      const float e = exp2_fast(s - (mn > -INFINITY ? mn : 0.0f)), w = FINE ? e : round_bf16(e);
-      l = l * f + w;
-      o0 = o0 * f + w * bf16_lo(v);
-      o1 = o1 * f + w * bf16_hi(v);
-      m = mn;
-    }
-    if (it.part >= 0) {
-      const size_t st = ((size_t)it.part * p.Hkv + h) * p.part_rows + (j - it.j0);
-      if (lane == 0) p.part_ml[st] = float2{l != l ? INFINITY : m, l};
-      *reinterpret_cast<float2*>(p.part_o + st * D + 2 * lane) = float2{o0, o1};
-    } else {
-      const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-      const uint32_t w = pack_bf16x2(o0 * inv, o1 * inv);
-      *reinterpret_cast<uint32_t*>(p.out + (qrow * p.Hq + head) * D + 2 * lane) = w;
-      if (p.out_sums) {
-        const float hs = wave_sum(bf16_lo(w) + bf16_hi(w));
-        if (lane == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
-      }
-    }
-  }
-}
-
 // An item of a workgroup of WAVES waves of 32 pairs, for one kv head.  All products run transposed
 // on the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32, h2 = lane / 32) holds one pair's scores
 // and outputs:
@@ -403,6 +351,11 @@ __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const Ragg
 // (16 x 26 nodes 47.2 -> 49.8 us, 8 x 64 nodes over 32k slots 265 -> 323, 16 single rows 33.1 -> 34.2); prompt
 // rows round their weights once, as the batch form of the prompt pass does (8001 rows: 517 us,
 // with FINE 713).
+// In an MFMA a weight of 0 times an infinity or a NaN in V is a NaN, also for rows whose mask hides that
+// key.  An item with sums that are not finite is therefore run again, MASKED: blocks that some row does not
+// see whole (FINE: any) and whose V holds such a value are multiplied key by key for the rows that attend it.  (500
+// rows from 1500, 16 / 8 heads, without such values 32 us, with a NaN in the last slot 76, in the first 46;
+// 1624 and 2384 where such rows were formed again from all of their keys.)
 // K and V blocks go straight from memory into LDS, RING buffers, one barrier a block; a row's
 // 16-byte chunk ch stands at place ch ^ (row % 16) (K) or ch ^ 4 (row % 4) (V): 16 neighbouring
 // lanes of a K read, 32 of a transposing read cover all banks (a load into LDS cannot pad rows,
@@ -423,9 +376,10 @@ __device__ __forceinline__ void exact_rows(const RaggedAttnParams& p, const Ragg
 // Measured and dropped: one half's softmax beside the other half's products (8 % slower), priorities
 // around the products (1-3 %), scheduling groups and iglp (0-4 %), two waves sharing the blocks of a
 // tile of up to 32 pairs (single rows 5 % faster, everything else 3-8 % slower: registers).
-template <bool TREE, int WAVES, int RING, bool FINE>
-__device__ __forceinline__ void attend_item(const RaggedAttnParams& p, const RaggedItem& it, int h, uint16_t* s_kv, int lane,
-                                            int wave, bool more) {
+// Returns the wave's pairs (bit c) whose sums are not finite, which were not written; MASKED: writes `only` those.
+template <bool TREE, int WAVES, int RING, bool FINE, bool MASKED>
+__device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const RaggedItem& it, int h, uint16_t* s_kv, int lane,
+                                                int wave, uint32_t only) {
   constexpr int D = RG_D;
   constexpr int ROWS = 32 * WAVES;             // pairs of a tile
   constexpr int WKEYS = RG_KEYS / WAVES;       // keys of a block that a wave loads
@@ -472,7 +426,7 @@ __device__ __forceinline__ void attend_item(const RaggedAttnParams& p, const Rag
 
   // ---- this lane's pair, and its q row as the B operand ----
   const int j = it.j0 + wave * 32 + c;
-  const bool wave_on = it.j0 + wave * 32 < it.pairs;       // some pair of the wave exists
+  const bool wave_on = it.j0 + wave * 32 < it.pairs && (!MASKED || only);   // some pair of the wave is to be done
   const int jj = min(j, it.pairs - 1);
   const int t = jj / p.G;
   const int head = h * p.G + (jj - t * p.G);
@@ -561,7 +515,7 @@ __device__ __forceinline__ void attend_item(const RaggedAttnParams& p, const Rag
 #pragma unroll
     for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
     mx = pair_max(mx) * p.scale_log2;
-    if (__any(mx > m + 8.0f)) {
+    if (__any(mx > m + (MASKED ? 0.0f : 8.0f))) {          // MASKED: no weight above 1, sums of huge values fit
       const float mn = fmaxf(m, mx);
       const float f = m > -INFINITY ? exp2_fast(m - mn) : 0.0f;
       l *= f;
@@ -571,6 +525,50 @@ __device__ __forceinline__ void attend_item(const RaggedAttnParams& p, const Rag
         for (int i = 0; i < 16; ++i) o[dt][i] *= f;
       m = mn;
       mref = mn > -INFINITY ? mn : 0.0f;
+    }
+    // ---- MASKED: where V holds an infinity or a NaN, key by key for the rows that attend it ----
+    if constexpr (MASKED) {
+      if (FINE || kb * RG_KEYS + RG_KEYS > mask_from) {    // FINE: a second word may be 0 or negative
+        bool odd = false;
+#pragma unroll 4
+        for (int i = 0; i < RG_KEYS / 4; ++i) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(bv + 4 * i * D + 8 * lane);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) odd |= (x[e] & 0x7F80u) == 0x7F80u || (x[e] & 0x7F800000u) == 0x7F800000u;
+        }
+        if (__any(odd)) {
+          const uint32_t unseen = __float_as_uint(-1.0f);  // no weight
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll 1
+            for (int i = 0; i < 16; ++i) {
+              const float x = s[n][i], e = exp2_fast(fmaf(x, p.scale_log2, -mref));
+              const uint32_t w = x == -INFINITY ? unseen : __float_as_uint(FINE ? e : round_bf16(e));
+              l += w == unseen ? 0.0f : __uint_as_float(w);
+              const auto two = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+#pragma unroll 1
+              for (int half = 0; half < 2; ++half) {
+                const uint32_t wk = half ? two[1] : two[0], sees = wk == unseen ? 0u : ~0u;
+                const float weight = __uint_as_float(wk & sees);
+                const int key = 32 * n + 8 * (i / 4) + 4 * half + i % 4;
+                const uint16_t* const v = bv + key * D + 4 * h2;
+#pragma unroll
+                for (int dt = 0; dt < 4; ++dt) {
+                  __builtin_amdgcn_sched_barrier(0);       // a few reads at a time: registers
+#pragma unroll
+                  for (int g = 0; g < 4; ++g) {
+                    const u32x2 y = *reinterpret_cast<const u32x2*>(v + ((4 * dt + g) ^ (4 * (key & 3))) * 8) & sees;
+                    o[dt][4 * g] = fmaf(weight, bf16_lo(y.x), o[dt][4 * g]);
+                    o[dt][4 * g + 1] = fmaf(weight, bf16_hi(y.x), o[dt][4 * g + 1]);
+                    o[dt][4 * g + 2] = fmaf(weight, bf16_lo(y.y), o[dt][4 * g + 2]);
+                    o[dt][4 * g + 3] = fmaf(weight, bf16_hi(y.y), o[dt][4 * g + 3]);
+                  }
+                }
+              }
+            }
+          continue;
+        }
+      }
     }
     uint32_t pw[2][8], pr[2][8];                           // bf16 weights, two keys a word; what their rounding left
 #pragma unroll
@@ -611,22 +609,19 @@ __device__ __forceinline__ void attend_item(const RaggedAttnParams& p, const Rag
     }
   }
 
-  // the buffers are free for the next item
-  if (more) loads_done_barrier();
   // ---- outputs: register i of o[dt] is dim 32 dt + 8 (i / 4) + 4 h2 + i % 4 of the lane's pair ----
-  if (!wave_on) return;
+  if (!wave_on) return 0;
   l = pair_sum(l);
-  // A weight of 0 times an infinity or a NaN in V is a NaN: a row whose sums are not finite is
-  // formed again from the keys that it attends alone, so that what a mask hides stays hidden.
-  float finite = 0.0f * l;
+  if constexpr (!MASKED) {
+    float finite = 0.0f * l;
 #pragma unroll
-  for (int dt = 0; dt < 4; ++dt)
+    for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) finite = fmaf(0.0f, o[dt][i], finite);
-  const unsigned long long odd = __ballot(finite != finite);
-  const uint32_t again = (uint32_t)(odd | odd >> 32);       // bit c: the pair of lanes c and c + 32
-  if (again) exact_rows<TREE, FINE>(p, it, h, it.j0 + wave * 32, again, lane);
-  const bool live = j < it.pairs && !(again >> c & 1);
+      for (int i = 0; i < 16; ++i) finite = fmaf(0.0f, o[dt][i], finite);
+    const unsigned long long odd = __ballot(finite != finite);
+    only = (uint32_t)(odd | odd >> 32);                    // bit c: the pair of lanes c and c + 32
+  }
+  const bool live = j < it.pairs && (only >> c & 1) == MASKED;
   if (it.part >= 0) {
     const size_t st = ((size_t)it.part * p.Hkv + h) * p.part_rows + wave * 32 + c;
     m = l != l ? INFINITY : m;                             // a row that saw a NaN stays one in the merge
@@ -639,7 +634,7 @@ __device__ __forceinline__ void attend_item(const RaggedAttnParams& p, const Rag
         for (int g = 0; g < 4; ++g)
           *reinterpret_cast<f32x4*>(dst + 32 * dt + 8 * g) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
     }
-    return;
+    return only;
   }
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);   // nothing attended: a zero row; NaN stays
   uint16_t* const dst = p.out + (qrow * p.Hq + head) * D + 8 * h2;
@@ -664,6 +659,7 @@ __device__ __forceinline__ void attend_item(const RaggedAttnParams& p, const Rag
     hs = pair_sum(hs);
     if (live && h2 == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
   }
+  return only;
 }
 
 // A workgroup takes a bin's items for one kv head, one after the other.
@@ -671,6 +667,7 @@ template <bool TREE, int WAVES, int RING>
 __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
   constexpr int ROWS = 32 * WAVES;             // pairs of a tile
   extern __shared__ __align__(256) uint16_t s_kv[];   // [RING][K, V][key][dim]
+  __shared__ uint32_t s_odd[WAVES];                   // an item's pairs whose sums are not finite
 
   const int h = blockIdx.x % p.Hkv;
   const int tile = TREE ? blockIdx.x / p.Hkv % p.tiles : 0;
@@ -709,8 +706,21 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
       it.kb1 = min(it.kb1, (it.kend + RG_KEYS - 1) / RG_KEYS);
     }
 
-    if (TREE || it.rows == 1) attend_item<TREE, WAVES, RING, true>(p, it, h, s_kv, lane, wave, at < end);
-    else attend_item<TREE, WAVES, RING, false>(p, it, h, s_kv, lane, wave, at < end);
+    const auto run = [&](auto fine) __attribute__((always_inline)) {
+      constexpr bool FINE = decltype(fine)::value;
+      const uint32_t odd = attend_item<TREE, WAVES, RING, FINE, false>(p, it, h, s_kv, lane, wave, 0);
+      if (it.kb0 >= it.kb1) return;
+      if (lane == 0) s_odd[wave] = odd;
+      lds_barrier();                                         // the buffers are free
+      uint32_t any = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) any |= s_odd[w];
+      if (!__builtin_amdgcn_readfirstlane(any)) return;
+      (void)attend_item<TREE, WAVES, RING, FINE, true>(p, it, h, s_kv, lane, wave, odd);
+      lds_barrier();
+    };
+    if (TREE || it.rows == 1) run(std::true_type{});
+    else run(std::false_type{});
   }
 }
 
