@@ -909,26 +909,27 @@ void* set_parts(t2i::RaggedAttnParams& p, void* ws, long long parts, int32_t row
 }
 
 // The kernel's forms: 4 waves (128 pairs a tile, two workgroups a CU, the next block on its
-// way) and 8 waves (256 pairs, one workgroup a CU, three blocks on their way).
+// way) and, for trees alone, 8 waves (256 pairs, one workgroup a CU, three blocks on their way).
 constexpr int lds_bytes(int ring) { return ring * 2 * t2i::RG_KEYS * t2i::RG_D * 2; }
 
 template <bool TREE>
-int launch_attention(const t2i::RaggedAttnParams& p, long long groups, hipStream_t s) {
-  if (p.tile_rows == 128) {
-    hipLaunchKernelGGL((t2i::ragged_attention_kernel<TREE, 4, 2>), dim3(groups), dim3(256), lds_bytes(2), s, p);
-  } else {
-    // more than 64 KB of LDS: asked for once a device (twice does no harm)
-    static std::atomic<bool> done[64];
-    int dev = 0;
-    if (int rc = t2i_host::hip_status(hipGetDevice(&dev), "device query")) return rc;
-    if (dev < 0 || dev >= 64 || !done[dev]) {
-      if (int rc = t2i_host::hip_status(hipFuncSetAttribute(reinterpret_cast<const void*>(&t2i::ragged_attention_kernel<TREE, 8, 4>),
-                                                            hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes(4)), "LDS attribute"))
-        return rc;
-      if (dev >= 0 && dev < 64) done[dev] = true;
-    }
-    hipLaunchKernelGGL((t2i::ragged_attention_kernel<TREE, 8, 4>), dim3(groups), dim3(512), lds_bytes(4), s, p);
+int launch_narrow(const t2i::RaggedAttnParams& p, long long groups, hipStream_t s) {
+  hipLaunchKernelGGL((t2i::ragged_attention_kernel<TREE, 4, 2>), dim3(groups), dim3(256), lds_bytes(2), s, p);
+  return t2i_host::hip_status(hipGetLastError(), "ragged attention launch");
+}
+
+int launch_wide_tree(const t2i::RaggedAttnParams& p, long long groups, hipStream_t s) {
+  // more than 64 KB of LDS: asked for once a device (twice does no harm)
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  if (int rc = t2i_host::hip_status(hipGetDevice(&dev), "device query")) return rc;
+  if (dev < 0 || dev >= 64 || !done[dev]) {
+    if (int rc = t2i_host::hip_status(hipFuncSetAttribute(reinterpret_cast<const void*>(&t2i::ragged_attention_kernel<true, 8, 4>),
+                                                          hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes(4)), "LDS attribute"))
+      return rc;
+    if (dev >= 0 && dev < 64) done[dev] = true;
   }
+  hipLaunchKernelGGL((t2i::ragged_attention_kernel<true, 8, 4>), dim3(groups), dim3(512), lds_bytes(4), s, p);
   return t2i_host::hip_status(hipGetLastError(), "ragged attention launch");
 }
 
@@ -1044,18 +1045,16 @@ extern "C" int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32
   if (!aligned4(items) || !aligned4(merges) || !aligned4(bins) || !aligned4(out_sums))
     return fail(T2I_ERR_ALIGN, "tables and out_sums must be 4-byte aligned");
   const size_t need = part_bytes(n_parts, Hkv, t2i_host::RG_ROWS);
-  const int tile_rows = t2i_host::RG_ROWS;
   if (need && (!workspace || workspace_bytes < need)) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
   if (need && !aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
   t2i::RaggedAttnParams p{};
   p.q = q; p.kc = k_cache; p.vc = v_cache; p.out = out; p.out_sums = out_sums; p.items = items; p.bins = bins;
-  p.tile_rows = tile_rows;
   p.rows = rows; p.n_cache = n_cache_rows; p.n_items = n_items; p.n_bins = n_bins; p.n_parts = n_parts;
   p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
   if (need) set_parts(p, workspace, n_parts, t2i_host::RG_ROWS);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (int rc = launch_attention<false>(p, (long long)n_bins * Hkv, s)) return rc;
+  if (int rc = launch_narrow<false>(p, (long long)n_bins * Hkv, s)) return rc;
   if (!need) return T2I_OK;
   p.items = merges;
   hipLaunchKernelGGL(t2i::ragged_merge_kernel<false>, dim3(n_merges * Hkv), dim3(256), 0, s, p);
@@ -1108,7 +1107,8 @@ extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, con
   if (!aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
   p.cuts = reinterpret_cast<int2*>(set_parts(p, workspace, 2LL * t.bins * t.tiles, t.rows));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (int rc = launch_attention<true>(p, (long long)t.bins * t.tiles * Hkv, s)) return rc;
+  const long long groups = (long long)t.bins * t.tiles * Hkv;
+  if (int rc = t.tile_rows == 128 ? launch_narrow<true>(p, groups, s) : launch_wide_tree(p, groups, s)) return rc;
   hipLaunchKernelGGL(t2i::ragged_merge_kernel<true>, dim3(B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS)), dim3(256), 0, s, p);
   return t2i_host::hip_status(hipGetLastError(), "tree attention merge launch");
 }
