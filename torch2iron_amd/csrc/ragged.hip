@@ -41,21 +41,19 @@ __device__ __forceinline__ int tree_parent(const int32_t* parents, int N, int la
   return p >= 0 && p < lane ? p : -1;
 }
 
-// Nodes above node `lane`, and their number, by doubling the steps: after k rounds a lane
+// Nodes above the lane's node, whose parent is p, by doubling the steps: after k rounds a lane
 // knows the nodes up to 2^k steps above it, and the one that stands there.
-__device__ __forceinline__ unsigned long long tree_above(int p, int lane, int& depth) {
+__device__ __forceinline__ unsigned long long tree_above(int p) {
   uint32_t lo = 0, hi = 0;
   if (p >= 0) (p < 32 ? lo : hi) = 1u << (p & 31);
-  depth = p >= 0 ? 1 : 0;
 #pragma unroll
   for (int k = 0; k < 6; ++k) {
     const int at = max(p, 0);
     const uint32_t l = __shfl(lo, at, 64), h = __shfl(hi, at, 64);
-    const int d = __shfl(depth, at, 64), q = __shfl(p, at, 64);
+    const int q = __shfl(p, at, 64);
     if (p >= 0) {
       lo |= l;
       hi |= h;
-      depth += d;
       p = q;
     }
   }
@@ -445,9 +443,8 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
   const int wave_end = TREE ? it.kend : it.start + t_last + 1;      // keys from it on by none
   uint32_t seen_lo = 0, seen_hi = 0;                       // tree: the nodes that the lane's node attends
   if (TREE && it.kb1 * RG_KEYS > it.start && it.kb0 < it.kb1) {
-    int depth;
     const unsigned long long own = 1ull << lane;
-    const unsigned long long s = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane), lane, depth) | own;
+    const unsigned long long s = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane)) | own;
     seen_lo = __shfl((uint32_t)s, t, 64);
     seen_hi = __shfl((uint32_t)(s >> 32), t, 64);
   }
