@@ -536,8 +536,9 @@ int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32_t* items, 
  * slots and a tree of node_counts[b] nodes (NULL: N; at most N <= 64): node i hangs from
  * node parents[b][i] < i (anything else makes it a root), stands in slot
  * context + i and has position context + its depth.  Arrays of nodes are [B, N]; entries
- * behind a sequence's count are neither read nor written.  A sequence whose context
- * is negative or whose nodes pass ctx_cap writes no slot; its attention rows are zero.
+ * behind a sequence's count must be readable but count for nothing, and of the outputs q_out, out
+ * and the caches those rows are left as they are (path is written whole).  A sequence whose
+ * context is negative or whose nodes pass ctx_cap writes no slot; its attention rows are zero.
  *
  * t2i_tree_qk_rope_kv: t2i_prefill_qk_rope_kv for the nodes; q_out bf16 [B, N, Hq, D].
  * t2i_tree_attention: node i attends the slots 0 .. context - 1, the nodes above it and

@@ -193,7 +193,7 @@ struct TreeWalk {
   __device__ __forceinline__ int blocks_of(const TreeSeq& t) const {
     return t.nodes == 0 ? 0 : t.ok ? (t.ctx + t.nodes + RG_KEYS - 1) / RG_KEYS : 1;
   }
-  // (32-bit products: the host keeps total below 2^23, n below 2^9)
+  // (32-bit products: the host keeps total below 2^23 and n at 2^9 or less, so that total n < 2^32)
   __device__ __forceinline__ int run_start(int i) const { return (int)((uint32_t)total * (uint32_t)i / (uint32_t)n); }
   // the run that holds block x
   __device__ __forceinline__ int run_of(int x) const { return (int)(((uint32_t)(x + 1) * (uint32_t)n - 1) / (uint32_t)total); }
