@@ -176,9 +176,8 @@ def stream_handle(device=None) -> int:
     """hipStream_t of torch's current stream on ``device``."""
     # torch's own raw accessor where the device is named: without the Stream object around the
     # handle a call takes 0.1 us in place of 2.0
-    index = getattr(device, "index", None)
-    if index is not None and _RAW_STREAM is not None:
-        return _RAW_STREAM(index)
+    if isinstance(device, torch.device) and device.index is not None and _RAW_STREAM is not None:
+        return _RAW_STREAM(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
