@@ -8,6 +8,8 @@ without synchronising.  Argument errors raise ``ValueError`` and HIP errors
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from torch2iron_amd import _lib
@@ -1032,6 +1034,14 @@ def _scratch(workspace: Workspace | None, key: str, nbytes: int, device):
     return workspace.get((key, size), size, device)
 
 
+def _integers(name: str, values) -> list:
+    """``values`` as Python integers; what is none (2.9) raises instead of being cut to one."""
+    try:
+        return [operator.index(x) for x in values]
+    except TypeError:
+        raise ValueError(f"{name} must be integers") from None
+
+
 class PackedPlan:
     """A batch of packed prompt rows: ``lengths[s]`` rows of sequence s (0: none), one
     sequence after the other, at cache slots ``starts[s] ..`` (0 by default) of cache row
@@ -1046,12 +1056,12 @@ class PackedPlan:
 
     def __init__(self, lengths, n_heads: int, n_kv_heads: int, ctx_cap: int, device, starts=None, cache_rows=None,
                  n_cache_rows: int | None = None):
-        lengths = [int(x) for x in lengths]
-        starts = [0] * len(lengths) if starts is None else [int(x) for x in starts]
+        lengths = _integers("lengths", lengths)
+        starts = [0] * len(lengths) if starts is None else _integers("starts", starts)
         if not lengths or len(starts) != len(lengths):
             raise ValueError("lengths must hold at least one sequence, and starts one entry for each")
         if cache_rows is not None:
-            cache_rows = [int(x) for x in cache_rows]
+            cache_rows = _integers("cache_rows", cache_rows)
             if len(cache_rows) != len(lengths):
                 raise ValueError("cache_rows must hold one entry for each sequence")
         if n_cache_rows is None:
