@@ -22,3 +22,12 @@ def test_integers_of_any_kind(make):
     plan = ops.PackedPlan(make([3, 0, 2]), 4, 2, 16, "cpu", starts=make([1, 2, 3]), cache_rows=make([2, 0, 1]))
     assert (plan.lengths, plan.starts, plan.cache_rows, plan.rows) == ([3, 0, 2], [1, 2, 3], [2, 0, 1], 5)
     assert all(type(x) is int for x in plan.lengths + plan.starts + plan.cache_rows)
+
+
+def test_plan_under_another_default_device():
+    """The plan is made in host memory whatever torch's default device: its entry point reads and writes it there
+    (a tensor on the default device has no host address)."""
+    want = ops.PackedPlan([40, 0, 3], 4, 2, 512, "cpu", starts=[0, 0, 500])
+    with torch.device("meta"):
+        plan = ops.PackedPlan([40, 0, 3], 4, 2, 512, "cpu", starts=[0, 0, 500])
+    assert plan.table.device.type == "cpu" and torch.equal(plan.table, want.table)

@@ -1076,12 +1076,13 @@ class PackedPlan:
         self.cache_rows = list(range(len(lengths))) if cache_rows is None else cache_rows
         self.n_heads, self.n_kv_heads, self.ctx_cap, self.n_cache_rows = n_heads, n_kv_heads, ctx_cap, n_cache_rows
         lib = _lib.load()
-        args = [torch.tensor(v, dtype=torch.int32) for v in (lengths, starts, self.cache_rows)]
-        sizes = torch.zeros(6, dtype=torch.int64)
+        # host memory, also where torch's default device is another
+        args = [torch.tensor(v, dtype=torch.int32, device="cpu") for v in (lengths, starts, self.cache_rows)]
+        sizes = torch.zeros(6, dtype=torch.int64, device="cpu")
         call = (*(a.data_ptr() for a in args), len(lengths), n_heads, n_kv_heads, n_cache_rows, ctx_cap)
         _lib.check(lib.t2i_packed_plan(*call, None, 0, sizes.data_ptr()), "t2i_packed_plan")
         self.rows, self.n_items, self.n_merges, self.n_parts, self.n_bins, words = sizes.tolist()
-        table = torch.empty(words, dtype=torch.int32)
+        table = torch.empty(words, dtype=torch.int32, device="cpu")
         _lib.check(lib.t2i_packed_plan(*call, table.data_ptr(), words, sizes.data_ptr()), "t2i_packed_plan")
         self.table = table.to(self.device)
         self._stream = _lib.stream_handle(self.device) if self.device.type == "cuda" else None
