@@ -400,7 +400,7 @@ extern "C" int t2i_token_logprobs(const void* logits, int32_t logits_type, int64
   if (((uintptr_t)logits % size) || (((uintptr_t)tokens | (uintptr_t)logprobs | (uintptr_t)entropy | (uintptr_t)top_logprobs | (uintptr_t)top_ids) & 3u))
     return fail(T2I_ERR_ALIGN, "token_logprobs arrays must be aligned to their values");
   const int splits = lp_splits(M, V);
-  if ((long long)M * splits > 0x7FFFFFFFLL) return fail(T2I_ERR_SHAPE, "M=%d exceeds the grid", M);
+  if ((long long)M * splits > 0xFFFFFFFFLL / t2i::LP_THREADS) return fail(T2I_ERR_SHAPE, "M=%d exceeds the grid", M);
   const size_t need = lp_bytes(M, splits, top_k);
   if (need && (!workspace || workspace_bytes < need)) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
   if (need && !t2i_host::aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");

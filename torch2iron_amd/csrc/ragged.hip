@@ -890,8 +890,9 @@ int check_heads(int32_t Hq, int32_t Hkv, int32_t D, int32_t cap) {
   return T2I_OK;
 }
 
-// Pairs, parts and workgroups stay below 2^31.
+// Pairs and parts stay below 2^31, the threads of a launch below 2^32.
 bool too_many(long long n) { return n > 0x7FFFFFFFLL; }
+bool past_grid(long long groups, int threads) { return groups > 0xFFFFFFFFLL / threads; }
 
 size_t part_bytes(long long parts, int32_t Hkv, int32_t rows) {
   return (size_t)parts * Hkv * rows * (t2i::RG_D * sizeof(float) + sizeof(float2));
@@ -1012,7 +1013,8 @@ extern "C" int t2i_packed_qk_rope_kv(const uint16_t* qkv, int32_t rows, const in
   if (!row_pos || !row_cache) return fail(T2I_ERR_NULL, "row_pos and row_cache must not be NULL");
   if (!aligned4(row_pos) || !aligned4(row_cache)) return fail(T2I_ERR_ALIGN, "row_pos and row_cache must be 4-byte aligned");
   if (int rc = check_heads(Hq, Hkv, D, ctx_cap)) return rc;
-  if (rows < 1 || n_cache_rows < 1) return fail(T2I_ERR_SHAPE, "rows=%d cache rows=%d invalid", rows, n_cache_rows);
+  if (rows < 1 || n_cache_rows < 1 || past_grid(rows, 256))
+    return fail(T2I_ERR_SHAPE, "rows=%d cache rows=%d invalid", rows, n_cache_rows);
   t2i::RaggedPrepParams p{};
   p.qkv = qkv; p.qn = q_norm; p.kn = k_norm; p.rope = rope; p.q = q_out; p.kc = k_cache; p.vc = v_cache;
   p.row_pos = row_pos; p.row_cache = row_cache; p.n_cache = n_cache_rows;
@@ -1035,7 +1037,7 @@ extern "C" int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32
   if (rows < 1 || n_cache_rows < 1 || n_items < 1 || n_bins < 1 || n_merges < 0 || n_parts < 0 ||
       (n_parts > 0 && (n_merges < 1 || !merges)))
     return fail(T2I_ERR_SHAPE, "rows=%d items=%d bins=%d merges=%d parts=%d invalid", rows, n_items, n_bins, n_merges, n_parts);
-  if (too_many((long long)n_bins * Hkv) || too_many((long long)n_merges * Hkv))
+  if (past_grid((long long)n_bins * Hkv, 256) || past_grid((long long)n_merges * Hkv, 256))
     return fail(T2I_ERR_SHAPE, "%d bins of %d kv heads exceed the grid", n_bins, Hkv);
   if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out))
     return fail(T2I_ERR_ALIGN, "packed attention tensors must be 16-byte aligned");
@@ -1066,7 +1068,7 @@ extern "C" int t2i_tree_qk_rope_kv(const uint16_t* qkv, const int32_t* parents, 
   if (int rc = check_prep(qkv, q_norm, k_norm, rope, q_out, k_cache, v_cache, eps, rope_style)) return rc;
   if (int rc = check_heads(Hq, Hkv, D, ctx_cap)) return rc;
   if (int rc = check_tree(parents, context_lens, node_counts, B, N, ctx_cap)) return rc;
-  if (too_many((long long)B * N)) return fail(T2I_ERR_SHAPE, "B=%d N=%d exceed the grid", B, N);
+  if (past_grid((long long)B * N, 256)) return fail(T2I_ERR_SHAPE, "B=%d N=%d exceed the grid", B, N);
   t2i::RaggedPrepParams p{};
   p.qkv = qkv; p.qn = q_norm; p.kn = k_norm; p.rope = rope; p.q = q_out; p.kc = k_cache; p.vc = v_cache;
   p.parents = parents; p.ctx = context_lens; p.counts = node_counts; p.N = N; p.n_cache = B;
@@ -1097,7 +1099,7 @@ extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, con
   p.tile_rows = t.tile_rows;
   p.n_bins = t.bins;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
-  if (too_many((long long)B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS)) || too_many((long long)B * N) ||
+  if (past_grid((long long)B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS), 256) || too_many((long long)B * N) ||
       (long long)B * ((ctx_cap + t2i::RG_KEYS - 1) / t2i::RG_KEYS) >= 1 << 23)
     return fail(T2I_ERR_SHAPE, "B=%d N=%d Hkv=%d over %d slots are too many", B, N, Hkv, ctx_cap);
   if (!workspace || workspace_bytes < t.bytes) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, t.bytes);
@@ -1119,7 +1121,7 @@ extern "C" int t2i_tree_commit(const int32_t* tokens, const int32_t* parents, co
     return fail(T2I_ERR_NULL, "tree commit pointers must not be NULL");
   if (int rc = check_heads(Hkv, Hkv, D, ctx_cap)) return rc;
   if (int rc = check_tree(parents, context_lens, node_counts, B, N, ctx_cap)) return rc;
-  if (layers < 1 || too_many((long long)layers * B * Hkv)) return fail(T2I_ERR_SHAPE, "layers=%d invalid", layers);
+  if (layers < 1 || past_grid((long long)layers * B * Hkv, 64)) return fail(T2I_ERR_SHAPE, "layers=%d invalid", layers);
   if (!aligned4(tokens) || !aligned4(picks) || !aligned4(path) || !aligned4(path_counts) || !aligned4(next_tokens) || !aligned4(context_out))
     return fail(T2I_ERR_ALIGN, "token and count arrays must be 4-byte aligned");
   if (!aligned16(k_cache) || !aligned16(v_cache)) return fail(T2I_ERR_ALIGN, "caches must be 16-byte aligned");

@@ -1333,6 +1333,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, w
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError("logits must be [M, V]")
     m, v = logits.shape
+    if max(m, v) >= 2**31:
+        raise ValueError(f"{m} rows of {v} logits are too many")
     stride = logits.stride(0) if m > 1 else v
     if (v > 1 and logits.stride(1) != 1) or stride < v:
         raise ValueError("logits rows must be contiguous and must not overlap")
