@@ -676,6 +676,22 @@ class Qwen3Model:
                 raise ValueError("prompt token id out of range")
         return [p.to(torch.int32) for p in prompts]
 
+    def _prompt_argument(self, prompt, prompt_mode: str):
+        """``generate``'s prompts: ``([B, T] ids, None)`` for one length, ``(None, list)`` where
+        lengths differ.  A list or tuple holds a row for each sequence and is checked as ``prefill_packed``'s,
+        whatever its lengths; of a tensor or array the ids must be whole numbers."""
+        if isinstance(prompt, (list, tuple)):
+            rows = self._prompt_list(prompt)
+            if len({p.numel() for p in rows}) == 1:
+                return torch.stack(rows), None
+            if prompt_mode != "prefill":
+                raise ValueError("prompts of different lengths need prompt_mode 'prefill'")
+            return None, rows
+        prompt = torch.as_tensor(prompt)
+        if prompt.is_floating_point() and not torch.equal(prompt, prompt.trunc()):
+            raise ValueError("token ids must be integers")
+        return prompt, None
+
     def _packed_pass(self, prompts: list):
         """The packed prompt pass from slot 0 of every cache row: ``(residual rows, plan)``."""
         c = self.cfg
@@ -864,24 +880,19 @@ class Qwen3Model:
         """
         if prompt_mode not in ("prefill", "decode"):
             raise ValueError("prompt_mode must be 'prefill' or 'decode'")
-        ragged = None
-        if isinstance(prompt, (list, tuple)) and all(hasattr(p, "__len__") for p in prompt) and len(set(map(len, prompt))) > 1:
-            if prompt_mode != "prefill":
-                raise ValueError("prompts of different lengths need prompt_mode 'prefill'")
-            ragged = self._prompt_list(prompt)
+        prompt, ragged = self._prompt_argument(prompt, prompt_mode)
+        if ragged is None:
+            b, plen = prompt.shape
+            if b != self.batch:
+                raise ValueError("prompt batch does not match the model batch size")
+            if int(prompt.min()) < 0 or int(prompt.max()) >= self.cfg.vocab:
+                raise ValueError("prompt token id out of range")
+            first = prompt[:, 0]
+        else:
             b, plen = len(ragged), max(p.numel() for p in ragged)
-            prompt = torch.zeros(b, plen, dtype=torch.int32)   # a first token each, for the eager step before a capture
-            prompt[:, 0] = torch.stack([p[0] for p in ragged])
-        elif isinstance(prompt, (list, tuple)) and all(isinstance(p, torch.Tensor) for p in prompt):
-            prompt = torch.stack(list(prompt))
-        prompt = torch.as_tensor(prompt)
-        b, plen = prompt.shape
-        if b != self.batch:
-            raise ValueError("prompt batch does not match the model batch size")
+            first = torch.stack([p[0] for p in ragged])
         if plen + new_tokens - 1 > self.ctx_cap:
             raise ValueError(f"prompt {plen} + {new_tokens} tokens exceed the cache capacity {self.ctx_cap}")
-        if int(prompt.min()) < 0 or int(prompt.max()) >= self.cfg.vocab:
-            raise ValueError("prompt token id out of range")
         # The KV cache is not cleared: attention reads only slots 0 .. position of a
         # sequence, and the prompt pass (or the decode step, for the current slot)
         # writes every one of them before it is read.
@@ -891,11 +902,13 @@ class Qwen3Model:
         if self.prompt is None or tuple(self.prompt.shape) != (b, plen):
             self.prompt = torch.empty(b, plen, dtype=torch.int32, device=self.device)
             self._captured = False
-        self.prompt.copy_(prompt.to(torch.int32))
+        if ragged is None:
+            self.prompt.copy_(prompt.to(torch.int32))
         if self.history is None or self.history.shape[1] < new_tokens:
             self.history = torch.zeros(b, new_tokens, dtype=torch.int32, device=self.device)
             self._captured = False      # the head graph holds the history pointer
-        self.tokens.copy_(self.prompt[:, 0])
+        first = first.to(device=self.device, dtype=torch.int32)
+        self.tokens.copy_(first)
         self.positions.zero_()
         self.step.zero_()
         ev = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
@@ -905,7 +918,7 @@ class Qwen3Model:
             torch.cuda.synchronize(self.device)
             self._capture()
             # restore the state the prompt pass starts from
-            self.tokens.copy_(self.prompt[:, 0])
+            self.tokens.copy_(first)
             self.positions.zero_()
             self.step.zero_()
             torch.cuda.synchronize(self.device)
