@@ -53,6 +53,33 @@ def small(gpu):
     return gm.Qwen3Model(gm.random_qwen3_tensors(cfg, seed=62, weights="centered"), cfg, batch=3, ctx_cap=96, device=gpu)
 
 
+def _prompts(lengths, seed):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randint(0, 2048, (n,), generator=g) for n in lengths]
+
+
+@pytest.mark.gpu
+def test_longer_ragged_prompts_keep_the_captured_steps(small):
+    """The decode graphs do not depend on a packed prompt pass: another longest prompt captures nothing anew, and the
+    calls before and behind it still replay what they captured."""
+    small.generate(_prompts([5, 9, 2], 1), 10)
+    step = small.micro[0].graphs["step"]
+    for seed, lengths in enumerate(([5, 30, 2], [70, 1, 12], [3, 4, 5])):
+        p = _prompts(lengths, seed)
+        got = small.generate(p, 10)
+        assert small.micro[0].graphs["step"] is step
+        assert torch.equal(got, small.generate(p, 10, use_graph=False))
+    batch = torch.stack(_prompts([20, 20, 20], 7))
+    for mode in ("decode", "prefill"):
+        want = small.generate(batch, 10, use_graph=False, prompt_mode=mode)
+        assert torch.equal(small.generate(batch, 10, prompt_mode=mode), want)
+        step = small.micro[0].graphs["step"]
+        small.generate(_prompts([8, 64, 2], 8), 10)
+        assert torch.equal(small.generate(batch, 10, prompt_mode=mode), want)
+        assert small.micro[0].graphs["step"] is step
+    assert torch.equal(small.generate(batch.tolist(), 10), small.generate(batch, 10))
+
+
 @pytest.mark.gpu
 def test_generate_refuses_what_is_no_integer(small):
     for bad in ([[1.9, 2.2], [3.7, 4.0], [1.0, 1.0]], torch.full((3, 2), 1.5)):

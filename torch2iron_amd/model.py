@@ -898,8 +898,9 @@ class Qwen3Model:
         # writes every one of them before it is read.
         # One prompt buffer per prompt shape: the captured prompt-bookkeeping graph
         # reads it by address (and its length), so a new shape needs a new capture
-        # and a new prompt of the same shape only new contents.
-        if self.prompt is None or tuple(self.prompt.shape) != (b, plen):
+        # and a new prompt of the same shape only new contents.  A packed pass does not
+        # read it: any buffer serves the capture, and the one that is there stays.
+        if self.prompt is None or (ragged is None and tuple(self.prompt.shape) != (b, plen)):
             self.prompt = torch.empty(b, plen, dtype=torch.int32, device=self.device)
             self._captured = False
         if ragged is None:
