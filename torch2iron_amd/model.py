@@ -757,8 +757,9 @@ class Qwen3Model:
         walk down each tree, and the accepted path's K/V rows left in their places.  Node 0
         stands for the sequence's pending token (``self.tokens``, put there by this call).
 
-        The state moves on as by as many decode steps: ``positions`` by the accepted nodes, ``tokens`` to
-        the token after the last of them.  Returns device int32 ``(new_tokens [B, N], counts [B])``: the
+        ``positions`` move on by the accepted nodes and ``tokens`` to the token after the last of them, as by
+        as many decode steps; ``history`` and ``step``, which record one token of every sequence a step, stay
+        as they are (sequences accept different numbers).  Returns device int32 ``(new_tokens [B, N], counts [B])``: the
         tokens that the step found, padded with -1 (the accepted drafted ones, then the one after
         them: what greedy decode emits), and how many.  A sequence without nodes or without
         room for them in the cache stays as it is, with count 0.  Nothing is read back: the
