@@ -735,6 +735,8 @@ class Qwen3Model:
         (token i + 1 after the tokens before it), ``entropy [n]`` (nats), ``top_logprobs`` and ``top_ids
         [n, top_k]`` of what may follow each token."""
         prompts = self._prompt_list(prompts)
+        if not 0 <= top_k <= min(ops.MAX_TOP_K, self.cfg.vocab):
+            raise ValueError(f"top_k must be 0 to {min(ops.MAX_TOP_K, self.cfg.vocab)}, got {top_k}")
         x, plan = self._packed_pass(prompts)
         target = torch.cat([torch.cat((p[1:], p.new_full((1,), -1))) for p in prompts]).to(self.device)
         xn = ops.rmsnorm(x, self.norm, self.cfg.eps)
