@@ -123,3 +123,14 @@ def test_cost_of_a_nan(gpu, slot):
     clean = _time(run)
     vc[:, :, slot, 3] = NAN
     assert _time(run) <= 10 * clean
+
+
+def test_cost_of_a_cache_of_nan(gpu):
+    """Trees over caches whose V is NaN throughout: blocks that every row sees whole stay matrix products, so that
+    the second pass costs about the first and the last two blocks' key by key products."""
+    q, parents, ctx, _, kc, vc, _ = _tree_case(gpu, 16, 8, 8192, [8000 - 61 * i for i in range(16)], 26, None, "random")
+    run = lambda: ops.tree_attention(q, parents, ctx, 8, kc, vc)  # noqa: E731
+    clean = _time(run)
+    vc[:] = NAN
+    assert _time(run) <= 5 * clean
+    assert run().isnan().all()

@@ -331,6 +331,12 @@ __device__ __forceinline__ float pair_sum(float v) {
   return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
 
+// Two bf16 values, 0 in the place of infinities and NaN.
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
+  if ((w & 0x7F80u) == 0x7F80u) w &= 0xFFFF0000u;
+  return (w & 0x7F800000u) == 0x7F800000u ? w & 0xFFFFu : w;
+}
+
 // An item of a workgroup of WAVES waves of 32 pairs, for one kv head.  All products run transposed
 // on the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32, h2 = lane / 32) holds one pair's scores
 // and outputs:
@@ -351,7 +357,8 @@ __device__ __forceinline__ float pair_sum(float v) {
 // with FINE 713).
 // In an MFMA a weight of 0 times an infinity or a NaN in V is a NaN, also for rows whose mask hides that
 // key.  An item with sums that are not finite is therefore run again, MASKED: blocks that some row does not
-// see whole (FINE: any) and whose V holds such a value are multiplied key by key for the rows that attend it.  (500
+// see whole and whose V holds such a value are multiplied key by key for the rows that attend it; FINE multiplies
+// its second words by V without such values, since they may be 0 or negative.  (500
 // rows from 1500, 16 / 8 heads, without such values 32 us, with a NaN in the last slot 76, in the first 46;
 // 1624 and 2384 where such rows were formed again from all of their keys.)
 // K and V blocks go straight from memory into LDS, RING buffers, one barrier a block; a row's
@@ -525,13 +532,13 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
     }
     // ---- MASKED: where V holds an infinity or a NaN, key by key for the rows that attend it ----
     if constexpr (MASKED) {
-      if (FINE || kb * RG_KEYS + RG_KEYS > mask_from) {    // FINE: a second word may be 0 or negative
+      if (kb * RG_KEYS + RG_KEYS > mask_from) {
         bool odd = false;
 #pragma unroll 4
         for (int i = 0; i < RG_KEYS / 4; ++i) {
           const u32x4 x = *reinterpret_cast<const u32x4*>(bv + 4 * i * D + 8 * lane);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= (x[e] & 0x7F80u) == 0x7F80u || (x[e] & 0x7F800000u) == 0x7F800000u;
+          for (int e = 0; e < 4; ++e) odd |= finite_or_zero(x[e]) != x[e];
         }
         if (__any(odd)) {
           const uint32_t unseen = __float_as_uint(-1.0f);  // no weight
@@ -600,8 +607,15 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
       }
       if constexpr (FINE) {
 #pragma unroll
-        for (int dt = 0; dt < 4; ++dt)
+        for (int dt = 0; dt < 4; ++dt) {
+          if (MASKED) {                                    // a second word may be 0 or negative
+            u32x4 x = __builtin_bit_cast(u32x4, va[dt]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = finite_or_zero(x[e]);
+            va[dt] = __builtin_bit_cast(bf16x8, x);
+          }
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[dt], __builtin_bit_cast(bf16x8, u32x4{r[0], r[1], r[2], r[3]}), o[dt], 0, 0, 0);
+        }
       }
     }
   }
