@@ -15,7 +15,6 @@
 // sequences of one row, which stand in for decode steps, multiply by weights of 16 bits.
 #include <math.h>
 
-#include <atomic>
 #include <exception>
 #include <type_traits>
 
@@ -27,6 +26,8 @@ namespace t2i {
 
 constexpr int RG_D = 128;
 constexpr int RG_KEYS = t2i_host::RG_KEYS;
+constexpr int RG_WAVES = 4;                  // waves of a workgroup of the attention, 32 pairs each
+constexpr int RG_ROWS = t2i_host::RG_ROWS;
 constexpr int RG_ITEM = t2i_host::RG_ITEM;
 constexpr int TREE_NODES = 64;               // nodes of a tree: one lane of a wave each
 
@@ -169,7 +170,7 @@ struct RaggedAttnParams {
   const int32_t* ctx;
   const int32_t* counts;
   long long rows;
-  int n_cache, n_items, n_bins, n_parts, part_rows, tile_rows, Hq, Hkv, G, cap, B, N, tiles;
+  int n_cache, n_items, n_bins, n_parts, part_rows, Hq, Hkv, G, cap, B, N, tiles;
   float scale_log2;         // D^-1/2 * log2(e)
 };
 
@@ -182,9 +183,9 @@ struct RaggedItem {
 // The even shares of a batch of trees: the key blocks of all sequences in a row, cut into `n`
 // equal runs.  A workgroup takes a run for one tile of pairs of one kv head; the tiles of a
 // sequence stand beside each other on one XCD and read the same K and V at the same time, so
-// memory gives them once (8 trees of two tiles over 32k slots: 307 us one tile after the other, 260
-// side by side).  A sequence that is cut leaves a part in each of its runs: slot 2 bin where it
-// is the run's first piece, 2 bin + 1 where it is the last of several.
+// memory gives them once (8 trees of two tiles over 32k slots, before weights had 16 bits: 307 us
+// one tile after the other, 260 side by side).  A sequence that is cut leaves a part in each of its
+// runs: slot 2 bin where it is the run's first piece, 2 bin + 1 where it is the last of several.
 struct TreeWalk {
   int n, total, b, blocks, kb;         // n: runs; the next piece starts at block kb of sequence b
   TreeSeq seq;
@@ -245,7 +246,7 @@ struct TreeWalk {
     it.rows = seq.nodes;
     it.start = seq.ctx;
     it.crow = b;
-    it.j0 = tile * p.tile_rows;
+    it.j0 = tile * RG_ROWS;
     it.pairs = seq.nodes * p.G;
     it.kend = seq.ctx + seq.nodes;
     it.kb0 = kb;
@@ -262,11 +263,6 @@ struct TreeWalk {
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
 
-// Until at most N of this wave's loads into LDS are in flight, and every wave is here.
-template <int N>
-__device__ __forceinline__ void loads_barrier() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
-}
 // Until every LDS operation of this wave is done, and every wave is here.
 __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -285,26 +281,19 @@ __device__ __forceinline__ void lds_load16(i32x4 rsrc, uint32_t at, uint32_t lds
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :: "s"(lds), "v"(at), "s"(rsrc) : "memory", "m0");
 }
-// 4 N keys from a buffer, four an instruction, the lane's chunk of instruction i's at byte at[i]
+// 16 keys from a buffer, four an instruction, the lane's chunk of instruction i's at byte at[i]
 // (from soff on, less 1024 i).  An instruction's offset counts for the memory address and for
 // the LDS address.
 // ONCE: past the caches' own order (nt), for keys that no other workgroup reads.
 #define T2I_KEYS(mod)                                                                                             \
-  if constexpr (N == 4)                                                                                           \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"                                                                \
-                 "buffer_load_dwordx4 %1, %5, %6 offen" mod " lds\n\t"                                            \
-                 "buffer_load_dwordx4 %2, %5, %6 offen offset:1024" mod " lds\n\t"                                \
-                 "buffer_load_dwordx4 %3, %5, %6 offen offset:2048" mod " lds\n\t"                                \
-                 "buffer_load_dwordx4 %4, %5, %6 offen offset:3072" mod " lds"                                    \
-                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(rsrc), "s"(soff) : "memory", "m0"); \
-  else                                                                                                            \
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"                                                                \
-                 "buffer_load_dwordx4 %1, %3, %4 offen" mod " lds\n\t"                                            \
-                 "buffer_load_dwordx4 %2, %3, %4 offen offset:1024" mod " lds"                                    \
-                 :: "s"(lds), "v"(at[0]), "v"(at[1]), "s"(rsrc), "s"(soff) : "memory", "m0")
-template <bool ONCE, int N>
-__device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[N], uint32_t soff, uint32_t lds) {
-  static_assert(N == 2 || N == 4, "instructions of a wave");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"                                                                  \
+               "buffer_load_dwordx4 %1, %5, %6 offen" mod " lds\n\t"                                              \
+               "buffer_load_dwordx4 %2, %5, %6 offen offset:1024" mod " lds\n\t"                                  \
+               "buffer_load_dwordx4 %3, %5, %6 offen offset:2048" mod " lds\n\t"                                  \
+               "buffer_load_dwordx4 %4, %5, %6 offen offset:3072" mod " lds"                                      \
+               :: "s"(lds), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "s"(rsrc), "s"(soff) : "memory", "m0")
+template <bool ONCE>
+__device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[4], uint32_t soff, uint32_t lds) {
   if constexpr (ONCE) {
     T2I_KEYS(" nt");
   } else {
@@ -337,9 +326,9 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
   return (w & 0x7F800000u) == 0x7F800000u ? w & 0xFFFFu : w;
 }
 
-// An item of a workgroup of WAVES waves of 32 pairs, for one kv head.  All products run transposed
-// on the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32, h2 = lane / 32) holds one pair's scores
-// and outputs:
+// An item of a workgroup, for one kv head: four waves of 32 pairs.  All products run transposed on
+// the 32 x 32 x 16 MFMA, so that a lane (c = lane % 32, h2 = lane / 32) holds one pair's scores and
+// outputs:
 //   S^T = K Q^T: A = K from LDS (lane: key 32 n + c, dims 16 ks + 8 h2 ..), B = the wave's q
 //     rows (registers); register i holds the score of key 32 n + 8 (i / 4) + 4 h2 + i % 4;
 //   the online softmax per lane: the row's maximum from its two lanes by one lane swap, the
@@ -361,16 +350,15 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
 // its second words by V without such values, since they may be 0 or negative.  (500
 // rows from 1500, 16 / 8 heads, without such values 32 us, with a NaN in the last slot 76, in the first 46;
 // 1624 and 2384 where such rows were formed again from all of their keys.)
-// K and V blocks go straight from memory into LDS, RING buffers, one barrier a block; a row's
+// K and V blocks go straight from memory into LDS, two buffers, one barrier a block; a row's
 // 16-byte chunk ch stands at place ch ^ (row % 16) (K) or ch ^ 4 (row % 4) (V): 16 neighbouring
 // lanes of a K read, 32 of a transposing read cover all banks (a load into LDS cannot pad rows,
 // but each lane chooses what it loads; with ch ^ 2 (row % 8) for both, half of the cycles of
 // LDS were bank conflicts).  Keys past the last one reload it: slots that no row attends are
 // never read.
-//   4 waves, 2 buffers (64 KB, two workgroups a CU): every packed call, and trees of up to 128
-//     pairs.  8 waves, 4 buffers (128 KB, one a CU): wider trees, whose K and V then come once
-//     for 256 pairs (8 x 64 nodes, 4 q heads a kv head, 32k slots: 264 -> 258 us; packed prompts
-//     are no faster for it, and 16 short ones 31 -> 38 us).
+//   The buffers take 64 KB: two workgroups a CU.  Eight waves and four buffers, whose K and V come once for
+// 256 pairs, were no faster for trees of more than 128 pairs either (8 x 64 nodes, 4 q heads a kv head,
+// 32k slots 318 us against 325, 1 x 64 over 4k 26.9 against 29.3, 2 x 64 of 8 q heads over 20k 138 against 137).
 // What bounds it (one MI355X; a large copy reaches 5.15 TB/s, an 8192^3 product 1.21 PFLOP/s):
 //   8001 rows from 0, 32 / 8 heads: 500-516 us, 1.02-1.05 PFLOP/s.  MFMAs take 54 % of a SIMD's
 //     cycles and VALU instructions as many beside them, at the 1.8-1.9 GHz that the card holds
@@ -382,12 +370,11 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
 // around the products (1-3 %), scheduling groups and iglp (0-4 %), two waves sharing the blocks of a
 // tile of up to 32 pairs (single rows 5 % faster, everything else 3-8 % slower: registers).
 // Returns the wave's pairs (bit c) whose sums are not finite, which were not written; MASKED: writes `only` those.
-template <bool TREE, int WAVES, int RING, bool FINE, bool MASKED>
+template <bool TREE, bool FINE, bool MASKED>
 __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const RaggedItem& it, int h, uint16_t* s_kv, int lane,
                                                 int wave, uint32_t only) {
   constexpr int D = RG_D;
-  constexpr int ROWS = 32 * WAVES;             // pairs of a tile
-  constexpr int WKEYS = RG_KEYS / WAVES;       // keys of a block that a wave loads
+  constexpr int WKEYS = RG_KEYS / RG_WAVES;    // keys of a block that a wave loads
   const int c = lane & 31, h2 = lane >> 5;
 
   // ---- K / V staging: a wave's instruction moves 4 keys (1 KB); 4 each of K and V a block ----
@@ -405,10 +392,10 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
   const i32x4 krsrc = keys_rsrc(p.kc + cache_base), vrsrc = keys_rsrc(p.vc + cache_base);
   // K and V block kb into its buffer
   auto stage = [&](int kb) __attribute__((always_inline)) {
-    const uint32_t lds = lds0 + ((kb - it.kb0) & (RING - 1)) * (4 * RG_KEYS * D);
+    const uint32_t lds = lds0 + ((kb - it.kb0) & 1) * (4 * RG_KEYS * D);
     if ((kb + 1) * RG_KEYS <= it.kend) {
       const uint32_t at = (uint32_t)kb * (RG_KEYS * D * 2);
-      if (it.pairs <= ROWS) {                              // the sequence's only tile: its keys are read once
+      if (it.pairs <= RG_ROWS) {                            // the sequence's only tile: its keys are read once
         lds_load_keys<true>(krsrc, kat, at, lds);
         lds_load_keys<true>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
       } else {
@@ -425,9 +412,7 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
       }
     }
   };
-#pragma unroll
-  for (int s = 0; s < RING - 1; ++s)
-    if (it.kb0 + s < it.kb1) stage(it.kb0 + s);
+  if (it.kb0 < it.kb1) stage(it.kb0);
 
   // ---- this lane's pair, and its q row as the B operand ----
   const int j = it.j0 + wave * 32 + c;
@@ -469,16 +454,10 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
   const int vcol = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);   // its 16-byte chunk within a 32-dim tile
 
   for (int kb = it.kb0; kb < it.kb1; ++kb) {
-    // this block is here (2 LOADS of each later one may be on their way; the first wait of an
-    // item, behind other kinds of memory operations, is for everything), and the buffer of the
-    // block before it is free
-    const int later = min(RING - 2, it.kb1 - 1 - kb);
-    if (RING > 3 && later == 2 && kb > it.kb0) loads_barrier<4 * LOADS>();
-    else if (RING > 2 && later == 1 && kb > it.kb0) loads_barrier<2 * LOADS>();
-    else loads_done_barrier();
-    if (kb + RING - 1 < it.kb1) stage(kb + RING - 1);
+    loads_done_barrier();                                  // this block is here, the buffer of the one before it free
+    if (kb + 1 < it.kb1) stage(kb + 1);
     if (!wave_on || kb * RG_KEYS >= wave_end) continue;
-    const uint16_t* const bk = s_kv + ((kb - it.kb0) & (RING - 1)) * (2 * RG_KEYS * D);
+    const uint16_t* const bk = s_kv + ((kb - it.kb0) & 1) * (2 * RG_KEYS * D);
     const uint16_t* const bv = bk + RG_KEYS * D;
     // ---- S^T = K Q^T ----
     f32x16 s[2];
@@ -674,11 +653,10 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
 }
 
 // A workgroup takes a bin's items for one kv head, one after the other.
-template <bool TREE, int WAVES, int RING>
-__global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
-  constexpr int ROWS = 32 * WAVES;             // pairs of a tile
-  extern __shared__ __align__(256) uint16_t s_kv[];   // [RING][K, V][key][dim]
-  __shared__ uint32_t s_odd[WAVES];                   // an item's pairs whose sums are not finite
+template <bool TREE>
+__global__ __launch_bounds__(64 * RG_WAVES, 2) void ragged_attention_kernel(const RaggedAttnParams p) {
+  extern __shared__ __align__(256) uint16_t s_kv[];   // [buffer][K, V][key][dim]
+  __shared__ uint32_t s_odd[RG_WAVES];                     // an item's pairs whose sums are not finite
 
   const int h = blockIdx.x % p.Hkv;
   const int tile = TREE ? blockIdx.x / p.Hkv % p.tiles : 0;
@@ -710,24 +688,24 @@ __global__ __launch_bounds__(64 * WAVES, 2) void ragged_attention_kernel(const R
       // a table that does not fit the tensors is not followed
       if (it.row0 < 0 || it.rows < 1 || it.row0 + (long long)it.rows > p.rows || it.start < 0 ||
           it.start > p.cap - it.rows || it.crow < 0 || it.crow >= p.n_cache || it.j0 < 0 ||
-          (long long)it.rows * p.G > 0x7FFFFFFF - ROWS || it.j0 >= it.pairs || it.part >= p.n_parts)
+          (long long)it.rows * p.G > 0x7FFFFFFF - RG_ROWS || it.j0 >= it.pairs || it.part >= p.n_parts)
         continue;
-      it.kend = it.start + (min(it.j0 + ROWS, it.pairs) - 1) / p.G + 1;
+      it.kend = it.start + (min(it.j0 + RG_ROWS, it.pairs) - 1) / p.G + 1;
       it.kb0 = max(it.kb0, 0);
       it.kb1 = min(it.kb1, (it.kend + RG_KEYS - 1) / RG_KEYS);
     }
 
     const auto run = [&](auto fine) __attribute__((always_inline)) {
       constexpr bool FINE = decltype(fine)::value;
-      const uint32_t odd = attend_item<TREE, WAVES, RING, FINE, false>(p, it, h, s_kv, lane, wave, 0);
+      const uint32_t odd = attend_item<TREE, FINE, false>(p, it, h, s_kv, lane, wave, 0);
       if (it.kb0 >= it.kb1) return;
       if (lane == 0) s_odd[wave] = odd;
       lds_barrier();                                         // the buffers are free
       uint32_t any = 0;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) any |= s_odd[w];
+      for (int w = 0; w < RG_WAVES; ++w) any |= s_odd[w];
       if (!__builtin_amdgcn_readfirstlane(any)) return;
-      (void)attend_item<TREE, WAVES, RING, FINE, true>(p, it, h, s_kv, lane, wave, odd);
+      (void)attend_item<TREE, FINE, true>(p, it, h, s_kv, lane, wave, odd);
       lds_barrier();
     };
     if (TREE || it.rows == 1) run(std::true_type{});
@@ -754,7 +732,7 @@ __global__ __launch_bounds__(256) void ragged_merge_kernel(const RaggedAttnParam
     row0 = b * p.N;
     rows = tree_seq(p.ctx, p.counts, b, p.N, p.cap).nodes;
     at += group * MERGE_PAIRS;
-    j0 = tile * p.tile_rows;
+    j0 = tile * RG_ROWS;
     if (j0 + group * MERGE_PAIRS >= rows * p.G) return;   // nothing was written for it
     const int2 w = p.cuts[b];
     if (w.x < 0) return;                       // one piece: its rows are written
@@ -920,43 +898,25 @@ void* set_parts(t2i::RaggedAttnParams& p, void* ws, long long parts, int32_t row
   return p.part_ml + (size_t)parts * p.Hkv * rows;
 }
 
-// The kernel's forms: 4 waves (128 pairs a tile, two workgroups a CU, the next block on its
-// way) and, for trees alone, 8 waves (256 pairs, one workgroup a CU, three blocks on their way).
-constexpr int lds_bytes(int ring) { return ring * 2 * t2i::RG_KEYS * t2i::RG_D * 2; }
+constexpr int LDS_BYTES = 2 * 2 * t2i::RG_KEYS * t2i::RG_D * 2;   // two buffers of K and V
 
 template <bool TREE>
-int launch_narrow(const t2i::RaggedAttnParams& p, long long groups, hipStream_t s) {
-  hipLaunchKernelGGL((t2i::ragged_attention_kernel<TREE, 4, 2>), dim3(groups), dim3(256), lds_bytes(2), s, p);
-  return t2i_host::hip_status(hipGetLastError(), "ragged attention launch");
-}
-
-int launch_wide_tree(const t2i::RaggedAttnParams& p, long long groups, hipStream_t s) {
-  // more than 64 KB of LDS: asked for once a device (twice does no harm)
-  static std::atomic<bool> done[64];
-  int dev = 0;
-  if (int rc = t2i_host::hip_status(hipGetDevice(&dev), "device query")) return rc;
-  if (dev < 0 || dev >= 64 || !done[dev]) {
-    if (int rc = t2i_host::hip_status(hipFuncSetAttribute(reinterpret_cast<const void*>(&t2i::ragged_attention_kernel<true, 8, 4>),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, lds_bytes(4)), "LDS attribute"))
-      return rc;
-    if (dev >= 0 && dev < 64) done[dev] = true;
-  }
-  hipLaunchKernelGGL((t2i::ragged_attention_kernel<true, 8, 4>), dim3(groups), dim3(512), lds_bytes(4), s, p);
+int launch_attention(const t2i::RaggedAttnParams& p, long long groups, hipStream_t s) {
+  hipLaunchKernelGGL(t2i::ragged_attention_kernel<TREE>, dim3(groups), dim3(64 * t2i::RG_WAVES), LDS_BYTES, s, p);
   return t2i_host::hip_status(hipGetLastError(), "ragged attention launch");
 }
 
 // A tree call's launch: tiles of a sequence, workgroups of a kv head, rows of a part's tile.
 struct TreePlan {
-  int tiles, bins, rows, tile_rows;
+  int tiles, bins, rows;
   size_t bytes;
 };
 TreePlan tree_plan(int32_t B, int32_t N, int32_t Hq, int32_t Hkv, int32_t cap) {
   TreePlan t;
   const int pairs = N * (Hq / Hkv);
-  t.tile_rows = pairs > 128 ? 256 : 128;
-  t.tiles = (pairs + t.tile_rows - 1) / t.tile_rows;
-  t.bins = t2i_host::tree_bins(B, t.tiles * Hkv, cap, t.tile_rows);
-  t.rows = std::min(t.tile_rows, (pairs + 31) / 32 * 32);
+  t.tiles = (pairs + t2i_host::RG_ROWS - 1) / t2i_host::RG_ROWS;
+  t.bins = t2i_host::tree_bins(B, t.tiles * Hkv, cap);
+  t.rows = std::min(t2i_host::RG_ROWS, (pairs + 31) / 32 * 32);
   t.bytes = part_bytes(2LL * t.bins * t.tiles, Hkv, t.rows) + (size_t)B * sizeof(int2);
   return t;
 }
@@ -1067,7 +1027,7 @@ extern "C" int t2i_packed_attention(const uint16_t* q, int32_t rows, const int32
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
   if (need) set_parts(p, workspace, n_parts, t2i_host::RG_ROWS);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (int rc = launch_narrow<false>(p, (long long)n_bins * Hkv, s)) return rc;
+  if (int rc = launch_attention<false>(p, (long long)n_bins * Hkv, s)) return rc;
   if (!need) return T2I_OK;
   p.items = merges;
   hipLaunchKernelGGL(t2i::ragged_merge_kernel<false>, dim3(n_merges * Hkv), dim3(256), 0, s, p);
@@ -1110,7 +1070,6 @@ extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, con
   const TreePlan t = tree_plan(B, N, Hq, Hkv, ctx_cap);
   p.rows = (long long)B * N; p.n_cache = B; p.Hq = Hq; p.Hkv = Hkv; p.G = Hq / Hkv; p.cap = ctx_cap; p.B = B; p.N = N;
   p.tiles = t.tiles;
-  p.tile_rows = t.tile_rows;
   p.n_bins = t.bins;
   p.scale_log2 = (float)(1.4426950408889634 / sqrt((double)D));
   if (past_grid((long long)B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS), 256) || too_many((long long)B * N) ||
@@ -1120,8 +1079,7 @@ extern "C" int t2i_tree_attention(const uint16_t* q, const int32_t* parents, con
   if (!aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
   p.cuts = reinterpret_cast<int2*>(set_parts(p, workspace, 2LL * t.bins * t.tiles, t.rows));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const long long groups = (long long)t.bins * t.tiles * Hkv;
-  if (int rc = t.tile_rows == 128 ? launch_narrow<true>(p, groups, s) : launch_wide_tree(p, groups, s)) return rc;
+  if (int rc = launch_attention<true>(p, (long long)t.bins * t.tiles * Hkv, s)) return rc;
   hipLaunchKernelGGL(t2i::ragged_merge_kernel<true>, dim3(B * t.tiles * Hkv * (t.rows / t2i::MERGE_PAIRS)), dim3(256), 0, s, p);
   return t2i_host::hip_status(hipGetLastError(), "tree attention merge launch");
 }

@@ -142,9 +142,9 @@ inline PackedTable packed_items(const int32_t* lengths, const int32_t* starts, c
 
 // A tree's attention: its contexts are on the device, where every workgroup finds its own even
 // share of the batch's key blocks (of at least two blocks).  Shares of a kv head's tile, at most:
-inline int tree_bins(int64_t B, int tiles_heads, int cap, int tile_rows) {
+inline int tree_bins(int64_t B, int tiles_heads, int cap) {
   const int64_t most = B * ((cap + RG_KEYS - 1) / RG_KEYS) / 2;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::max(1, (tile_rows == 128 ? 512 : 256) / tiles_heads), most));
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::max(1, RG_SLOTS / tiles_heads), most));
 }
 
 }  // namespace t2i_host
