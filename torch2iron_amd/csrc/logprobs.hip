@@ -181,8 +181,8 @@ __device__ __forceinline__ void lp_finish(const LpParams& p, int row, LpState st
 // starts as its lanes' largest values of the first pieces, in order; after that it looks at a
 // piece's order only where a lane's largest value passes the k-th best of its own list and of
 // the other waves' (which only grow, so an older one of them is as good).  2043 rows of 151936
-// fp32 logits, 20 best: 227-238 us, 5.2-5.5 TB/s (a large copy reaches 5.15), 228-230 without lists: memory,
-// with VALU instructions in 84 % of a SIMD's cycles beside it.  416 bf16 rows: 32 us without best lists,
+// fp32 logits, 20 best: 225-238 us, 5.2-5.5 TB/s (a bulk read reaches 6.7), 217 without lists: VALU
+// instructions in 87 % of a SIMD's cycles beside memory.  416 bf16 or fp16 rows: 32.5 us without best lists,
 // 51-54 with 8 (7 of them the merge): VALU instructions, 83 % of a SIMD's cycles.
 // Measured and dropped: twice the pieces on their way (1-14 % slower), lists of the waves joined by
 // rank (2 %), fewer and longer parts (3-10 %).

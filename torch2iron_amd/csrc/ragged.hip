@@ -97,8 +97,9 @@ struct RaggedPrepParams {
 
 // One workgroup (4 waves) per row, a head vector to a 16-lane row of a wave, as
 // prefill_prep_kernel (same bits): RG_PREP_NB batches of 16 vectors in flight.  A row whose
-// position, slot or cache row lies outside the cache writes nothing.  Bound by HBM: every byte
-// is read and written once (4997 rows, 16 / 8 heads: 20.8 us, 3.9 TB/s; 416 nodes: 4.9 us).
+// position, slot or cache row lies outside the cache writes nothing.  Bound by HBM where rows are
+// many, every byte read and written once (4997 rows, 16 / 8 heads: 21 us, 3.9 TB/s), by the latency
+// of a workgroup's own chain where they are few (416 nodes: 4.9 us for 6.8 MB).
 constexpr int RG_PREP_NB = 2;
 
 template <bool TREE>
@@ -341,7 +342,7 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
 // FINE: what the rounding of the weights left is a second bf16 word and V is multiplied by both:
 // weights of 16 bits, whose error the output's own rounding hides, normalised by their fp32 sum.  Trees
 // and sequences of one row take it, since they stand in for decode steps, whose weights are fp32
-// (16 x 26 nodes 47.2 -> 49.8 us, 8 x 64 nodes over 32k slots 265 -> 323, 16 single rows 33.1 -> 34.2); prompt
+// (16 x 26 nodes 46 -> 48 us, 8 x 64 nodes over 32k slots 270 -> 330, 16 single rows 32.8 -> 34.1); prompt
 // rows round their weights once, as the batch form of the prompt pass does (8001 rows: 517 us,
 // with FINE 713).
 // In an MFMA a weight of 0 times an infinity or a NaN in V is a NaN, also for rows whose mask hides that
@@ -356,15 +357,17 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
 // but each lane chooses what it loads; with ch ^ 2 (row % 8) for both, half of the cycles of
 // LDS were bank conflicts).  Keys past the last one reload it: slots that no row attends are
 // never read.
-//   The buffers take 64 KB: two workgroups a CU.  Eight waves and four buffers, whose K and V come once for
-// 256 pairs, were no faster for trees of more than 128 pairs either (8 x 64 nodes, 4 q heads a kv head,
-// 32k slots 318 us against 325, 1 x 64 over 4k 26.9 against 29.3, 2 x 64 of 8 q heads over 20k 138 against 137).
-// What bounds it (one MI355X; a large copy reaches 5.15 TB/s, an 8192^3 product 1.21 PFLOP/s):
-//   8001 rows from 0, 32 / 8 heads: 500-516 us, 1.02-1.05 PFLOP/s.  MFMAs take 54 % of a SIMD's
+//   The buffers take 64 KB: two workgroups a CU.  Eight waves with four buffers, whose K and V come once
+// for 256 pairs, gained nothing for trees of more than 128 pairs (this form / eight waves: 8 x 64 nodes, 4 q
+// heads a kv head, 32k slots 318 / 325 us; 1 x 64 over 4k 26.9 / 29.3; 2 x 64 of 8 q heads over 20k 138 / 137).
+// What bounds it (one MI355X; a bulk read reaches 6.7 TB/s, an 8192^3 product 1.21 PFLOP/s):
+//   8001 rows from 0, 32 / 8 heads: 500-530 us, 0.99-1.05 PFLOP/s.  MFMAs take 54 % of a SIMD's
 //     cycles and VALU instructions as many beside them, at the 1.8-1.9 GHz that the card holds
-//     under this load; LDS 26 % of a CU's, no bank conflicts.
-//   16 x 26 nodes over 901 to 4001 slots, 16 / 8 heads: 46-49 us with the merge; 41 without, in which
-//     157 MB come from memory (3.8 TB/s) and waves wait 70 % of their time.
+//     under this load; LDS 27 % of a CU's, no bank conflicts.
+//   16 x 26 nodes over 901 to 4001 slots, 16 / 8 heads: 48 us with the merge; 42 without, in which
+//     164 MB come from memory (3.9 TB/s) and waves wait 67 % of their time.
+//   8 x 64 nodes over 15007 to 32003 slots, 32 / 8 heads: 318-345 us with the merge (10): MFMA 52 % of a
+//     SIMD's cycles, a third of them for the second words; 781 MB, 2.4 TB/s.
 //   16 prompts of 37 to 1021 rows: 29-32 us: first loads and outputs of items of up to 16 blocks.
 // Measured and dropped: one half's softmax beside the other half's products (8 % slower), priorities
 // around the products (1-3 %), scheduling groups and iglp (0-4 %), two waves sharing the blocks of a

@@ -55,7 +55,7 @@ inline PackedTable packed_items(const int32_t* lengths, const int32_t* starts, c
 //          ends; the parts of a cut tile are joined by a second launch.
 // Measured (us, whole / even; taken): 1999 rows from 6001, 32 / 8 heads 237 / 258 (whole); 1000 rows
 // from 6001 151 / 132 (even); 32 x 500 rows 129 / 213 (whole); 2000 rows from 0, 16 / 8 47 / 42
-// (even); 16 single rows from 4000 113 / 47, 4 of them 108 / 19 (even); 4 x 300 rows 11.4 / 16.5 (whole).
+// (even); 16 single rows from 4000, 4 q heads, 131 / 50, 4 of 2 126 / 19 (even); 4 x 300 rows 11.0 / 16.7 (whole).
 inline PackedTable packed_table(const int32_t* lengths, const int32_t* starts, const int32_t* cache_rows, int n, int G,
                                 int Hkv) {
   PackedTable t = packed_items(lengths, starts, cache_rows, n, G, Hkv);
