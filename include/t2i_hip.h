@@ -508,7 +508,8 @@ int t2i_prompt_advance(const int32_t* prompt, int32_t B, int32_t P, int32_t* tok
  *
  * t2i_packed_attention: row r of a sequence attends its slots 0 .. starts + r (causal;
  * fp32 scores and softmax, weights rounded to bf16 for the product with V, those of a
- * sequence of one row to 16 bits); q bf16 [rows, Hq, D], out bf16 [rows, Hq * D].  Slots that no row attends are never read.
+ * sequence of one row to 16 bits); q bf16 [rows, Hq, D], out bf16 [rows, Hq * D].
+ * Slots that no row attends are never read.
  * out_sums (nullable): fp32 [Hq][rows], as t2i_prefill_attention_sums.  The workspace
  * (t2i_packed_attention_workspace_bytes, 0: none needed) is scratch: no initial
  * value, nothing kept; calls that overlap in time must not share one.

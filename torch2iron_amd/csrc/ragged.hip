@@ -346,11 +346,11 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
 // rows round their weights once, as the batch form of the prompt pass does (8001 rows: 517 us,
 // with FINE 713).
 // In an MFMA a weight of 0 times an infinity or a NaN in V is a NaN, also for rows whose mask hides that
-// key.  An item with sums that are not finite is therefore run again, MASKED: blocks that some row does not
-// see whole and whose V holds such a value are multiplied key by key for the rows that attend it; FINE multiplies
-// its second words by V without such values, since they may be 0 or negative.  (500
-// rows from 1500, 16 / 8 heads, without such values 32 us, with a NaN in the last slot 76, in the first 46;
-// 1624 and 2384 where such rows were formed again from all of their keys.)
+// key.  An item with sums that are not finite is therefore run again, MASKED: blocks that some row does
+// not see whole and whose V holds such a value are multiplied key by key for the rows that attend it; FINE
+// multiplies its second words by V without such values, since they may be 0 or negative.  (500 rows from
+// 1500, 16 / 8 heads, without such values 32 us, with a NaN in the last slot 76, in the first 46; 1624 and
+// 2384 where such rows were formed again from all of their keys.)
 // K and V blocks go straight from memory into LDS, two buffers, one barrier a block; a row's
 // 16-byte chunk ch stands at place ch ^ (row % 16) (K) or ch ^ 4 (row % 4) (V): 16 neighbouring
 // lanes of a K read, 32 of a transposing read cover all banks (a load into LDS cannot pad rows,
