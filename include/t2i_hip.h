@@ -591,6 +591,52 @@ int t2i_token_logprobs(const void* logits, int32_t logits_type, int64_t row_stri
                        void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Rows of many sequences over a KV cache in pages.  k_pages / v_pages bf16 [n_pages, Hkv,
+ * page_slots, D]; slot j of sequence s is place j % page_slots of page pages[s][j / page_slots]
+ * (int32 [n_seqs, max_pages]; entries behind a sequence's last slot are never looked at, and several
+ * sequences may share a page).  Rows row_starts[s] .. row_starts[s + 1] - 1 (int32 [n_seqs + 1],
+ * ascending within 0 .. rows) are sequence s's; row r of them has position, and slot,
+ * context_lens[s] + r: a chunk of a prompt, a token to decode with drafted ones behind it, or one
+ * token.  All of these arrays are on the device, so that a captured step serves every later one.
+ * page_slots: a power of two, 16 to 65536; n_seqs at most 4096.
+ *
+ * t2i_paged_plan: the step's plan (t2i_paged_plan_words words on the device), which the two calls below
+ * take for every layer; made anew whenever row_starts or context_lens change.  A sequence whose
+ * context is negative or whose rows pass max_pages * page_slots has no slots.  row_starts that do not
+ * ascend: no row is anyone's.
+ *
+ * t2i_paged_qk_rope_kv: t2i_prefill_qk_rope_kv for these rows (the same bits); q_out bf16
+ * [rows, Hq, D].  A row without a slot, and rows that are no sequence's, write nothing; a row whose page
+ * lies outside the pool writes q alone.
+ *
+ * t2i_paged_attention: row r of a sequence attends its slots 0 .. context + r, whose k and v are in
+ * the pages by then; q bf16 [rows, Hq, D], out bf16 [rows, Hq * D], out_sums as
+ * t2i_packed_attention's.  fp32 scores and softmax; weights enter the product with V with 16 bits where
+ * a sequence's rows times Hq / Hkv are at most 128, else rounded to bf16.  Rows of a sequence without
+ * slots are zero, rows that are no sequence's stay as they are.  Slots that no row attends are never
+ * read.  Where a slot's page lies outside the pool the rows that attend it (and others of their sequence)
+ * are NaN.  The workspace (t2i_paged_attention_workspace_bytes) is scratch as t2i_packed_attention's.
+ * D = 128; Hq % Hkv == 0; Hq <= 1024.
+ * The reference's counterpart is its cache of 64-slot packets of one sequence
+ * (quantized_qwen3/batch_decode_fused.py:300-539).
+ */
+int64_t t2i_paged_plan_words(int32_t rows, int32_t n_seqs, int32_t Hq, int32_t Hkv);
+int t2i_paged_plan(const int32_t* row_starts, const int32_t* context_lens, int32_t n_seqs, int32_t rows,
+                   int32_t max_pages, int32_t page_slots, int32_t Hq, int32_t Hkv, int32_t* plan,
+                   int64_t plan_words, void* stream);
+int t2i_paged_qk_rope_kv(const uint16_t* qkv, int32_t rows, const int32_t* plan, int64_t plan_words,
+                         const int32_t* pages, int32_t n_seqs, int32_t max_pages, int32_t n_pages,
+                         int32_t page_slots, int32_t Hq, int32_t Hkv, int32_t D, const uint16_t* q_norm,
+                         const uint16_t* k_norm, float eps, const uint16_t* rope, int32_t rope_style,
+                         uint16_t* q_out, uint16_t* k_pages, uint16_t* v_pages, void* stream);
+size_t t2i_paged_attention_workspace_bytes(int32_t rows, int32_t Hq, int32_t Hkv);
+int t2i_paged_attention(const uint16_t* q, int32_t rows, const int32_t* plan, int64_t plan_words,
+                        const int32_t* pages, int32_t n_seqs, int32_t max_pages, int32_t n_pages,
+                        int32_t page_slots, int32_t Hq, int32_t Hkv, int32_t D, const uint16_t* k_pages,
+                        const uint16_t* v_pages, uint16_t* out, float* out_sums, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Measurement helper, no counterpart in the reference: the HBM read ceiling that
  * a linear's bandwidth is compared with.  Reads `bytes` (a positive multiple of
  * 16) from src with 16-byte loads, loads_per_thread (1, 2, 4 or 8) per thread in

@@ -125,6 +125,16 @@ SIGNATURES = {
     "t2i_token_logprobs_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
     "t2i_token_logprobs": (c_int32, [c_void_p, c_int32, c_int64, c_int32, c_int32, c_void_p, c_int32, c_void_p,
                                      c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "t2i_paged_plan_words": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
+    "t2i_paged_plan": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p,
+                                 c_int64, c_void_p]),
+    "t2i_paged_qk_rope_kv": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32,
+                                       c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_float, c_void_p,
+                                       c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "t2i_paged_attention_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "t2i_paged_attention": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_int32,
+                                      c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_size_t, c_void_p]),
     "t2i_stream_read_out_words": (ctypes.c_int64, [c_size_t, c_int32]),
     "t2i_stream_read": (c_int32, [c_void_p, c_size_t, c_int32, c_void_p, c_void_p]),
 }

@@ -1361,6 +1361,152 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, w
     return lp, entropy, top, ids
 
 
+# ---- a cache in pages ----
+class PagedPlan:
+    """A step of many sequences over a KV cache in pages: ``rows`` packed rows, of which
+    ``row_starts[s] .. row_starts[s + 1] - 1`` (int32 ``[S + 1]``) are sequence s's new tokens (a chunk of a
+    prompt, a token with drafted ones behind it, one token, or none) behind its ``context_lens[s]`` (int32
+    ``[S]``) slots.  Slot j of sequence s is place ``j % page_slots`` of page ``page_table[s, j // page_slots]``
+    (int32 ``[S, max_pages]``; entries behind the last slot in use are never looked at, and sequences may
+    share pages); ``page_slots`` a power of two from 16 on.
+
+    All three are device tensors, which the plan keeps and reads again: after a change of
+    ``row_starts`` or ``context_lens`` call ``refresh`` (one launch, which can be captured: a captured step
+    then serves every later one).  A sequence whose context is negative or whose rows pass ``max_pages *
+    page_slots`` has no slots: it writes none and its attention rows are zero.  ``row_starts`` that do not
+    ascend within ``0 .. rows`` give no sequence any rows.
+
+    One plan serves every layer of the step; keep it as long as a captured call may be replayed."""
+
+    def __init__(self, rows: int, row_starts: torch.Tensor, context_lens: torch.Tensor, page_table: torch.Tensor,
+                 n_heads: int, n_kv_heads: int, page_slots: int):
+        for n, t in (("row_starts", row_starts), ("context_lens", context_lens), ("page_table", page_table)):
+            _check_dev(n, t, torch.int32)
+        if page_table.dim() != 2 or page_table.shape[0] < 1 or page_table.shape[1] < 1:
+            raise ValueError("page_table must be [sequences, pages of a sequence]")
+        rows, n_heads, n_kv_heads, page_slots = _integers("rows, n_heads, n_kv_heads and page_slots",
+                                                          (rows, n_heads, n_kv_heads, page_slots))
+        self.n_seqs, self.max_pages = page_table.shape
+        if row_starts.numel() != self.n_seqs + 1 or context_lens.numel() != self.n_seqs:
+            raise ValueError(f"row_starts must hold {self.n_seqs + 1} values and context_lens {self.n_seqs}")
+        if not 0 <= rows < 2**31 or not 1 <= n_heads <= 1024 or not 1 <= n_kv_heads <= n_heads or n_heads % n_kv_heads:
+            raise ValueError(f"{rows} rows of {n_heads} heads over {n_kv_heads} kv heads are unsupported")
+        if not 16 <= page_slots <= 65536 or page_slots & (page_slots - 1):
+            raise ValueError(f"page_slots must be a power of two from 16 to 65536, got {page_slots}")
+        self.device = page_table.device
+        _same_device(self.device, row_starts=row_starts, context_lens=context_lens)
+        self.rows, self.n_heads, self.n_kv_heads, self.page_slots = rows, n_heads, n_kv_heads, page_slots
+        self.row_starts, self.context_lens, self.page_table = row_starts, context_lens, page_table
+        self._words = 0
+        if rows == 0:
+            return
+        lib = _lib.load()
+        self._words = lib.t2i_paged_plan_words(rows, self.n_seqs, n_heads, n_kv_heads)
+        if self._words <= 0:
+            raise ValueError(f"a step of {rows} rows of {self.n_seqs} sequences is too large (at most 4096 sequences)")
+        self._nbytes = lib.t2i_paged_attention_workspace_bytes(rows, n_heads, n_kv_heads)
+        self._stream = _lib.stream_handle(self.device)
+        self.table = torch.empty(self._words, dtype=torch.int32, device=self.device)
+        self.refresh()
+
+    def refresh(self):
+        """The plan of what ``row_starts`` and ``context_lens`` hold by now (on the current stream)."""
+        if self.rows:
+            self._use()
+            _launch(self.device, "t2i_paged_plan",
+                    self.row_starts.data_ptr(), self.context_lens.data_ptr(), self.n_seqs, self.rows, self.max_pages,
+                    self.page_slots, self.n_heads, self.n_kv_heads, self.table.data_ptr(), self._words)
+
+    def _use(self):
+        """The plan's memory waits for the current stream before it is given to another tensor."""
+        if _lib.stream_handle(self.device) != self._stream:
+            stream = torch.cuda.current_stream(self.device)
+            for t in (self.table, self.row_starts, self.context_lens, self.page_table):
+                t.record_stream(stream)
+
+    def _check(self, k_pages, v_pages, d: int):
+        _check_dev("k_pages", k_pages, BF16)
+        _check_dev("v_pages", v_pages, BF16)
+        want = (self.n_kv_heads, self.page_slots, d)
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[0] < 1 or tuple(k_pages.shape[1:]) != want:
+            raise ValueError(f"k_pages and v_pages must be [pages, {want[0]}, {want[1]}, {d}] of equal shape")
+        if k_pages.shape[0] >= 2**31:
+            raise ValueError(f"a pool of {k_pages.shape[0]} pages is too large")
+
+    def _args(self):
+        return self.table.data_ptr(), self._words, self.page_table.data_ptr(), self.n_seqs, self.max_pages
+
+
+def paged_qk_rope_kv(qkv: torch.Tensor, plan: PagedPlan, q_norm: torch.Tensor, k_norm: torch.Tensor, eps: float,
+                     rope: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, rope_style: int = ROPE_HALVES,
+                     q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``prefill_qk_rope_kv`` for the rows of ``plan`` (the same bits): q/k RMSNorm + RoPE at each row's
+    position and the write of its k and v into its sequence's page.
+
+    ``qkv`` bf16 ``[rows, (Hq + 2 Hkv) * D]``, ``k_pages`` and ``v_pages`` bf16 ``[pages, Hkv, page_slots, D]``, ``rope``
+    with a row for each of a sequence's ``max_pages * page_slots`` slots; returns q bf16 ``[rows, Hq, D]``.
+    Rows without a slot are left as they are, in ``q_out`` too; a row whose page id lies outside the pool
+    writes its q alone."""
+    for n, t in (("qkv", qkv), ("q_norm", q_norm), ("k_norm", k_norm), ("rope", rope)):
+        _check_dev(n, t, BF16)
+    d = q_norm.numel()
+    plan._check(k_pages, v_pages, d)
+    if k_norm.numel() != d:
+        raise ValueError("q_norm and k_norm must both hold head_dim values")
+    if qkv.numel() != plan.rows * (plan.n_heads + 2 * plan.n_kv_heads) * d:
+        raise ValueError("qkv must be [rows, (Hq + 2 Hkv) * D]")
+    if rope.dim() != 2 or rope.shape[0] < plan.max_pages * plan.page_slots or rope.shape[1] != d:
+        raise ValueError(f"rope table must be [>= {plan.max_pages * plan.page_slots}, D], a row for every slot of a sequence")
+    if q_out is None:
+        q_out = torch.empty(plan.rows, plan.n_heads, d, dtype=BF16, device=qkv.device)
+    _check_dev("q_out", q_out, BF16)
+    if q_out.numel() != plan.rows * plan.n_heads * d:
+        raise ValueError("q_out must be [rows, Hq, D]")
+    _same_device(plan.device, qkv=qkv, q_norm=q_norm, k_norm=k_norm, rope=rope, k_pages=k_pages, v_pages=v_pages,
+                 q_out=q_out)
+    if plan.rows == 0:
+        return q_out
+    plan._use()
+    _launch(plan.device, "t2i_paged_qk_rope_kv",
+            qkv.data_ptr(), plan.rows, *plan._args(), k_pages.shape[0], plan.page_slots, plan.n_heads, plan.n_kv_heads, d,
+            q_norm.data_ptr(), k_norm.data_ptr(), float(eps), rope.data_ptr(), int(rope_style), q_out.data_ptr(),
+            k_pages.data_ptr(), v_pages.data_ptr())
+    return q_out
+
+
+def paged_attention(q: torch.Tensor, plan: PagedPlan, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                    out: torch.Tensor | None = None, out_sums: torch.Tensor | None = None,
+                    workspace: Workspace | None = None) -> torch.Tensor:
+    """Causal GQA attention of the rows of ``plan`` (``q [rows, Hq, D]``) over the pages: row r of sequence s over its
+    slots ``0 .. context_lens[s] + r``, whose k and v stand in the pages by then (``paged_qk_rope_kv``).
+    Returns bf16 ``[rows, Hq * D]``; ``out_sums`` (fp32 ``[Hq, rows]``) as ``prefill_attention``.
+
+    Slots that no row attends are never read.  Rows of a sequence without slots are zero, rows that are no
+    sequence's are left as they are (unset without ``out``), and a page id outside the pool makes the rows that
+    attend it NaN (and others of their sequence)."""
+    _check_dev("q", q, BF16)
+    if q.dim() != 3 or q.shape[0] != plan.rows or q.shape[1] != plan.n_heads:
+        raise ValueError(f"q must be [{plan.rows}, {plan.n_heads}, D], as the plan was made for")
+    d = q.shape[2]
+    plan._check(k_pages, v_pages, d)
+    if out is None:
+        out = torch.empty(plan.rows, plan.n_heads * d, dtype=BF16, device=q.device)
+    _check_dev("out", out, BF16)
+    if out.numel() != plan.rows * plan.n_heads * d:
+        raise ValueError("out must be [rows, Hq * D]")
+    if out_sums is not None:
+        _check_sums("out_sums", out_sums, plan.rows, plan.n_heads)
+    _same_device(plan.device, q=q, k_pages=k_pages, v_pages=v_pages, out=out, out_sums=out_sums)
+    if plan.rows == 0:
+        return out
+    ws = _scratch(workspace, "paged_attn", plan._nbytes, q.device)
+    plan._use()
+    _launch(plan.device, "t2i_paged_attention",
+            q.data_ptr(), plan.rows, *plan._args(), k_pages.shape[0], plan.page_slots, plan.n_heads, plan.n_kv_heads, d,
+            k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _lib.ptr(out_sums), _lib.ptr(ws), plan._nbytes)
+    return out
+
+
 def stream_read(src, nbytes: int | None = None, offset: int = 0, loads_per_thread: int = 4, out=None):
     """Read ``nbytes`` of ``src`` from byte ``offset`` with the HBM read-ceiling
     kernel (``t2i_stream_read``) and return the per-wave XOR words (uint32 bit
