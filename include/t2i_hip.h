@@ -637,6 +637,34 @@ int t2i_paged_attention(const uint16_t* q, int32_t rows, const int32_t* plan, in
                         size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Drafted tokens held to the model's probabilities with given random numbers, and the next token
+ * drawn.  Rows row_starts[s] .. row_starts[s + 1] - 1 (int32 [n_seqs + 1]) of M rows of V logits (types and
+ * alignment as t2i_token_logprobs) are sequence s's: row i gives p_i = softmax(logits / T),
+ * tokens[row + 1] is the draft behind every row but the last, taken from q = draft_probs[row] (fp32 rows
+ * probs_stride apart, those of last rows never read; NULL: from a distribution that is 1 at the draft), T =
+ * temperatures[s] (NULL: 1).
+ * A draft y stays where uniforms[row] * q(y) < p(y).  Behind the first that does not stay the next token is
+ * drawn from max(p - q, 0) of that row (from p, where nothing is left of it), else from the last row's p: the
+ * first token whose running sum passes uniforms[last row] times the whole sum (the last with a weight, for a number of
+ * 1 or more).  T not above 0: a draft stays where it is the first of the row's largest logits, which else is
+ * the next token.  A sequence of one row samples.
+ * counts [n_seqs]: drafts that stay; next_tokens [n_seqs]; logprobs [M]: behind rows first .. first + count
+ * the log probability (at T, or at 1 where T is not above 0) of the token that came out there, 0 behind the other rows.
+ * Logits of -inf have probability 0.  Behind a row that holds a NaN or +inf, or nothing but -inf, no draft
+ * stays, the next token is -1 and its log probability NaN.  A draft outside [0, V) does not stay.  A sequence
+ * without rows (or whose rows do not lie in the batch): count 0, next token -1.
+ * Weights and sums are fp64.  The workspace (t2i_verify_drafts_workspace_bytes) is scratch as for
+ * t2i_packed_attention.  n_seqs at most 2^20.
+ * No counterpart in the reference, which decodes greedily (qwen_npu.py:321).
+ */
+size_t t2i_verify_drafts_workspace_bytes(int32_t M, int32_t V, int32_t n_seqs, int32_t with_probs);
+int t2i_verify_drafts(const void* logits, int32_t logits_type, int64_t row_stride, int32_t M, int32_t V,
+                      const int32_t* row_starts, int32_t n_seqs, const int32_t* tokens, const float* uniforms,
+                      const float* draft_probs, int64_t probs_stride, const float* temperatures,
+                      int32_t* counts, int32_t* next_tokens, float* logprobs, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Measurement helper, no counterpart in the reference: the HBM read ceiling that
  * a linear's bandwidth is compared with.  Reads `bytes` (a positive multiple of
  * 16) from src with 16-byte loads, loads_per_thread (1, 2, 4 or 8) per thread in

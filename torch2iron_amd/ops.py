@@ -1317,6 +1317,27 @@ def tree_commit(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     return path.view(b, n), counts, nxt, context
 
 
+def _check_rows(name: str, t: torch.Tensor):
+    """``[M, V]`` rows, contiguous within and apart from each other; returns ``(M, V, row stride)``."""
+    if t.dim() != 2 or t.shape[1] < 1:
+        raise ValueError(f"{name} must be [M, V]")
+    m, v = t.shape
+    if max(m, v) >= 2**31:
+        raise ValueError(f"{m} rows of {v} {name} are too many")
+    stride = t.stride(0) if m > 1 else v
+    if (v > 1 and t.stride(1) != 1) or stride < v:
+        raise ValueError(f"{name} rows must be contiguous and must not overlap")
+    return m, v, stride
+
+
+def _check_logits(logits: torch.Tensor):
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        raise ValueError("logits must be a GPU tensor (the W4A16 path has no CPU fallback)")
+    if logits.dtype not in _LOGITS_TYPES:
+        raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    return _check_rows("logits", logits)
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, workspace: Workspace | None = None):
     """Log probabilities of ``tokens`` (int32 ``[M]``) under the rows of ``logits`` (fp32, bf16 or
     fp16 ``[M, V]``; rows may be strided), each row's entropy (nats), and its ``top_k`` (0 to 32)
@@ -1326,18 +1347,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top_k: int = 0, w
     int32; alternatives best first, the lower index first among equal logits.  A token outside
     ``[0, V)`` (padding) gives 0.  Logits of -inf have probability 0; a row with a NaN, a +inf
     or nothing but -inf gives NaN."""
-    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
-        raise ValueError("logits must be a GPU tensor (the W4A16 path has no CPU fallback)")
-    if logits.dtype not in _LOGITS_TYPES:
-        raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-    if logits.dim() != 2 or logits.shape[1] < 1:
-        raise ValueError("logits must be [M, V]")
-    m, v = logits.shape
-    if max(m, v) >= 2**31:
-        raise ValueError(f"{m} rows of {v} logits are too many")
-    stride = logits.stride(0) if m > 1 else v
-    if (v > 1 and logits.stride(1) != 1) or stride < v:
-        raise ValueError("logits rows must be contiguous and must not overlap")
+    m, v, stride = _check_logits(logits)
     _check_dev("tokens", tokens, torch.int32)
     if tokens.numel() != m:
         raise ValueError(f"tokens must hold {m} ids")
@@ -1505,6 +1515,65 @@ def paged_attention(q: torch.Tensor, plan: PagedPlan, k_pages: torch.Tensor, v_p
             q.data_ptr(), plan.rows, *plan._args(), k_pages.shape[0], plan.page_slots, plan.n_heads, plan.n_kv_heads, d,
             k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), _lib.ptr(out_sums), _lib.ptr(ws), plan._nbytes)
     return out
+
+
+def verify_drafts(logits: torch.Tensor, row_starts: torch.Tensor, tokens: torch.Tensor, uniforms: torch.Tensor,
+                  draft_probs: torch.Tensor | None = None, temperatures: torch.Tensor | None = None,
+                  workspace: Workspace | None = None):
+    """Drafted tokens held to the model's probabilities with given random numbers, and the token after them drawn:
+    what comes out is distributed as the model's own samples.  A sequence of one row samples.
+
+    Rows ``row_starts[s] .. row_starts[s + 1] - 1`` (int32 ``[S + 1]``) of ``logits`` (fp32, bf16 or fp16 ``[M, V]``;
+    rows may be strided) are sequence s's, ``tokens`` int32 ``[M]`` the tokens that they stand behind: the draft after
+    a row is the next row's token.  ``draft_probs`` fp32 ``[M, V]``: the distribution that the draft after a row was drawn from (rows
+    that have none are never read); without it drafts count as certain (looked up, or a small model's greedy choice).
+    ``uniforms`` fp32 ``[M]`` in [0, 1): the number behind a draft decides on it, the one of the last row
+    draws the next token.  ``temperatures`` fp32 ``[S]`` (1 without); not above 0: greedy.
+
+    With p = softmax(logits / T) and q a row of ``draft_probs``, a draft y stays where ``u * q[y] < p[y]``, up to the
+    first that does not; the next token is drawn from ``max(p - q, 0)`` of that row, else from the last row's p, as the first token whose
+    running sum passes u times the whole.  fp64 throughout.  Returns int32 ``counts [S]`` (drafts that stay), int32 ``next_tokens
+    [S]``, fp32 ``logprobs [M]`` (log p of the token that came out behind each row, 0 behind the rest; greedy rows at T = 1).
+
+    Logits of -inf have probability 0; a row with a NaN, a +inf or nothing but -inf ends its sequence with the token -1
+    and log probability NaN.  A draft outside ``[0, V)`` does not stay.  A sequence without rows: count 0, token -1."""
+    m, v, stride = _check_logits(logits)
+    for n, t, dtype in (("row_starts", row_starts, torch.int32), ("tokens", tokens, torch.int32),
+                        ("uniforms", uniforms, torch.float32)):
+        _check_dev(n, t, dtype)
+    n_seqs = row_starts.numel() - 1
+    if n_seqs < 1:
+        raise ValueError("row_starts must hold at least two values")
+    if tokens.numel() != m or uniforms.numel() != m:
+        raise ValueError(f"tokens and uniforms must hold {m} values")
+    dev, probs_stride = logits.device, 0
+    if draft_probs is not None:
+        if not isinstance(draft_probs, torch.Tensor) or draft_probs.dtype != torch.float32:
+            raise ValueError("draft_probs must be a float32 tensor")
+        if tuple(draft_probs.shape) != (m, v):
+            raise ValueError(f"draft_probs must be [{m}, {v}], as the logits")
+        probs_stride = _check_rows("draft_probs", draft_probs)[2]
+    if temperatures is not None:
+        _check_dev("temperatures", temperatures, torch.float32)
+        if temperatures.numel() != n_seqs:
+            raise ValueError(f"temperatures must hold {n_seqs} values")
+    _same_device(dev, row_starts=row_starts, tokens=tokens, uniforms=uniforms, draft_probs=draft_probs,
+                 temperatures=temperatures)
+    rec = torch.empty(2 * n_seqs, dtype=torch.int32, device=dev)   # one allocation for the two
+    counts, nxt = rec.split((n_seqs, n_seqs))
+    logprobs = torch.empty(m, dtype=torch.float32, device=dev)
+    if m == 0:
+        counts.zero_()
+        nxt.fill_(-1)
+        return counts, nxt, logprobs
+    lib = _lib.load()
+    nbytes = lib.t2i_verify_drafts_workspace_bytes(m, v, n_seqs, draft_probs is not None)
+    ws = _scratch(workspace, "verify", nbytes, dev)
+    _launch(dev, "t2i_verify_drafts",
+            logits.data_ptr(), _LOGITS_TYPES[logits.dtype], stride, m, v, row_starts.data_ptr(), n_seqs, tokens.data_ptr(),
+            uniforms.data_ptr(), _lib.ptr(draft_probs), probs_stride, _lib.ptr(temperatures), counts.data_ptr(),
+            nxt.data_ptr(), logprobs.data_ptr(), _lib.ptr(ws), nbytes)
+    return counts, nxt, logprobs
 
 
 def stream_read(src, nbytes: int | None = None, offset: int = 0, loads_per_thread: int = 4, out=None):
