@@ -665,6 +665,33 @@ int t2i_verify_drafts(const void* logits, int32_t logits_type, int64_t row_strid
                       size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a shared projection.
+ *
+ * t2i_adapter_plan: the M rows of a step by their adapters ids[row] (0 .. n_adapters - 1, at most 511;
+ * any other id: none), as t2i_adapter_plan_words words on the device, for every projection of the step.
+ *
+ * t2i_adapter_add: out[r] = y[r] + scales[a] * B_a (A_a x[r]) with a = ids[r], y[r] itself for rows without an
+ * adapter; y bf16 [M, N] is the shared projection's output, x bf16 [M, K] its input, out may be y.  a bf16
+ * [n_adapters, parts * R, K] and b bf16 [n_adapters, N, R] with R = rank (1 to 256) rounded up to a
+ * multiple of 16, the places behind rank 0; scales fp32 [n_adapters] (NULL: 1).  The columns may be several
+ * projections' beside each other (parts up to 4): slice i of widths[i] columns (host memory; multiples
+ * of 64, parts 1: NULL) has rows i * R .. of a; or, paired (parts 2), alternate between them (column 2j of slice 0, gate, column
+ * 2j + 1 of slice 1, up; as t2i_w4a16_gate_up without SwiGLU leaves them interleaved in one linear).  swiglu (paired alone): out
+ * bf16 [M, N / 2] = silu(gate) * up.  Sums are fp32, A x enters the second product with 16 bits, the result is rounded
+ * once.  The workspace (t2i_adapter_add_workspace_bytes) is scratch as t2i_packed_attention's.
+ * K % 32 == 0, N % 16 == 0.
+ * No counterpart in the reference, which has one set of weights.
+ */
+int64_t t2i_adapter_plan_words(int32_t M, int32_t n_adapters);
+int t2i_adapter_plan(const int32_t* ids, int32_t M, int32_t n_adapters, int32_t* plan, int64_t plan_words,
+                     void* stream);
+size_t t2i_adapter_add_workspace_bytes(int32_t M, int32_t parts, int32_t rank);
+int t2i_adapter_add(const uint16_t* y, const uint16_t* x, int32_t M, int32_t K, int32_t N, const int32_t* plan,
+                    int64_t plan_words, const uint16_t* a, const uint16_t* b, const float* scales,
+                    int32_t n_adapters, int32_t rank, int32_t parts, const int32_t* widths, int32_t paired,
+                    int32_t swiglu, uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Measurement helper, no counterpart in the reference: the HBM read ceiling that
  * a linear's bandwidth is compared with.  Reads `bytes` (a positive multiple of
  * 16) from src with 16-byte loads, loads_per_thread (1, 2, 4 or 8) per thread in

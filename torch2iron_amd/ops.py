@@ -999,6 +999,7 @@ def prompt_advance(prompt, tokens, positions):
 # ---- ragged batches: packed prompts, drafted trees, token probabilities ----
 MAX_TREE_NODES = 64
 MAX_TOP_K = 32
+MAX_ADAPTERS = 511
 _LOGITS_TYPES = {torch.float32: _lib.T2I_LOGITS_FP32, torch.bfloat16: _lib.T2I_LOGITS_BF16,
                  torch.float16: _lib.T2I_LOGITS_FP16}
 
@@ -1574,6 +1575,150 @@ def verify_drafts(logits: torch.Tensor, row_starts: torch.Tensor, tokens: torch.
             uniforms.data_ptr(), _lib.ptr(draft_probs), probs_stride, _lib.ptr(temperatures), counts.data_ptr(),
             nxt.data_ptr(), logprobs.data_ptr(), _lib.ptr(ws), nbytes)
     return counts, nxt, logprobs
+
+
+# ---- adapters of many requests ----
+class Adapters:
+    """A pool of low-rank adapters of one projection: adapter i adds ``scales[i] * B_i (A_i x)`` to its output.
+
+    ``a`` bf16 ``[n, R, K]``, ``b`` bf16 ``[n, N, R]`` (n up to 511, R up to 256, K a multiple of 32, N of 16), ``scales``
+    fp32 ``[n]`` (1 by default).  Of a fused projection: ``a [n, slices, R, K]``, ``b``'s rows in the order of the fused columns, and either
+    ``widths`` (the columns of up to 4 projections beside each other, multiples of 64, as q|k|v) or ``paired=True`` (two
+    projections' columns in turn, as ``formats.interleave_gate_up``).  Smaller ranks among them: zeros in the last places.
+
+    The pool keeps its own copy, laid out once; ``put`` replaces one adapter's values in place, so captured calls keep serving."""
+
+    def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor | None = None, widths=None,
+                 paired: bool = False):
+        for n, t in (("a", a), ("b", b)):
+            _check_dev(n, t, BF16)
+        if a.dim() == 3:
+            a = a.unsqueeze(1)
+        if a.dim() != 4 or b.dim() != 3 or b.shape[0] != a.shape[0] or b.shape[2] != a.shape[2]:
+            raise ValueError("a must be [n, R, K] or [n, slices, R, K], and b [n, N, R]")
+        self.n, self.parts, self.rank, self.K = a.shape
+        self.N, self.paired = b.shape[1], bool(paired)
+        if not 1 <= self.n <= MAX_ADAPTERS or not 1 <= self.rank <= 256:
+            raise ValueError(f"1 to {MAX_ADAPTERS} adapters of rank 1 to 256, got {self.n} of {self.rank}")
+        if self.K < 32 or self.K % 32 or self.N < 16 or self.N % 16 or max(self.K, self.N) > 2**20:
+            raise ValueError(f"K={self.K} must be a multiple of 32 and N={self.N} of 16")
+        if paired and (self.parts != 2 or widths is not None):
+            raise ValueError("paired columns have two slices and no widths")
+        if not paired:
+            widths = [self.N] if widths is None else _integers("widths", widths)
+            if len(widths) != self.parts or sum(widths) != self.N:
+                raise ValueError(f"widths must hold {self.parts} values that make {self.N} columns")
+            if self.parts > 4 or (self.parts > 1 and any(w < 64 or w % 64 for w in widths)):
+                raise ValueError("up to 4 slices of multiples of 64 columns")
+        # host memory, also where torch's default device is another
+        self.widths = None if paired else torch.tensor(widths, dtype=torch.int32, device="cpu")
+        self.device = a.device
+        pad = -self.rank % 16
+        self.a = torch.nn.functional.pad(a, (0, 0, 0, pad)).reshape(self.n, -1, self.K).contiguous().clone()
+        self.b = torch.nn.functional.pad(b, (0, pad)).contiguous().clone()
+        if scales is None:
+            scales = torch.ones(self.n, dtype=torch.float32, device=self.device)
+        _check_dev("scales", scales, torch.float32)
+        if scales.numel() != self.n:
+            raise ValueError(f"scales must hold {self.n} values")
+        self.scales = scales.reshape(-1).clone()
+        _same_device(self.device, b=b, scales=scales)
+
+    def put(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0):
+        """Adapter ``slot`` becomes ``a`` (``[R, K]`` or ``[slices, R, K]``), ``b`` (``[N, R]``), ``scale``; a smaller rank
+        leaves the places behind it 0."""
+        slot = _integers("slot", (slot,))[0]
+        if not 0 <= slot < self.n:
+            raise ValueError(f"slot must be 0 to {self.n - 1}, got {slot}")
+        for n, t in (("a", a), ("b", b)):
+            if not isinstance(t, torch.Tensor) or t.dtype != BF16:
+                raise ValueError(f"{n} must be a bfloat16 tensor")
+        a = a.unsqueeze(0) if a.dim() == 2 else a
+        if a.dim() != 3 or a.shape[0] != self.parts or a.shape[2] != self.K or not 1 <= a.shape[1] <= self.rank:
+            raise ValueError(f"a must be [{self.parts}, up to {self.rank}, {self.K}]")
+        if tuple(b.shape) != (self.N, a.shape[1]):
+            raise ValueError(f"b must be [{self.N}, {a.shape[1]}]")
+        r = a.shape[1]
+        mine = self.a[slot].view(self.parts, -1, self.K)
+        mine[:, :r].copy_(a)
+        mine[:, r:].zero_()
+        self.b[slot, :, :r].copy_(b)
+        self.b[slot, :, r:].zero_()
+        self.scales[slot].fill_(float(scale))
+
+
+class AdapterPlan:
+    """The rows of a step by their adapters: ``ids`` int32 ``[M]`` on the device, an adapter's number below
+    ``n_adapters`` or anything else for none.  The plan keeps ``ids`` and reads them again in ``refresh`` (one launch, which
+    can be captured).  One plan serves every projection of the step whose pool has ``n_adapters`` adapters; keep it as
+    long as a captured call may be replayed."""
+
+    def __init__(self, ids: torch.Tensor, n_adapters: int):
+        _check_dev("ids", ids, torch.int32)
+        if ids.dim() != 1:
+            raise ValueError("ids must be [M]")
+        n_adapters = _integers("n_adapters", (n_adapters,))[0]
+        if not 1 <= n_adapters <= MAX_ADAPTERS:
+            raise ValueError(f"1 to {MAX_ADAPTERS} adapters, got {n_adapters}")
+        self.rows, self.n, self.ids, self.device = ids.numel(), n_adapters, ids, ids.device
+        if self.rows == 0:
+            return
+        if self.rows >= 2**24:
+            raise ValueError(f"{self.rows} rows are too many")
+        self._words = _lib.load().t2i_adapter_plan_words(self.rows, n_adapters)
+        self._stream = _lib.stream_handle(self.device)
+        self.table = torch.empty(self._words, dtype=torch.int32, device=self.device)
+        self.refresh()
+
+    def refresh(self):
+        """The plan of what ``ids`` hold by now (on the current stream)."""
+        if self.rows:
+            self._use()
+            _launch(self.device, "t2i_adapter_plan", self.ids.data_ptr(), self.rows, self.n, self.table.data_ptr(),
+                    self._words)
+
+    def _use(self):
+        """The plan's memory waits for the current stream before it is given to another tensor."""
+        if _lib.stream_handle(self.device) != self._stream:
+            for t in (self.table, self.ids):
+                t.record_stream(torch.cuda.current_stream(self.device))
+
+
+def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: AdapterPlan, out: torch.Tensor | None = None,
+                swiglu: bool = False, workspace: Workspace | None = None) -> torch.Tensor:
+    """``y`` (bf16 ``[M, N]``, a shared projection of ``x`` bf16 ``[M, K]``) plus each row's adapter of ``x``; in
+    place without ``out``.  ``swiglu`` (paired columns): bf16 ``[M, N / 2]`` of silu(gate) * up, a tensor of its own.
+
+    fp32 sums, one rounding of the result: rows without an adapter keep their bits (with ``swiglu`` they are ``gate_up``'s
+    up to its two more roundings)."""
+    if not isinstance(adapters, Adapters) or not isinstance(plan, AdapterPlan):
+        raise ValueError("adapters must be an Adapters and plan an AdapterPlan")
+    _check_dev("y", y, BF16)
+    _check_dev("x", x, BF16)
+    m, n, k = plan.rows, adapters.N, adapters.K
+    if plan.n != adapters.n:
+        raise ValueError(f"the plan is for {plan.n} adapters, the pool has {adapters.n}")
+    if tuple(x.shape) != (m, k) or tuple(y.shape) != (m, n):
+        raise ValueError(f"x must be [{m}, {k}] and y [{m}, {n}]")
+    if swiglu and not adapters.paired:
+        raise ValueError("SwiGLU needs paired columns")
+    if out is None:
+        out = torch.empty(m, n // 2, dtype=BF16, device=y.device) if swiglu else y
+    _check_dev("out", out, BF16)
+    if tuple(out.shape) != (m, n // 2 if swiglu else n):
+        raise ValueError(f"out must be [{m}, {n // 2 if swiglu else n}]")
+    _same_device(adapters.device, y=y, x=x, out=out, ids=plan.ids)
+    if m == 0:
+        return out
+    lib = _lib.load()
+    nbytes = lib.t2i_adapter_add_workspace_bytes(m, adapters.parts, adapters.rank)
+    ws = _scratch(workspace, "adapters", nbytes, y.device)
+    plan._use()
+    _launch(y.device, "t2i_adapter_add",
+            y.data_ptr(), x.data_ptr(), m, k, n, plan.table.data_ptr(), plan._words, adapters.a.data_ptr(),
+            adapters.b.data_ptr(), adapters.scales.data_ptr(), adapters.n, adapters.rank, adapters.parts,
+            _lib.ptr(adapters.widths), adapters.paired, swiglu, out.data_ptr(), _lib.ptr(ws), nbytes)
+    return out
 
 
 def stream_read(src, nbytes: int | None = None, offset: int = 0, loads_per_thread: int = 4, out=None):
