@@ -286,6 +286,95 @@ class PromptScore(NamedTuple):
     top_ids: torch.Tensor        # [n, top_k]
 
 
+class LayerAdapters(NamedTuple):
+    """The pools of one layer's adapted projections (all of one size; None: the projection has none)."""
+
+    qkv: ops.Adapters | None = None        # three slices: q, k and v columns
+    o: ops.Adapters | None = None
+    gate_up: ops.Adapters | None = None    # paired
+    down: ops.Adapters | None = None
+
+
+class PagedCache:
+    """K and V of many requests in pages of ``page_slots`` tokens, for ``Qwen3Model.paged_step``: pools bf16
+    ``[layers, n_pages, Hkv, page_slots, D]``, a page table int32 ``[n_seqs, max_pages]`` (-1: none) and the slots in use
+    ``lens`` int32 ``[n_seqs]`` on the device; the free pages on the host."""
+
+    def __init__(self, cfg: Qwen3Config, n_seqs: int, n_pages: int, max_pages: int, device, page_slots: int = 32):
+        if min(n_seqs, n_pages, max_pages) < 1:
+            raise ValueError("a cache has at least one sequence and one page")
+        shape = (cfg.n_layers, n_pages, cfg.n_kv_heads, page_slots, cfg.head_dim)
+        self.k, self.v = (torch.zeros(shape, dtype=BF16, device=device) for _ in range(2))
+        self.table = torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(n_seqs, dtype=torch.int32, device=device)
+        self.n_seqs, self.n_pages, self.max_pages, self.page_slots = n_seqs, n_pages, max_pages, page_slots
+        self._free = list(range(n_pages - 1, -1, -1))
+        self._held: list[list[int]] = [[] for _ in range(n_seqs)]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def reserve(self, seq: int, slots: int) -> None:
+        """Pages for sequence ``seq`` up to ``slots`` slots in all (those it has stay).  ``ValueError`` past its part of
+        the table; ``RuntimeError``, and nothing given out, where the pool has not that many left."""
+        if not 0 <= seq < self.n_seqs or slots < 0 or slots > self.max_pages * self.page_slots:
+            raise ValueError(f"sequence {seq} of {self.n_seqs} with {slots} slots, at most {self.max_pages * self.page_slots}")
+        held = self._held[seq]
+        more = -(-slots // self.page_slots) - len(held)
+        if more <= 0:
+            return
+        if more > len(self._free):
+            raise RuntimeError(f"{more} pages needed, {len(self._free)} free")
+        new = [self._free.pop() for _ in range(more)]
+        self.table[seq, len(held):len(held) + more] = torch.tensor(new, dtype=torch.int32)
+        held += new
+
+    def release(self, seq: int) -> None:
+        """Sequence ``seq`` is empty again and its pages free."""
+        if not 0 <= seq < self.n_seqs:
+            raise ValueError(f"sequence {seq} of {self.n_seqs}")
+        self._free += reversed(self._held[seq])
+        self._held[seq] = []
+        self.table[seq] = -1
+        self.lens[seq] = 0
+
+
+class PagedBatch:
+    """What a step takes of each sequence of a ``PagedCache``: ``rows[s]`` tokens (0: none), the last ``drafts[s]`` of
+    them drafted (0 by default, less than ``rows[s]`` where there are any).  Host integers; made once, it serves every step
+    of that shape (keep it as long as a captured step may be replayed).
+
+    ``rows``: tokens in all; ``head_rows``: those whose logits are formed, a sequence's last drafts + 1."""
+
+    def __init__(self, rows, drafts=None, device="cuda"):
+        rows = ops._integers("rows", rows)
+        drafts = [0] * len(rows) if drafts is None else ops._integers("drafts", drafts)
+        if not rows or len(drafts) != len(rows):
+            raise ValueError("rows must hold at least one sequence, and drafts one entry for each")
+        if any(r < 0 or d < 0 or d > max(r - 1, 0) for r, d in zip(rows, drafts)):
+            raise ValueError("every sequence has drafts of 0 to its rows - 1")
+        ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cpu").to(device)  # noqa: E731
+        ends = np.cumsum([0] + rows).tolist()
+        heads = [range(e - d - 1, e) for e, d, r in zip(ends[1:], drafts, rows) if r]
+        self.n_seqs, self.rows = len(rows), ends[-1]
+        self.row_starts = ints(ends)
+        self.row_seq = ints([s for s, r in enumerate(rows) for _ in range(r)]).long()
+        self.head_rows = ints([i for h in heads for i in h])
+        self.head_starts = ints(np.cumsum([0] + [d + 1 if r else 0 for r, d in zip(rows, drafts)]).tolist())
+        self.fed = ints([r - d for r, d in zip(rows, drafts)])
+        self.device = self.row_starts.device
+
+
+class PagedStep(NamedTuple):
+    """What ``Qwen3Model.paged_step`` says (device tensors)."""
+
+    counts: torch.Tensor         # int32 [S] drafts that stay
+    next_tokens: torch.Tensor    # int32 [S] the token behind them (-1: a sequence without rows, or without a distribution)
+    logprobs: torch.Tensor       # fp32 [head rows] of the token behind each of them, as ``ops.verify_drafts``
+    logits: torch.Tensor         # fp32 [head rows, vocab]
+
+
 class _Micro:
     """One micro-batch: rows ``b0:b1`` of the batch, its stream, buffers and graphs."""
 
@@ -629,10 +718,11 @@ class Qwen3Model:
         return logits.clone() if want_logits else None
 
     # ---- prompts of different lengths, scoring, drafted trees ----
-    def _rows_pass(self, tokens: torch.Tensor, prep, attend) -> torch.Tensor:
+    def _rows_pass(self, tokens: torch.Tensor, prep, attend, adapters=None, adapter_plan=None) -> torch.Tensor:
         """Every layer over ``len(tokens)`` rows of any sequences; returns the residual rows.
         ``prep(i, qkv)`` does layer i's q/k norm, RoPE and cache write and returns q;
-        ``attend(i, q, out, out_sums)`` its attention, and returns ``out_sums`` where it gave them."""
+        ``attend(i, q, out, out_sums)`` its attention, and returns ``out_sums`` where it gave them.
+        ``adapters``: a ``LayerAdapters`` a layer, for the rows of ``adapter_plan``."""
         c, r, dev = self.cfg, tokens.numel(), self.device
         empty = lambda *shape, dtype=BF16: torch.empty(*shape, dtype=dtype, device=dev)  # noqa: E731
         x, xn, qkv = empty(r, c.hidden), empty(r, c.hidden), empty(r, c.qkv_dim)
@@ -642,22 +732,37 @@ class Qwen3Model:
             xs_n, xs_ctx, xs_h = (empty(n, r, dtype=torch.float32) for n in
                                   (c.hidden // 128, c.n_heads, c.intermediate // 64))
         ops.rmsnorm(self.embed, self.layers[0].w.ln1, c.eps, out=xn, tokens=tokens, x_out=x, out_sums=xs_n)
+        ws = self.micro[0].buf.workspace
         for i, layer in enumerate(self.layers):
-            w = layer.w
-            if i > 0 and r <= 64:       # decode-sized: the norm inside the linear
+            w, a = layer.w, LayerAdapters() if adapters is None else adapters[i]
+
+            def adapt(pool, y, rows, **kw):
+                if pool is not None:
+                    ops.adapter_add(y, rows, pool, adapter_plan, workspace=ws, **kw)
+
+            if i > 0 and r <= 64 and a.qkv is None:       # decode-sized: the norm inside the linear
                 ops.rmsnorm_linear(x, w.ln1, c.eps, w.qkv, out=qkv)
             else:
                 if i > 0:
                     ops.rmsnorm(x, w.ln1, c.eps, out=xn, out_sums=xs_n)
                 ops.linear(xn, w.qkv, out=qkv, x_sums=xs_n)
+                adapt(a.qkv, qkv, xn)
             sums = attend(i, prep(i, qkv), ctx, xs_ctx)
             ops.linear(ctx, w.o, residual=x, out=x, x_sums=sums)
-            if r <= 64:
+            adapt(a.o, x, ctx)
+            if r <= 64 and a.gate_up is None:
                 ops.rmsnorm_gate_up(x, w.ln2, c.eps, w.gate_up, swiglu=True, out=h)
             else:
                 ops.rmsnorm(x, w.ln2, c.eps, out=xn, out_sums=xs_n)
-                ops.gate_up(xn, w.gate_up, swiglu=True, out=h, x_sums=xs_n, out_sums=xs_h)
-            ops.linear(h, w.down, residual=x, out=x, x_sums=xs_h, sum_parts=2)
+                if a.gate_up is None:
+                    ops.gate_up(xn, w.gate_up, swiglu=True, out=h, x_sums=xs_n, out_sums=xs_h)
+                else:                   # the adapter comes before the SwiGLU
+                    adapt(a.gate_up, ops.linear(xn, w.gate_up, x_sums=xs_n), xn, out=h, swiglu=True)
+            if a.gate_up is None:
+                ops.linear(h, w.down, residual=x, out=x, x_sums=xs_h, sum_parts=2)
+            else:
+                ops.linear(h, w.down, residual=x, out=x)
+            adapt(a.down, x, h)
         return x
 
     def _prompt_list(self, prompts) -> list:
@@ -798,6 +903,90 @@ class Qwen3Model:
         self.tokens.copy_(torch.where(counts > 0, nxt, self.tokens))
         self.positions.copy_(after)
         return new, counts
+
+    def paged_step(self, cache: PagedCache, batch: PagedBatch, tokens: torch.Tensor, uniforms: torch.Tensor | None = None,
+                   temperatures: torch.Tensor | None = None, draft_probs: torch.Tensor | None = None,
+                   adapters=None, adapter_ids: torch.Tensor | None = None) -> PagedStep:
+        """One step of many requests at once over a cache in pages: prompt chunks, single tokens and tokens with drafted
+        ones behind them in one pass, each request with its own adapter; then the drafts held to the model's
+        probabilities and each request's next token drawn.
+
+        ``tokens`` int32 ``[batch.rows]``: each sequence's tokens behind its ``cache.lens`` (a chunk of its prompt, or its
+        pending token and ``drafts`` drafted ones).  ``uniforms`` fp32 ``[head rows]`` and ``draft_probs`` fp32 ``[head rows,
+        vocab]`` as ``ops.verify_drafts`` over the rows ``batch.head_rows``; ``temperatures`` fp32 ``[S]``.  Without
+        ``uniforms`` every sequence is greedy.  ``adapters``: a ``LayerAdapters`` for each layer; ``adapter_ids`` int32
+        ``[S]`` each sequence's adapter (-1: none).
+
+        The pages must have room (``cache.reserve``): a token without a slot gives NaN logits, and the next token -1.
+        ``cache.lens`` move on by the tokens that were fed and the drafts that stay (what a refused draft left in
+        the pages is written over by the next step).  Nothing is read back: the call can be captured once its
+        workspaces exist."""
+        c, ws = self.cfg, self.micro[0].buf.workspace
+        ops._check_dev("tokens", tokens, torch.int32)
+        if not isinstance(cache, PagedCache) or not isinstance(batch, PagedBatch) or batch.n_seqs != cache.n_seqs:
+            raise ValueError("batch must be a PagedBatch of the cache's sequences")
+        if cache.k.shape[0] != c.n_layers or tuple(cache.k.shape[2:]) != (c.n_kv_heads, cache.page_slots, c.head_dim):
+            raise ValueError("the cache was made for another model")
+        if batch.rows < 1 or tokens.numel() != batch.rows:
+            raise ValueError(f"tokens must hold {batch.rows} ids, at least one")
+        if cache.max_pages * cache.page_slots > self.rope.shape[0]:
+            raise ValueError(f"sequences of {cache.max_pages * cache.page_slots} slots exceed the model's {self.rope.shape[0]} positions")
+        n_head, plan = batch.head_rows.numel(), None
+        if uniforms is None:
+            if temperatures is not None or draft_probs is not None:
+                raise ValueError("temperatures and draft_probs need uniforms")
+            uniforms = torch.zeros(n_head, dtype=torch.float32, device=self.device)
+            temperatures = torch.zeros(batch.n_seqs, dtype=torch.float32, device=self.device)
+        # (everything is refused before the pass writes into the pages)
+        ops._check_dev("uniforms", uniforms, torch.float32)
+        if uniforms.numel() != n_head:
+            raise ValueError(f"uniforms must hold {n_head} values, one for each head row")
+        if temperatures is not None:
+            ops._check_dev("temperatures", temperatures, torch.float32)
+            if temperatures.numel() != batch.n_seqs:
+                raise ValueError(f"temperatures must hold {batch.n_seqs} values")
+        if draft_probs is not None:
+            ops._check_dev("draft_probs", draft_probs, torch.float32)
+            if tuple(draft_probs.shape) != (n_head, c.vocab):
+                raise ValueError(f"draft_probs must be [{n_head}, {c.vocab}]")
+        ops._same_device(cache.table.device, tokens=tokens, row_starts=batch.row_starts, uniforms=uniforms,
+                         temperatures=temperatures, draft_probs=draft_probs, adapter_ids=adapter_ids, rope=self.rope)
+        if adapters is not None:
+            if len(adapters) != c.n_layers or adapter_ids is None:
+                raise ValueError("adapters must hold a LayerAdapters for each layer, and adapter_ids each sequence's")
+            ops._check_dev("adapter_ids", adapter_ids, torch.int32)
+            q = c.n_heads * c.head_dim
+            want = LayerAdapters((c.hidden, c.qkv_dim, False), (q, c.hidden, False), (c.hidden, 2 * c.intermediate, True),
+                                 (c.intermediate, c.hidden, False))
+            for a in adapters:
+                for name, pool, shape in zip(LayerAdapters._fields, LayerAdapters(*a), want):
+                    if pool is not None and (pool.K, pool.N, pool.paired) != shape:
+                        raise ValueError(f"adapters of {name} must be [{shape[1]}, {shape[0]}]{', paired' if shape[2] else ''}")
+            pools = {p.n for a in adapters for p in a if p is not None}
+            if len(pools) > 1 or adapter_ids.numel() != batch.n_seqs:
+                raise ValueError(f"the pools must be of one size, and adapter_ids hold {batch.n_seqs} values")
+            plan = ops.AdapterPlan(adapter_ids[batch.row_seq], pools.pop()) if pools else None
+        pages = ops.PagedPlan(batch.rows, batch.row_starts, cache.lens, cache.table, c.n_heads, c.n_kv_heads, cache.page_slots)
+
+        def prep(i, qkv):
+            layer = self.layers[i]
+            return ops.paged_qk_rope_kv(qkv, pages, layer.w.q_norm, layer.w.k_norm, c.eps, self.rope, cache.k[i], cache.v[i],
+                                        rope_style=layer.rope_style)
+
+        def attend(i, q, out, out_sums):
+            ops.paged_attention(q, pages, cache.k[i], cache.v[i], out=out, out_sums=out_sums, workspace=ws)
+            return out_sums
+
+        x = self._rows_pass(tokens, prep, attend, adapters=adapters, adapter_plan=plan)
+        keys = torch.empty(n_head, dtype=torch.int64, device=self.device)
+        head = torch.empty(n_head, c.hidden, dtype=BF16, device=self.device)
+        xn = ops.rmsnorm(x, self.norm, c.eps, out=head, tokens=batch.head_rows, x_out=torch.empty_like(head), argmax_keys=keys)
+        logits = torch.empty(n_head, c.vocab, dtype=torch.float32, device=self.device)
+        ops.lm_head_argmax(xn, self.lm_head, keys, logits=logits)
+        counts, nxt, lp = ops.verify_drafts(logits, batch.head_starts, tokens[batch.head_rows.long()], uniforms,
+                                            draft_probs=draft_probs, temperatures=temperatures, workspace=ws)
+        cache.lens += batch.fed + counts
+        return PagedStep(counts, nxt, lp, logits)
 
     # ---- graph-captured greedy generation ----
     def _capture_graph(self, stream, fn):
