@@ -1,8 +1,8 @@
 """Drafted tokens verified on the MI355X against the definition in float64, row by row on the CPU.
 
 Tokens and counts are whole numbers and must be equal: weights and running sums are float64 on both sides (a weight off
-by 1e-14 relative, sums of up to 152k of them by a few 1e-14), so a number u falls between the two sides' borders with a
-probability of tokens * 1e-13 at most; `_near` proves for each case that no number lies that near.
+by 1e-13 relative, sums of them no more), so a number u falls between the two sides' borders with a probability of tokens *
+2e-13 at most; `_reference` asserts for each case that no number lies within 1e-12 of a border.
 Log probabilities: fp32 rounding of a float64 value, 2^-24 relative, and 1e-13 of the float64 terms' size."""
 
 import math
@@ -114,7 +114,8 @@ def _check(args, got, near=1e-13):
 
 
 SHAPES = [([1], 5), ([1], 1), ([2], 1), ([3, 1, 4], 7), ([5, 0, 1, 9], 1000), ([4] * 6, 1023), ([2, 6], 1024), ([9, 3], 1025),
-          ([5] * 5, 4099), ([1] * 40, 30011), ([17, 2], 2049), ([5, 3, 1], 151936)]
+          ([5] * 5, 4099), ([1] * 40, 30011), ([17, 2], 2049), ([5, 3, 1], 151936), ([2, 3], 300001),
+          ([2, 1], 1100003)]
 
 
 @pytest.mark.parametrize("with_probs", [False, True], ids=["certain", "probs"])
@@ -188,6 +189,15 @@ def test_extreme_temperatures_and_numbers(gpu):
         args = list(_case(gpu, [1] * 4, 500, torch.float32, with_probs, seed=7, greedy_every=9))
         args[3] = torch.tensor([0.0, 1.0, 2.0, 1 - 2.0 ** -24], device=gpu)
         _check(args, ops.verify_drafts(*args[:4], draft_probs=args[4], temperatures=args[5]))
+
+
+def test_logits_of_any_size(gpu):
+    """Differences are taken before they are scaled: rows far from 0, and of huge values."""
+    for with_probs in (False, True):
+        for scale, shift in ((1.0, 3e4), (1.0, -2e6), (1e30, 0.0), (1e3, 1e9), (1e-20, 0.0)):
+            args = list(_case(gpu, [3, 1, 4], 2500, torch.float32, with_probs, seed=17))
+            args[0] = args[0] * scale + shift
+            _check(args, ops.verify_drafts(*args[:4], draft_probs=args[4], temperatures=args[5]), near=1e-13 * max(1.0, scale))
 
 
 def test_nothing_left_of_the_rest(gpu):

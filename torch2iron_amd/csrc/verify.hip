@@ -18,8 +18,9 @@
 namespace t2i {
 
 constexpr int VD_CHUNK = 1024;               // tokens whose sum is kept: a wave's, sixteen a lane
-constexpr int VD_WAVES = 4;
-constexpr int VD_THREADS = 64 * VD_WAVES;
+constexpr int VD_WAVES = 4;                  // waves of a workgroup over the rows
+constexpr int VD_BLOCK = 1024;               // threads of a workgroup over a sequence: a thread a token of a chunk
+constexpr int VD_HELD = 4;                   // chunks of a lane that stay in registers: rows of up to 262144 tokens
 
 struct VdChunk {
   double z;                                  // sum of exp((x - m) / T)
@@ -27,11 +28,12 @@ struct VdChunk {
   int best;                                  // T <= 0: its first place
 };
 
-// What was decided for a sequence whose refused draft has probabilities (else one kernel goes on with it).
+// What was decided for a sequence: the row that its next token comes from, by which weights, and all that the draw needs.
 struct VdChoice {
-  double z;
-  float m;
-  int row, mode, best;
+  double c, inv_z, log_z;                    // the row's scale and sum
+  double start, target;                      // the sum before the chunk, and the one that the token's has to pass
+  float m, u;                                // its largest logit, the number for the draw
+  int row, mode, best, draft, chunk;         // row -1: no rows; draft: the refused one (-1: none); chunk: -1 not found yet
 };
 enum VdMode { VD_NONE, VD_BEST, VD_ALL, VD_WITHOUT, VD_REST };   // no token; the best; by p; by p without the draft; by max(p - q, 0)
 
@@ -49,47 +51,109 @@ struct VdParams {
   double* rest;                              // [B][n_chunks] sums of max(p - q, 0)
   VdChoice* choice;                          // [B]
   long long stride, probs_stride;
-  int M, V, B, n_chunks, splits;
+  int M, V, B, n_chunks, splits;             // workgroups of a row (of a sequence)
 };
 
-// 2^y for y <= 0 or so (fp64, relative error 1e-14): the whole part as an exponent, 2^f = e^(f ln 2) by its Taylor
-// series (|f| <= 1/2: the first term left out is 0.347^12 / 12! = 6e-15).  Below 2^-1100 (and for -inf) 0; NaN stays.
-__device__ __forceinline__ double exp2_f64(double y) {
-  y = y < -1100.0 ? -1100.0 : y;
-  const double n = __builtin_rint(y);
-  const double t = (y - n) * 0.69314718055994530942;
-  double p = 1.0 / 39916800.0;
-  p = __builtin_fma(p, t, 1.0 / 3628800.0);
-  p = __builtin_fma(p, t, 1.0 / 362880.0);
-  p = __builtin_fma(p, t, 1.0 / 40320.0);
-  p = __builtin_fma(p, t, 1.0 / 5040.0);
-  p = __builtin_fma(p, t, 1.0 / 720.0);
-  p = __builtin_fma(p, t, 1.0 / 120.0);
-  p = __builtin_fma(p, t, 1.0 / 24.0);
-  p = __builtin_fma(p, t, 1.0 / 6.0);
-  p = __builtin_fma(p, t, 0.5);
-  p = __builtin_fma(p, t, 1.0);
-  p = __builtin_fma(p, t, 1.0);
-  return __builtin_amdgcn_ldexp(p, (int)n);
+// ---- exp((x - m) / T) in fp64 ----
+// With y = (x - m) 32 log2(e) / T = 32 n + j + f (j of 0 .. 31, |f| <= 1/2): 2^n 2^(j / 32) 2^(f / 32), the second from a
+// table in LDS (32 doubles stand in 64 banks: no conflict), the third by its interpolation at five Chebyshev nodes
+// (relative error 8e-14).  Half the instructions of a series for 2^(y / 32 - n).
+constexpr int VD_EXP = 32;
+__device__ __forceinline__ double vd_fraction(double f) {
+  double p = 9.172607532092245e-09;
+  p = __builtin_fma(p, f, 1.6938633903155644e-06);
+  p = __builtin_fma(p, f, 0.0002345961981994449);
+  p = __builtin_fma(p, f, 0.02166084939172217);
+  return __builtin_fma(p, f, 1.0);
 }
 
-// exp((x - m) / T) with c = log2(e) / T; 0 for a logit of -inf, whatever m and c are
-__device__ __forceinline__ double vd_weight(float x, float m, double c) {
-  return x == -INFINITY ? 0.0 : exp2_f64(((double)x - (double)m) * c);
-}
-
-// log2(e) / T; a temperature that is not above 0 (greedy) counts as 1 where probabilities are formed
-__device__ __forceinline__ double vd_scale(float t) { return 1.44269504088896340736 / (t > 0.0f ? (double)t : 1.0); }
-
-__device__ __forceinline__ double vd_wave_sum(double v) {
+// The table: s_exp[j] = 2^(j / 32) by the series of e^t (the first term left out is 0.68^17 / 17! = 4e-18), and s_add[j] the
+// same with j 2^15 taken from its high word, so that 2^n comes with an addition.  A barrier behind it is the caller's.
+__device__ __forceinline__ void vd_table(double* s_exp, double* s_add = nullptr) {
+  if (threadIdx.x < VD_EXP) {
+    const double t = (double)threadIdx.x * (0.69314718055994530942 / VD_EXP);
+    double p = 1.0;
 #pragma unroll
-  for (int s = 32; s; s >>= 1) v += __shfl_xor(v, s, 64);
+    for (int k = 16; k > 0; --k) p = __builtin_fma(p * t, 1.0 / k, 1.0);
+    s_exp[threadIdx.x] = p;
+    if (s_add) s_add[threadIdx.x] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) - ((uint64_t)threadIdx.x << 47));
+  }
+}
+
+// 2^(y / 32): 0 far below; an infinite y gives NaN.
+__device__ __forceinline__ double vd_exp(double y, const double* s_exp) {
+  const double k = __builtin_rint(y);
+  int n;
+  asm("v_cvt_i32_f64 %0, %1" : "=v"(n) : "v"(k));          // (saturates)
+  return __builtin_amdgcn_ldexp(vd_fraction(y - k) * s_exp[n & (VD_EXP - 1)], n >> 5);
+}
+
+// z + 2^(d c / 32), for a row's sums: -32000 < d c < 2^20.  The whole part k = 32 n + j comes out of the low bits of
+// d c + 1.5 2^52, and k 2^15, added to the high word of the table's value, is j 2^15 + n 2^20: n more in its exponent.
+// The constants stay in registers (an instruction takes one from elsewhere, and copies would be a tenth of all).
+struct VdAdd {
+  double c, whole, p[4];
+  const u32x2* table;
+  __device__ __forceinline__ VdAdd(double scale, const double* s_add) : c(scale), whole(6755399441055744.0),
+      p{9.172607532092245e-09, 1.6938633903155644e-06, 0.0002345961981994449, 0.02166084939172217} {
+    table = reinterpret_cast<const u32x2*>(s_add);
+    asm("" : "+v"(c), "+v"(whole), "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]));
+  }
+  __device__ __forceinline__ double operator()(double d, double z) const {
+    const double s = __builtin_fma(d, c, whole);
+    const double f = __builtin_fma(d, c, whole - s);
+    const uint32_t k = __builtin_bit_cast(u32x2, s).x;
+    u32x2 e = table[k & (VD_EXP - 1)];
+    e.y += k << 15;
+    double v = __builtin_fma(p[0], f, p[1]);
+    v = __builtin_fma(v, f, p[2]);
+    v = __builtin_fma(v, f, p[3]);
+    v = __builtin_fma(v, f, 1.0);
+    return __builtin_fma(v, __builtin_bit_cast(double, e), z);
+  }
+};
+
+// exp((x - m) / T) with c = 32 log2(e) / T; 0 for a logit of -inf, whatever m and c are
+__device__ __forceinline__ double vd_weight(float x, float m, double c, const double* s_exp) {
+  const double w = vd_exp(((double)x - (double)m) * c, s_exp);
+  return x == -INFINITY ? 0.0 : w;
+}
+
+// 32 log2(e) / T; a temperature that is not above 0 (greedy) counts as 1 where probabilities are formed
+__device__ __forceinline__ double vd_scale(float t) { return VD_EXP * 1.44269504088896340736 / (t > 0.0f ? (double)t : 1.0); }
+// log p of a logit x, given the row's m and z
+__device__ __forceinline__ float vd_logprob(float x, float m, double c, double log_z) {
+  return (float)(((double)x - (double)m) * c * (0.69314718055994530942 / VD_EXP) - log_z);
+}
+
+// ---- sums, maxima and minima of a wave, in every lane ----
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double vd_shift(double v) {     // 0 where there is no lane to take from
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// the sum of the lanes up to this one
+__device__ __forceinline__ double vd_upto(double v) {
+  v += vd_shift<0x111, 0xF>(v);              // row_shr 1, 2, 4, 8: within 16 lanes
+  v += vd_shift<0x112, 0xF>(v);
+  v += vd_shift<0x114, 0xF>(v);
+  v += vd_shift<0x118, 0xF>(v);
+  v += vd_shift<0x142, 0xA>(v);              // row_bcast 15: into rows 1 and 3
+  v += vd_shift<0x143, 0xC>(v);              // row_bcast 31: into rows 2 and 3
   return v;
 }
+__device__ __forceinline__ double vd_lane(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane) << 32 |
+                                        (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane));
+}
+__device__ __forceinline__ double vd_wave_sum(double v) { return vd_lane(vd_upto(v), 63); }
 __device__ __forceinline__ float vd_wave_max(float v) {
-#pragma unroll
-  for (int s = 32; s; s >>= 1) v = fmaxf(v, __shfl_xor(v, s, 64));
-  return v;
+  v = row_max16(v);
+  return fmaxf(fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 0)), __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16))),
+               fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 32)), __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 48))));
 }
 __device__ __forceinline__ int vd_wave_min(int v) {
 #pragma unroll
@@ -165,138 +229,212 @@ __device__ __forceinline__ int vd_rows(const VdParams& p, int b, int& first) {
 // ============================================================================
 // largest value and sum of every chunk of every row
 // ============================================================================
-// A wave a chunk: its logits in one go, the maximum, then the weights.  Lane l holds the pieces l, l + 64, ...
+// A wave takes every step-th chunk of a row, the next one's logits on their way while it adds the weights of one: the largest
+// logit first, then the weights.  Lane l holds the pieces l, l + 64, ... of a chunk (16 bytes, at any alignment of the values).
 template <typename T>
-__global__ __launch_bounds__(VD_THREADS) void verify_rows_kernel(const VdParams p) {
+__global__ __launch_bounds__(64 * VD_WAVES) void verify_rows_kernel(const VdParams p) {
   constexpr int PER = 16 / VdType<T>::SIZE, PIECES = VD_CHUNK / 64 / PER;
-  __shared__ int s_seq;
+  __shared__ double s_exp[VD_EXP], s_add[VD_EXP];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = blockIdx.x / p.splits;
-  const int chunk = (blockIdx.x - row * p.splits) * VD_WAVES + wave;
-  const char* const src = vd_row<T>(p, row);
-  float x[PIECES][PER];
-  if (chunk < p.n_chunks) {
+  const int from = (blockIdx.x - row * p.splits) * VD_WAVES + wave, step = p.splits * VD_WAVES;   // all waves side by side
+  const int whole = p.V / VD_CHUNK;                        // chunks that lie in the row to their end
+  const char* const src = vd_row<T>(p, row) + (size_t)lane * 16;
+  u32x4 next[PIECES];
+  const auto fetch = [&](int chunk) {
+    if (chunk < whole) {
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) vd_load<T>(src, chunk * VD_CHUNK + (64 * i + lane) * PER, p.V, x[i]);
-  }
-  // the row's sequence, for its temperature
+      for (int i = 0; i < PIECES; ++i)
+        next[i] = *reinterpret_cast<const u32x4_any*>(src + (size_t)chunk * (VD_CHUNK * VdType<T>::SIZE) + 1024 * i);
+    }
+  };
+  fetch(from);
+  // the row's sequence, for its temperature: the last that starts at the row or before it
   float t = 1.0f;
   if (p.temperatures) {
-    if (threadIdx.x == 0) s_seq = -1;
-    __syncthreads();
-    for (int b = threadIdx.x; b < p.B; b += VD_THREADS)
-      if (p.row_starts[b] <= row && row < p.row_starts[b + 1]) s_seq = b;
-    __syncthreads();
-    if (s_seq >= 0) t = p.temperatures[s_seq];
+    int s = -1;
+    for (int base = 0; base < p.B; base += 64)
+      s += __builtin_popcountll(__ballot(base + lane < p.B && p.row_starts[min(base + lane, p.B - 1)] <= row));
+    if (s >= 0) t = p.temperatures[s];
   }
-  if (chunk >= p.n_chunks) return;
+  vd_table(s_exp, s_add);
+  __syncthreads();
   const double c = vd_scale(t);
-  float m = -INFINITY;
+  const VdAdd add(c, s_add);
+  const float down = t > 0.0f ? 690.0f * t : 690.0f;       // 690 / ln 2 = 995.5 powers of two
+  for (int chunk = from; chunk < p.n_chunks; chunk += step) {
+    float x[PIECES][PER];
+    if (chunk < whole) {
 #pragma unroll
-  for (int i = 0; i < PIECES; ++i)
+      for (int i = 0; i < PIECES; ++i) VdType<T>::get(next[i], x[i]);
+    } else {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) m = fmaxf(m, x[i][j]);
-  m = vd_wave_max(m);
-  double z = 0.0;
+      for (int i = 0; i < PIECES; ++i) vd_load<T>(vd_row<T>(p, row), chunk * VD_CHUNK + (64 * i + lane) * PER, p.V, x[i]);
+    }
+    fetch(chunk + step);
+    float m = -INFINITY, low = INFINITY;
 #pragma unroll
-  for (int i = 0; i < PIECES; ++i)
+    for (int i = 0; i < PIECES; ++i)
 #pragma unroll
-    for (int j = 0; j < PER; ++j) z += vd_weight(x[i][j], m, c);
-  z = vd_wave_sum(z);
-  int best = 0;
-  if (!(t > 0.0f)) {
-    best = 0x7FFFFFFF;
+      for (int j = 0; j < PER; j += 2) {
+        m = fmaxf(fmaxf(x[i][j], x[i][j + 1]), m);
+        low = fminf(fminf(x[i][j], x[i][j + 1]), low);
+      }
+    m = vd_wave_max(m);
+    double z = 0.0;
+    if (m < INFINITY && !__ballot(!(m - low < down)) && c < 1e6) {   // (a NaN makes z one)
+      const double md = (double)m;
 #pragma unroll
-    for (int i = PIECES - 1; i >= 0; --i)
+      for (int i = 0; i < PIECES; ++i)
 #pragma unroll
-      for (int j = PER - 1; j >= 0; --j)
-        if (x[i][j] == m) best = chunk * VD_CHUNK + (64 * i + lane) * PER + j;
-    best = vd_wave_min(best);
+        for (int j = 0; j < PER; ++j) z = add((double)x[i][j] - md, z);
+    } else {                                               // masked tokens, the row's end, infinities; temperatures near 0
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+        for (int j = 0; j < PER; ++j) z += vd_weight(x[i][j], m, c, s_exp);
+    }
+    z = vd_wave_sum(z);
+    int best = 0;
+    if (!(t > 0.0f)) {
+      best = 0x7FFFFFFF;
+#pragma unroll
+      for (int i = PIECES - 1; i >= 0; --i)
+#pragma unroll
+        for (int j = PER - 1; j >= 0; --j)
+          if (x[i][j] == m) best = chunk * VD_CHUNK + (64 * i + lane) * PER + j;
+      best = vd_wave_min(best);
+    }
+    if (lane == 0) p.chunks[(size_t)row * p.n_chunks + chunk] = VdChunk{z, m, best};
   }
-  if (lane == 0) p.chunks[(size_t)row * p.n_chunks + chunk] = VdChunk{z, m, best};
-  if (threadIdx.x == 0 && chunk == 0) p.logprobs[row] = 0.0f;
+  if (threadIdx.x == 0 && from == 0) p.logprobs[row] = 0.0f;
 }
 
 // ============================================================================
 // which drafts stay
 // ============================================================================
-// A row's largest logit and sum (a wave; every lane receives them), and the first place of the largest.
-__device__ __forceinline__ void vd_join(const VdParams& p, int row, double c, int lane, float& m, double& z, int& best) {
+// A row's largest logit and sum (a wave; every lane receives them), and the first place of the largest; part: this lane's
+// chunks (lane, lane + 64, ...) in units of the row's largest weight.
+__device__ __forceinline__ void vd_join(const VdParams& p, int row, double c, const double* s_exp, bool greedy, int lane, float& m,
+                                        double& z, int& best, double (&part)[VD_HELD]) {
   const VdChunk* const at = p.chunks + (size_t)row * p.n_chunks;
+  VdChunk held[VD_HELD];
+#pragma unroll
+  for (int i = 0; i < VD_HELD; ++i) held[i] = at[min(64 * i + lane, p.n_chunks - 1)];
   m = -INFINITY;
-  for (int i = lane; i < p.n_chunks; i += 64) m = fmaxf(m, at[i].m);
+#pragma unroll
+  for (int i = 0; i < VD_HELD; ++i) m = fmaxf(m, held[i].m);
+  for (int i = 64 * VD_HELD + lane; i < p.n_chunks; i += 64) m = fmaxf(m, at[i].m);
   m = vd_wave_max(m);
-  z = 0.0;
+  double sum = 0.0;
   best = 0x7FFFFFFF;
-  for (int i = lane; i < p.n_chunks; i += 64) {
-    const VdChunk s = at[i];
-    z += s.m > -INFINITY ? s.z * vd_weight(s.m, m, c) : s.z;   // (nothing but -inf: 0; NaN stays)
+  const auto add = [&](const VdChunk& s) {
+    const double w = s.m > -INFINITY ? s.z * vd_weight(s.m, m, c, s_exp) : s.z;   // (nothing but -inf: 0; NaN stays)
+    sum += w;
     if (s.m == m) best = min(best, s.best);
+    return w;
+  };
+#pragma unroll
+  for (int i = 0; i < VD_HELD; ++i) part[i] = 64 * i + lane < p.n_chunks ? add(held[i]) : 0.0;
+  for (int i = 64 * VD_HELD + lane; i < p.n_chunks; i += 64) (void)add(at[i]);
+  z = vd_wave_sum(sum);
+  if (greedy) best = vd_wave_min(best);
+}
+
+// The chunk of the token that ch's number draws, by a wave that holds all the row's parts; left open where the draft's
+// chunk holds hardly anything else (the difference would not be exact), or no chunk is found.
+__device__ __forceinline__ void vd_chunk_of(VdChoice& ch, double (&part)[VD_HELD], double taken, int V, int lane) {
+  bool open = false;
+  double total = 0.0, upto[VD_HELD], before[VD_HELD];
+#pragma unroll
+  for (int i = 0; i < VD_HELD; ++i) {
+    if (ch.mode == VD_WITHOUT && ch.draft >= 0 && ch.draft < V && ch.draft / VD_CHUNK == 64 * i + lane) {
+      const double left = part[i] - taken;
+      open = !(left > 1e-3 * part[i]);
+      part[i] = left;
+    }
+    upto[i] = vd_upto(part[i]);
+    before[i] = total;
+    total += vd_lane(upto[i], 63);
   }
-  z = vd_wave_sum(z);
-  best = vd_wave_min(best);
+  if (__ballot(open) || !(total > 0.0)) return;
+  const double target = (double)ch.u * total;
+#pragma unroll
+  for (int i = VD_HELD - 1; i >= 0; --i) {
+    const unsigned long long hit = __ballot(part[i] > 0.0 && before[i] + upto[i] > target);
+    if (!hit) continue;
+    const int at = __builtin_ctzll(hit);
+    ch.chunk = 64 * i + at;
+    ch.start = at ? before[i] + vd_lane(upto[i], at - 1) : before[i];
+    ch.target = target;
+  }
 }
 
 // A workgroup's decision for sequence b: what its next token is drawn by, from which row.  Waves take rows in turn;
-// each remembers the first of its rows behind which no draft stays.  WRITE: the log probabilities of the drafts that stay.
+// each remembers the first of its rows behind which no draft stays, and its parts: where the token comes from p itself (or p
+// without the draft) the wave of that row finds the chunk too, without another look at memory.  WRITE: the log
+// probabilities of the drafts that stay.
 template <typename T, bool WRITE>
-__device__ __forceinline__ VdChoice vd_decide(const VdParams& p, int b, int* s_row, VdChoice* s_choice) {
+__device__ __forceinline__ VdChoice vd_decide(const VdParams& p, int b, const double* s_exp, int* s_row, VdChoice* s_choice) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int first;
   const int n = vd_rows(p, b, first);
   const float t = p.temperatures ? p.temperatures[b] : 1.0f;
+  const float draw = n ? p.uniforms[first + n - 1] : 0.0f;
   const bool greedy = !(t > 0.0f);
   const double c = vd_scale(t);
+  VdChoice mine{c, 0.0, 0.0, 0.0, 0.0, 0.0f, draw, -1, VD_NONE, 0, -1, -1};
+  double part[VD_HELD] = {}, taken = 0.0;                  // of the row of `mine`; the draft's weight
   if (threadIdx.x == 0) {
     *s_row = first + n - 1;
-    *s_choice = VdChoice{0.0, 0.0f, -1, VD_NONE, 0};
+    *s_choice = mine;
   }
-  __syncthreads();
-  VdChoice mine{0.0, 0.0f, -1, VD_NONE, 0};
-  for (int row = first + wave; row < first + n && mine.row < 0; row += VD_WAVES) {
+  __syncthreads();                                         // (also the table's)
+  for (int row = first + wave; row < first + n && mine.row < 0; row += VD_BLOCK / 64) {
+    const bool last = row + 1 == first + n;
+    const int y = last ? -1 : p.tokens[row + 1];
+    const bool in = y >= 0 && y < p.V;
+    const float x = in ? VdType<T>::one(vd_row<T>(p, row) + (size_t)y * VdType<T>::SIZE) : 0.0f;
+    const double q = in && p.probs ? (double)p.probs[(size_t)row * p.probs_stride + y] : 1.0;
+    const double u = (double)p.uniforms[row];
     float m;
     double z;
     int best;
-    vd_join(p, row, c, lane, m, z, best);
+    vd_join(p, row, c, s_exp, greedy, lane, m, z, best, part);
+    taken = in ? vd_weight(x, m, c, s_exp) : 0.0;
     const bool fine = z > 0.0 && z < INFINITY;             // no NaN, no +inf, not all -inf
-    bool stays = false;
-    float lp = 0.0f;
-    if (row + 1 < first + n) {
-      const int y = p.tokens[row + 1];
-      if (fine && y >= 0 && y < p.V) {
-        const float x = VdType<T>::one(vd_row<T>(p, row) + (size_t)y * VdType<T>::SIZE);
-        const double q = p.probs ? (double)p.probs[(size_t)row * p.probs_stride + y] : 1.0;
-        stays = greedy ? y == best : (double)p.uniforms[row] * q < vd_weight(x, m, c) / z;
-        lp = (float)(((double)x - (double)m) * c * 0.69314718055994530942 - log(z));
-      }
-    }
+    const bool stays = fine && in && (greedy ? y == best : u * q * z < taken);
     if (stays) {
-      if (WRITE && lane == 0) p.logprobs[row] = lp;
+      if (WRITE && lane == 0) p.logprobs[row] = vd_logprob(x, m, c, log(z));
     } else {
-      const bool last = row + 1 == first + n;
-      mine = VdChoice{z, m, row, !fine ? VD_NONE : greedy ? VD_BEST : last ? VD_ALL : p.probs ? VD_REST : VD_WITHOUT, best};
-      if (lane == 0) atomicMin(s_row, row);
+      mine = VdChoice{c, 1.0 / z, log(z), 0.0, 0.0, m, draw, row, !fine ? VD_NONE : greedy ? VD_BEST : last ? VD_ALL : p.probs ? VD_REST : VD_WITHOUT,
+                      best, y, -1};
+      if (lane == 0) atomicMin(s_row, row);                // (a lane a wave)
     }
   }
   __syncthreads();
-  if (mine.row >= 0 && mine.row == *s_row && lane == 0) *s_choice = mine;
-  __syncthreads();
-  const VdChoice out = *s_choice;
-  if (WRITE) {
-    for (int row = out.row + 1 + (int)threadIdx.x; row < first + n; row += VD_THREADS) p.logprobs[row] = 0.0f;
-    if (threadIdx.x == 0) p.counts[b] = out.row < 0 ? 0 : out.row - first;
+  const int at = *s_row;
+  if (mine.row >= 0 && mine.row == at) {
+    if ((mine.mode == VD_ALL || mine.mode == VD_WITHOUT) && p.n_chunks <= 64 * VD_HELD) vd_chunk_of(mine, part, taken, p.V, lane);
+    if (lane == 0) *s_choice = mine;
   }
-  return out;
+  if (WRITE) {
+    for (int row = at + 1 + (int)threadIdx.x; row < first + n; row += VD_BLOCK) p.logprobs[row] = 0.0f;
+    if (threadIdx.x == 0) p.counts[b] = n ? at - first : 0;
+  }
+  __syncthreads();
+  return *s_choice;
 }
 
-// The weights by which a token is drawn.
+// The weights by which a token is drawn, in units of 1 / z where there are draft probabilities.
 struct VdWeights {
   double c, inv_z;
   float m;
   int mode, without;
   const float* q;                            // VD_REST: the row of draft probabilities
+  const double* s_exp;
   __device__ __forceinline__ double of(float x, int at) const {
-    const double e = vd_weight(x, m, c);
+    const double e = vd_weight(x, m, c, s_exp);
     if (mode == VD_REST) {
       const double w = e * inv_z - (double)q[at];
       return w > 0.0 ? w : 0.0;
@@ -305,184 +443,211 @@ struct VdWeights {
   }
 };
 
-// The weights of a chunk of a row, four neighbouring tokens a thread of VD_THREADS.
-template <typename T>
-__device__ __forceinline__ void vd_four(const VdParams& p, const char* row, int chunk, const VdWeights& w, double (&v)[4]) {
-  const int first = chunk * VD_CHUNK + 4 * (int)threadIdx.x;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) v[j] = first + j < p.V ? w.of(VdType<T>::one(row + (size_t)(first + j) * VdType<T>::SIZE), first + j) : 0.0;
-}
+constexpr int VD_BLOCK_WAVES = VD_BLOCK / 64;
 
-// Sums over the workgroup: those of the threads before this one, and all.
+// Sums over the workgroup of VD_BLOCK: those of the threads before this one, and all.
 __device__ __forceinline__ double vd_scan(double v, double* s_wave, double& all) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  double x = v;
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    const double u = __shfl_up(x, s, 64);
-    if (lane >= s) x += u;
-  }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const double x = vd_upto(v);
   __syncthreads();
   if (lane == 63) s_wave[wave] = x;
   __syncthreads();
-  double before = 0.0;
-  all = 0.0;
-  for (int w = 0; w < VD_WAVES; ++w) {
-    if (w < wave) before += s_wave[w];
-    all += s_wave[w];
-  }
-  const double up = __shfl_up(x, 1, 64);
-  return before + (lane ? up : 0.0);
+  // every wave's 16 lanes hold the waves' sums
+  const double w = s_wave[lane & (VD_BLOCK_WAVES - 1)];
+  const double up = vd_upto(lane < VD_BLOCK_WAVES ? w : 0.0);
+  all = vd_lane(up, VD_BLOCK_WAVES - 1);
+  const double before = wave ? vd_lane(up, wave - 1) : 0.0;
+  return before + vd_shift<0x138, 0xF>(x);                 // wave_shr 1
+}
+
+// The first and the last thread of the workgroup of which `hit` and `some` hold (none: past every one, -1).
+struct VdEnds {
+  int first, last;
+};
+__device__ __forceinline__ VdEnds vd_ends(bool hit, bool some, int2* s_ends) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned long long h = __ballot(hit), s = __ballot(some);
+  __syncthreads();                                         // the words of the call before are read
+  if (lane == 0)
+    s_ends[wave] = int2{h ? 64 * wave + __builtin_ctzll(h) : 0x7FFFFFFF, s ? 64 * wave + 63 - __builtin_clzll(s) : -1};
+  __syncthreads();
+  const int2 w = s_ends[lane & (VD_BLOCK_WAVES - 1)];
+  const uint32_t f = (uint32_t)__ballot(lane < VD_BLOCK_WAVES && w.x < 0x7FFFFFFF);
+  const uint32_t l = (uint32_t)__ballot(lane < VD_BLOCK_WAVES && w.y >= 0);
+  return VdEnds{f ? __builtin_amdgcn_readlane(w.x, __builtin_ctz(f)) : 0x7FFFFFFF,
+                l ? __builtin_amdgcn_readlane(w.y, 31 - __builtin_clz(l)) : -1};
 }
 
 // The next token of sequence b, from what was decided: first the chunk, then the token within it.
 template <typename T>
-__device__ __forceinline__ void vd_pick(const VdParams& p, int b, VdChoice ch) {
-  __shared__ double s_wave[VD_WAVES];
+__device__ __forceinline__ void vd_pick(const VdParams& p, int b, VdChoice ch, const double* s_exp) {
+  __shared__ double s_wave[VD_BLOCK_WAVES];
   __shared__ double s_before;
-  __shared__ int s_chunk, s_last, s_token, s_some;
-  int first;
-  const int n = vd_rows(p, b, first);
-  if (ch.mode == VD_NONE || ch.mode == VD_BEST) {          // (no rows: ch.row is -1)
+  __shared__ int2 s_ends[VD_BLOCK_WAVES];
+  if (ch.mode == VD_NONE || ch.mode == VD_BEST) {
     if (threadIdx.x == 0) {
       p.next[b] = ch.mode == VD_BEST ? ch.best : -1;
-      if (ch.row >= 0) p.logprobs[ch.row] = ch.mode == VD_BEST ? (float)-log(ch.z) : __uint_as_float(0x7FC00000u);
+      if (ch.row >= 0) p.logprobs[ch.row] = ch.mode == VD_BEST ? (float)-ch.log_z : __uint_as_float(0x7FC00000u);
     }
     return;
   }
   const char* const row = vd_row<T>(p, ch.row);
+  const VdChunk* const chunks = p.chunks + (size_t)ch.row * p.n_chunks;
+  const double* const rest = p.rest + (size_t)b * p.n_chunks;
   VdWeights w;
-  w.c = vd_scale(p.temperatures ? p.temperatures[b] : 1.0f);
-  w.inv_z = 1.0 / ch.z;
+  w.c = ch.c;
+  w.inv_z = ch.inv_z;
   w.m = ch.m;
   w.mode = ch.mode;
-  w.without = ch.row + 1 < first + n ? p.tokens[ch.row + 1] : -1;
+  w.without = ch.draft;
   w.q = p.probs ? p.probs + (size_t)ch.row * p.probs_stride : nullptr;
-  const VdChunk* const chunks = p.chunks + (size_t)ch.row * p.n_chunks;
-  double without = 0.0, total = 0.0;
-  const int odd = w.mode == VD_WITHOUT && w.without >= 0 && w.without < p.V ? w.without / VD_CHUNK : -1;
-  if (odd >= 0) {                                          // the draft's own chunk, without it
-    double v[4];
-    vd_four<T>(p, row, odd, w, v);
-    (void)vd_scan((v[0] + v[1]) + (v[2] + v[3]), s_wave, without);
-  }
-  const auto sum_of = [&](int i) {
-    if (i >= p.n_chunks) return 0.0;
-    if (w.mode == VD_REST) return p.rest[(size_t)b * p.n_chunks + i];
-    return i == odd && w.mode == VD_WITHOUT ? without : chunks[i].m > -INFINITY ? chunks[i].z * vd_weight(chunks[i].m, w.m, w.c) : 0.0;
+  w.s_exp = s_exp;
+  float x = 0.0f;                                          // the logit of this thread's token of a chunk
+  const auto token_weight = [&](int chunk) {
+    const int at = chunk * VD_CHUNK + (int)threadIdx.x;
+    if (at >= p.V) return 0.0;
+    x = VdType<T>::one(row + (size_t)at * VdType<T>::SIZE);
+    return w.of(x, at);
   };
-  for (;;) {
-    total = 0.0;
-    for (int base = 0; base < p.n_chunks; base += VD_THREADS) {
-      double all;
-      (void)vd_scan(sum_of(base + threadIdx.x), s_wave, all);
-      total += all;
+  int chunk = ch.chunk;
+  double start = ch.start, target = ch.target;
+  if (chunk < 0) {                                         // not found yet: from the sums of the chunks
+    double without = 0.0;
+    const int odd = w.mode == VD_WITHOUT && w.without >= 0 && w.without < p.V ? w.without / VD_CHUNK : -1;
+    if (odd >= 0) (void)vd_scan(token_weight(odd), s_wave, without);   // the draft's own chunk, without it
+    const auto sum_of = [&](int i) {
+      if (i >= p.n_chunks) return 0.0;
+      if (w.mode == VD_REST) return rest[i];
+      const VdChunk s = chunks[i];
+      return i == odd && w.mode == VD_WITHOUT ? without : s.m > -INFINITY ? s.z * vd_weight(s.m, w.m, w.c, s_exp) : 0.0;
+    };
+    double total, v = 0.0, upto = 0.0;                       // (rows of up to 2^20 tokens: one round, kept for the search)
+    for (;;) {
+      total = 0.0;
+      for (int base = 0; base < p.n_chunks; base += VD_BLOCK) {
+        double all;
+        v = sum_of(base + threadIdx.x);
+        upto = vd_scan(v, s_wave, all);
+        total += all;
+      }
+      if (total > 0.0 || w.mode == VD_ALL) break;
+      w.mode = VD_ALL;                                       // nothing is left: by p itself
     }
-    if (total > 0.0 || w.mode == VD_ALL) break;
-    w.mode = VD_ALL;                                       // nothing is left: by p itself
-  }
-  if (threadIdx.x == 0) {
-    s_chunk = s_token = 0x7FFFFFFF;
-    s_last = s_some = -1;
-  }
-  __syncthreads();
-  const double target = (double)p.uniforms[first + n - 1] * total;
-  double before = 0.0;
-  for (int base = 0; base < p.n_chunks; base += VD_THREADS) {
-    const int i = base + threadIdx.x;
-    const double v = sum_of(i);
-    double all;
-    const double upto = before + vd_scan(v, s_wave, all);
-    if (v > 0.0 && upto + v > target) atomicMin(&s_chunk, i);
-    if (v > 0.0) atomicMax(&s_last, i);
-    before += all;
-    __syncthreads();
-    if (s_chunk == i) s_before = upto;
-    __syncthreads();
-    if (s_chunk < 0x7FFFFFFF) break;
-    if (s_last == i) s_before = upto;                      // u of 1 or more: the last token with a weight
-    __syncthreads();
-  }
-  __syncthreads();
-  const int chunk = s_chunk < 0x7FFFFFFF ? s_chunk : s_last;
-  const double start = s_before;
-  if (chunk < 0) {                                         // (a NaN among the draft's probabilities)
-    if (threadIdx.x == 0) p.next[b] = -1;
-    return;
-  }
-  double v[4], all;
-  vd_four<T>(p, row, chunk, w, v);
-  double upto = start + vd_scan((v[0] + v[1]) + (v[2] + v[3]), s_wave, all);
-  const int at = chunk * VD_CHUNK + 4 * (int)threadIdx.x;
-  bool found = false;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    upto += v[j];
-    if (v[j] > 0.0) {
-      if (!found && upto > target) atomicMin(&s_token, at + j), found = true;
-      atomicMax(&s_some, at + j);
+    target = (double)ch.u * total;
+    double before = 0.0;
+    for (int base = 0; base < p.n_chunks; base += VD_BLOCK) {
+      double all = 0.0;
+      if (p.n_chunks > VD_BLOCK) {
+        v = sum_of(base + threadIdx.x);
+        upto = before + vd_scan(v, s_wave, all);
+      }
+      const VdEnds e = vd_ends(v > 0.0 && upto + v > target, v > 0.0, s_ends);
+      const int at = e.first < 0x7FFFFFFF ? e.first : e.last;   // a number of 1 or more: the last with a weight
+      if (at >= 0) {
+        chunk = base + at;
+        if ((int)threadIdx.x == at) s_before = upto;
+      }
+      before += all;
+      if (e.first < 0x7FFFFFFF) break;
     }
+    if (chunk < 0) {                                       // (a NaN among the draft's probabilities)
+      if (threadIdx.x == 0) {
+        p.next[b] = -1;
+        p.logprobs[ch.row] = __uint_as_float(0x7FC00000u);
+      }
+      return;
+    }
+    __syncthreads();
+    start = s_before;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const int token = s_token < 0x7FFFFFFF ? s_token : s_some;
-    p.next[b] = token;
-    const float x = token >= 0 ? VdType<T>::one(row + (size_t)token * VdType<T>::SIZE) : 0.0f;
-    p.logprobs[ch.row] = (float)(((double)x - (double)ch.m) * w.c * 0.69314718055994530942 - log(ch.z));
+  double all;
+  const double mine = token_weight(chunk);
+  const double to = start + vd_scan(mine, s_wave, all) + mine;
+  const VdEnds e = vd_ends(mine > 0.0 && to > target, mine > 0.0, s_ends);
+  const int at = e.first < 0x7FFFFFFF ? e.first : e.last;
+  if ((int)threadIdx.x == max(at, 0)) {
+    p.next[b] = at < 0 ? -1 : chunk * VD_CHUNK + at;
+    p.logprobs[ch.row] = at < 0 ? __uint_as_float(0x7FC00000u) : vd_logprob(x, ch.m, w.c, ch.log_z);
   }
 }
 
-// No draft probabilities: everything behind the rows' sums, a workgroup a sequence.
+// Everything behind the rows' sums, a workgroup a sequence; but where a refused draft has probabilities only the
+// decision, which the next two launches go on with.
 template <typename T>
-__global__ __launch_bounds__(VD_THREADS) void verify_kernel(const VdParams p) {
+__global__ __launch_bounds__(VD_BLOCK) void verify_kernel(const VdParams p) {
+  __shared__ double s_exp[VD_EXP];
   __shared__ int s_row;
   __shared__ VdChoice s_choice;
-  const VdChoice ch = vd_decide<T, true>(p, blockIdx.x, &s_row, &s_choice);
-  __syncthreads();
-  vd_pick<T>(p, blockIdx.x, ch);
+  vd_table(s_exp);
+  const VdChoice ch = vd_decide<T, true>(p, blockIdx.x, s_exp, &s_row, &s_choice);
+  if (p.probs && threadIdx.x == 0) p.choice[blockIdx.x] = ch;
+  if (ch.mode != VD_REST) vd_pick<T>(p, blockIdx.x, ch, s_exp);
 }
 
-// With draft probabilities: first each chunk's sum of max(p - q, 0) behind a refused draft, `splits` workgroups a sequence
-// (each decides for itself; the first writes it down), a wave a chunk.
+// Each chunk's sum of max(p - q, 0) behind a refused draft, `splits` workgroups a sequence, a wave a chunk.
 template <typename T>
-__global__ __launch_bounds__(VD_THREADS) void verify_rest_kernel(const VdParams p) {
-  __shared__ int s_row;
-  __shared__ VdChoice s_choice;
-  const int b = blockIdx.x / p.splits, split = blockIdx.x - b * p.splits;
-  VdChoice ch;
-  if (split == 0) {
-    ch = vd_decide<T, true>(p, b, &s_row, &s_choice);
-    if (threadIdx.x == 0) p.choice[b] = ch;
-  } else {
-    ch = vd_decide<T, false>(p, b, &s_row, &s_choice);
-  }
-  if (ch.mode != VD_REST) return;
+__device__ __forceinline__ void vd_rest(const VdParams& p, int b, const VdChoice& ch, int first, int step, const double* s_exp) {
   constexpr int PER = 16 / VdType<T>::SIZE, PIECES = VD_CHUNK / 64 / PER;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const double c = vd_scale(p.temperatures ? p.temperatures[b] : 1.0f), inv_z = 1.0 / ch.z;
+  const int lane = threadIdx.x & 63;
   const char* const row = vd_row<T>(p, ch.row);
   const float* const q = p.probs + (size_t)ch.row * p.probs_stride;
-  for (int chunk = split * VD_WAVES + wave; chunk < p.n_chunks; chunk += p.splits * VD_WAVES) {
-    double z = 0.0;
+  for (int chunk = first; chunk < p.n_chunks; chunk += step) {
+    float x[PIECES][PER], y[PIECES][PER];
 #pragma unroll
     for (int i = 0; i < PIECES; ++i) {
-      const int first = chunk * VD_CHUNK + (64 * i + lane) * PER;
-      float x[PER], y[PER];
-      vd_load<T>(row, first, p.V, x);
-      vd_load<float>(reinterpret_cast<const char*>(q), first, p.V, y);
-#pragma unroll
-      for (int j = 0; j < PER; ++j) {
-        const double w = vd_weight(x[j], ch.m, c) * inv_z - (double)y[j];
-        z += first + j < p.V && w > 0.0 ? w : 0.0;
-      }
+      const int at = chunk * VD_CHUNK + (64 * i + lane) * PER;
+      vd_load<T>(row, at, p.V, x[i]);
+      vd_load<float>(reinterpret_cast<const char*>(q), at, p.V, y[i]);
     }
+    double z = 0.0;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {                      // (behind the row's end y is -inf, and the weight is left out)
+        const double w = vd_weight(x[i][j], ch.m, ch.c, s_exp) * ch.inv_z - (double)y[i][j];
+        z += w > 0.0 && y[i][j] > -INFINITY ? w : 0.0;
+      }
     z = vd_wave_sum(z);
     if (lane == 0) p.rest[(size_t)b * p.n_chunks + chunk] = z;
   }
 }
 template <typename T>
-__global__ __launch_bounds__(VD_THREADS) void verify_pick_kernel(const VdParams p) {
-  vd_pick<T>(p, blockIdx.x, p.choice[blockIdx.x]);
+__global__ __launch_bounds__(64 * VD_WAVES) void verify_rest_kernel(const VdParams p) {
+  __shared__ double s_exp[VD_EXP];
+  const int b = blockIdx.x / p.splits, split = blockIdx.x - b * p.splits;
+  const VdChoice ch = p.choice[b];
+  if (ch.mode != VD_REST) return;
+  vd_table(s_exp);
+  __syncthreads();
+  vd_rest<T>(p, b, ch, split * VD_WAVES + (threadIdx.x >> 6), p.splits * VD_WAVES, s_exp);
+}
+// Few sequences: each of these workgroups decides for itself, and the first writes it down (or draws at once where
+// there is no rest), which saves a launch.
+template <typename T>
+__global__ __launch_bounds__(VD_BLOCK) void verify_decide_rest_kernel(const VdParams p) {
+  __shared__ double s_exp[VD_EXP];
+  __shared__ int s_row;
+  __shared__ VdChoice s_choice;
+  const int b = blockIdx.x / p.splits, split = blockIdx.x - b * p.splits;
+  VdChoice ch;
+  vd_table(s_exp);
+  if (split == 0) {
+    ch = vd_decide<T, true>(p, b, s_exp, &s_row, &s_choice);
+    if (threadIdx.x == 0) p.choice[b] = ch;
+    if (ch.mode != VD_REST) vd_pick<T>(p, b, ch, s_exp);
+  } else {
+    ch = vd_decide<T, false>(p, b, s_exp, &s_row, &s_choice);
+  }
+  if (ch.mode == VD_REST) vd_rest<T>(p, b, ch, split * VD_BLOCK_WAVES + (threadIdx.x >> 6), p.splits * VD_BLOCK_WAVES, s_exp);
+}
+template <typename T>
+__global__ __launch_bounds__(VD_BLOCK) void verify_pick_kernel(const VdParams p) {
+  __shared__ double s_exp[VD_EXP];
+  vd_table(s_exp);
+  const VdChoice ch = p.choice[blockIdx.x];
+  if (ch.mode != VD_REST) return;            // (drawn already)
+  __syncthreads();
+  vd_pick<T>(p, blockIdx.x, ch, s_exp);
 }
 
 }  // namespace t2i
@@ -521,8 +686,10 @@ extern "C" int t2i_verify_drafts(const void* logits, int32_t logits_type, int64_
     return fail(T2I_ERR_ALIGN, "verify_drafts arrays must be aligned to their values");
   t2i::VdParams p{};
   p.n_chunks = vd_chunks(V);
-  p.splits = (p.n_chunks + t2i::VD_WAVES - 1) / t2i::VD_WAVES;
-  if ((long long)M * p.splits > 0xFFFFFFFFLL / t2i::VD_THREADS || n_seqs > 1 << 20)
+  // chunks of a wave: enough waves for every CU's eight a SIMD, else one after the other
+  const int run = (int)std::max<long long>(1, std::min<long long>(((long long)M * p.n_chunks + 8191) / 8192, 16));
+  p.splits = (p.n_chunks + t2i::VD_WAVES * run - 1) / (t2i::VD_WAVES * run);
+  if ((long long)M * p.splits > 0xFFFFFFFFLL / (64 * t2i::VD_WAVES) || n_seqs > 1 << 20)
     return fail(T2I_ERR_SHAPE, "M=%d rows of %d logits, %d sequences exceed the grid", M, V, n_seqs);
   const size_t need = vd_bytes(M, V, n_seqs, draft_probs != nullptr);
   if (!workspace || workspace_bytes < need) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
@@ -534,24 +701,30 @@ extern "C" int t2i_verify_drafts(const void* logits, int32_t logits_type, int64_
   p.choice = reinterpret_cast<t2i::VdChoice*>(p.chunks + (size_t)M * p.n_chunks);
   p.rest = reinterpret_cast<double*>(p.choice + (draft_probs ? n_seqs : 0));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  // workgroups of a sequence's rest: about two a CU in all
-  const int rest_splits = std::max(1, std::min(p.splits, (512 + n_seqs - 1) / n_seqs));
-#define T2I_VD(ty)                                                                                                       \
-  hipLaunchKernelGGL((t2i::verify_rows_kernel<ty>), dim3(M * p.splits), dim3(t2i::VD_THREADS), 0, s, p);                 \
-  if (int rc = t2i_host::hip_status(hipGetLastError(), "verify_drafts launch")) return rc;                               \
-  if (!draft_probs) {                                                                                                    \
-    hipLaunchKernelGGL((t2i::verify_kernel<ty>), dim3(n_seqs), dim3(t2i::VD_THREADS), 0, s, p);                          \
-    return t2i_host::hip_status(hipGetLastError(), "verify_drafts launch");                                              \
-  }                                                                                                                      \
-  p.splits = rest_splits;                                                                                                \
-  hipLaunchKernelGGL((t2i::verify_rest_kernel<ty>), dim3(n_seqs * rest_splits), dim3(t2i::VD_THREADS), 0, s, p);         \
-  if (int rc = t2i_host::hip_status(hipGetLastError(), "verify_drafts launch")) return rc;                               \
-  hipLaunchKernelGGL((t2i::verify_pick_kernel<ty>), dim3(n_seqs), dim3(t2i::VD_THREADS), 0, s, p);                       \
-  return t2i_host::hip_status(hipGetLastError(), "verify_drafts launch")
+  // few sequences: their workgroups decide for themselves, so long as all of them run at once
+  const int wide = (p.n_chunks + t2i::VD_BLOCK_WAVES - 1) / t2i::VD_BLOCK_WAVES;
+  const bool fused = draft_probs && (long long)n_seqs * wide <= 256;
+#define T2I_VD_LAUNCH(kernel, ty, groups, threads)                                                                    \
+  hipLaunchKernelGGL((t2i::kernel<ty>), dim3(groups), dim3(threads), 0, s, p);                                        \
+  if (int rc = t2i_host::hip_status(hipGetLastError(), "verify_drafts launch")) return rc
+#define T2I_VD(ty)                                                                                                    \
+  T2I_VD_LAUNCH(verify_rows_kernel, ty, M * p.splits, 64 * t2i::VD_WAVES);                                            \
+  if (!fused) { T2I_VD_LAUNCH(verify_kernel, ty, n_seqs, t2i::VD_BLOCK); }                                            \
+  if (!draft_probs) return T2I_OK;                                                                                    \
+  if (fused) {                                                                                                        \
+    p.splits = wide;                                                                                                  \
+    T2I_VD_LAUNCH(verify_decide_rest_kernel, ty, n_seqs * p.splits, t2i::VD_BLOCK);                                   \
+  } else {                                                                                                            \
+    p.splits = std::max(1, std::min((p.n_chunks + t2i::VD_WAVES - 1) / t2i::VD_WAVES, (4096 + n_seqs - 1) / n_seqs)); \
+    T2I_VD_LAUNCH(verify_rest_kernel, ty, n_seqs * p.splits, 64 * t2i::VD_WAVES);                                     \
+  }                                                                                                                   \
+  T2I_VD_LAUNCH(verify_pick_kernel, ty, n_seqs, t2i::VD_BLOCK);                                                       \
+  return T2I_OK
   switch (logits_type) {
     case T2I_LOGITS_FP32: { T2I_VD(float); }
     case T2I_LOGITS_BF16: { T2I_VD(t2i::VdBf16); }
     default: { T2I_VD(t2i::VdF16); }
   }
 #undef T2I_VD
+#undef T2I_VD_LAUNCH
 }
