@@ -652,9 +652,9 @@ int t2i_paged_attention(const uint16_t* q, int32_t rows, const int32_t* plan, in
  * the log probability (at T, or at 1 where T is not above 0) of the token that came out there, 0 behind the other rows.
  * Logits of -inf have probability 0.  Behind a row that holds a NaN or +inf, or nothing but -inf, no draft
  * stays, the next token is -1 and its log probability NaN.  A draft outside [0, V) does not stay.  A sequence
- * without rows (or whose rows do not lie in the batch): count 0, next token -1.
+ * without rows: count 0, next token -1; so all of them where row_starts do not ascend within 0 .. M.
  * Weights and sums are fp64.  The workspace (t2i_verify_drafts_workspace_bytes) is scratch as for
- * t2i_packed_attention.  n_seqs at most 2^20.
+ * t2i_packed_attention.  n_seqs at most 65536.
  * No counterpart in the reference, which decodes greedily (qwen_npu.py:321).
  */
 size_t t2i_verify_drafts_workspace_bytes(int32_t M, int32_t V, int32_t n_seqs, int32_t with_probs);
@@ -671,11 +671,13 @@ int t2i_verify_drafts(const void* logits, int32_t logits_type, int64_t row_strid
  * any other id: none), as t2i_adapter_plan_words words on the device, for every projection of the step.
  *
  * t2i_adapter_add: out[r] = y[r] + scales[a] * B_a (A_a x[r]) with a = ids[r], y[r] itself for rows without an
- * adapter; y bf16 [M, N] is the shared projection's output, x bf16 [M, K] its input, out may be y.  a bf16
- * [n_adapters, parts * R, K] and b bf16 [n_adapters, N, R] with R = rank (1 to 256) rounded up to a
- * multiple of 16, the places behind rank 0; scales fp32 [n_adapters] (NULL: 1).  The columns may be several
+ * adapter; y bf16 [M, N] is the shared projection's output, x bf16 [M, K] its input, out may be y.  With R = rank (1 to
+ * 256) rounded up to a multiple of 16, a is A bf16 [n_adapters, parts * R, K] and b is B bf16 [n_adapters, N, R], the places behind
+ * rank 0, in the order that the kernels take them: a [n][parts * R / 16][K / 32][g 4][c 16][8] holds rank 16 i + c and k 32 s
+ * + 8 g .., b [n][ceil(N / 128)][R / 16][t 8][g 2][c 16][8] column 128 i + 8 c + t and ranks 16 s + 8 g .. (columns behind N 0);
+ * scales fp32 [n_adapters] (NULL: 1).  The columns may be several
  * projections' beside each other (parts up to 4): slice i of widths[i] columns (host memory; multiples
- * of 64, parts 1: NULL) has rows i * R .. of a; or, paired (parts 2), alternate between them (column 2j of slice 0, gate, column
+ * of 128, parts 1: NULL) has rows i * R .. of A; or, paired (parts 2), alternate between them (column 2j of slice 0, gate, column
  * 2j + 1 of slice 1, up; as t2i_w4a16_gate_up without SwiGLU leaves them interleaved in one linear).  swiglu (paired alone): out
  * bf16 [M, N / 2] = silu(gate) * up.  Sums are fp32, A x enters the second product with 16 bits, the result is rounded
  * once.  The workspace (t2i_adapter_add_workspace_bytes) is scratch as t2i_packed_attention's.
@@ -685,7 +687,7 @@ int t2i_verify_drafts(const void* logits, int32_t logits_type, int64_t row_strid
 int64_t t2i_adapter_plan_words(int32_t M, int32_t n_adapters);
 int t2i_adapter_plan(const int32_t* ids, int32_t M, int32_t n_adapters, int32_t* plan, int64_t plan_words,
                      void* stream);
-size_t t2i_adapter_add_workspace_bytes(int32_t M, int32_t parts, int32_t rank);
+size_t t2i_adapter_add_workspace_bytes(int32_t M, int32_t n_adapters, int32_t parts, int32_t rank);
 int t2i_adapter_add(const uint16_t* y, const uint16_t* x, int32_t M, int32_t K, int32_t N, const int32_t* plan,
                     int64_t plan_words, const uint16_t* a, const uint16_t* b, const float* scales,
                     int32_t n_adapters, int32_t rank, int32_t parts, const int32_t* widths, int32_t paired,

@@ -21,8 +21,9 @@ def _add(y=FAKE, x=FAKE, m=9, k=128, n=128, plan=FAKE, words=10**9, a=FAKE, b=FA
 
 @pytest.mark.parametrize("kw", [dict(m=0), dict(m=1 << 24), dict(pool=0), dict(pool=512), dict(k=0), dict(k=48), dict(n=8), dict(n=24),
                                 dict(k=1 << 21), dict(n=1 << 21), dict(rank=0), dict(rank=257), dict(parts=0), dict(parts=5),
-                                dict(parts=1, paired=1), dict(parts=3, paired=1), dict(parts=2, widths=[64, 32]),
-                                dict(parts=2, widths=[32, 96]), dict(parts=2, widths=[64, 128]), dict(parts=2, widths=[-64, 192]),
+                                dict(parts=1, paired=1), dict(parts=3, paired=1), dict(parts=2, n=256, widths=[128, 64]),
+                                dict(parts=2, n=256, widths=[64, 192]), dict(parts=2, n=256, widths=[128, 256]),
+                                dict(parts=2, n=256, widths=[-128, 384]),
                                 dict(m=(1 << 24) - 1, n=1 << 20)], ids=str)
 def test_sizes(kw):
     assert _add(**kw) == _lib.T2I_ERR_SHAPE
@@ -36,11 +37,12 @@ def test_pointers_and_values():
     assert _add(scales=0x10002) == E.T2I_ERR_ALIGN and _add(ws=0x10008) == E.T2I_ERR_ALIGN
     assert _add(parts=2) == E.T2I_ERR_NULL
     assert _add(swiglu=1) == E.T2I_ERR_VALUE and _add(swiglu=1, paired=1, parts=2, out=FAKE) == E.T2I_ERR_VALUE
-    need, words = lib.t2i_adapter_add_workspace_bytes(9, 1, 8), lib.t2i_adapter_plan_words(9, 3)
-    assert need == 9 * 16 * 4 and words > 9
+    need, words = lib.t2i_adapter_add_workspace_bytes(9, 3, 1, 8), lib.t2i_adapter_plan_words(9, 3)
+    assert need > 9 * 16 * 4 and words > 9
     assert _add(nbytes=need - 1) == E.T2I_ERR_WORKSPACE and _add(ws=None) == E.T2I_ERR_WORKSPACE
     assert _add(words=words - 1) == E.T2I_ERR_WORKSPACE and _plan(words=words - 1) == E.T2I_ERR_WORKSPACE
-    assert lib.t2i_adapter_add_workspace_bytes(9, 5, 8) == 0 and lib.t2i_adapter_add_workspace_bytes(9, 1, 257) == 0
+    assert lib.t2i_adapter_add_workspace_bytes(9, 3, 5, 8) == 0 and lib.t2i_adapter_add_workspace_bytes(9, 3, 1, 257) == 0
+    assert lib.t2i_adapter_add_workspace_bytes(0, 3, 1, 8) == 0 and lib.t2i_adapter_add_workspace_bytes(9, 512, 1, 8) == 0
     assert _plan(ids=None) == E.T2I_ERR_NULL and _plan(plan=None) == E.T2I_ERR_NULL
     assert _plan(ids=0x10002) == E.T2I_ERR_ALIGN and _plan(plan=0x10004) == E.T2I_ERR_ALIGN
     assert _plan(m=0) == E.T2I_ERR_SHAPE and _plan(n=0) == E.T2I_ERR_SHAPE and _plan(n=512) == E.T2I_ERR_SHAPE

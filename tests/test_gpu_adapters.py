@@ -78,8 +78,8 @@ CASES = [
     (32, [16], False, 1, 1, 1, "one"),
     (128, [16], False, 8, 3, 5, "mixed"),
     (1024, [2048, 1024, 1024], False, 16, 32, 16, "mixed"),
-    (1024, [64, 128, 64], False, 20, 4, 70, "runs"),
-    (256, [64, 64, 64, 64], False, 64, 5, 257, "mixed"),
+    (1024, [128, 256, 128], False, 20, 4, 70, "runs"),
+    (256, [128, 128, 128, 128], False, 64, 5, 257, "mixed"),
     (2048, [1024], False, 128, 2, 33, "one"),
     (160, [272], False, 33, 7, 300, "runs"),
     (1024, [48], False, 256, 3, 66, "mixed"),
@@ -118,16 +118,16 @@ def test_plan_keeps_every_row_once(gpu):
         ids = _ids(gpu, kind, m, pool, seed=m)
         plan = ops.AdapterPlan(ids, pool)
         cap = m // 64 + min(pool + 1, m)
-        tiles, order = plan.table[:4 * cap].view(cap, 4).cpu(), plan.table[4 * cap:].cpu()
-        i = ids.cpu().long()
+        tiles, i = plan.table.view(cap, 68).cpu().tolist(), ids.cpu().long()
         i = torch.where((i < 0) | (i >= pool), pool, i)
-        assert torch.equal(order.long(), torch.sort(i, stable=True).indices)
-        at = 0
-        for a, first, rows, _ in tiles.tolist():
+        order, at = [], 0
+        for a, first, rows, _, *places in tiles:
             if rows:
                 assert first == at and rows <= 64
-                assert (i[order[at:at + rows].long()] == (a if a >= 0 else pool)).all()
+                order += places[:rows]
+                assert all(int(i[r]) == (a if a >= 0 else pool) for r in places[:rows])
                 at += rows
+        assert order == torch.sort(i, stable=True).indices.tolist()
         assert at == m
 
 
@@ -156,15 +156,15 @@ def test_rows_do_not_touch_each_other(gpu):
 
 
 def test_put(gpu):
-    g, a, b, scales, pool_ = _make(gpu, 128, [64, 64], False, 24, 3)
-    x, y = torch.randn(6, 128, device=gpu, generator=g).to(BF16), torch.randn(6, 128, device=gpu, generator=g).to(BF16)
+    g, a, b, scales, pool_ = _make(gpu, 128, [128, 128], False, 24, 3)
+    x, y = torch.randn(6, 128, device=gpu, generator=g).to(BF16), torch.randn(6, 256, device=gpu, generator=g).to(BF16)
     ids = torch.tensor([0, 1, 2, 1, -1, 1], dtype=torch.int32, device=gpu)
     plan = ops.AdapterPlan(ids, 3)
-    na, nb = torch.randn(2, 8, 128, device=gpu, generator=g).to(BF16), torch.randn(128, 8, device=gpu, generator=g).to(BF16)
+    na, nb = torch.randn(2, 8, 128, device=gpu, generator=g).to(BF16), torch.randn(256, 8, device=gpu, generator=g).to(BF16)
     pool_.put(1, na, nb, 0.5)
     a[1], b[1], scales[1] = 0, 0, 0.5
     a[1, :, :8], b[1, :, :8] = na, nb
-    _check(ops.adapter_add(y, x, pool_, plan, out=torch.empty_like(y)), *_reference(y, x, a, b, scales, [64, 64], False, ids))
+    _check(ops.adapter_add(y, x, pool_, plan, out=torch.empty_like(y)), *_reference(y, x, a, b, scales, [128, 128], False, ids))
     for args in ((3, na, nb), (-1, na, nb), (1, na[0], nb), (1, na, nb[:, :4]), (1, na.float(), nb), (1, na[:, :, :64], nb)):
         with pytest.raises(ValueError):
             pool_.put(*args)
@@ -234,15 +234,15 @@ def test_no_rows(gpu):
 
 
 def test_refusals(gpu):
-    g, a, b, scales, pool_ = _make(gpu, 128, [64, 64], False, 8, 3)
-    x, y = torch.zeros(5, 128, dtype=BF16, device=gpu), torch.zeros(5, 128, dtype=BF16, device=gpu)
+    g, a, b, scales, pool_ = _make(gpu, 128, [128, 128], False, 8, 3)
+    x, y = torch.zeros(5, 128, dtype=BF16, device=gpu), torch.zeros(5, 256, dtype=BF16, device=gpu)
     ids = torch.zeros(5, dtype=torch.int32, device=gpu)
     plan = ops.AdapterPlan(ids, 3)
-    make = lambda **kw: ops.Adapters(**{**dict(a=a, b=b, scales=scales, widths=[64, 64]), **kw})  # noqa: E731
+    make = lambda **kw: ops.Adapters(**{**dict(a=a, b=b, scales=scales, widths=[128, 128]), **kw})  # noqa: E731
     make()
     for kw in (dict(a=a.float()), dict(a=a.cpu()), dict(a=a[:2]), dict(a=a[0]), dict(b=b[:, :, :4].contiguous()), dict(widths=None),
-               dict(widths=[32, 96]), dict(widths=[64, 128]), dict(widths=[64.0, 64]), dict(paired=True), dict(scales=scales[:2]),
-               dict(scales=scales.double()), dict(a=a[..., :100].contiguous()), dict(b=b[:, :120].contiguous(), widths=[64, 56])):
+               dict(widths=[64, 192]), dict(widths=[128, 256]), dict(widths=[128.0, 128]), dict(paired=True), dict(scales=scales[:2]),
+               dict(scales=scales.double()), dict(a=a[..., :100].contiguous()), dict(b=b[:, :248].contiguous(), widths=[128, 120])):
         with pytest.raises(ValueError):
             make(**kw)
     wide = torch.zeros(1, 32, 64, dtype=BF16, device=gpu)
@@ -254,7 +254,7 @@ def test_refusals(gpu):
         with pytest.raises(ValueError):
             ops.AdapterPlan(*args)
     for kw in (dict(y=y[:4]), dict(x=x[:, :64].contiguous()), dict(x=x.float()), dict(plan=ops.AdapterPlan(ids, 4)), dict(swiglu=True),
-               dict(out=torch.empty(5, 64, dtype=BF16, device=gpu)), dict(out=torch.empty(5, 128, device=gpu)), dict(y=y.T),
+               dict(out=torch.empty(5, 128, dtype=BF16, device=gpu)), dict(out=torch.empty(5, 256, device=gpu)), dict(y=y.T),
                dict(adapters=None), dict(plan=None)):
         with pytest.raises(ValueError):
             ops.adapter_add(**{**dict(y=y, x=x, adapters=pool_, plan=plan), **kw})

@@ -14,7 +14,7 @@ def _call(logits=FAKE, kind=0, stride=40, m=5, v=40, starts=FAKE, n=2, tokens=FA
 
 
 @pytest.mark.parametrize("kw", [dict(m=0), dict(v=0), dict(n=0), dict(m=-1), dict(stride=39), dict(probs_stride=39),
-                                dict(m=2**24, v=4096, stride=4096, probs_stride=4096), dict(n=2**20 + 1)], ids=str)
+                                dict(m=2**24, v=4096, stride=4096, probs_stride=4096), dict(n=2**16 + 1)], ids=str)
 def test_sizes(kw):
     assert _call(**kw) == _lib.T2I_ERR_SHAPE
 

@@ -141,7 +141,7 @@ SIGNATURES = {
                                     c_void_p]),
     "t2i_adapter_plan_words": (c_int64, [c_int32, c_int32]),
     "t2i_adapter_plan": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_int64, c_void_p]),
-    "t2i_adapter_add_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32]),
+    "t2i_adapter_add_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
     "t2i_adapter_add": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p,
                                   c_void_p, c_int32, c_int32, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
                                   c_size_t, c_void_p]),

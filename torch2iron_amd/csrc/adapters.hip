@@ -17,13 +17,13 @@ namespace t2i {
 constexpr int AD_THREADS = 1024;             // of the plan
 constexpr int AD_MOST = 511;                 // adapters of a pool
 constexpr int AD_TILE = 64;                  // rows of a tile: one adapter's
-constexpr int AD_REC = 4;                    // words of a tile: {adapter (-1: none), its first place in the order, rows, 0}
+constexpr int AD_HEAD = 4;                   // words of a tile: {adapter (-1: none), its first place in the order, rows, 0},
+constexpr int AD_REC = AD_HEAD + AD_TILE;    //   then its rows, so that one look at the plan gives all
 constexpr int AD_PARTS = 4;                  // slices of a projection's columns
 
 struct AdapterPlanParams {
   const int32_t* ids;                        // [M]
   int32_t* tiles;                            // [tiles_cap][AD_REC]
-  int32_t* order;                            // [M] rows by adapter, those without one last
   int M, n, tiles_cap;
 };
 
@@ -44,7 +44,7 @@ __device__ __forceinline__ int adapter_scan(int v, int* s_wave) {
   return before + x - v;
 }
 
-// One workgroup: a counting sort that keeps the rows of an adapter in their order.  A wave takes its share of
+// One workgroup: a counting sort (by adapter, those rows last that have none) that keeps the rows of an adapter in their order.  A wave takes its share of
 // the rows 64 at a time, adapter by adapter of those there are among them.
 __global__ __launch_bounds__(AD_THREADS) void adapter_plan_kernel(const AdapterPlanParams p) {
   extern __shared__ int s_count[];           // [16 waves][n + 1]: rows, then the next place, of a wave's adapter
@@ -109,11 +109,11 @@ __global__ __launch_bounds__(AD_THREADS) void adapter_plan_kernel(const AdapterP
       rec.y = s_start[lo] + (t - s_tile[lo]) * AD_TILE;
       rec.z = min(s_start[lo + 1] - rec.y, AD_TILE);
     }
-    reinterpret_cast<int4*>(p.tiles)[t] = rec;
+    *reinterpret_cast<int4*>(p.tiles + (size_t)t * AD_REC) = rec;
   }
   walk([&](int row, int a, unsigned long long same, bool is) {
-    const int at = mine[a];
-    if (is) p.order[at + __builtin_popcountll(same & ((1ull << lane) - 1))] = row;
+    const int at = mine[a], in = at + __builtin_popcountll(same & ((1ull << lane) - 1)) - s_start[a];   // of its adapter's rows
+    if (is) p.tiles[(size_t)(s_tile[a] + in / AD_TILE) * AD_REC + AD_HEAD + in % AD_TILE] = row;
     if (lane == 0) mine[a] = at + __builtin_popcountll(same);
   });
 }
@@ -122,158 +122,192 @@ struct AdapterParams {
   const uint16_t* x;                         // [M, K]
   const uint16_t* y;                         // [M, N]
   uint16_t* out;                             // [M, N], or [M, N / 2]
-  const uint16_t* a;                         // [n, parts * R, K], R a multiple of 16
-  const uint16_t* b;                         // [n, N, R]
+  const uint16_t* a;                         // [n][parts * R / 16][K / 32][4 groups of 8 k][16 ranks][8 k], R a multiple of 16
+  const uint16_t* b;                         // [n][N / 128 rounded up][R / 16][8 t][2 groups of 8 ranks][16 c][8 ranks]: column 8 c + t
   const float* scales;                       // [n] or NULL
   const int32_t* tiles;
-  const int32_t* order;
-  uint16_t* h;                               // [M][parts * R / 16][hi 16, lo 16]: rows in the plan's order
+  uint16_t* h;                               // [tiles * 4][parts * R / 16][hi 0-7, hi 8-15, lo 0-7, lo 8-15][16 rows][8 ranks]
   int M, K, N, n, R, rank, parts, ends[AD_PARTS], blocks, swiglu;   // ends: column behind each slice
 };
 
 // A tile as the plan has it, checked; rows 0: nothing to do.
 struct AdapterTile {
   int adapter, first, rows;
+  const int32_t* row;
+  // (a place behind the tile's last row is never asked for)
+  __device__ __forceinline__ int at(const AdapterParams& p, int i) const { return min(max(row[i], 0), p.M - 1); }
 };
 __device__ __forceinline__ AdapterTile adapter_tile(const AdapterParams& p, int t) {
-  const int4 w = reinterpret_cast<const int4*>(p.tiles)[t];
-  AdapterTile r{w.x, w.y, w.z};
+  const int32_t* const rec = p.tiles + (size_t)t * AD_REC;
+  const int4 w = *reinterpret_cast<const int4*>(rec);
+  AdapterTile r{w.x, w.y, w.z, rec + AD_HEAD};
   if (r.adapter >= p.n || r.first < 0 || r.rows < 0 || r.rows > AD_TILE || r.first > p.M - r.rows) r.rows = 0;
   return r;
 }
-__device__ __forceinline__ int adapter_row(const AdapterParams& p, int at) { return min(max(p.order[at], 0), p.M - 1); }
 
 // ============================================================================
 // h = scale A x
 // ============================================================================
-// A workgroup 16 rows of a tile by NC x 16 ranks; its waves share K and meet in LDS.  Both operands come straight from
-// memory: lane (c, g) holds 8 neighbouring k of row c (x) and of rank c (A).
-constexpr int AD_WAVES = 8;
-
-template <int NC>
-__global__ __launch_bounds__(64 * AD_WAVES) void adapter_shrink_kernel(const AdapterParams p) {
-  __shared__ float s_part[AD_WAVES][NC][16][17];
+// A workgroup RT x 16 rows of a tile by NC x 16 ranks; its waves take 128 k in turn and meet in LDS.  A comes in the order
+// that the MFMA takes it (1 KB a load instruction).  An operand's lanes want 16 rows of x at once: loaded that way four
+// neighbouring lanes ask for four lines, and the loads alone took 16 us of 4001 rows' 19 (K 6144, two fragments of
+// ranks).  So an instruction takes 256 bytes of four rows, and the rows turn into operands in the wave's own part of LDS, a
+// row's 16-byte piece q at place q ^ row: 16 lanes of a write or a read cover all banks.
+template <int NC, int RT, int W>
+__global__ __launch_bounds__(64 * W) void adapter_shrink_kernel(const AdapterParams p) {
+  constexpr int STEPS = 4;                                 // of 32 k
+  union Lds {
+    uint16_t x[W][RT][16 * 32 * STEPS];
+    float part[W][RT * NC][16][17];
+  };
+  __shared__ __align__(16) Lds lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int block = blockIdx.x % p.blocks, sub = blockIdx.x / p.blocks % (AD_TILE / 16);
-  const AdapterTile t = adapter_tile(p, blockIdx.x / p.blocks / (AD_TILE / 16));
+  const int block = blockIdx.x % p.blocks, sub = blockIdx.x / p.blocks % (AD_TILE / 16 / RT) * RT;
+  const int tile = blockIdx.x / p.blocks / (AD_TILE / 16 / RT);
+  const AdapterTile t = adapter_tile(p, tile);
   if (t.adapter < 0 || sub * 16 >= t.rows) return;
   const int c = lane & 15, g = lane >> 4;
-  const int ranks = p.parts * p.R, r0 = block * NC * 16;
-  const uint16_t* const x = p.x + (size_t)adapter_row(p, t.first + min(sub * 16 + c, t.rows - 1)) * p.K + 8 * g;
+  const int groups = p.parts * p.R / 16, g0 = block * NC, steps = p.K / 32;
+  const uint16_t* x[RT][4];                                // rows 4 q + g, from the lane's piece on
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) x[i][q] = p.x + (size_t)t.at(p, min((sub + i) * 16 + 4 * q + g, t.rows - 1)) * p.K;
   const uint16_t* a[NC];
 #pragma unroll
-  for (int j = 0; j < NC; ++j) a[j] = p.a + ((size_t)t.adapter * ranks + min(r0 + 16 * j + c, ranks - 1)) * p.K + 8 * g;
-  const int steps = p.K / 32, k0 = wave * steps / AD_WAVES, k1 = (wave + 1) * steps / AD_WAVES;
-  f32x4 acc[NC];
+  for (int j = 0; j < NC; ++j) a[j] = p.a + ((size_t)t.adapter * groups + min(g0 + j, groups - 1)) * p.K * 16 + 8 * lane;
+  f32x4 acc[RT][NC];
 #pragma unroll
-  for (int j = 0; j < NC; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int k = k0; k < k1; ++k) {
-    const u32x4 xv = *reinterpret_cast<const u32x4*>(x + 32 * k);
+  for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const u32x4 av = *reinterpret_cast<const u32x4*>(a[j] + 32 * k);
-      acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xv), __builtin_bit_cast(bf16x8, av), acc[j], 0, 0, 0);
+    for (int j = 0; j < NC; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  u32x4 xv[RT][4], av[STEPS][NC];
+  const auto fetch = [&](int s0) __attribute__((always_inline)) {
+    const int k = min(32 * s0 + 8 * c, p.K - 8);           // (what lies behind K is not multiplied)
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) xv[i][q] = *reinterpret_cast<const u32x4*>(x[i][q] + k);
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) av[u][j] = *reinterpret_cast<const u32x4*>(a[j] + (size_t)min(s0 + u, steps - 1) * 512);
+  };
+  if (STEPS * wave < steps) fetch(STEPS * wave);
+  for (int s0 = STEPS * wave; s0 < steps; s0 += STEPS * W) {
+    u32x4 an[STEPS][NC];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<u32x4*>(&lds.x[wave][i][(4 * q + g) * 128 + 8 * (c ^ (4 * q + g))]) = xv[i][q];
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) an[u][j] = av[u][j];
+    if (s0 + STEPS * W < steps) fetch(s0 + STEPS * W);
+#pragma unroll
+    for (int u = 0; u < STEPS; ++u) {
+      if (s0 + u >= steps) break;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const u32x4 xo = *reinterpret_cast<const u32x4*>(&lds.x[wave][i][c * 128 + 8 * ((4 * u + g) ^ c)]);
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xo), __builtin_bit_cast(bf16x8, an[u][j]), acc[i][j], 0, 0, 0);
+      }
     }
   }
-  // register i: row 4 g + i, rank c
+  __syncthreads();                                         // the rows of x are done with
+  // register e: row 4 g + e, rank c
 #pragma unroll
-  for (int j = 0; j < NC; ++j)
+  for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s_part[wave][j][4 * g + i][c] = acc[j][i];
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lds.part[wave][i * NC + j][4 * g + e][c] = acc[i][j][e];
   __syncthreads();
   const float scale = p.scales ? p.scales[t.adapter] : 1.0f;
-  for (int e = threadIdx.x; e < NC * 256; e += 64 * AD_WAVES) {
-    const int j = e >> 8, row = e >> 4 & 15, col = e & 15;
-    const int rank = r0 + 16 * j + col;
-    if (sub * 16 + row >= t.rows || rank >= ranks) continue;
+  for (int e = threadIdx.x; e < RT * NC * 256; e += 64 * W) {
+    const int f = e >> 8, i = f / NC, group = g0 + f % NC, row = e >> 4 & 15, col = e & 15;
+    if (group >= groups) continue;
     float h = 0.0f;
 #pragma unroll
-    for (int w = 0; w < AD_WAVES; ++w) h += s_part[w][j][row][col];
-    h = rank % p.R < p.rank ? h * scale : 0.0f;            // (a rank of the padding may be 0 times an infinity)
+    for (int w = 0; w < W; ++w) h += lds.part[w][f][row][col];
+    h = (16 * group + col) % p.R < p.rank ? h * scale : 0.0f;   // (a rank of the padding may be 0 times an infinity)
     const uint32_t hi = f32_to_bf16(h);
     const float left = h - bf16_to_f32(hi);
-    uint16_t* const dst = p.h + ((size_t)(t.first + sub * 16 + row) * ranks + (r0 + 16 * j)) * 2 + col;
+    uint16_t* const dst = p.h + (((size_t)tile * (AD_TILE / 16) + sub + i) * groups + group) * 512 + (col >> 3) * 128 + row * 8 + (col & 7);
     dst[0] = hi;
-    dst[16] = fabsf(left) < INFINITY ? f32_to_bf16(left) : 0;   // an infinity stays one
+    dst[256] = fabsf(left) < INFINITY ? f32_to_bf16(left) : 0;   // an infinity stays one
   }
 }
 
 // ============================================================================
 // out = y + B h
 // ============================================================================
-// A workgroup a tile by 256 columns, a wave 64 of them, 16 rows at a time.  Run transposed (B's rows as the
-// MFMA's rows), with B's rows in an order that leaves a lane 16 neighbouring columns of one row:
-// register i of part t holds column 16 g + 4 t + i (paired: gate 8 g + 4 (t % 2) + i for t < 2, up behind).
+// A wave 16 rows of a tile by 128 columns; a workgroup the tile's 64 rows, or where the tile has up to 16 rows four times
+// the columns.  B comes in the order that the MFMA takes it, and in one that leaves a lane (c, g) 8 neighbouring
+// columns of rows 4 g .. 4 g + 3 (register i of product t: column 8 c + t of row 4 g + i): y and out move as 256 bytes of
+// four rows an instruction.  Of paired columns the even products are gate's, the odd ones up's.
 template <bool PAIRED>
 __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = (blockIdx.x % p.blocks * 4 + wave) * 64;
-  const AdapterTile t = adapter_tile(p, blockIdx.x / p.blocks);
-  if (n0 >= p.N || t.rows == 0) return;
+  const int tile = blockIdx.x / p.blocks;
+  const AdapterTile t = adapter_tile(p, tile);
+  const bool few = t.rows <= 16;
+  const int block = few ? 4 * (blockIdx.x % p.blocks) + wave : blockIdx.x % p.blocks, n0 = 128 * block;
+  const int sub = few ? 0 : wave;
+  if (n0 >= p.N || sub * 16 >= t.rows) return;
   if (t.adapter < 0 && !p.swiglu && p.out == p.y) return;  // nothing to add in place
   const int c = lane & 15, g = lane >> 4;
-  const int groups = p.parts * p.R / 16, steps = p.R / 16;
-  int slice = 0;                                           // of the wave's columns
-  if (!PAIRED)
-    for (int s = 0; s < AD_PARTS - 1; ++s) slice += s < p.parts - 1 && n0 >= p.ends[s];
-  const uint16_t* b[4];
+  const int col = n0 + 8 * c;
+  int row[4];
+  u32x4 y[4];
 #pragma unroll
-  for (int t4 = 0; t4 < 4; ++t4) {
-    const int col = PAIRED ? 2 * (4 * (t4 & 1) + (c & 3)) + (t4 >> 1) : 4 * t4 + (c & 3);
-    b[t4] = p.b + ((size_t)max(t.adapter, 0) * p.N + min(n0 + 16 * (c >> 2) + col, p.N - 1)) * p.R + 8 * (g & 1);
+  for (int i = 0; i < 4; ++i) {
+    row[i] = t.at(p, min(sub * 16 + 4 * g + i, t.rows - 1));
+    y[i] = *reinterpret_cast<const u32x4*>(p.y + (size_t)row[i] * p.N + min(col, p.N - 8));
   }
-  const int col = n0 + 16 * g;                             // the lane's columns
-  for (int sub = 0; sub * 16 < t.rows; ++sub) {
-    const int at = t.first + min(sub * 16 + c, t.rows - 1);
-    const int row = adapter_row(p, at);
-    const bool live = sub * 16 + c < t.rows && col < p.N;
-    u32x4 y0 = u32x4{0, 0, 0, 0}, y1 = y0;
-    if (live) {
-      y0 = *reinterpret_cast<const u32x4*>(p.y + (size_t)row * p.N + col);
-      y1 = *reinterpret_cast<const u32x4*>(p.y + (size_t)row * p.N + col + 8);
+  f32x4 acc[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (t.adapter >= 0) {
+    const int groups = p.parts * p.R / 16, steps = p.R / 16;
+    int slice = 0;                                         // of the wave's columns
+    if (!PAIRED)
+      for (int s = 0; s < AD_PARTS - 1; ++s) slice += s < p.parts - 1 && n0 >= p.ends[s];
+    const uint16_t* const h = p.h + (((size_t)tile * (AD_TILE / 16) + sub) * groups + slice * steps) * 512 + 8 * lane;
+    const uint16_t* const b = p.b + ((size_t)t.adapter * ((p.N + 127) / 128) + block) * p.R * 128 + 8 * (lane & 31);
+#pragma unroll 2
+    for (int s = 0; s < steps; ++s) {
+      u32x4 hv[2], bv[8];
+      hv[0] = *reinterpret_cast<const u32x4*>(h + 512 * s);
+      if (PAIRED) hv[1] = *reinterpret_cast<const u32x4*>(h + 512 * (s + steps));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) bv[k] = *reinterpret_cast<const u32x4*>(b + (8 * s + k) * 256);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hv[PAIRED ? k & 1 : 0]),
+                                                         __builtin_bit_cast(bf16x8, bv[k]), acc[k], 0, 0, 0);
     }
-    f32x4 acc[4];
+  }
+  if (col >= p.N) return;
 #pragma unroll
-    for (int t4 = 0; t4 < 4; ++t4) acc[t4] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (t.adapter >= 0) {
-      const uint16_t* const h = p.h + ((size_t)at * groups + slice * steps) * 32 + 8 * g;
-      for (int s = 0; s < steps; ++s) {
-        u32x4 hv[2];
-        hv[0] = *reinterpret_cast<const u32x4*>(h + 32 * s);
-        if (PAIRED) hv[1] = *reinterpret_cast<const u32x4*>(h + 32 * (s + steps));
+  for (int i = 0; i < 4; ++i) {
+    if (sub * 16 + 4 * g + i >= t.rows) break;
+    float f[8];
+    unpack8(y[i], f);
 #pragma unroll
-        for (int t4 = 0; t4 < 4; ++t4) {
-          const u32x4 bv = *reinterpret_cast<const u32x4*>(b[t4] + 16 * s);
-          acc[t4] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, bv),
-                                                            __builtin_bit_cast(bf16x8, hv[PAIRED ? t4 >> 1 : 0]), acc[t4], 0, 0, 0);
-        }
-      }
-    }
-    float f[16];
-    {
-      float lo[8], hi[8];
-      unpack8(y0, lo);
-      unpack8(y1, hi);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = lo[i], f[8 + i] = hi[i];
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      f[e] += PAIRED ? acc[2 * (e & 1) + (e >> 3)][e >> 1 & 3] : acc[e >> 2][e & 3];
-    if (!live) continue;
+    for (int k = 0; k < 8; ++k) f[k] += acc[k][i];
     if (p.swiglu) {                                        // silu(gate) * up, rounded once
-      float r[8];
+      float r[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = silu_f32(f[2 * i]) * f[2 * i + 1];
-      *reinterpret_cast<u32x4*>(p.out + (size_t)row * (p.N / 2) + col / 2) =
-          u32x4{pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3]), pack_bf16x2(r[4], r[5]), pack_bf16x2(r[6], r[7])};
+      for (int k = 0; k < 4; ++k) r[k] = silu_f32(f[2 * k]) * f[2 * k + 1];
+      *reinterpret_cast<u32x2*>(p.out + (size_t)row[i] * (p.N / 2) + col / 2) = u32x2{pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3])};
     } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<u32x4*>(p.out + (size_t)row * p.N + col + 8 * i) =
-            u32x4{pack_bf16x2(f[8 * i], f[8 * i + 1]), pack_bf16x2(f[8 * i + 2], f[8 * i + 3]),
-                  pack_bf16x2(f[8 * i + 4], f[8 * i + 5]), pack_bf16x2(f[8 * i + 6], f[8 * i + 7])};
+      *reinterpret_cast<u32x4*>(p.out + (size_t)row[i] * p.N + col) =
+          u32x4{pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7])};
     }
   }
 }
@@ -288,7 +322,7 @@ namespace {
 bool aligned4(const void* p) { return ((uintptr_t)p & 3u) == 0; }
 
 int tiles_cap(int32_t M, int32_t n) { return M / t2i::AD_TILE + std::min(n + 1, M); }
-int64_t plan_words(int32_t M, int32_t n) { return (int64_t)tiles_cap(M, n) * t2i::AD_REC + M; }
+int64_t plan_words(int32_t M, int32_t n) { return (int64_t)tiles_cap(M, n) * t2i::AD_REC; }
 int padded(int32_t rank) { return (rank + 15) / 16 * 16; }
 
 int check_rows(int32_t M, int32_t n) {
@@ -312,15 +346,15 @@ extern "C" int t2i_adapter_plan(const int32_t* ids, int32_t M, int32_t n_adapter
     return fail(T2I_ERR_WORKSPACE, "the plan holds %lld words, %lld needed", (long long)words, (long long)plan_words(M, n_adapters));
   t2i::AdapterPlanParams p{};
   p.ids = ids; p.M = M; p.n = n_adapters; p.tiles_cap = tiles_cap(M, n_adapters);
-  p.tiles = plan; p.order = plan + (size_t)p.tiles_cap * t2i::AD_REC;
+  p.tiles = plan;
   const size_t lds = (size_t)(t2i::AD_THREADS / 64) * (n_adapters + 1) * sizeof(int);
   hipLaunchKernelGGL(t2i::adapter_plan_kernel, dim3(1), dim3(t2i::AD_THREADS), lds, reinterpret_cast<hipStream_t>(stream), p);
   return t2i_host::hip_status(hipGetLastError(), "adapter plan launch");
 }
 
-extern "C" size_t t2i_adapter_add_workspace_bytes(int32_t M, int32_t parts, int32_t rank) {
-  if (M < 1 || parts < 1 || parts > t2i::AD_PARTS || rank < 1 || rank > 256) return 0;
-  return (size_t)M * parts * padded(rank) * 4;
+extern "C" size_t t2i_adapter_add_workspace_bytes(int32_t M, int32_t n_adapters, int32_t parts, int32_t rank) {
+  if (check_rows(M, n_adapters) || parts < 1 || parts > t2i::AD_PARTS || rank < 1 || rank > 256) return 0;
+  return (size_t)tiles_cap(M, n_adapters) * (t2i::AD_TILE / 16) * (parts * padded(rank) / 16) * 1024;
 }
 
 extern "C" int t2i_adapter_add(const uint16_t* y, const uint16_t* x, int32_t M, int32_t K, int32_t N, const int32_t* plan,
@@ -345,7 +379,7 @@ extern "C" int t2i_adapter_add(const uint16_t* y, const uint16_t* x, int32_t M, 
   if (!paired && parts > 1) {
     long long at = 0;
     for (int i = 0; i < parts; ++i) {
-      if (widths[i] < 64 || widths[i] % 64) return fail(T2I_ERR_SHAPE, "a slice of %d columns (multiples of 64)", widths[i]);
+      if (widths[i] < 128 || widths[i] % 128) return fail(T2I_ERR_SHAPE, "a slice of %d columns (multiples of 128)", widths[i]);
       p.ends[i] = (int)(at += widths[i]);
       if (at > N) break;
     }
@@ -353,25 +387,33 @@ extern "C" int t2i_adapter_add(const uint16_t* y, const uint16_t* x, int32_t M, 
   }
   if (words < plan_words(M, n_adapters))
     return fail(T2I_ERR_WORKSPACE, "the plan holds %lld words, %lld needed", (long long)words, (long long)plan_words(M, n_adapters));
-  const size_t need = t2i_adapter_add_workspace_bytes(M, parts, rank);
+  const size_t need = t2i_adapter_add_workspace_bytes(M, n_adapters, parts, rank);
   if (!workspace || workspace_bytes < need) return fail(T2I_ERR_WORKSPACE, "workspace of %zu bytes, %zu needed", workspace ? workspace_bytes : 0, need);
   if (!aligned16(workspace)) return fail(T2I_ERR_ALIGN, "the workspace must be 16-byte aligned");
   const int cap = tiles_cap(M, n_adapters);
   p.x = x; p.y = y; p.out = out; p.a = a; p.b = b; p.scales = scales;
-  p.tiles = plan; p.order = plan + (size_t)cap * t2i::AD_REC; p.h = reinterpret_cast<uint16_t*>(workspace);
+  p.tiles = plan; p.h = reinterpret_cast<uint16_t*>(workspace);
   p.M = M; p.K = K; p.N = N; p.n = n_adapters; p.R = padded(rank); p.rank = rank; p.parts = parts; p.swiglu = swiglu != 0;
-  const int fragments = parts * p.R / 16, expand_blocks = (N + 255) / 256;
-  if ((long long)cap * 4 * fragments > 0xFFFFFFFFLL / 512 || (long long)cap * expand_blocks > 0xFFFFFFFFLL / 256)
+  const int fragments = parts * p.R / 16, expand_blocks = (N + 127) / 128;
+  if ((long long)cap * 4 * fragments > 0xFFFFFFFFLL / 1024 || (long long)cap * expand_blocks > 0xFFFFFFFFLL / 256)
     return fail(T2I_ERR_SHAPE, "M=%d N=%d rank=%d exceed the grid", M, N, rank);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  // few rows: 16 ranks a workgroup, so that there are enough of them
-  if (M <= 256 || fragments == 1) {
-    p.blocks = fragments;
-    hipLaunchKernelGGL(t2i::adapter_shrink_kernel<1>, dim3(cap * 4 * p.blocks), dim3(64 * t2i::AD_WAVES), 0, s, p);
-  } else {
-    p.blocks = (fragments + 3) / 4;
-    hipLaunchKernelGGL(t2i::adapter_shrink_kernel<4>, dim3(cap * 4 * p.blocks), dim3(64 * t2i::AD_WAVES), 0, s, p);
+  // few rows: 16 ranks a workgroup, so that there are enough of them; else all ranks up to 64; many rows: 32 a workgroup
+  const int nc = M <= 256 ? 1 : std::min(fragments, 4), rt = M > 4096 ? 2 : 1;
+  p.blocks = (fragments + nc - 1) / nc;
+#define T2I_SHRINK(NC, RT, W) \
+  hipLaunchKernelGGL((t2i::adapter_shrink_kernel<NC, RT, W>), dim3(cap * (4 / RT) * p.blocks), dim3(64 * W), 0, s, p)
+  switch (nc + 4 * (rt - 1)) {
+    case 1: T2I_SHRINK(1, 1, 8); break;
+    case 2: T2I_SHRINK(2, 1, 8); break;
+    case 3: T2I_SHRINK(3, 1, 8); break;
+    case 4: T2I_SHRINK(4, 1, 8); break;
+    case 5: T2I_SHRINK(1, 2, 8); break;
+    case 6: T2I_SHRINK(2, 2, 8); break;
+    case 7: T2I_SHRINK(3, 2, 8); break;
+    default: T2I_SHRINK(4, 2, 8); break;
   }
+#undef T2I_SHRINK
   if (int rc = t2i_host::hip_status(hipGetLastError(), "adapter shrink launch")) return rc;
   p.blocks = expand_blocks;
   if (paired) hipLaunchKernelGGL(t2i::adapter_expand_kernel<true>, dim3(cap * p.blocks), dim3(256), 0, s, p);

@@ -1537,7 +1537,8 @@ def verify_drafts(logits: torch.Tensor, row_starts: torch.Tensor, tokens: torch.
     [S]``, fp32 ``logprobs [M]`` (log p of the token that came out behind each row, 0 behind the rest; greedy rows at T = 1).
 
     Logits of -inf have probability 0; a row with a NaN, a +inf or nothing but -inf ends its sequence with the token -1
-    and log probability NaN.  A draft outside ``[0, V)`` does not stay.  A sequence without rows: count 0, token -1."""
+    and log probability NaN.  A draft outside ``[0, V)`` does not stay.  A sequence without rows: count 0, token -1; so all of
+    them where ``row_starts`` (of up to 65536 sequences) do not ascend within ``0 .. M``."""
     m, v, stride = _check_logits(logits)
     for n, t, dtype in (("row_starts", row_starts, torch.int32), ("tokens", tokens, torch.int32),
                         ("uniforms", uniforms, torch.float32)):
@@ -1583,10 +1584,10 @@ class Adapters:
 
     ``a`` bf16 ``[n, R, K]``, ``b`` bf16 ``[n, N, R]`` (n up to 511, R up to 256, K a multiple of 32, N of 16), ``scales``
     fp32 ``[n]`` (1 by default).  Of a fused projection: ``a [n, slices, R, K]``, ``b``'s rows in the order of the fused columns, and either
-    ``widths`` (the columns of up to 4 projections beside each other, multiples of 64, as q|k|v) or ``paired=True`` (two
+    ``widths`` (the columns of up to 4 projections beside each other, multiples of 128, as q|k|v) or ``paired=True`` (two
     projections' columns in turn, as ``formats.interleave_gate_up``).  Smaller ranks among them: zeros in the last places.
 
-    The pool keeps its own copy, laid out once; ``put`` replaces one adapter's values in place, so captured calls keep serving."""
+    The pool keeps its own copy, laid out once in the order of the kernels' operands; ``put`` replaces one adapter's values in place, so captured calls keep serving."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor | None = None, widths=None,
                  paired: bool = False):
@@ -1608,14 +1609,12 @@ class Adapters:
             widths = [self.N] if widths is None else _integers("widths", widths)
             if len(widths) != self.parts or sum(widths) != self.N:
                 raise ValueError(f"widths must hold {self.parts} values that make {self.N} columns")
-            if self.parts > 4 or (self.parts > 1 and any(w < 64 or w % 64 for w in widths)):
-                raise ValueError("up to 4 slices of multiples of 64 columns")
+            if self.parts > 4 or (self.parts > 1 and any(w < 128 or w % 128 for w in widths)):
+                raise ValueError("up to 4 slices of multiples of 128 columns")
         # host memory, also where torch's default device is another
         self.widths = None if paired else torch.tensor(widths, dtype=torch.int32, device="cpu")
         self.device = a.device
-        pad = -self.rank % 16
-        self.a = torch.nn.functional.pad(a, (0, 0, 0, pad)).reshape(self.n, -1, self.K).contiguous().clone()
-        self.b = torch.nn.functional.pad(b, (0, pad)).contiguous().clone()
+        self.a, self.b = self._laid_a(a), self._laid_b(b)
         if scales is None:
             scales = torch.ones(self.n, dtype=torch.float32, device=self.device)
         _check_dev("scales", scales, torch.float32)
@@ -1623,6 +1622,20 @@ class Adapters:
             raise ValueError(f"scales must hold {self.n} values")
         self.scales = scales.reshape(-1).clone()
         _same_device(self.device, b=b, scales=scales)
+
+    def _laid_a(self, a: torch.Tensor) -> torch.Tensor:
+        """``[n, slices, up to R, K]`` as ``[n, slices * R / 16, K / 32, 4, 16, 8]``, zeros behind the ranks there are."""
+        r = -(-self.rank // 16) * 16
+        a = torch.nn.functional.pad(a, (0, 0, 0, r - a.shape[2]))
+        a = a.reshape(a.shape[0], self.parts * r // 16, 16, self.K // 32, 4, 8)
+        return a.permute(0, 1, 3, 4, 2, 5).contiguous()
+
+    def _laid_b(self, b: torch.Tensor) -> torch.Tensor:
+        """``[n, N, up to R]`` as ``[n, ceil(N / 128), R / 16, 8, 2, 16, 8]``, zeros behind the ranks and columns there are."""
+        r = -(-self.rank // 16) * 16
+        b = torch.nn.functional.pad(b, (0, r - b.shape[2], 0, -self.N % 128))
+        b = b.reshape(b.shape[0], -1, 16, 8, r // 16, 2, 8)
+        return b.permute(0, 1, 4, 3, 5, 2, 6).contiguous()
 
     def put(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0):
         """Adapter ``slot`` becomes ``a`` (``[R, K]`` or ``[slices, R, K]``), ``b`` (``[N, R]``), ``scale``; a smaller rank
@@ -1638,12 +1651,8 @@ class Adapters:
             raise ValueError(f"a must be [{self.parts}, up to {self.rank}, {self.K}]")
         if tuple(b.shape) != (self.N, a.shape[1]):
             raise ValueError(f"b must be [{self.N}, {a.shape[1]}]")
-        r = a.shape[1]
-        mine = self.a[slot].view(self.parts, -1, self.K)
-        mine[:, :r].copy_(a)
-        mine[:, r:].zero_()
-        self.b[slot, :, :r].copy_(b)
-        self.b[slot, :, r:].zero_()
+        self.a[slot].copy_(self._laid_a(a.unsqueeze(0))[0])
+        self.b[slot].copy_(self._laid_b(b.unsqueeze(0))[0])
         self.scales[slot].fill_(float(scale))
 
 
@@ -1711,7 +1720,7 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Adap
     if m == 0:
         return out
     lib = _lib.load()
-    nbytes = lib.t2i_adapter_add_workspace_bytes(m, adapters.parts, adapters.rank)
+    nbytes = lib.t2i_adapter_add_workspace_bytes(m, adapters.n, adapters.parts, adapters.rank)
     ws = _scratch(workspace, "adapters", nbytes, y.device)
     plan._use()
     _launch(y.device, "t2i_adapter_add",
