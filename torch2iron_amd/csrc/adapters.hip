@@ -127,15 +127,18 @@ struct AdapterParams {
   const float* scales;                       // [n] or NULL
   const int32_t* tiles;
   uint16_t* h;                               // [tiles * 4][parts * R / 16][hi 0-7, hi 8-15, lo 0-7, lo 8-15][16 rows][8 ranks]
-  int M, K, N, n, R, rank, parts, ends[AD_PARTS], blocks, swiglu;   // ends: column behind each slice
+  int M, K, N, n, R, rank, parts, ends[AD_PARTS], blocks, swiglu, tiles_cap;   // ends: column behind each slice
 };
 
 // A tile as the plan has it, checked; rows 0: nothing to do.
 struct AdapterTile {
   int adapter, first, rows;
   const int32_t* row;
-  // (a place behind the tile's last row is never asked for)
-  __device__ __forceinline__ int at(const AdapterParams& p, int i) const { return min(max(row[i], 0), p.M - 1); }
+  // Row i (below AD_TILE) of the tile, its first one behind the last: read without waiting for the count.
+  __device__ __forceinline__ int at(const AdapterParams& p, int i) const {
+    const int r = row[i], r0 = row[0];
+    return min(max(i < rows ? r : r0, 0), p.M - 1);
+  }
 };
 __device__ __forceinline__ AdapterTile adapter_tile(const AdapterParams& p, int t) {
   const int32_t* const rec = p.tiles + (size_t)t * AD_REC;
@@ -148,96 +151,84 @@ __device__ __forceinline__ AdapterTile adapter_tile(const AdapterParams& p, int 
 // ============================================================================
 // h = scale A x
 // ============================================================================
-// A workgroup RT x 16 rows of a tile by NC x 16 ranks; its waves take 128 k in turn and meet in LDS.  A comes in the order
+// A workgroup 16 rows of a tile by NC x 16 ranks; its waves take 128 k in turn and meet in LDS.  A comes in the order
 // that the MFMA takes it (1 KB a load instruction).  An operand's lanes want 16 rows of x at once: loaded that way four
 // neighbouring lanes ask for four lines, and the loads alone took 16 us of 4001 rows' 19 (K 6144, two fragments of
 // ranks).  So an instruction takes 256 bytes of four rows, and the rows turn into operands in the wave's own part of LDS, a
 // row's 16-byte piece q at place q ^ row: 16 lanes of a write or a read cover all banks.
-template <int NC, int RT, int W>
-__global__ __launch_bounds__(64 * W) void adapter_shrink_kernel(const AdapterParams p) {
-  constexpr int STEPS = 4;                                 // of 32 k
+// Sixteen waves in place of eight gained nothing (4001 rows 22.0 us, 8192 56).
+constexpr int AD_WAVES = 8;
+
+template <int NC>
+__global__ __launch_bounds__(64 * AD_WAVES, 4) void adapter_shrink_kernel(const AdapterParams p) {
+  constexpr int STEPS = 4, W = AD_WAVES;                   // steps of 32 k
   union Lds {
-    uint16_t x[W][RT][16 * 32 * STEPS];
-    float part[W][RT * NC][16][17];
+    uint16_t x[W][16 * 32 * STEPS];
+    float part[W][NC][16][17];
   };
   __shared__ __align__(16) Lds lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int block = blockIdx.x % p.blocks, sub = blockIdx.x / p.blocks % (AD_TILE / 16 / RT) * RT;
-  const int tile = blockIdx.x / p.blocks / (AD_TILE / 16 / RT);
+  // (workgroups go round the eight XCDs: those that share rows of x stand eight apart, behind one L2)
+  const int block = blockIdx.x / 8 % p.blocks, rows16 = blockIdx.x / 8 / p.blocks * 8 + blockIdx.x % 8;
+  const int sub = rows16 % (AD_TILE / 16), tile = rows16 / (AD_TILE / 16);
+  const int c = lane & 15, g = lane >> 4;
+  if (tile >= p.tiles_cap) return;
   const AdapterTile t = adapter_tile(p, tile);
   if (t.adapter < 0 || sub * 16 >= t.rows) return;
-  const int c = lane & 15, g = lane >> 4;
+  const uint16_t* x[4];                                    // rows 4 q + g
+#pragma unroll
+  for (int q = 0; q < 4; ++q) x[q] = p.x + (size_t)t.at(p, sub * 16 + 4 * q + g) * p.K;
   const int groups = p.parts * p.R / 16, g0 = block * NC, steps = p.K / 32;
-  const uint16_t* x[RT][4];                                // rows 4 q + g, from the lane's piece on
-#pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) x[i][q] = p.x + (size_t)t.at(p, min((sub + i) * 16 + 4 * q + g, t.rows - 1)) * p.K;
   const uint16_t* a[NC];
 #pragma unroll
   for (int j = 0; j < NC; ++j) a[j] = p.a + ((size_t)t.adapter * groups + min(g0 + j, groups - 1)) * p.K * 16 + 8 * lane;
-  f32x4 acc[RT][NC];
+  f32x4 acc[NC];
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
-#pragma unroll
-    for (int j = 0; j < NC; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  u32x4 xv[RT][4], av[STEPS][NC];
+  for (int j = 0; j < NC; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  u32x4 xv[4];
   const auto fetch = [&](int s0) __attribute__((always_inline)) {
     const int k = min(32 * s0 + 8 * c, p.K - 8);           // (what lies behind K is not multiplied)
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) xv[i][q] = *reinterpret_cast<const u32x4*>(x[i][q] + k);
+    for (int q = 0; q < 4; ++q) xv[q] = *reinterpret_cast<const u32x4*>(x[q] + k);
+  };
+  if (STEPS * wave < steps) fetch(STEPS * wave);
+  for (int s0 = STEPS * wave; s0 < steps; s0 += STEPS * W) {
+    u32x4 av[STEPS][NC];
 #pragma unroll
     for (int u = 0; u < STEPS; ++u)
 #pragma unroll
       for (int j = 0; j < NC; ++j) av[u][j] = *reinterpret_cast<const u32x4*>(a[j] + (size_t)min(s0 + u, steps - 1) * 512);
-  };
-  if (STEPS * wave < steps) fetch(STEPS * wave);
-  for (int s0 = STEPS * wave; s0 < steps; s0 += STEPS * W) {
-    u32x4 an[STEPS][NC];
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<u32x4*>(&lds.x[wave][i][(4 * q + g) * 128 + 8 * (c ^ (4 * q + g))]) = xv[i][q];
-#pragma unroll
-    for (int u = 0; u < STEPS; ++u)
-#pragma unroll
-      for (int j = 0; j < NC; ++j) an[u][j] = av[u][j];
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<u32x4*>(&lds.x[wave][(4 * q + g) * 128 + 8 * (c ^ (4 * q + g))]) = xv[q];
     if (s0 + STEPS * W < steps) fetch(s0 + STEPS * W);
 #pragma unroll
     for (int u = 0; u < STEPS; ++u) {
       if (s0 + u >= steps) break;
+      const u32x4 xo = *reinterpret_cast<const u32x4*>(&lds.x[wave][c * 128 + 8 * ((4 * u + g) ^ c)]);
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        const u32x4 xo = *reinterpret_cast<const u32x4*>(&lds.x[wave][i][c * 128 + 8 * ((4 * u + g) ^ c)]);
-#pragma unroll
-        for (int j = 0; j < NC; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xo), __builtin_bit_cast(bf16x8, an[u][j]), acc[i][j], 0, 0, 0);
-      }
+      for (int j = 0; j < NC; ++j)
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, xo), __builtin_bit_cast(bf16x8, av[u][j]), acc[j], 0, 0, 0);
     }
   }
   __syncthreads();                                         // the rows of x are done with
   // register e: row 4 g + e, rank c
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+  for (int j = 0; j < NC; ++j)
 #pragma unroll
-    for (int j = 0; j < NC; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) lds.part[wave][i * NC + j][4 * g + e][c] = acc[i][j][e];
+    for (int e = 0; e < 4; ++e) lds.part[wave][j][4 * g + e][c] = acc[j][e];
   __syncthreads();
   const float scale = p.scales ? p.scales[t.adapter] : 1.0f;
-  for (int e = threadIdx.x; e < RT * NC * 256; e += 64 * W) {
-    const int f = e >> 8, i = f / NC, group = g0 + f % NC, row = e >> 4 & 15, col = e & 15;
+  for (int e = threadIdx.x; e < NC * 256; e += 64 * W) {
+    const int j = e >> 8, group = g0 + j, row = e >> 4 & 15, col = e & 15;
     if (group >= groups) continue;
     float h = 0.0f;
 #pragma unroll
-    for (int w = 0; w < W; ++w) h += lds.part[w][f][row][col];
+    for (int w = 0; w < W; ++w) h += lds.part[w][j][row][col];
     h = (16 * group + col) % p.R < p.rank ? h * scale : 0.0f;   // (a rank of the padding may be 0 times an infinity)
     const uint32_t hi = f32_to_bf16(h);
     const float left = h - bf16_to_f32(hi);
-    uint16_t* const dst = p.h + (((size_t)tile * (AD_TILE / 16) + sub + i) * groups + group) * 512 + (col >> 3) * 128 + row * 8 + (col & 7);
+    uint16_t* const dst = p.h + (((size_t)tile * (AD_TILE / 16) + sub) * groups + group) * 512 + (col >> 3) * 128 + row * 8 + (col & 7);
     dst[0] = hi;
     dst[256] = fabsf(left) < INFINITY ? f32_to_bf16(left) : 0;   // an infinity stays one
   }
@@ -266,7 +257,7 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterParams
   u32x4 y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    row[i] = t.at(p, min(sub * 16 + 4 * g + i, t.rows - 1));
+    row[i] = t.at(p, sub * 16 + 4 * g + i);
     y[i] = *reinterpret_cast<const u32x4*>(p.y + (size_t)row[i] * p.N + min(col, p.N - 8));
   }
   f32x4 acc[8];
@@ -300,10 +291,10 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterParams
     unpack8(y[i], f);
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] += acc[k][i];
-    if (p.swiglu) {                                        // silu(gate) * up, rounded once
+    if (p.swiglu) {                                        // silu(gate) * up, rounded once (the exponential and the reciprocal are off by an ulp)
       float r[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) r[k] = silu_f32(f[2 * k]) * f[2 * k + 1];
+      for (int k = 0; k < 4; ++k) r[k] = f[2 * k] * __builtin_amdgcn_rcpf(1.0f + exp2_fast(-1.4426950408889634f * f[2 * k])) * f[2 * k + 1];
       *reinterpret_cast<u32x2*>(p.out + (size_t)row[i] * (p.N / 2) + col / 2) = u32x2{pack_bf16x2(r[0], r[1]), pack_bf16x2(r[2], r[3])};
     } else {
       *reinterpret_cast<u32x4*>(p.out + (size_t)row[i] * p.N + col) =
@@ -393,27 +384,22 @@ extern "C" int t2i_adapter_add(const uint16_t* y, const uint16_t* x, int32_t M, 
   const int cap = tiles_cap(M, n_adapters);
   p.x = x; p.y = y; p.out = out; p.a = a; p.b = b; p.scales = scales;
   p.tiles = plan; p.h = reinterpret_cast<uint16_t*>(workspace);
-  p.M = M; p.K = K; p.N = N; p.n = n_adapters; p.R = padded(rank); p.rank = rank; p.parts = parts; p.swiglu = swiglu != 0;
+  p.M = M; p.K = K; p.N = N; p.n = n_adapters; p.tiles_cap = cap; p.R = padded(rank); p.rank = rank; p.parts = parts; p.swiglu = swiglu != 0;
   const int fragments = parts * p.R / 16, expand_blocks = (N + 127) / 128;
-  if ((long long)cap * 4 * fragments > 0xFFFFFFFFLL / 1024 || (long long)cap * expand_blocks > 0xFFFFFFFFLL / 256)
+  if (((long long)cap * 4 + 8) * fragments > 0xFFFFFFFFLL / 1024 || (long long)cap * expand_blocks > 0xFFFFFFFFLL / 256)
     return fail(T2I_ERR_SHAPE, "M=%d N=%d rank=%d exceed the grid", M, N, rank);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  // few rows: 16 ranks a workgroup, so that there are enough of them; else all ranks up to 64; many rows: 32 a workgroup
-  const int nc = M <= 256 ? 1 : std::min(fragments, 4), rt = M > 4096 ? 2 : 1;
+  // as many fragments of ranks a workgroup (up to four) as leave one for every CU (1, 2, 3, 4 of them, us: 331 rows
+  // of 8 16.9, 17.0, 17.8, 18.6; 16 of 3 6.0, 6.4, 6.8, 6.8; 4001 of 2 22.9, 21.8; 8192 of 3 54.4, 56.0, 54.0)
+  const int nc = (int)std::min<long long>(std::min(fragments, 4), std::max<long long>(1, ((long long)M * fragments + 4095) / 4096));
   p.blocks = (fragments + nc - 1) / nc;
-#define T2I_SHRINK(NC, RT, W) \
-  hipLaunchKernelGGL((t2i::adapter_shrink_kernel<NC, RT, W>), dim3(cap * (4 / RT) * p.blocks), dim3(64 * W), 0, s, p)
-  switch (nc + 4 * (rt - 1)) {
-    case 1: T2I_SHRINK(1, 1, 8); break;
-    case 2: T2I_SHRINK(2, 1, 8); break;
-    case 3: T2I_SHRINK(3, 1, 8); break;
-    case 4: T2I_SHRINK(4, 1, 8); break;
-    case 5: T2I_SHRINK(1, 2, 8); break;
-    case 6: T2I_SHRINK(2, 2, 8); break;
-    case 7: T2I_SHRINK(3, 2, 8); break;
-    default: T2I_SHRINK(4, 2, 8); break;
+  const dim3 grid((cap * 4 + 7) / 8 * 8 * p.blocks), threads(64 * t2i::AD_WAVES);
+  switch (nc) {
+    case 1: hipLaunchKernelGGL(t2i::adapter_shrink_kernel<1>, grid, threads, 0, s, p); break;
+    case 2: hipLaunchKernelGGL(t2i::adapter_shrink_kernel<2>, grid, threads, 0, s, p); break;
+    case 3: hipLaunchKernelGGL(t2i::adapter_shrink_kernel<3>, grid, threads, 0, s, p); break;
+    default: hipLaunchKernelGGL(t2i::adapter_shrink_kernel<4>, grid, threads, 0, s, p); break;
   }
-#undef T2I_SHRINK
   if (int rc = t2i_host::hip_status(hipGetLastError(), "adapter shrink launch")) return rc;
   p.blocks = expand_blocks;
   if (paired) hipLaunchKernelGGL(t2i::adapter_expand_kernel<true>, dim3(cap * p.blocks), dim3(256), 0, s, p);
