@@ -147,6 +147,7 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
     if (t < n_tiles) {
       int32_t* w = p.tiles + (size_t)t * PG_TILE;
       w[0] = row0; w[1] = rows; w[2] = ctx; w[3] = s; w[4] = j0; w[5] = first; w[6] = units; w[7] = 0;
+      if (t < PG_THREADS) s_count[t] = first;
       float alone, shared;
       plan_times(pairs, alone, shared);
       atomicAdd(&s_pairs, pairs);
@@ -167,12 +168,13 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
   const float even_time = 9.0f + fmaxf(work / n * 1.3f, work * heads) + (n_tiles + n) * heads * 2.5f + merged * p.Hkv * 1024e-7f;
   if (whole_time <= even_time) {
     // longest first: a tile's place is the number of tiles of more units, by buckets of like ones
+    const int longest = s_units;
+    const auto bucket = [&](int units) { return (int)((float)(longest - units) / (float)longest * (PG_THREADS - 1)); };
     s_count[tid] = 0;
     __syncthreads();
-    const int longest = s_units;
     for (int base = 0; base < n_tiles; base += PG_THREADS) {
       const int t = base + tid;
-      if (t < n_tiles) atomicAdd(&s_count[(int)((long long)(longest - p.tiles[(size_t)t * PG_TILE + 6]) * (PG_THREADS - 1) / longest)], 1);
+      if (t < n_tiles) atomicAdd(&s_count[bucket(p.tiles[(size_t)t * PG_TILE + 6])], 1);
     }
     __syncthreads();
     const int mine = s_count[tid];
@@ -186,29 +188,35 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
       if (t >= n_tiles) continue;
       const int first = p.tiles[(size_t)t * PG_TILE + 5], units = p.tiles[(size_t)t * PG_TILE + 6];
       // (the order within a bucket is of no account: every tile is a workgroup's own)
-      const int at = atomicAdd(&s_count[(int)((long long)(longest - units) * (PG_THREADS - 1) / longest)], 1);
+      const int at = atomicAdd(&s_count[bucket(units)], 1);
       int32_t* w = p.bins + (size_t)at * PG_BIN;
       w[0] = t; w[1] = first; w[2] = first + units; w[3] = 0;
     }
     return;
   }
-  const auto run_start = [&](int i) { return (int)((long long)total * i / n); };
-  const auto run_of = [&](int x) { return (int)(((long long)(x + 1) * n - 1) / total); };
-  for (int base = 0; base < n_tiles; base += PG_THREADS) {
-    const int t = base + tid;
-    if (t >= n_tiles) continue;
-    const int32_t* rec = p.tiles + (size_t)t * PG_TILE;
-    const int first = rec[5], end = first + rec[6];
-    const int run = run_of(first), last = run_of(end - 1);
-    for (int i = run_start(run) < first ? run + 1 : run; i < n && run_start(i) < end; ++i) {
-      int32_t* w = p.bins + (size_t)i * PG_BIN;
-      w[0] = t; w[1] = run_start(i); w[2] = run_start(i + 1); w[3] = 0;
-    }
-    if (run < last) {                                      // cut: joined by the entry of the run that ends it
-      int32_t* w = p.merges + (size_t)last * PG_MERGE;
-      w[0] = rec[0]; w[2] = rec[4]; w[3] = 2 * run + (run_start(run) != first); w[4] = 2 * (run + 1); w[5] = last - run + 1;
-      w[1] = rec[1];
-    }
+  // a thread a share: total i / n without 64-bit division (the remainder and n stay below 2^9)
+  const int each = total / n, left = total - each * n;
+  const auto run_start = [&](int i) { return each * i + left * i / n; };
+  if (tid >= n) return;                                    // (shares are at most RG_SLOTS)
+  const int from = run_start(tid), to = run_start(tid + 1);
+  const auto first_unit = [&](int t) { return n_tiles <= PG_THREADS ? s_count[t] : p.tiles[(size_t)t * PG_TILE + 5]; };
+  int t = 0;
+  for (int hi = n_tiles; hi - t > 1;) {                    // the tile that holds the share's first unit
+    const int mid = (t + hi) / 2;
+    if (first_unit(mid) <= from) t = mid;
+    else hi = mid;
+  }
+  int32_t* const bin = p.bins + (size_t)tid * PG_BIN;
+  bin[0] = t; bin[1] = from; bin[2] = to; bin[3] = 0;
+  const int32_t* const rec = p.tiles + (size_t)t * PG_TILE;
+  const int first = rec[5], end = first + rec[6];
+  if (from > first && to >= end) {                         // the share ends a tile that others began: its merge
+    int run = min((int)((float)first * n / total), tid);   // the share that holds the tile's first unit, about; then exactly
+    while (run_start(run + 1) <= first) ++run;
+    while (run_start(run) > first) --run;
+    int32_t* const w = p.merges + (size_t)tid * PG_MERGE;
+    w[0] = rec[0]; w[2] = rec[4]; w[3] = 2 * run + (run_start(run) != first); w[4] = 2 * (run + 1); w[5] = tid - run + 1;
+    w[1] = rec[1];
   }
 }
 
