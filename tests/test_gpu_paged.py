@@ -134,6 +134,42 @@ def test_values_behind_a_mask_stay_there(gpu):
             assert (mine[:, keep].float() - was[:, keep].float()).abs().max() < 0.05
 
 
+def test_single_tokens_and_drafts_among_long_chunks(gpu):
+    """The form of narrow tiles among wide ones: values, values behind a mask, pages outside the pool."""
+    lens, ctx, hq, hkv = [300, 1, 5, 1, 3, 7], [800, 1099, 500, 0, 31, 2050], 32, 8
+    for page in (16, 128):
+        c = Case(gpu, hq, hkv, page, lens, ctx)
+        clean = ops.paged_attention(c.q, c.plan, c.k, c.v)
+        ref, mag = c.reference()
+        _check(clean, ref, mag)
+        start = torch.tensor([0] + lens).cumsum(0).tolist()
+        for s in (2, 5):                                   # drafts: the last row alone attends the last slot
+            last = lens[s] + ctx[s] - 1
+            was = c.v[int(c.table[s, last // page]), :, last % page, 5].clone()
+            for bad in (NAN, math.inf):
+                c.v[int(c.table[s, last // page]), :, last % page, 5] = bad
+                out = ops.paged_attention(c.q, c.plan, c.k, c.v)
+                row = start[s + 1] - 1
+                at = torch.arange(c.rows, device=gpu)
+                own = (at >= start[s]) & (at <= row)
+                assert torch.equal(out[~own], clean[~own])
+                # Rows that share a tile with such a value are formed again, with fp32 weights on that block (and
+                # two bf16 words relative to another maximum on the others), where the clean call took two words
+                # throughout: each is within the tolerance of the reference (errors of 2^-17 before the output's
+                # rounding), but not the other's bits.
+                _check(out[own & (at != row)], ref[own & (at != row)], mag[own & (at != row)])
+                mine = torch.isfinite(out[row].view(hq, D).float())
+                assert not mine[:, 5].any() and torch.equal(mine.sum(-1), torch.full((hq,), D - 1, device=gpu))
+            c.v[int(c.table[s, last // page]), :, last % page, 5] = was
+        for s in (1, 4):
+            was = int(c.table[s, 0])
+            c.table[s, 0] = c.k.shape[0]
+            out = ops.paged_attention(c.q, c.plan, c.k, c.v)
+            mine = (torch.arange(c.rows, device=gpu) >= start[s]) & (torch.arange(c.rows, device=gpu) < start[s + 1])
+            assert torch.isnan(out[mine]).all() and torch.equal(out[~mine], clean[~mine])
+            c.table[s, 0] = was
+
+
 def test_sequences_without_slots_and_rows_of_nobody(gpu):
     """A context below zero, or rows past the pages: zero rows, nothing written; rows behind the last sequence and
     row_starts that do not ascend: nothing at all."""

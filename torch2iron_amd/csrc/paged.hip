@@ -24,8 +24,9 @@ namespace t2i {
 constexpr int PG_THREADS = 1024;
 constexpr int PG_SEQS = 4096;                // sequences of a plan
 constexpr int PG_TILE = 8;                   // words of a tile: {first row, rows, context, sequence, first pair, first unit, units, 0}
-constexpr int PG_BIN = 4;                    // of a bin: {first tile (-1: none), first unit, unit behind the last, 0}
+constexpr int PG_BIN = 4;                    // of a bin: {first tile (-1: none), first unit, unit behind the last, whether narrow tiles stand among wide ones}
 constexpr int PG_MERGE = 8;                  // of a merge: {first row, rows (0: none), first pair, first part, first second part, parts, 0, 0}
+constexpr int PG_NARROW = 32;                // pairs that one wave multiplies
 constexpr int PG_ROW = 2;                    // of a row: {position (-1: none), sequence}
 
 // A unit is a key block of a tile; all tiles' units stand in a row.
@@ -81,8 +82,8 @@ __device__ __forceinline__ int plan_rows(const PagedPlanParams& p, int s) {
 // Times in us that the choice below goes by: those of the packed plan (ragged_plan.h), in which a key block of a
 // workgroup costs `alone` with a CU to itself and `shared` where two workgroups fill one.
 __device__ __forceinline__ void plan_times(int pairs, float& alone, float& shared) {
-  alone = pairs > 32 ? 1.35f : 1.95f;
-  shared = pairs > 32 ? 1.1f : 1.45f;
+  alone = pairs > PG_NARROW ? 1.35f : 1.95f;
+  shared = pairs > PG_NARROW ? 1.1f : 1.45f;
 }
 
 // Workgroup 0: the tiles and how they are handed out; the others: a thread a row.  As in the packed plan a tile goes
@@ -104,7 +105,7 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
   __shared__ int s_first[PG_SEQS + 1];       // first tile of each sequence
   __shared__ int s_wave[PG_THREADS / 64], s_count[PG_THREADS];
   __shared__ int s_work, s_longest;          // times of all tiles (0.05 us), and of the longest (a float's bits)
-  __shared__ int s_pairs, s_units;           // pairs of all tiles; units of the longest
+  __shared__ int s_pairs, s_units, s_wide;   // pairs of all tiles; units of the longest; is any tile wider than PG_NARROW
 
   // ---- tiles of each sequence ----
   int falls = 0;                             // row_starts that do not ascend make no tiles
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
   }
   if (tid == 0) {
     s_first[p.B] = n_tiles;
-    s_work = s_longest = s_pairs = s_units = 0;
+    s_work = s_longest = s_pairs = s_units = s_wide = 0;
   }
   for (int i = tid; i < p.bins_cap; i += PG_THREADS) p.bins[PG_BIN * i] = -1;
   for (int i = tid; i < p.shares; i += PG_THREADS) p.merges[PG_MERGE * i + 1] = 0;
@@ -152,6 +153,7 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
       plan_times(pairs, alone, shared);
       atomicAdd(&s_pairs, pairs);
       atomicMax(&s_units, units);
+      if (pairs > PG_NARROW) s_wide = 1;
       atomicMax(&s_longest, __float_as_int(units * alone));   // positive floats order as integers
       atomicAdd(&s_work, (int)(units * shared * 20.0f + 0.5f));   // whole numbers: in any order the same sum
     }
@@ -190,7 +192,7 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
       // (the order within a bucket is of no account: every tile is a workgroup's own)
       const int at = atomicAdd(&s_count[bucket(units)], 1);
       int32_t* w = p.bins + (size_t)at * PG_BIN;
-      w[0] = t; w[1] = first; w[2] = first + units; w[3] = 0;
+      w[0] = t; w[1] = first; w[2] = first + units; w[3] = s_wide;
     }
     return;
   }
@@ -307,7 +309,10 @@ __device__ __forceinline__ void poison_item(const RaggedAttnParams& p, const Rag
 }
 
 // A workgroup takes a bin's units for one kv head, tile by tile.  Sequences of one tile (single tokens, drafted
-// tokens, short chunks) multiply by weights of 16 bits: their products hide behind the loads.
+// tokens, short chunks) multiply by weights of 16 bits: their products hide behind the loads.  Single tokens among the
+// tiles of long chunks, one workgroup each, are as slow as their own chain of loads: they take the form with more
+// of them on their way (two chunks of 509 and 701 rows with 24 tokens 146 -> 131 us).  Where they fill the chip themselves
+// that form has more barriers for nothing (32 tokens 56.9 -> 58.7 us, 64 after 4090 slots 170 -> 179).
 __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const RaggedAttnParams p, const PagedTables tab) {
   extern __shared__ __align__(256) uint16_t s_kv[];   // [buffer][K, V][key][dim]
   __shared__ uint32_t s_odd[RG_WAVES];                     // an item's pairs whose sums are not finite
@@ -319,6 +324,7 @@ __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const
   int tile = tab.bins[(size_t)bin * PG_BIN];
   if (tile < 0) return;
   const int at0 = tab.bins[(size_t)bin * PG_BIN + 1], end = tab.bins[(size_t)bin * PG_BIN + 2];
+  const bool among_wide = tab.bins[(size_t)bin * PG_BIN + 3] != 0;
   for (int at = at0; at < end && tile < tab.tiles_cap; ++tile) {
     const int32_t* w = tab.tiles + (size_t)tile * PG_TILE;
     RaggedItem it;
@@ -339,10 +345,14 @@ __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const
     if (it.start < 0) it.kb1 = it.kb0;                     // does not fit its pages: zero rows
     else if (it.kb1 > (it.kend + RG_KEYS - 1) / RG_KEYS) return;
 
-    const auto run = [&](auto fine) __attribute__((always_inline)) {
-      constexpr bool FINE = decltype(fine)::value;
+    const auto run = [&](auto fine, auto narrow) __attribute__((always_inline)) {
+      constexpr bool FINE = decltype(fine)::value, NARROW = decltype(narrow)::value;
+      if (NARROW) {                                          // blocks of 32 keys
+        it.kb0 *= 2;
+        it.kb1 = min(2 * it.kb1, (it.kend + 31) / 32);
+      }
       bool bad = false;
-      const uint32_t odd = attend_item<RG_PAGED, FINE, false>(p, it, h, s_kv, lane, wave, 0, bad);
+      const uint32_t odd = attend_item<RG_PAGED, FINE, false, NARROW>(p, it, h, s_kv, lane, wave, 0, bad);
       if (it.kb0 >= it.kb1) return;
       // (a wave writes these words after a barrier of the item, behind which no wave reads the last item's)
       if (lane == 0) s_odd[wave] = odd, s_bad[wave] = bad;
@@ -356,11 +366,12 @@ __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const
         return;
       }
       if (!__builtin_amdgcn_readfirstlane(any)) return;
-      (void)attend_item<RG_PAGED, FINE, true>(p, it, h, s_kv, lane, wave, odd, bad);
+      (void)attend_item<RG_PAGED, FINE, true, NARROW>(p, it, h, s_kv, lane, wave, odd, bad);
       lds_barrier();
     };
-    if (it.pairs <= RG_ROWS) run(std::true_type{});
-    else run(std::false_type{});
+    if (among_wide && it.pairs <= PG_NARROW) run(std::true_type{}, std::true_type{});
+    else if (it.pairs <= RG_ROWS) run(std::true_type{}, std::false_type{});
+    else run(std::false_type{}, std::false_type{});
   }
 }
 

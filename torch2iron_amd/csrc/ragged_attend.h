@@ -132,6 +132,13 @@ __device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[4
   }
 }
 #undef T2I_KEYS
+// The same for 8 keys.
+__device__ __forceinline__ void lds_load_keys(i32x4 rsrc, const uint32_t (&at)[2], uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\t"
+               "buffer_load_dwordx4 %1, %3, 0 offen nt lds\n\t"
+               "buffer_load_dwordx4 %2, %3, 0 offen offset:1024 nt lds"
+               :: "s"(lds), "v"(at[0]), "v"(at[1]), "s"(rsrc) : "memory", "m0");
+}
 // A buffer over everything from p on (every offset used is inside the cache: checked or clamped).
 __device__ __forceinline__ i32x4 keys_rsrc(const void* p) {
   const uint64_t a = (uint64_t)(uintptr_t)p;
@@ -206,12 +213,17 @@ __device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
 // Pages: a wave's 16 keys of a block lie in one page (pages hold 16 2^n slots), whose id comes by a scalar load a
 // block ahead; the buffer starts at its first slot, so that offsets stay small whatever the pool's size.  An id
 // outside the pool is read as page 0 and raises `bad`.
-template <RaggedForm FORM, bool FINE, bool MASKED>
+// NARROW (pages, up to 32 pairs): one wave multiplies, and what counts is how much is on its way from memory.  Blocks of 32
+// keys (kb0 and kb1 count those) in four buffers: three are loading while one is multiplied, where two buffers of
+// 64 keys leave half of them.
+template <RaggedForm FORM, bool FINE, bool MASKED, bool NARROW = false>
 __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const RaggedItem& it, int h, uint16_t* s_kv, int lane,
                                                 int wave, uint32_t only, bool& bad) {
   constexpr int D = RG_D;
   constexpr bool TREE = FORM == RG_TREE, PAGED = FORM == RG_PAGED;
-  constexpr int WKEYS = RG_KEYS / RG_WAVES;    // keys of a block that a wave loads
+  static_assert(!NARROW || PAGED);
+  constexpr int KEYS = NARROW ? 32 : RG_KEYS, STAGES = NARROW ? 4 : 2;   // keys of a block, blocks in LDS
+  constexpr int WKEYS = KEYS / RG_WAVES;       // keys of a block that a wave loads
   const int c = lane & 31, h2 = lane >> 5;
 
   // ---- K / V staging: a wave's instruction moves 4 keys (1 KB); 4 each of K and V a block ----
@@ -229,7 +241,7 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
   }
   i32x4 krsrc = keys_rsrc(p.kc + cache_base), vrsrc = keys_rsrc(p.vc + cache_base);
   // pages: the wave's first key of a block (at most the last key there is), and its page
-  auto wave_key = [&](int kb) __attribute__((always_inline)) { return min(kb * RG_KEYS + wave * WKEYS, it.kend - 1) & -WKEYS; };
+  auto wave_key = [&](int kb) __attribute__((always_inline)) { return min(kb * KEYS + wave * WKEYS, it.kend - 1) & -WKEYS; };
   auto page_of = [&](int kb) __attribute__((always_inline)) {
     typedef const __attribute__((address_space(4))) int32_t* scalar_ptr;
     return ((scalar_ptr)(uintptr_t)(p.pages + (size_t)it.crow * p.max_pages))[wave_key(kb) >> p.page_shift];
@@ -238,7 +250,7 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
   if (PAGED && it.kb0 < it.kb1) page = page_of(it.kb0);
   // K and V block kb into its buffer
   auto stage = [&](int kb) __attribute__((always_inline)) {
-    const uint32_t lds = lds0 + ((kb - it.kb0) & 1) * (4 * RG_KEYS * D);
+    const uint32_t lds = lds0 + ((kb - it.kb0) & (STAGES - 1)) * (4 * KEYS * D);
     if constexpr (PAGED) {
       const bool in = (uint32_t)page < (uint32_t)p.n_pages;
       bad |= !in;
@@ -247,26 +259,31 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
       vrsrc = keys_rsrc(p.vc + first * D);
       page = page_of(min(kb + 1, it.kb1 - 1));
     }
-    if ((kb + 1) * RG_KEYS <= it.kend) {
-      const uint32_t at = PAGED ? 0u : (uint32_t)kb * (RG_KEYS * D * 2);
-      if (it.pairs <= RG_ROWS) {                            // the sequence's only tile: its keys are read once
+    if ((kb + 1) * KEYS <= it.kend) {
+      const uint32_t at = PAGED ? 0u : (uint32_t)kb * (KEYS * D * 2);
+      if constexpr (NARROW) {
+        lds_load_keys(krsrc, kat, lds);
+        lds_load_keys(vrsrc, vat, lds + 2 * KEYS * D);
+      } else if (it.pairs <= RG_ROWS) {                     // the sequence's only tile: its keys are read once
         lds_load_keys<true>(krsrc, kat, at, lds);
-        lds_load_keys<true>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
+        lds_load_keys<true>(vrsrc, vat, at, lds + 2 * KEYS * D);
       } else {
         lds_load_keys<false>(krsrc, kat, at, lds);
-        lds_load_keys<false>(vrsrc, vat, at, lds + 2 * RG_KEYS * D);
+        lds_load_keys<false>(vrsrc, vat, at, lds + 2 * KEYS * D);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const int at = wave * WKEYS + 4 * i + srow;
-        const uint32_t key = (uint32_t)(PAGED ? min(4 * i + srow, it.kend - 1 - wave_key(kb)) : min(kb * RG_KEYS + at, it.kend - 1)) * (D * 2);
+        const uint32_t key = (uint32_t)(PAGED ? min(4 * i + srow, it.kend - 1 - wave_key(kb)) : min(kb * KEYS + at, it.kend - 1)) * (D * 2);
         lds_load16(krsrc, key + 16 * (place ^ (at & 15)), lds + i * 4 * D * 2);
-        lds_load16(vrsrc, key + 16 * (place ^ (4 * srow)), lds + 2 * RG_KEYS * D + i * 4 * D * 2);
+        lds_load16(vrsrc, key + 16 * (place ^ (4 * srow)), lds + 2 * KEYS * D + i * 4 * D * 2);
       }
     }
   };
-  if (it.kb0 < it.kb1) stage(it.kb0);
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (it.kb0 + s < it.kb1) stage(it.kb0 + s);
 
   // ---- this lane's pair, and its q row as the B operand ----
   const int j = it.j0 + wave * 32 + c;
@@ -288,7 +305,7 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
   const int mask_from = TREE ? it.start : it.start + t_first + 1;   // keys below it are seen by every row
   const int wave_end = TREE ? it.kend : it.start + t_last + 1;      // keys from it on by none
   uint32_t seen_lo = 0, seen_hi = 0;                       // tree: the nodes that the lane's node attends
-  if (TREE && it.kb1 * RG_KEYS > it.start && it.kb0 < it.kb1) {
+  if (TREE && it.kb1 * KEYS > it.start && it.kb0 < it.kb1) {
     const unsigned long long own = 1ull << lane;
     const unsigned long long s = tree_above(tree_parent(p.parents + (size_t)it.row0, p.N, lane)) | own;
     seen_lo = __shfl((uint32_t)s, t, 64);
@@ -307,16 +324,29 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
   const int vi = lane & 15, vrow = 4 * h2 + (vi >> 2);     // key of the 8 that the lane's read names
   const int vcol = 2 * ((lane >> 4) & 1) + ((vi & 3) >> 1);   // its 16-byte chunk within a 32-dim tile
 
+  if constexpr (NARROW) {
+    // The loop counts its own loads, four a block: nothing else may be on its way in it.  (Not known to the compiler,
+    // which so waits for the q rows here and not at their use.)
+    asm volatile("s_waitcnt vmcnt(0)"
+                 : "+v"(qb[0]), "+v"(qb[1]), "+v"(qb[2]), "+v"(qb[3]), "+v"(qb[4]), "+v"(qb[5]), "+v"(qb[6]), "+v"(qb[7]) :: "memory");
+  }
   for (int kb = it.kb0; kb < it.kb1; ++kb) {
-    loads_done_barrier();                                  // this block is here, the buffer of the one before it free
-    if (kb + 1 < it.kb1) stage(kb + 1);
-    if (!wave_on || kb * RG_KEYS >= wave_end) continue;
-    const uint16_t* const bk = s_kv + ((kb - it.kb0) & 1) * (2 * RG_KEYS * D);
-    const uint16_t* const bv = bk + RG_KEYS * D;
+    // this block is here, the buffer of the one before it free
+    if constexpr (NARROW) {
+      if (kb + 2 < it.kb1) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      else if (kb + 1 < it.kb1) asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      else loads_done_barrier();
+    } else {
+      loads_done_barrier();
+    }
+    if (kb + STAGES - 1 < it.kb1) stage(kb + STAGES - 1);
+    if (!wave_on || kb * KEYS >= wave_end) continue;
+    const uint16_t* const bk = s_kv + ((kb - it.kb0) & (STAGES - 1)) * (2 * KEYS * D);
+    const uint16_t* const bv = bk + KEYS * D;
     // ---- S^T = K Q^T ----
-    f32x16 s[2];
+    f32x16 s[KEYS / 32];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < KEYS / 32; ++n) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[n][i] = 0.0f;
 #pragma unroll
@@ -327,30 +357,30 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
       }
     }
     // ---- masks, only on blocks that some row does not see whole ----
-    if (kb * RG_KEYS + RG_KEYS > mask_from) {
+    if (kb * KEYS + KEYS > mask_from) {
       if (TREE) {
-        const int rel = kb * RG_KEYS - it.start;           // node of the block's first key (negative: a context slot)
+        const int rel = kb * KEYS - it.start;           // node of the block's first key (negative: a context slot)
         const unsigned long long w = (unsigned long long)seen_hi << 32 | seen_lo;
         unsigned long long bm = rel >= 64 ? 0ull : rel >= 0 ? w >> rel : (w << -rel) | ((1ull << -rel) - 1);
         bm >>= 4 * h2;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < KEYS / 32; ++n)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (!((uint32_t)(bm >> (32 * n)) & (1u << (8 * (i / 4) + i % 4)))) s[n][i] = -INFINITY;
       } else {
-        const int rel = qpos - kb * RG_KEYS - 4 * h2;
+        const int rel = qpos - kb * KEYS - 4 * h2;
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < KEYS / 32; ++n)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             if (32 * n + 8 * (i / 4) + i % 4 > rel) s[n][i] = -INFINITY;
       }
     }
     // ---- online softmax (log2 domain) ----
-    float mx = fmaxf(s[0][0], s[1][0]);
+    float mx = fmaxf(s[0][0], s[KEYS / 32 - 1][0]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[1][i]));
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, fmaxf(s[0][i], s[KEYS / 32 - 1][i]));
     mx = pair_max(mx) * p.scale_log2;
     if (__any(mx > m + (MASKED ? 0.0f : 8.0f))) {          // MASKED: no weight above 1, sums of huge values fit
       const float mn = fmaxf(m, mx);
@@ -365,10 +395,10 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
     }
     // ---- MASKED: where V holds an infinity or a NaN, key by key for the rows that attend it ----
     if constexpr (MASKED) {
-      if (kb * RG_KEYS + RG_KEYS > mask_from) {
+      if (kb * KEYS + KEYS > mask_from) {
         bool odd = false;
 #pragma unroll 4
-        for (int i = 0; i < RG_KEYS / 4; ++i) {
+        for (int i = 0; i < KEYS / 4; ++i) {
           const u32x4 x = *reinterpret_cast<const u32x4*>(bv + 4 * i * D + 8 * lane);
 #pragma unroll
           for (int e = 0; e < 4; ++e) odd |= finite_or_zero(x[e]) != x[e];
@@ -376,7 +406,7 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
         if (__any(odd)) {
           const uint32_t unseen = __float_as_uint(-1.0f);  // no weight
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < KEYS / 32; ++n)
 #pragma unroll 1
             for (int i = 0; i < 16; ++i) {
               const float x = s[n][i], e = exp2_fast(fmaf(x, p.scale_log2, -mref));
@@ -407,9 +437,9 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
         }
       }
     }
-    uint32_t pw[2][8], pr[2][8];                           // bf16 weights, two keys a word; what their rounding left
+    uint32_t pw[KEYS / 32][8], pr[KEYS / 32][8];                           // bf16 weights, two keys a word; what their rounding left
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < KEYS / 32; ++n)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
         const float e0 = exp2_fast(fmaf(s[n][i], p.scale_log2, -mref)), e1 = exp2_fast(fmaf(s[n][i + 1], p.scale_log2, -mref));
@@ -424,7 +454,7 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
       }
     // ---- O^T += V^T P^T ----
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < KEYS / 16; ++u) {
       const uint32_t* const w = pw[u / 2] + 4 * (u % 2);
       const uint32_t* const r = pr[u / 2] + 4 * (u % 2);
       bf16x8 va[4];
