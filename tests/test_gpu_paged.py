@@ -201,6 +201,20 @@ def test_sequences_without_slots_and_rows_of_nobody(gpu):
         assert (ops.paged_attention(c.q, c.plan, c.k, c.v, out=out) == 3.0).all()
 
 
+@pytest.mark.parametrize("starts", [[0, 3, 2, 45, 50], [-1, 3, 43, 45, 50], [0, 3, 43, 45, 54], [0, 50, 3, 45, 50]])
+def test_row_starts_that_do_not_ascend_write_nothing(gpu, starts):
+    c = Case(gpu, 8, 4, 16, [3, 40, 2, 5], [20, 100, 7, 30], behind=3)
+    c.row_starts.copy_(torch.tensor(starts, dtype=torch.int32))
+    c.plan.refresh()
+    qkv = _normal(_gen(gpu, 1), c.rows, (8 + 2 * 4) * D)
+    norm, rope = torch.ones(D, dtype=BF16, device=gpu), gm.rope_table(D, c.table.shape[1] * 16, 1e6, gpu)
+    k, v = c.k.clone(), c.v.clone()
+    q = torch.full((c.rows, 8, D), 3.0, dtype=BF16, device=gpu)
+    ops.paged_qk_rope_kv(qkv, c.plan, norm, norm, 1e-6, rope, k, v, q_out=q)
+    assert (q == 3.0).all()
+    assert torch.equal(k.nan_to_num(9.0), c.k.nan_to_num(9.0)) and torch.equal(v.nan_to_num(9.0), c.v.nan_to_num(9.0))
+
+
 def test_rows_that_start_behind_the_first(gpu):
     """Rows before the first sequence's are no sequence's."""
     c = Case(gpu, 8, 4, 16, [3, 5], [20, 33], behind=4)

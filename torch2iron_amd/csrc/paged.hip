@@ -92,12 +92,15 @@ __device__ __forceinline__ void plan_times(int pairs, float& alone, float& share
 // serve every later one.
 __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanParams p) {
   const int tid = threadIdx.x;
+  int falls = 0;                             // row_starts that do not ascend: no row is anyone's
+  for (int s = tid; s < p.B; s += PG_THREADS) falls |= p.row_starts[s] < 0 || p.row_starts[s] > p.row_starts[s + 1] || p.row_starts[s + 1] > p.rows;
+  const bool ascends = !__syncthreads_or(falls);
   if (blockIdx.x > 0) {
     const int row = (blockIdx.x - 1) * PG_THREADS + tid;
     if (row >= p.rows) return;
     const int s = plan_find(p.row_starts, p.B, row);
     const int n = plan_rows(p, s), r = row - p.row_starts[s], ctx = p.ctx[s];
-    const bool ok = r >= 0 && r < n && ctx >= 0 && ctx <= p.cap - n;
+    const bool ok = ascends && r >= 0 && r < n && ctx >= 0 && ctx <= p.cap - n;
     p.row[PG_ROW * row] = ok ? ctx + r : -1;
     p.row[PG_ROW * row + 1] = s;
     return;
@@ -108,9 +111,6 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
   __shared__ int s_pairs, s_units, s_wide;   // pairs of all tiles; units of the longest; is any tile wider than PG_NARROW
 
   // ---- tiles of each sequence ----
-  int falls = 0;                             // row_starts that do not ascend make no tiles
-  for (int s = tid; s < p.B; s += PG_THREADS) falls |= p.row_starts[s] < 0 || p.row_starts[s] > p.row_starts[s + 1] || p.row_starts[s + 1] > p.rows;
-  const bool ascends = !__syncthreads_or(falls);
   int n_tiles = 0;
   for (int base = 0; base < p.B; base += PG_THREADS) {
     const int s = base + tid;
