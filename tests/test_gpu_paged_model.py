@@ -249,6 +249,28 @@ def test_a_sequence_without_room(gpu, setup):
     assert torch.equal(res[0].logits[0], res[1].logits[0]) and torch.isnan(res[1].logits[1]).any()
 
 
+def test_a_sequence_past_its_part_of_the_table(gpu, setup):
+    """Its tokens have no slots at all: NaN logits and the token -1, and the others do not notice."""
+    cfg, _, _, _ = setup
+    m = _model(setup, gpu)
+    g = torch.Generator().manual_seed(9)
+    tokens = torch.randint(0, cfg.vocab, (60,), generator=g, dtype=torch.int32).to(gpu)
+    res = []
+    for first in (3, 59):
+        cache = gm.PagedCache(cfg, 2, 8, 4, gpu, page_slots=16)
+        for s in range(2):
+            cache.reserve(s, 64)
+        m.paged_step(cache, gm.PagedBatch([first, 1], device=gpu), tokens[59 - first:])
+        k = cache.k.clone()
+        u = torch.zeros(6, device=gpu)
+        res.append(m.paged_step(cache, gm.PagedBatch([6, 1], [4, 0], device=gpu), tokens[:7], uniforms=u))
+    assert (res[0].next_tokens >= 0).all() and torch.isfinite(res[0].logits).all()
+    assert res[1].next_tokens[0] == -1 and res[1].counts[0] == 0 and torch.isnan(res[1].logits[:5]).all()
+    held = cache.table[0].long()
+    assert torch.equal(cache.k[:, held], k[:, held])
+    assert res[1].next_tokens[1] == res[0].next_tokens[1] and torch.equal(res[1].logits[5], res[0].logits[5])
+
+
 def test_refusals(gpu, setup):
     cfg, _, _, pools = setup
     m = _model(setup, gpu)

@@ -360,7 +360,9 @@ class PagedBatch:
         self.n_seqs, self.rows = len(rows), ends[-1]
         self.row_starts = ints(ends)
         self.row_seq = ints([s for s, r in enumerate(rows) for _ in range(r)]).long()
+        self.seq_rows = ints(rows)
         self.head_rows = ints([i for h in heads for i in h])
+        self.head_seq = self.row_seq[self.head_rows.long()]
         self.head_starts = ints(np.cumsum([0] + [d + 1 if r else 0 for r, d in zip(rows, drafts)]).tolist())
         self.fed = ints([r - d for r, d in zip(rows, drafts)])
         self.device = self.row_starts.device
@@ -967,6 +969,7 @@ class Qwen3Model:
                 raise ValueError(f"the pools must be of one size, and adapter_ids hold {batch.n_seqs} values")
             plan = ops.AdapterPlan(adapter_ids[batch.row_seq], pools.pop()) if pools else None
         pages = ops.PagedPlan(batch.rows, batch.row_starts, cache.lens, cache.table, c.n_heads, c.n_kv_heads, cache.page_slots)
+        past = cache.lens > cache.max_pages * cache.page_slots - batch.seq_rows   # their rows attend nothing
 
         def prep(i, qkv):
             layer = self.layers[i]
@@ -981,6 +984,7 @@ class Qwen3Model:
         keys = torch.empty(n_head, dtype=torch.int64, device=self.device)
         head = torch.empty(n_head, c.hidden, dtype=BF16, device=self.device)
         xn = ops.rmsnorm(x, self.norm, c.eps, out=head, tokens=batch.head_rows, x_out=torch.empty_like(head), argmax_keys=keys)
+        xn.masked_fill_(past[batch.head_seq].unsqueeze(1), math.nan)
         logits = torch.empty(n_head, c.vocab, dtype=torch.float32, device=self.device)
         ops.lm_head_argmax(xn, self.lm_head, keys, logits=logits)
         counts, nxt, lp = ops.verify_drafts(logits, batch.head_starts, tokens[batch.head_rows.long()], uniforms,
