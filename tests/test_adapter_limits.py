@@ -47,3 +47,11 @@ def test_pointers_and_values():
     assert _plan(ids=0x10002) == E.T2I_ERR_ALIGN and _plan(plan=0x10004) == E.T2I_ERR_ALIGN
     assert _plan(m=0) == E.T2I_ERR_SHAPE and _plan(n=0) == E.T2I_ERR_SHAPE and _plan(n=512) == E.T2I_ERR_SHAPE
     assert lib.t2i_adapter_plan_words(0, 3) == 0 and lib.t2i_adapter_plan_words(9, 512) == 0
+
+
+@pytest.mark.parametrize("swiglu", [0, 1])
+def test_out_over_a_part_of_y(swiglu):
+    """Other rows than a workgroup's own would be written before they are read."""
+    size = 9 * 128 * 2
+    for y, out in ((FAKE, FAKE + 16), (FAKE, FAKE + size - 16), (FAKE + 16, FAKE), (FAKE + (size >> swiglu) - 16, FAKE)):
+        assert _add(y=y, out=out, swiglu=swiglu, paired=swiglu, parts=1 + swiglu) == _lib.T2I_ERR_VALUE

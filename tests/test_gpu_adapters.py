@@ -261,3 +261,16 @@ def test_refusals(gpu):
     pair = ops.Adapters(a, b, scales, paired=True)
     with pytest.raises(ValueError, match="must not be y|out must be"):
         ops.adapter_add(y, x, pair, plan, out=y, swiglu=True)
+
+
+def test_out_may_be_x(gpu):
+    """x is done with when the first result is written."""
+    g = torch.Generator(device=gpu).manual_seed(5)
+    rnd = lambda *s: torch.randn(*s, device=gpu, generator=g).to(torch.bfloat16)  # noqa: E731
+    for m in (3, 700):
+        x, y = rnd(m, 256), rnd(m, 256)
+        pool = ops.Adapters(rnd(3, 8, 256), rnd(3, 256, 8))
+        plan = ops.AdapterPlan((torch.arange(m, device=gpu) % 4).to(torch.int32), 3)
+        want = ops.adapter_add(y, x, pool, plan, out=torch.empty_like(y))
+        got = ops.adapter_add(y, x, pool, plan, out=x)
+        assert got is x and torch.equal(got, want)

@@ -388,6 +388,10 @@ extern "C" int t2i_adapter_add(const uint16_t* y, const uint16_t* x, int32_t M, 
   const int fragments = parts * p.R / 16, expand_blocks = (N + 127) / 128;
   if (((long long)cap * 4 + 8) * fragments > 0xFFFFFFFFLL / 1024 || (long long)cap * expand_blocks > 0xFFFFFFFFLL / 256)
     return fail(T2I_ERR_SHAPE, "M=%d N=%d rank=%d exceed the grid", M, N, rank);
+  const uintptr_t y0 = (uintptr_t)y, out0 = (uintptr_t)out;
+  const uintptr_t y_bytes = 2 * (uintptr_t)M * N, out_bytes = swiglu ? y_bytes / 2 : y_bytes;
+  if (out0 != y0 && out0 < y0 + y_bytes && y0 < out0 + out_bytes)
+    return fail(T2I_ERR_VALUE, "out must be y itself or lie beside it");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   // as many fragments of ranks a workgroup (up to four) as leave one for every CU (1, 2, 3, 4 of them, us: 331 rows
   // of 8 16.9, 17.0, 17.8, 18.6; 16 of 3 6.0, 6.4, 6.8, 6.8; 4001 of 2 22.9, 21.8; 8192 of 3 54.4, 56.0, 54.0)

@@ -964,6 +964,8 @@ class Qwen3Model:
                 for name, pool, shape in zip(LayerAdapters._fields, LayerAdapters(*a), want):
                     if pool is not None and (pool.K, pool.N, pool.paired) != shape:
                         raise ValueError(f"adapters of {name} must be [{shape[1]}, {shape[0]}]{', paired' if shape[2] else ''}")
+                    if pool is not None and pool.device != tokens.device:
+                        raise ValueError(f"adapters of {name} are on {pool.device}, not on {tokens.device}")
             pools = {p.n for a in adapters for p in a if p is not None}
             if len(pools) > 1 or adapter_ids.numel() != batch.n_seqs:
                 raise ValueError(f"the pools must be of one size, and adapter_ids hold {batch.n_seqs} values")

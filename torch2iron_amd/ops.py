@@ -1699,7 +1699,7 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Adap
     place without ``out``.  ``swiglu`` (paired columns): bf16 ``[M, N / 2]`` of silu(gate) * up, a tensor of its own.
 
     fp32 sums, one rounding of the result: rows without an adapter keep their bits (with ``swiglu`` they are ``gate_up``'s
-    up to its two more roundings)."""
+    up to its two more roundings).  ``out`` may be ``x``, but no part of ``y`` other than ``y`` itself."""
     if not isinstance(adapters, Adapters) or not isinstance(plan, AdapterPlan):
         raise ValueError("adapters must be an Adapters and plan an AdapterPlan")
     _check_dev("y", y, BF16)
