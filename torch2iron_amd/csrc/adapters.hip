@@ -270,18 +270,31 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterParams
       for (int s = 0; s < AD_PARTS - 1; ++s) slice += s < p.parts - 1 && n0 >= p.ends[s];
     const uint16_t* const h = p.h + (((size_t)tile * (AD_TILE / 16) + sub) * groups + slice * steps) * 512 + 8 * lane;
     const uint16_t* const b = p.b + ((size_t)t.adapter * ((p.N + 127) / 128) + block) * p.R * 128 + 8 * (lane & 31);
-#pragma unroll 2
-    for (int s = 0; s < steps; ++s) {
-      u32x4 hv[2], bv[8];
+    // the operands of a step come while the one before it is multiplied
+    u32x4 hv[2], bv[8];
+    const auto fetch_h = [&](int s) __attribute__((always_inline)) {
       hv[0] = *reinterpret_cast<const u32x4*>(h + 512 * s);
       if (PAIRED) hv[1] = *reinterpret_cast<const u32x4*>(h + 512 * (s + steps));
+    };
+    const auto fetch_b = [&](int s, int k) __attribute__((always_inline)) { bv[k] = *reinterpret_cast<const u32x4*>(b + (8 * s + k) * 256); };
+    const auto multiply = [&](int k, u32x4 x) __attribute__((always_inline)) {
+      acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, bv[k]), acc[k], 0, 0, 0);
+    };
+    fetch_h(0);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) bv[k] = *reinterpret_cast<const u32x4*>(b + (8 * s + k) * 256);
+    for (int k = 0; k < 8; ++k) fetch_b(0, k);
+#pragma unroll 1
+    for (int s = 1; s < steps; ++s) {
+      const u32x4 x[2] = {hv[0], hv[1]};
+      fetch_h(s);
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, hv[PAIRED ? k & 1 : 0]),
-                                                         __builtin_bit_cast(bf16x8, bv[k]), acc[k], 0, 0, 0);
+      for (int k = 0; k < 8; ++k) {
+        multiply(k, x[PAIRED ? k & 1 : 0]);
+        fetch_b(s, k);
+      }
     }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) multiply(k, hv[PAIRED ? k & 1 : 0]);
   }
   if (col >= p.N) return;
 #pragma unroll
