@@ -35,9 +35,9 @@ struct PagedPlanParams {
   const int32_t* ctx;                        // [B]
   int32_t* tiles;                            // [tiles_cap][PG_TILE]
   int32_t* bins;                             // [bins_cap][PG_BIN]
-  int32_t* merges;                           // [shares][PG_MERGE]
+  int32_t* merges;                           // [merges_cap][PG_MERGE]: a cut tile's, at its number or at its last share's
   int32_t* row;                              // [rows][PG_ROW]
-  int rows, B, G, Hkv, cap, tiles_cap, bins_cap, shares;
+  int rows, B, G, Hkv, cap, tiles_cap, bins_cap, shares, merges_cap;
 };
 
 // Sums of the values of the threads before this one, and of all (LDS: one word a wave).
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
     s_work = s_longest = s_pairs = s_units = s_wide = 0;
   }
   for (int i = tid; i < p.bins_cap; i += PG_THREADS) p.bins[PG_BIN * i] = -1;
-  for (int i = tid; i < p.shares; i += PG_THREADS) p.merges[PG_MERGE * i + 1] = 0;
+  for (int i = tid; i < p.merges_cap; i += PG_THREADS) p.merges[PG_MERGE * i + 1] = 0;
   __syncthreads();
 
   // ---- the tiles, and their units in a row ----
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanP
     int run = min((int)((float)first * n / total), tid);   // the share that holds the tile's first unit, about; then exactly
     while (run_start(run + 1) <= first) ++run;
     while (run_start(run) > first) --run;
-    int32_t* const w = p.merges + (size_t)tid * PG_MERGE;
+    int32_t* const w = p.merges + (size_t)(p.merges_cap < p.shares ? t : tid) * PG_MERGE;
     w[0] = rec[0]; w[2] = rec[4]; w[3] = 2 * run + (run_start(run) != first); w[4] = 2 * (run + 1); w[5] = tid - run + 1;
     w[1] = rec[1];
   }
@@ -408,7 +408,7 @@ constexpr long long INT_MOST = 0x7FFFFFFF;
 
 // What a plan holds: words of each of its tables.
 struct PlanSizes {
-  int tiles, bins, shares;
+  int tiles, bins, shares, merges;
   int64_t words;
 };
 PlanSizes plan_sizes(int32_t rows, int32_t B, int32_t G, int32_t Hkv) {
@@ -416,7 +416,8 @@ PlanSizes plan_sizes(int32_t rows, int32_t B, int32_t G, int32_t Hkv) {
   z.tiles = (int)((long long)rows * G / t2i_host::RG_ROWS + B);
   z.shares = std::max(1, t2i_host::RG_SLOTS / Hkv);
   z.bins = std::max(z.tiles, z.shares);
-  z.words = (int64_t)z.tiles * t2i::PG_TILE + (int64_t)z.bins * t2i::PG_BIN + (int64_t)z.shares * t2i::PG_MERGE + (int64_t)rows * t2i::PG_ROW;
+  z.merges = std::min(z.tiles, z.shares);
+  z.words = (int64_t)z.tiles * t2i::PG_TILE + (int64_t)z.bins * t2i::PG_BIN + (int64_t)z.merges * t2i::PG_MERGE + (int64_t)rows * t2i::PG_ROW;
   return z;
 }
 
@@ -458,7 +459,7 @@ struct PlanTables {
     tiles = const_cast<int32_t*>(plan);
     bins = tiles + (size_t)z.tiles * t2i::PG_TILE;
     merges = bins + (size_t)z.bins * t2i::PG_BIN;
-    row = merges + (size_t)z.shares * t2i::PG_MERGE;
+    row = merges + (size_t)z.merges * t2i::PG_MERGE;
   }
 };
 
@@ -484,7 +485,7 @@ extern "C" int t2i_paged_plan(const int32_t* row_starts, const int32_t* context_
   t2i::PagedPlanParams p{};
   p.row_starts = row_starts; p.ctx = context_lens; p.tiles = t.tiles; p.bins = t.bins; p.merges = t.merges; p.row = t.row;
   p.rows = rows; p.B = n_seqs; p.G = Hq / Hkv; p.Hkv = Hkv; p.cap = max_pages * page_slots;
-  p.tiles_cap = z.tiles; p.bins_cap = z.bins; p.shares = z.shares;
+  p.tiles_cap = z.tiles; p.bins_cap = z.bins; p.shares = z.shares; p.merges_cap = z.merges;
   const int groups = 1 + (rows + t2i::PG_THREADS - 1) / t2i::PG_THREADS;
   hipLaunchKernelGGL(t2i::paged_plan_kernel, dim3(groups), dim3(t2i::PG_THREADS), 0, reinterpret_cast<hipStream_t>(stream), p);
   return t2i_host::hip_status(hipGetLastError(), "paged plan launch");
@@ -546,6 +547,6 @@ extern "C" int t2i_paged_attention(const uint16_t* q, int32_t rows, const int32_
   constexpr int LDS_BYTES = 2 * 2 * t2i::RG_KEYS * t2i::RG_D * 2;   // two buffers of K and V
   hipLaunchKernelGGL(t2i::paged_attention_kernel, dim3(z.bins * Hkv), dim3(64 * t2i::RG_WAVES), LDS_BYTES, s, p, tab);
   if (int rc = t2i_host::hip_status(hipGetLastError(), "paged attention launch")) return rc;
-  hipLaunchKernelGGL(t2i::paged_merge_kernel, dim3(z.shares * Hkv * (p.part_rows / t2i::MERGE_PAIRS)), dim3(256), 0, s, p, tab);
+  hipLaunchKernelGGL(t2i::paged_merge_kernel, dim3(z.merges * Hkv * (p.part_rows / t2i::MERGE_PAIRS)), dim3(256), 0, s, p, tab);
   return t2i_host::hip_status(hipGetLastError(), "paged attention merge launch");
 }
