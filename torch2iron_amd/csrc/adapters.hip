@@ -269,32 +269,42 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterParams
     if (!PAIRED)
       for (int s = 0; s < AD_PARTS - 1; ++s) slice += s < p.parts - 1 && n0 >= p.ends[s];
     const uint16_t* const h = p.h + (((size_t)tile * (AD_TILE / 16) + sub) * groups + slice * steps) * 512 + 8 * lane;
-    const uint16_t* const b = p.b + ((size_t)t.adapter * ((p.N + 127) / 128) + block) * p.R * 128 + 8 * (lane & 31);
-    // the operands of a step come while the one before it is multiplied
-    u32x4 hv[2], bv[8];
+    const uint16_t* const b = p.b + ((size_t)t.adapter * ((p.N + 127) / 128) + block) * p.R * 128 + 8 * lane;
+    // The operands of a step come while the one before it is multiplied.  Both halves of a wave take the same of B (for the
+    // two words of h): a load brings two products' to the halves, and a swap gives either to both.
+    u32x4 hv[2], bv[4];
     const auto fetch_h = [&](int s) __attribute__((always_inline)) {
       hv[0] = *reinterpret_cast<const u32x4*>(h + 512 * s);
       if (PAIRED) hv[1] = *reinterpret_cast<const u32x4*>(h + 512 * (s + steps));
     };
-    const auto fetch_b = [&](int s, int k) __attribute__((always_inline)) { bv[k] = *reinterpret_cast<const u32x4*>(b + (8 * s + k) * 256); };
-    const auto multiply = [&](int k, u32x4 x) __attribute__((always_inline)) {
-      acc[k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, bv[k]), acc[k], 0, 0, 0);
+    const auto fetch_b = [&](int s, int k) __attribute__((always_inline)) { bv[k] = *reinterpret_cast<const u32x4*>(b + (4 * s + k) * 512); };
+    const auto multiply = [&](int k, u32x4 w, u32x4 x0, u32x4 x1) __attribute__((always_inline)) {
+      u32x4 w0, w1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const auto both = __builtin_amdgcn_permlane32_swap(w[e], w[e], false, false);
+        w0[e] = both[0];
+        w1[e] = both[1];
+      }
+      acc[2 * k] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x0), __builtin_bit_cast(bf16x8, w0), acc[2 * k], 0, 0, 0);
+      acc[2 * k + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x1), __builtin_bit_cast(bf16x8, w1), acc[2 * k + 1], 0, 0, 0);
     };
     fetch_h(0);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) fetch_b(0, k);
+    for (int k = 0; k < 4; ++k) fetch_b(0, k);
 #pragma unroll 1
     for (int s = 1; s < steps; ++s) {
-      const u32x4 x[2] = {hv[0], hv[1]};
+      const u32x4 x0 = hv[0], x1 = hv[PAIRED];
       fetch_h(s);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        multiply(k, x[PAIRED ? k & 1 : 0]);
+      for (int k = 0; k < 4; ++k) {
+        const u32x4 w = bv[k];
         fetch_b(s, k);
+        multiply(k, w, x0, x1);
       }
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) multiply(k, hv[PAIRED ? k & 1 : 0]);
+    for (int k = 0; k < 4; ++k) multiply(k, bv[k], hv[0], hv[PAIRED]);
   }
   if (col >= p.N) return;
 #pragma unroll
