@@ -97,6 +97,7 @@ CASES = [
     (16, 8, 16, [5] * 16, [901 + 200 * i for i in range(16)]),
     (32, 8, 64, [1] * 70, [37 * i for i in range(70)]),
     (150, 1, 16, [2, 1], [30, 200]),                           # more q heads a kv head than a tile has pairs
+    (32, 8, 64, [1, 40, 2] + [1] * 70, [9000, 4000, 100] + [11 * i for i in range(70)]),   # many tiles, the longest cut
 ]
 IDS = [f"{c[0]}-{c[1]}-p{c[2]}-" + "_".join(map(str, c[3][:6])) for c in CASES]
 

@@ -375,22 +375,24 @@ __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const
   }
 }
 
-// The parts of a cut tile joined, as the contiguous caches' merge: eight pairs a workgroup.
+// The parts of a cut tile joined, as the contiguous caches' merge; LANES lanes a pair.
+template <int LANES>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const RaggedAttnParams p, const PagedTables tab) {
-  const int lane = threadIdx.x & 31;
+  constexpr int JOINED = 256 / LANES;        // pairs of a workgroup
+  const int lane = threadIdx.x & (LANES - 1);
   const int h = blockIdx.x % p.Hkv;
-  const int groups = p.part_rows / MERGE_PAIRS;
+  const int groups = p.part_rows / JOINED;
   const int group = blockIdx.x / p.Hkv % groups;
   const int32_t* w = tab.merges + (size_t)(blockIdx.x / p.Hkv / groups) * PG_MERGE;
   const int row0 = w[0], rows = w[1], j0 = w[2], first = w[3], second = w[4], parts = w[5];
   if (rows < 1 || row0 < 0 || row0 + (long long)rows > p.rows || j0 < 0 || first < 0 || parts < 2 || second < 0 ||
       first >= p.n_parts || second + 2 * (parts - 2) >= p.n_parts)
     return;
-  const int at = group * MERGE_PAIRS + (threadIdx.x >> 5);
+  const int at = group * JOINED + (int)threadIdx.x / LANES;
   const int j = j0 + at;
-  if (j >= (long long)rows * p.G) return;      // 32 lanes together
+  if (j >= (long long)rows * p.G) return;      // a pair's lanes together
   const int t = j / p.G;
-  join_parts(p, h, at, first, second, 2, parts, (size_t)row0 + t, h * p.G + (j - t * p.G), lane);
+  join_parts<LANES>(p, h, at, first, second, 2, parts, (size_t)row0 + t, h * p.G + (j - t * p.G), lane);
 }
 
 }  // namespace t2i
@@ -547,6 +549,14 @@ extern "C" int t2i_paged_attention(const uint16_t* q, int32_t rows, const int32_
   constexpr int LDS_BYTES = 2 * 2 * t2i::RG_KEYS * t2i::RG_D * 2;   // two buffers of K and V
   hipLaunchKernelGGL(t2i::paged_attention_kernel, dim3(z.bins * Hkv), dim3(64 * t2i::RG_WAVES), LDS_BYTES, s, p, tab);
   if (int rc = t2i_host::hip_status(hipGetLastError(), "paged attention launch")) return rc;
-  hipLaunchKernelGGL(t2i::paged_merge_kernel, dim3(z.merges * Hkv * (p.part_rows / t2i::MERGE_PAIRS)), dim3(256), 0, s, p, tab);
+  // Tiles enough for all shares are mostly handed out whole, and then what this launch takes is its waves that find
+  // nothing to do: a quarter of them with 8 lanes a pair (16 prompts of 37 to 1021 rows 36.9 -> 34.5 us).  Few tiles are cut into many
+  // parts, which more lanes join sooner (a single token 10.6 us, with 8 lanes 11.6; 2 x 9 drafts 45.6, 48.8).
+  const auto merge = [&](auto lanes) {
+    constexpr int LANES = decltype(lanes)::value;
+    hipLaunchKernelGGL(t2i::paged_merge_kernel<LANES>, dim3(z.merges * Hkv * (p.part_rows * LANES / 256)), dim3(256), 0, s, p, tab);
+  };
+  if (z.tiles >= z.shares) merge(std::integral_constant<int, 8>{});
+  else merge(std::integral_constant<int, 32>{});
   return t2i_host::hip_status(hipGetLastError(), "paged attention merge launch");
 }

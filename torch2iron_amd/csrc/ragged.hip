@@ -286,7 +286,7 @@ __global__ __launch_bounds__(256) void ragged_merge_kernel(const RaggedAttnParam
   if (j >= (long long)rows * p.G) return;      // 32 lanes together
   const int t = j / p.G;
   const int head = h * p.G + (j - t * p.G);
-  join_parts(p, h, at, first, second, step, parts, (size_t)row0 + t, head, lane);
+  join_parts<32>(p, h, at, first, second, step, parts, (size_t)row0 + t, head, lane);
 }
 
 // ============================================================================

@@ -536,32 +536,37 @@ __device__ __forceinline__ uint32_t attend_item(const RaggedAttnParams& p, const
   return only;
 }
 
-// The parts of a tile joined, for one (row, q head) pair: 32 lanes, four dims each; parts in their order
+// The parts of a tile joined, for one (row, q head) pair: LANES lanes, 128 / LANES dims each; parts in their order
 // (first, then second, second + step, ...), MERGE_AHEAD of them in flight, with a running maximum.
 constexpr int MERGE_AHEAD = 4;
 constexpr int MERGE_PAIRS = t2i_host::RG_MERGE;
 
+template <int LANES>
 __device__ __forceinline__ void join_parts(const RaggedAttnParams& p, int h, int at, int first, int second, int step, int parts,
                                            size_t qrow, int head, int lane) {
-  constexpr int D = RG_D;
+  constexpr int D = RG_D, PER = D / 4 / LANES;             // dims 4 lane + 4 LANES i
   float M = -INFINITY, l = 0.0f;
-  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 o[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < parts; s0 += MERGE_AHEAD) {
     float2 ml[MERGE_AHEAD];
-    f32x4 v[MERGE_AHEAD];
+    f32x4 v[MERGE_AHEAD][PER];
 #pragma unroll
     for (int u = 0; u < MERGE_AHEAD; ++u) {
       const int s = min(s0 + u, parts - 1), part = s == 0 ? first : second + (s - 1) * step;
       const size_t st = ((size_t)part * p.Hkv + h) * p.part_rows + at;
       ml[u] = p.part_ml[st];
-      v[u] = *reinterpret_cast<const f32x4*>(p.part_o + st * D + 4 * lane);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[u][i] = *reinterpret_cast<const f32x4*>(p.part_o + st * D + 4 * lane + 4 * LANES * i);
     }
     float mn = M;
 #pragma unroll
     for (int u = 0; u < MERGE_AHEAD; ++u) mn = fmaxf(mn, ml[u].x);
     const float f = state_weight(M, mn);
     l *= f;
-    o *= f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) o[i] *= f;
     M = mn;
 #pragma unroll
     for (int u = 0; u < MERGE_AHEAD; ++u) {
@@ -569,15 +574,27 @@ __device__ __forceinline__ void join_parts(const RaggedAttnParams& p, int h, int
       const float g = exp2_fast(ml[u].x - M);
       l += some ? g * ml[u].y : 0.0f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] += some ? g * v[u][e] : 0.0f;
+      for (int i = 0; i < PER; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] += some ? g * v[u][i][e] : 0.0f;
     }
   }
   const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-  const u32x2 w = u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
-  *reinterpret_cast<u32x2*>(p.out + (qrow * p.Hq + head) * D + 4 * lane) = w;
+  float hs = 0.0f;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const u32x2 w = u32x2{pack_bf16x2(o[i][0] * inv, o[i][1] * inv), pack_bf16x2(o[i][2] * inv, o[i][3] * inv)};
+    *reinterpret_cast<u32x2*>(p.out + (qrow * p.Hq + head) * D + 4 * lane + 4 * LANES * i) = w;
+    hs += (bf16_lo(w.x) + bf16_hi(w.x)) + (bf16_lo(w.y) + bf16_hi(w.y));
+  }
   if (p.out_sums) {
-    float hs = row_sum16((bf16_lo(w.x) + bf16_hi(w.x)) + (bf16_lo(w.y) + bf16_hi(w.y)));
-    hs += __shfl_xor(hs, 16, 32);
+    if constexpr (LANES == 32) {
+      hs = row_sum16(hs);
+      hs += __shfl_xor(hs, 16, 32);
+    } else {
+#pragma unroll
+      for (int s = LANES / 2; s; s >>= 1) hs += __shfl_xor(hs, s, LANES);
+    }
     if (lane == 0) p.out_sums[(size_t)head * p.rows + qrow] = hs;
   }
 }
