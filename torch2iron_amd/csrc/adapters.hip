@@ -44,8 +44,9 @@ __device__ __forceinline__ int adapter_scan(int v, int* s_wave) {
   return before + x - v;
 }
 
-// One workgroup: a counting sort (by adapter, those rows last that have none) that keeps the rows of an adapter in their order.  A wave takes its share of
-// the rows 64 at a time, adapter by adapter of those there are among them.
+// One workgroup: a counting sort (by adapter, those rows last that have none) that keeps the rows of an adapter in their
+// order.  A wave takes its share of the rows 64 at a time, adapter by adapter of those there are among them.  5 to 7 us for up
+// to 4001 rows, 12 for 8192: latency, once a step of all projections.
 __global__ __launch_bounds__(AD_THREADS) void adapter_plan_kernel(const AdapterPlanParams p) {
   extern __shared__ int s_count[];           // [16 waves][n + 1]: rows, then the next place, of a wave's adapter
   __shared__ int s_wave[AD_THREADS / 64], s_tile[AD_THREADS + 1], s_start[AD_THREADS + 1];
@@ -157,6 +158,8 @@ __device__ __forceinline__ AdapterTile adapter_tile(const AdapterParams& p, int 
 // ranks).  So an instruction takes 256 bytes of four rows, and the rows turn into operands in the wave's own part of LDS, a
 // row's 16-byte piece q at place q ^ row: 16 lanes of a write or a read cover all banks.
 // Sixteen waves in place of eight gained nothing (4001 rows 22.0 us, 8192 56).
+// 4001 rows 12-13 us (49 MB of x, 4 TB/s; nothing hides a wave's first and last loads: six rounds a wave), 8192 of K 2048 13 (34 MB), 331
+// 5.3, 16 3.3 (two rounds of dependent loads).
 constexpr int AD_WAVES = 8;
 
 template <int NC>
@@ -237,18 +240,20 @@ __global__ __launch_bounds__(64 * AD_WAVES, 4) void adapter_shrink_kernel(const 
 // ============================================================================
 // out = y + B h
 // ============================================================================
-// A wave 16 rows of a tile by 128 columns; a workgroup the tile's 64 rows, or where the tile has up to 16 rows four times
-// the columns.  B comes in the order that the MFMA takes it, and in one that leaves a lane (c, g) 8 neighbouring
+// A wave 16 rows of a tile by 128 columns; a workgroup the tile's 64 rows.  (Tiles of up to 16 rows with four times the columns
+// a workgroup in place of three waves that leave at once: 64 single rows 9.8 us for 8.5, 32 x 5 17.2 for 16.4.)  B comes in the order that the MFMA takes it, and in one that leaves a lane (c, g) 8 neighbouring
 // columns of rows 4 g .. 4 g + 3 (register i of product t: column 8 c + t of row 4 g + i): y and out move as 256 bytes of
 // four rows an instruction.  Of paired columns the even products are gate's, the odd ones up's.
+// 8192 rows of rank 16 37 us (201 MB, 5.4 TB/s: the rate of a copy), 4001 of rank 32 8 (33 MB), 331 of rank 64 7.5 (23 MB: the plan's
+// word, then B, then the results, one after the other), 16 3.  Higher ranks wait for B and h in the caches: 5100 rows of
+// 12288 paired columns 38, 59, 85 us at rank 16, 64, 128.  B of 64 ranks in LDS for the four waves of a workgroup gained
+// 4 % at rank 128 and 5 % for the 8192 rows and cost 2 to 3 % for 16 and 331 rows.
 template <bool PAIRED>
 __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int tile = blockIdx.x / p.blocks;
   const AdapterTile t = adapter_tile(p, tile);
-  const bool few = t.rows <= 16;
-  const int block = few ? 4 * (blockIdx.x % p.blocks) + wave : blockIdx.x % p.blocks, n0 = 128 * block;
-  const int sub = few ? 0 : wave;
+  const int block = blockIdx.x % p.blocks, n0 = 128 * block, sub = wave;
   if (n0 >= p.N || sub * 16 >= t.rows) return;
   if (t.adapter < 0 && !p.swiglu && p.out == p.y) return;  // nothing to add in place
   const int c = lane & 15, g = lane >> 4;
@@ -417,7 +422,7 @@ extern "C" int t2i_adapter_add(const uint16_t* y, const uint16_t* x, int32_t M, 
     return fail(T2I_ERR_VALUE, "out must be y itself or lie beside it");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   // as many fragments of ranks a workgroup (up to four) as leave one for every CU (1, 2, 3, 4 of them, us: 331 rows
-  // of 8 16.9, 17.0, 17.8, 18.6; 16 of 3 6.0, 6.4, 6.8, 6.8; 4001 of 2 22.9, 21.8; 8192 of 3 54.4, 56.0, 54.0)
+  // of 8 12.8, 13.0, 13.7, 14.5; 16 of 3 5.7, 6.1, 6.5, 6.5; 4001 of 2 21.5, 20.7; 8192 of 3 52.4, 53.8, 51.8)
   const int nc = (int)std::min<long long>(std::min(fragments, 4), std::max<long long>(1, ((long long)M * fragments + 4095) / 4096));
   p.blocks = (fragments + nc - 1) / nc;
   const dim3 grid((cap * 4 + 7) / 8 * 8 * p.blocks), threads(64 * t2i::AD_WAVES);

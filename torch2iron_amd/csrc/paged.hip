@@ -90,6 +90,9 @@ __device__ __forceinline__ void plan_times(int pairs, float& alone, float& share
 // to a workgroup whole, longest first, or the units are cut into equal shares whose tiles' parts a second launch
 // joins, whichever the times say ends sooner; here the device decides, so that a captured step may
 // serve every later one.
+// A chain of scans and look-ups in one workgroup, bound by their latency: 32 single tokens 10.5 us, 16 x 5 drafts 8.3, 4997 rows
+// of 16 prompts 15, once a step of all layers.  A thread finds its own share (one after the other took 13.2 us for
+// the 32 tokens), and shares are cut without 64-bit division.
 __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanParams p) {
   const int tid = threadIdx.x;
   int falls = 0;                             // row_starts that do not ascend: no row is anyone's
@@ -242,7 +245,8 @@ struct PagedPrepParams {
 constexpr int PG_PREP_NB = 2;
 
 // One workgroup (4 waves) a row, as the contiguous caches' ragged_prep_kernel, whose bits it gives: only where a
-// row goes is another matter.  The page's id is needed at the stores alone.
+// row goes is another matter.  The page's id is needed at the stores alone.  4997 rows of 16 / 8 heads 21 us (82 MB, 3.9 TB/s,
+// as over a contiguous cache); up to 80 rows 4 us, a launch and three dependent loads.
 __global__ __launch_bounds__(256) void paged_prep_kernel(const PagedPrepParams p) {
   constexpr int D = RG_D;
   const int row = blockIdx.x;
@@ -313,6 +317,12 @@ __device__ __forceinline__ void poison_item(const RaggedAttnParams& p, const Rag
 // tiles of long chunks, one workgroup each, are as slow as their own chain of loads: they take the form with more
 // of them on their way (two chunks of 509 and 701 rows with 24 tokens 146 -> 131 us).  Where they fill the chip themselves
 // that form has more barriers for nothing (32 tokens 56.9 -> 58.7 us, 64 after 4090 slots 170 -> 179).
+// What bounds it (16 / 8 and 32 / 8 heads, this launch alone):
+//   tokens and drafts: memory.  64 tokens after 4090 slots 6.3 TB/s, 8 after 30000 6.5, of the 6.85 that a bulk read reaches; 32 after
+//     1000 to 4000 52 us (5.7 TB/s: shares of 9 blocks, whose first loads nothing hides), MFMA 12 % and VALU 14 % of a SIMD's cycles.
+//   1999 rows after 30001: 0.96-1.05 ms by the card, 0.97-1.05 PFLOP/s: MFMA 54 %, VALU 51 % at 1.7-1.9 GHz, as packed rows.
+//   two chunks with 24 tokens: 122 us, 2.8 TB/s and 0.52 PFLOP/s: the longest chains of loads beside the chunks' products.
+// Measured and dropped: wide tiles first; bins that carry their first tile's words; heavier shares where a CU has one workgroup.
 __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const RaggedAttnParams p, const PagedTables tab) {
   extern __shared__ __align__(256) uint16_t s_kv[];   // [buffer][K, V][key][dim]
   __shared__ uint32_t s_odd[RG_WAVES];                     // an item's pairs whose sums are not finite
@@ -375,7 +385,8 @@ __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const
   }
 }
 
-// The parts of a cut tile joined, as the contiguous caches' merge; LANES lanes a pair.
+// The parts of a cut tile joined, as the contiguous caches' merge; LANES lanes a pair.  4 us behind 32 tokens, 6 behind 16 x 5
+// drafts (a launch, the merge's words, two rounds of parts), 2-3 where nothing was cut.
 template <int LANES>
 __global__ __launch_bounds__(256) void paged_merge_kernel(const RaggedAttnParams p, const PagedTables tab) {
   constexpr int JOINED = 256 / LANES;        // pairs of a workgroup
