@@ -231,7 +231,7 @@ __device__ __forceinline__ int vd_rows(const VdParams& p, int b, int& first) {
 // ============================================================================
 // A wave takes every step-th chunk of a row, the next one's logits on their way while it adds the weights of one: the largest
 // logit first, then the weights.  Lane l holds the pieces l, l + 64, ... of a chunk (16 bytes, at any alignment of the values).
-// 122 rows of 151936 bf16 logits 16-17 us (37 MB, VALU 73 % of a SIMD's cycles at 1.9 GHz), 432 of fp32 56 (262 MB, 4.7 TB/s, VALU 74 %).
+// 122 rows of 151936 bf16 logits 16-17 us (37 MB, VALU 79 % of a SIMD's cycles at 1.9 GHz), 432 of fp32 56 (262 MB, 4.7 TB/s, VALU 79 %).
 // Fewer instructions did not make it faster: a degree less with a table of 64 (19 % fewer) 25.0 -> 24.6 us for the whole call, no
 // difference to the largest logit (5 %) none; nor did chunks two ahead (25.9), five waves a SIMD (93 for 83 us of fp32).
 template <typename T>
