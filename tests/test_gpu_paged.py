@@ -116,6 +116,25 @@ def test_paged_attention(gpu, hq, hkv, page, lens, ctx):
     assert ((sums.double() - want).abs() <= bound + 1e-30).all()
 
 
+@pytest.mark.parametrize("longest", [90, 9000], ids=["whole", "cut"])
+def test_more_tiles_than_the_plan_has_threads(gpu, longest):
+    n = 2500
+    c = Case(gpu, 2, 1, 16, [1 + i % 2 for i in range(n)], [longest if i == 1234 else i % 40 for i in range(n)])
+    out = ops.paged_attention(c.q, c.plan, c.k, c.v)
+    _check(out, *c.reference())
+
+
+def test_more_kv_heads_than_workgroups_run_at_once(gpu):
+    c = Case(gpu, 520, 520, 16, [3, 1, 2], [40, 700, 7])
+    _check(ops.paged_attention(c.q, c.plan, c.k, c.v), *c.reference())
+
+
+def test_as_many_sequences_as_a_plan_takes(gpu):
+    n = 4096
+    c = Case(gpu, 1, 1, 16, [i % 3 for i in range(n)], [i % 70 for i in range(n)])
+    _check(ops.paged_attention(c.q, c.plan, c.k, c.v), *c.reference())
+
+
 def test_values_behind_a_mask_stay_there(gpu):
     """NaN and infinities in slots that a row does not attend do not reach it; rows that attend them take them."""
     for bad in (NAN, math.inf, -math.inf):

@@ -116,7 +116,7 @@ def _check(args, got, near=1e-13):
 
 SHAPES = [([1], 5), ([1], 1), ([2], 1), ([3, 1, 4], 7), ([5, 0, 1, 9], 1000), ([4] * 6, 1023), ([2, 6], 1024), ([9, 3], 1025),
           ([5] * 5, 4099), ([1] * 40, 30011), ([17, 2], 2049), ([5, 3, 1], 151936), ([2, 3], 300001),
-          ([2, 1], 1100003)]
+          ([2, 1], 1100003), ([3, 1] * 150, 1500), ([2, 0, 1] * 700, 65)]
 
 
 @pytest.mark.parametrize("with_probs", [False, True], ids=["certain", "probs"])
