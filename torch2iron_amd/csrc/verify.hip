@@ -55,20 +55,18 @@ struct VdParams {
 };
 
 // ---- exp((x - m) / T) in fp64 ----
-// With y = (x - m) 32 log2(e) / T = 32 n + j + f (j of 0 .. 31, |f| <= 1/2): 2^n 2^(j / 32) 2^(f / 32), the second from a
-// table in LDS (32 doubles stand in 64 banks: no conflict), the third by its interpolation at five Chebyshev nodes
-// (relative error 8e-14).  Half the instructions of a series for 2^(y / 32 - n).
-constexpr int VD_EXP = 32;
+// With y = (x - m) 256 log2(e) / T = 256 n + j + f (j of 0 .. 255, |f| <= 1/2): 2^n 2^(j / 256) 2^(f / 256), the second from a
+// table in LDS, the third 1 + f times the quadratic of the smallest largest error there is (2.4e-14).  A third of the instructions of
+// a series for 2^(y / 256 - n).  (A table of 32 with no bank twice and a degree more, 8e-14: 122 bf16 rows 24.9 -> 24.2 us, 432 of
+// fp32 86.5 -> 84.)
+constexpr int VD_EXP = 256, VD_LOG = 8;
+constexpr double VD_P1 = 0.002707606174062412, VD_P2 = 3.665566060705425e-06, VD_P3 = 3.3083022204273407e-09;
 __device__ __forceinline__ double vd_fraction(double f) {
-  double p = 9.172607532092245e-09;
-  p = __builtin_fma(p, f, 1.6938633903155644e-06);
-  p = __builtin_fma(p, f, 0.0002345961981994449);
-  p = __builtin_fma(p, f, 0.02166084939172217);
-  return __builtin_fma(p, f, 1.0);
+  return __builtin_fma(__builtin_fma(__builtin_fma(VD_P3, f, VD_P2), f, VD_P1), f, 1.0);
 }
 
-// The table: s_exp[j] = 2^(j / 32) by the series of e^t (the first term left out is 0.68^17 / 17! = 4e-18), and s_add[j] the
-// same with j 2^15 taken from its high word, so that 2^n comes with an addition.  A barrier behind it is the caller's.
+// The table: s_exp[j] = 2^(j / 256) by the series of e^t (the first term left out is 0.7^17 / 17! = 7e-18), and s_add[j] the
+// same with j 2^12 taken from its high word, so that 2^n comes with an addition.  A barrier behind it is the caller's.
 __device__ __forceinline__ void vd_table(double* s_exp, double* s_add = nullptr) {
   if (threadIdx.x < VD_EXP) {
     const double t = (double)threadIdx.x * (0.69314718055994530942 / VD_EXP);
@@ -76,50 +74,48 @@ __device__ __forceinline__ void vd_table(double* s_exp, double* s_add = nullptr)
 #pragma unroll
     for (int k = 16; k > 0; --k) p = __builtin_fma(p * t, 1.0 / k, 1.0);
     s_exp[threadIdx.x] = p;
-    if (s_add) s_add[threadIdx.x] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) - ((uint64_t)threadIdx.x << 47));
+    if (s_add) s_add[threadIdx.x] = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, p) - ((uint64_t)threadIdx.x << (52 - VD_LOG)));
   }
 }
 
-// 2^(y / 32): 0 far below; an infinite y gives NaN.
+// 2^(y / 256): 0 far below; an infinite y gives NaN.
 __device__ __forceinline__ double vd_exp(double y, const double* s_exp) {
   const double k = __builtin_rint(y);
   int n;
   asm("v_cvt_i32_f64 %0, %1" : "=v"(n) : "v"(k));          // (saturates)
-  return __builtin_amdgcn_ldexp(vd_fraction(y - k) * s_exp[n & (VD_EXP - 1)], n >> 5);
+  return __builtin_amdgcn_ldexp(vd_fraction(y - k) * s_exp[n & (VD_EXP - 1)], n >> VD_LOG);
 }
 
-// z + 2^(d c / 32), for a row's sums: -32000 < d c < 2^20.  The whole part k = 32 n + j comes out of the low bits of
-// d c + 1.5 2^52, and k 2^15, added to the high word of the table's value, is j 2^15 + n 2^20: n more in its exponent.
+// z + 2^(d c / 256), for a row's sums: -2^18 < d c < 2^20.  The whole part k = 256 n + j comes out of the low bits of
+// d c + 1.5 2^52, and k 2^12, added to the high word of the table's value, is j 2^12 + n 2^20: n more in its exponent.
 // The constants stay in registers (an instruction takes one from elsewhere, and copies would be a tenth of all).
 struct VdAdd {
-  double c, whole, p[4];
+  double c, whole, p[3];
   const u32x2* table;
-  __device__ __forceinline__ VdAdd(double scale, const double* s_add) : c(scale), whole(6755399441055744.0),
-      p{9.172607532092245e-09, 1.6938633903155644e-06, 0.0002345961981994449, 0.02166084939172217} {
+  __device__ __forceinline__ VdAdd(double scale, const double* s_add) : c(scale), whole(6755399441055744.0), p{VD_P3, VD_P2, VD_P1} {
     table = reinterpret_cast<const u32x2*>(s_add);
-    asm("" : "+v"(c), "+v"(whole), "+v"(p[0]), "+v"(p[1]), "+v"(p[2]), "+v"(p[3]));
+    asm("" : "+v"(c), "+v"(whole), "+v"(p[0]), "+v"(p[1]), "+v"(p[2]));
   }
   __device__ __forceinline__ double operator()(double d, double z) const {
     const double s = __builtin_fma(d, c, whole);
     const double f = __builtin_fma(d, c, whole - s);
     const uint32_t k = __builtin_bit_cast(u32x2, s).x;
     u32x2 e = table[k & (VD_EXP - 1)];
-    e.y += k << 15;
+    e.y += k << (20 - VD_LOG);
     double v = __builtin_fma(p[0], f, p[1]);
     v = __builtin_fma(v, f, p[2]);
-    v = __builtin_fma(v, f, p[3]);
     v = __builtin_fma(v, f, 1.0);
     return __builtin_fma(v, __builtin_bit_cast(double, e), z);
   }
 };
 
-// exp((x - m) / T) with c = 32 log2(e) / T; 0 for a logit of -inf, whatever m and c are
+// exp((x - m) / T) with c = 256 log2(e) / T; 0 for a logit of -inf, whatever m and c are
 __device__ __forceinline__ double vd_weight(float x, float m, double c, const double* s_exp) {
   const double w = vd_exp(((double)x - (double)m) * c, s_exp);
   return x == -INFINITY ? 0.0 : w;
 }
 
-// 32 log2(e) / T; a temperature that is not above 0 (greedy) counts as 1 where probabilities are formed
+// 256 log2(e) / T; a temperature that is not above 0 (greedy) counts as 1 where probabilities are formed
 __device__ __forceinline__ double vd_scale(float t) { return VD_EXP * 1.44269504088896340736 / (t > 0.0f ? (double)t : 1.0); }
 // log p of a logit x, given the row's m and z
 __device__ __forceinline__ float vd_logprob(float x, float m, double c, double log_z) {
@@ -232,8 +228,8 @@ __device__ __forceinline__ int vd_rows(const VdParams& p, int b, int& first) {
 // A wave takes every step-th chunk of a row, the next one's logits on their way while it adds the weights of one: the largest
 // logit first, then the weights.  Lane l holds the pieces l, l + 64, ... of a chunk (16 bytes, at any alignment of the values).
 // 122 rows of 151936 bf16 logits 16-17 us (37 MB, VALU 79 % of a SIMD's cycles at 1.9 GHz), 432 of fp32 56 (262 MB, 4.7 TB/s, VALU 79 %).
-// Fewer instructions did not make it faster: a degree less with a table of 64 (19 % fewer) 25.0 -> 24.6 us for the whole call, no
-// difference to the largest logit (5 %) none; nor did chunks two ahead (25.9), five waves a SIMD (93 for 83 us of fp32).
+// Without the weights it takes 11 and 48 us: launch, a wave's first loads, the reductions.  No difference to the largest
+// logit (an instruction of 20 less) gained nothing; chunks two ahead (25.9 us for the whole call) and five waves a SIMD (93 for 83 us of fp32) lost.
 template <typename T>
 __global__ __launch_bounds__(64 * VD_WAVES) void verify_rows_kernel(const VdParams p) {
   constexpr int PER = 16 / VdType<T>::SIZE, PIECES = VD_CHUNK / 64 / PER;
