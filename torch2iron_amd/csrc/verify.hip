@@ -660,10 +660,11 @@ namespace {
 
 int vd_chunks(int V) { return (int)(((long long)V + t2i::VD_CHUNK - 1) / t2i::VD_CHUNK); }
 
-// Workgroups of a row.  A wave takes up to four chunks, one after the other, where there are enough waves for all CUs
-// (us for 1, 2, 4, 8, 19 chunks: 122 bf16 rows 24.5, 24.1, 24.5, 28.7, 34.3, 576 fp32 rows 82.5, 82.7, 82.1, 84.4, 91.6).
+// Workgroups of a row.  A wave takes two chunks, one after the other, where that leaves enough waves for all CUs
+// (us of the whole call for 1, 2, 4, 8 chunks: 16 fp32 rows of 151936 11.1, 12.1, 14.4, 20.4; 120 21.8, 22.4, 23.2, 26.5; 432 86.2, 83.7, 84.6, 86.1; bf16,
+// 61 rows 16.7, 16.8, 18.2, 21.7; 122 25.2, 24.3, 24.7, 28.8; 250 31.2, 29.7, 30.8, 32.3).
 int vd_splits(int M, int n_chunks) {
-  const long long run = std::max(1LL, std::min((long long)M * n_chunks / 8192, 4LL));
+  const long long run = (long long)M * n_chunks < 16384 ? 1 : 2;
   return (int)((n_chunks + t2i::VD_WAVES * run - 1) / (t2i::VD_WAVES * run));
 }
 
