@@ -1439,7 +1439,7 @@ class PagedPlan:
         _check_dev("k_pages", k_pages, BF16)
         _check_dev("v_pages", v_pages, BF16)
         want = (self.n_kv_heads, self.page_slots, d)
-        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[0] < 1 or tuple(k_pages.shape[1:]) != want:
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[0] < 1 or k_pages.shape[1:] != want:
             raise ValueError(f"k_pages and v_pages must be [pages, {want[0]}, {want[1]}, {d}] of equal shape")
         if k_pages.shape[0] >= 2**31:
             raise ValueError(f"a pool of {k_pages.shape[0]} pages is too large")
@@ -1552,7 +1552,7 @@ def verify_drafts(logits: torch.Tensor, row_starts: torch.Tensor, tokens: torch.
     if draft_probs is not None:
         if not isinstance(draft_probs, torch.Tensor) or draft_probs.dtype != torch.float32:
             raise ValueError("draft_probs must be a float32 tensor")
-        if tuple(draft_probs.shape) != (m, v):
+        if draft_probs.shape != (m, v):
             raise ValueError(f"draft_probs must be [{m}, {v}], as the logits")
         probs_stride = _check_rows("draft_probs", draft_probs)[2]
     if temperatures is not None:
@@ -1675,6 +1675,7 @@ class AdapterPlan:
         if self.rows >= 2**24:
             raise ValueError(f"{self.rows} rows are too many")
         self._words = _lib.load().t2i_adapter_plan_words(self.rows, n_adapters)
+        self._bytes = {}
         self._stream = _lib.stream_handle(self.device)
         self.table = torch.empty(self._words, dtype=torch.int32, device=self.device)
         self.refresh()
@@ -1685,6 +1686,13 @@ class AdapterPlan:
             self._use()
             _launch(self.device, "t2i_adapter_plan", self.ids.data_ptr(), self.rows, self.n, self.table.data_ptr(),
                     self._words)
+
+    def _workspace(self, parts: int, rank: int) -> int:
+        """Bytes of scratch that ``adapter_add`` takes, asked for once for each kind of pool."""
+        nbytes = self._bytes.get((parts, rank))
+        if nbytes is None:
+            nbytes = self._bytes[parts, rank] = _lib.load().t2i_adapter_add_workspace_bytes(self.rows, self.n, parts, rank)
+        return nbytes
 
     def _use(self):
         """The plan's memory waits for the current stream before it is given to another tensor."""
@@ -1707,20 +1715,19 @@ def adapter_add(y: torch.Tensor, x: torch.Tensor, adapters: Adapters, plan: Adap
     m, n, k = plan.rows, adapters.N, adapters.K
     if plan.n != adapters.n:
         raise ValueError(f"the plan is for {plan.n} adapters, the pool has {adapters.n}")
-    if tuple(x.shape) != (m, k) or tuple(y.shape) != (m, n):
+    if x.shape != (m, k) or y.shape != (m, n):
         raise ValueError(f"x must be [{m}, {k}] and y [{m}, {n}]")
     if swiglu and not adapters.paired:
         raise ValueError("SwiGLU needs paired columns")
     if out is None:
         out = torch.empty(m, n // 2, dtype=BF16, device=y.device) if swiglu else y
     _check_dev("out", out, BF16)
-    if tuple(out.shape) != (m, n // 2 if swiglu else n):
+    if out.shape != (m, n // 2 if swiglu else n):
         raise ValueError(f"out must be [{m}, {n // 2 if swiglu else n}]")
     _same_device(adapters.device, y=y, x=x, out=out, ids=plan.ids)
     if m == 0:
         return out
-    lib = _lib.load()
-    nbytes = lib.t2i_adapter_add_workspace_bytes(m, adapters.n, adapters.parts, adapters.rank)
+    nbytes = plan._workspace(adapters.parts, adapters.rank)
     ws = _scratch(workspace, "adapters", nbytes, y.device)
     plan._use()
     _launch(y.device, "t2i_adapter_add",
