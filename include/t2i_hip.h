@@ -671,17 +671,18 @@ int t2i_verify_drafts(const void* logits, int32_t logits_type, int64_t row_strid
  * any other id: none), as t2i_adapter_plan_words words on the device, for every projection of the step.
  *
  * t2i_adapter_add: out[r] = y[r] + scales[a] * B_a (A_a x[r]) with a = ids[r], y[r] itself for rows without an
- * adapter; y bf16 [M, N] is the shared projection's output, x bf16 [M, K] its input, out may be y
- * (any other overlap of the two is refused).  With R = rank (1 to
- * 256) rounded up to a multiple of 16, a is A bf16 [n_adapters, parts * R, K] and b is B bf16 [n_adapters, N, R], the places behind
- * rank 0, in the order that the kernels take them: a [n][parts * R / 16][K / 32][g 4][c 16][8] holds rank 16 i + c and k 32 s
- * + 8 g .., b [n][ceil(N / 128)][R / 16][t 8][g 2][c 16][8] column 128 i + 8 c + t and ranks 16 s + 8 g .. (columns behind N 0);
- * scales fp32 [n_adapters] (NULL: 1).  The columns may be several
- * projections' beside each other (parts up to 4): slice i of widths[i] columns (host memory; multiples
- * of 128, parts 1: NULL) has rows i * R .. of A; or, paired (parts 2), alternate between them (column 2j of slice 0, gate, column
- * 2j + 1 of slice 1, up; as t2i_w4a16_gate_up without SwiGLU leaves them interleaved in one linear).  swiglu (paired alone): out
- * bf16 [M, N / 2] = silu(gate) * up.  Sums are fp32, A x enters the second product with 16 bits, the result is rounded
- * once.  An infinity among an adapter's weights may give its rows NaN where an infinity is due.  The workspace (t2i_adapter_add_workspace_bytes) is scratch as t2i_packed_attention's.
+ * adapter; y bf16 [M, N] is the shared projection's output, x bf16 [M, K] its input, out may be y (any other
+ * overlap of the two is refused).  With R = rank (1 to 256) rounded up to a multiple of 16, a is A bf16
+ * [n_adapters, parts * R, K] and b is B bf16 [n_adapters, N, R], the places behind rank 0, in the order that
+ * the kernels take them: a [n][parts * R / 16][K / 32][g 4][c 16][8] holds rank 16 i + c and k 32 s + 8 g .., b
+ * [n][ceil(N / 128)][R / 16][t 8][g 2][c 16][8] column 128 i + 8 c + t and ranks 16 s + 8 g .. (columns behind
+ * N 0); scales fp32 [n_adapters] (NULL: 1).  The columns may be several projections' beside each other (parts
+ * up to 4): slice i of widths[i] columns (host memory; multiples of 128, parts 1: NULL) has rows i * R .. of A;
+ * or, paired (parts 2), alternate between them (column 2j of slice 0, gate, column 2j + 1 of slice 1, up; as
+ * t2i_w4a16_gate_up without SwiGLU leaves them interleaved in one linear).  swiglu (paired alone): out bf16 [M,
+ * N / 2] = silu(gate) * up.  Sums are fp32, A x enters the second product with 16 bits, the result is rounded
+ * once.  An infinity among an adapter's weights may give its rows NaN where an infinity is due.  The workspace
+ * (t2i_adapter_add_workspace_bytes) is scratch as t2i_packed_attention's.
  * K % 32 == 0, N % 16 == 0.
  * No counterpart in the reference, which has one set of weights.
  */

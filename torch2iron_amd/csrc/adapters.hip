@@ -158,8 +158,8 @@ __device__ __forceinline__ AdapterTile adapter_tile(const AdapterParams& p, int 
 // ranks).  So an instruction takes 256 bytes of four rows, and the rows turn into operands in the wave's own part of LDS, a
 // row's 16-byte piece q at place q ^ row: 16 lanes of a write or a read cover all banks.
 // Sixteen waves in place of eight gained nothing (4001 rows 22.0 us, 8192 56).
-// 4001 rows 12-13 us (49 MB of x, 4 TB/s; nothing hides a wave's first and last loads: six rounds a wave), 8192 of K 2048 13 (34 MB), 331
-// 5.3, 16 3.3 (two rounds of dependent loads).
+// 4001 rows 12-13 us (49 MB of x, 4 TB/s; nothing hides a wave's first and last loads: six rounds a wave), 8192 of K 2048
+// 13 (34 MB), 331 5.3, 16 3.3 (two rounds of dependent loads).
 constexpr int AD_WAVES = 8;
 
 template <int NC>
@@ -241,13 +241,14 @@ __global__ __launch_bounds__(64 * AD_WAVES, 4) void adapter_shrink_kernel(const 
 // out = y + B h
 // ============================================================================
 // A wave 16 rows of a tile by 128 columns; a workgroup the tile's 64 rows.  (Tiles of up to 16 rows with four times the columns
-// a workgroup in place of three waves that leave at once: 64 single rows 9.8 us for 8.5, 32 x 5 17.2 for 16.4.)  B comes in the order that the MFMA takes it, and in one that leaves a lane (c, g) 8 neighbouring
-// columns of rows 4 g .. 4 g + 3 (register i of product t: column 8 c + t of row 4 g + i): y and out move as 256 bytes of
-// four rows an instruction.  Of paired columns the even products are gate's, the odd ones up's.
-// 8192 rows of rank 16 37 us (201 MB, 5.4 TB/s: the rate of a copy), 4001 of rank 32 8 (33 MB), 331 of rank 64 7.5 (23 MB: the plan's
-// word, then B, then the results, one after the other), 16 3.  Higher ranks wait for B and h in the caches: 5100 rows of
-// 12288 paired columns 38, 59, 85 us at rank 16, 64, 128.  B of 64 ranks in LDS for the four waves of a workgroup gained
-// 4 % at rank 128 and 5 % for the 8192 rows and cost 2 to 3 % for 16 and 331 rows.
+// a workgroup in place of three waves that leave at once: 64 single rows 9.8 us for 8.5, 32 x 5 17.2 for 16.4.)  B comes in
+// the order that the MFMA takes it, and in one that leaves a lane (c, g) 8 neighbouring columns of rows 4 g .. 4 g + 3
+// (register i of product t: column 8 c + t of row 4 g + i): y and out move as 256 bytes of four rows an instruction.  Of
+// paired columns the even products are gate's, the odd ones up's. 8192 rows of rank 16 37 us (201 MB, 5.4 TB/s: the rate of
+// a copy), 4001 of rank 32 8 (33 MB), 331 of rank 64 7.5 (23 MB: the plan's word, then B, then the results, one after the
+// other), 16 3.  Higher ranks wait for B and h in the caches: 5100 rows of 12288 paired columns 38, 59, 85 us at rank 16,
+// 64, 128.  B of 64 ranks in LDS for the four waves of a workgroup gained 4 % at rank 128 and 5 % for the 8192 rows and
+// cost 2 to 3 % for 16 and 331 rows.
 template <bool PAIRED>
 __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

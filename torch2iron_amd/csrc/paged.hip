@@ -24,7 +24,7 @@ namespace t2i {
 constexpr int PG_THREADS = 1024;
 constexpr int PG_SEQS = 4096;                // sequences of a plan
 constexpr int PG_TILE = 8;                   // words of a tile: {first row, rows, context, sequence, first pair, first unit, units, 0}
-constexpr int PG_BIN = 4;                    // of a bin: {first tile (-1: none), first unit, unit behind the last, whether narrow tiles stand among wide ones}
+constexpr int PG_BIN = 4;                    // of a bin: {first tile (-1: none), first unit, unit behind the last, narrow ones among wide?}
 constexpr int PG_MERGE = 8;                  // of a merge: {first row, rows (0: none), first pair, first part, first second part, parts, 0, 0}
 constexpr int PG_NARROW = 32;                // pairs that one wave multiplies
 constexpr int PG_ROW = 2;                    // of a row: {position (-1: none), sequence}
@@ -90,9 +90,9 @@ __device__ __forceinline__ void plan_times(int pairs, float& alone, float& share
 // to a workgroup whole, longest first, or the units are cut into equal shares whose tiles' parts a second launch
 // joins, whichever the times say ends sooner; here the device decides, so that a captured step may
 // serve every later one.
-// A chain of scans and look-ups in one workgroup, bound by their latency: 32 single tokens 10.5 us, 16 x 5 drafts 8.3, 4997 rows
-// of 16 prompts 15, once a step of all layers.  A thread finds its own share (one after the other took 13.2 us for
-// the 32 tokens), and shares are cut without 64-bit division.
+// A chain of scans and look-ups in one workgroup, bound by their latency: 32 single tokens 10.5 us, 16 x 5 drafts 8.3, 4997
+// rows of 16 prompts 15, once a step of all layers.  A thread finds its own share (one after the other took 13.2 us for the
+// 32 tokens), and shares are cut without 64-bit division.
 __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanParams p) {
   const int tid = threadIdx.x;
   int falls = 0;                             // row_starts that do not ascend: no row is anyone's
@@ -322,7 +322,8 @@ __device__ __forceinline__ void poison_item(const RaggedAttnParams& p, const Rag
 //     1000 to 4000 52 us (5.7 TB/s: shares of 9 blocks, whose first loads nothing hides), MFMA 12 % and VALU 14 % of a SIMD's cycles.
 //   1999 rows after 30001: 0.96-1.05 ms by the card, 0.97-1.05 PFLOP/s: MFMA 54 %, VALU 51 % at 1.7-1.9 GHz, as packed rows.
 //   two chunks with 24 tokens: 122 us, 2.8 TB/s and 0.52 PFLOP/s: the longest chains of loads beside the chunks' products.
-// Measured and dropped: wide tiles first; bins that carry their first tile's words; heavier shares where a CU has one workgroup.
+// Measured and dropped: wide tiles first; bins that carry their first tile's words; heavier shares where a CU has one
+// workgroup.
 __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const RaggedAttnParams p, const PagedTables tab) {
   extern __shared__ __align__(256) uint16_t s_kv[];   // [buffer][K, V][key][dim]
   __shared__ uint32_t s_odd[RG_WAVES];                     // an item's pairs whose sums are not finite
@@ -561,8 +562,8 @@ extern "C" int t2i_paged_attention(const uint16_t* q, int32_t rows, const int32_
   hipLaunchKernelGGL(t2i::paged_attention_kernel, dim3(z.bins * Hkv), dim3(64 * t2i::RG_WAVES), LDS_BYTES, s, p, tab);
   if (int rc = t2i_host::hip_status(hipGetLastError(), "paged attention launch")) return rc;
   // Tiles enough for all shares are mostly handed out whole, and then what this launch takes is its waves that find
-  // nothing to do: a quarter of them with 8 lanes a pair (16 prompts of 37 to 1021 rows 36.9 -> 34.5 us).  Few tiles are cut into many
-  // parts, which more lanes join sooner (a single token 10.6 us, with 8 lanes 11.6; 2 x 9 drafts 45.6, 48.8).
+  // nothing to do: a quarter of them with 8 lanes a pair (16 prompts of 37 to 1021 rows 36.9 -> 34.5 us).  Few tiles are
+  // cut into many parts, which more lanes join sooner (a single token 10.6 us, with 8 lanes 11.6; 2 x 9 drafts 45.6, 48.8).
   const auto merge = [&](auto lanes) {
     constexpr int LANES = decltype(lanes)::value;
     hipLaunchKernelGGL(t2i::paged_merge_kernel<LANES>, dim3(z.merges * Hkv * (p.part_rows * LANES / 256)), dim3(256), 0, s, p, tab);

@@ -56,9 +56,9 @@ struct VdParams {
 
 // ---- exp((x - m) / T) in fp64 ----
 // With y = (x - m) 256 log2(e) / T = 256 n + j + f (j of 0 .. 255, |f| <= 1/2): 2^n 2^(j / 256) 2^(f / 256), the second from a
-// table in LDS, the third 1 + f times the quadratic of the smallest largest error there is (2.4e-14).  A third of the instructions of
-// a series for 2^(y / 256 - n).  (A table of 32 with no bank twice and a degree more, 8e-14: 122 bf16 rows 24.9 -> 24.2 us, 432 of
-// fp32 86.5 -> 84.)
+// table in LDS, the third 1 + f times the quadratic of the smallest largest error there is (2.4e-14).  A third of the
+// instructions of a series for 2^(y / 256 - n).  (A table of 32 with no bank twice and a degree more, 8e-14: 122 bf16 rows
+// 24.9 -> 24.2 us, 432 of fp32 86.5 -> 84.)
 constexpr int VD_EXP = 256, VD_LOG = 8;
 constexpr double VD_P1 = 0.002707606174062412, VD_P2 = 3.665566060705425e-06, VD_P3 = 3.3083022204273407e-09;
 __device__ __forceinline__ double vd_fraction(double f) {
@@ -227,9 +227,11 @@ __device__ __forceinline__ int vd_rows(const VdParams& p, int b, int& first) {
 // ============================================================================
 // A wave takes every step-th chunk of a row, the next one's logits on their way while it adds the weights of one: the largest
 // logit first, then the weights.  Lane l holds the pieces l, l + 64, ... of a chunk (16 bytes, at any alignment of the values).
-// 122 rows of 151936 bf16 logits 16-17 us (37 MB, VALU 79 % of a SIMD's cycles at 1.9 GHz), 432 of fp32 56 (262 MB, 4.7 TB/s, VALU 79 %).
+// 122 rows of 151936 bf16 logits 16-17 us (37 MB, VALU 81 % of a SIMD's cycles at 1.9 GHz), 432 of fp32 56 (262 MB,
+// 4.7 TB/s, VALU 78 %).
 // Without the weights it takes 11 and 48 us: launch, a wave's first loads, the reductions.  No difference to the largest
-// logit (an instruction of 20 less) gained nothing; chunks two ahead (25.9 us for the whole call) and five waves a SIMD (93 for 83 us of fp32) lost.
+// logit (an instruction of 20 less) gained nothing; chunks two ahead (25.9 us for the whole call) and five waves a SIMD (93
+// for 83 us of fp32) lost.
 template <typename T>
 __global__ __launch_bounds__(64 * VD_WAVES) void verify_rows_kernel(const VdParams p) {
   constexpr int PER = 16 / VdType<T>::SIZE, PIECES = VD_CHUNK / 64 / PER;
@@ -369,11 +371,11 @@ __device__ __forceinline__ void vd_chunk_of(VdChoice& ch, double (&part)[VD_HELD
   }
 }
 
-// A workgroup's decision for sequence b: what its next token is drawn by, from which row (with the draw 6.3 us for 32 sequences of
-// four drafts: five loads that depend on each other).  Waves take rows in turn;
-// each remembers the first of its rows behind which no draft stays, and its parts: where the token comes from p itself (or p
-// without the draft) the wave of that row finds the chunk too, without another look at memory.  WRITE: the log
-// probabilities of the drafts that stay.
+// A workgroup's decision for sequence b: what its next token is drawn by, from which row (with the draw 6.3 us for 32
+// sequences of four drafts: five loads that depend on each other).  Waves take rows in turn; each remembers the first of
+// its rows behind which no draft stays, and its parts: where the token comes from p itself (or p without the draft) the
+// wave of that row finds the chunk too, without another look at memory.  WRITE: the log probabilities of the drafts that
+// stay.
 template <typename T, bool WRITE>
 __device__ __forceinline__ VdChoice vd_decide(const VdParams& p, int b, const double* s_exp, int* s_row, VdChoice* s_choice) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -661,8 +663,9 @@ namespace {
 int vd_chunks(int V) { return (int)(((long long)V + t2i::VD_CHUNK - 1) / t2i::VD_CHUNK); }
 
 // Workgroups of a row.  A wave takes two chunks, one after the other, where that leaves enough waves for all CUs
-// (us of the whole call for 1, 2, 4, 8 chunks: 16 fp32 rows of 151936 11.1, 12.1, 14.4, 20.4; 120 21.8, 22.4, 23.2, 26.5; 432 86.2, 83.7, 84.6, 86.1; bf16,
-// 61 rows 16.7, 16.8, 18.2, 21.7; 122 25.2, 24.3, 24.7, 28.8; 250 31.2, 29.7, 30.8, 32.3).
+// (us of the whole call for 1, 2, 4, 8 chunks: 16 fp32 rows of 151936 11.1, 12.1, 14.4, 20.4; 120 21.8, 22.4, 23.2, 26.5;
+// 432 86.2, 83.7, 84.6, 86.1; bf16, 61 rows 16.7, 16.8, 18.2, 21.7; 122 25.2, 24.3, 24.7, 28.8; 250 31.2, 29.7, 30.8,
+// 32.3).
 int vd_splits(int M, int n_chunks) {
   const long long run = (long long)M * n_chunks < 16384 ? 1 : 2;
   return (int)((n_chunks + t2i::VD_WAVES * run - 1) / (t2i::VD_WAVES * run));

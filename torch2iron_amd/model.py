@@ -932,7 +932,8 @@ class Qwen3Model:
         if batch.rows < 1 or tokens.numel() != batch.rows:
             raise ValueError(f"tokens must hold {batch.rows} ids, at least one")
         if cache.max_pages * cache.page_slots > self.rope.shape[0]:
-            raise ValueError(f"sequences of {cache.max_pages * cache.page_slots} slots exceed the model's {self.rope.shape[0]} positions")
+            raise ValueError(f"sequences of {cache.max_pages * cache.page_slots} slots exceed the model's "
+                             f"{self.rope.shape[0]} positions")
         n_head, plan = batch.head_rows.numel(), None
         if uniforms is None:
             if temperatures is not None or draft_probs is not None:

@@ -1524,21 +1524,24 @@ def verify_drafts(logits: torch.Tensor, row_starts: torch.Tensor, tokens: torch.
     """Drafted tokens held to the model's probabilities with given random numbers, and the token after them drawn:
     what comes out is distributed as the model's own samples.  A sequence of one row samples.
 
-    Rows ``row_starts[s] .. row_starts[s + 1] - 1`` (int32 ``[S + 1]``) of ``logits`` (fp32, bf16 or fp16 ``[M, V]``;
-    rows may be strided) are sequence s's, ``tokens`` int32 ``[M]`` the tokens that they stand behind: the draft after
-    a row is the next row's token.  ``draft_probs`` fp32 ``[M, V]``: the distribution that the draft after a row was drawn from (rows
-    that have none are never read); without it drafts count as certain (looked up, or a small model's greedy choice).
-    ``uniforms`` fp32 ``[M]`` in [0, 1): the number behind a draft decides on it, the one of the last row
-    draws the next token.  ``temperatures`` fp32 ``[S]`` (1 without); not above 0: greedy.
+    Rows ``row_starts[s] .. row_starts[s + 1] - 1`` (int32 ``[S + 1]``) of ``logits`` (fp32, bf16 or fp16
+    ``[M, V]``; rows may be strided) are sequence s's, ``tokens`` int32 ``[M]`` the tokens that they stand
+    behind: the draft after a row is the next row's token. ``draft_probs`` fp32 ``[M, V]``: the distribution
+    that the draft after a row was drawn from (rows that have none are never read); without it drafts count as
+    certain (looked up, or a small model's greedy choice). ``uniforms`` fp32 ``[M]`` in [0, 1): the number
+    behind a draft decides on it, the one of the last row draws the next token. ``temperatures`` fp32 ``[S]``
+    (1 without); not above 0: greedy.
 
-    With p = softmax(logits / T) and q a row of ``draft_probs``, a draft y stays where ``u * q[y] < p[y]``, up to the
-    first that does not; the next token is drawn from ``max(p - q, 0)`` of that row, else from the last row's p, as the first token whose
-    running sum passes u times the whole.  fp64 throughout.  Returns int32 ``counts [S]`` (drafts that stay), int32 ``next_tokens
-    [S]``, fp32 ``logprobs [M]`` (log p of the token that came out behind each row, 0 behind the rest; greedy rows at T = 1).
+    With p = softmax(logits / T) and q a row of ``draft_probs``, a draft y stays where ``u * q[y] < p[y]``, up
+    to the first that does not; the next token is drawn from ``max(p - q, 0)`` of that row, else from the last
+    row's p, as the first token whose running sum passes u times the whole. fp64 throughout. Returns int32
+    ``counts [S]`` (drafts that stay), int32 ``next_tokens [S]``, fp32 ``logprobs [M]`` (log p of the token
+    that came out behind each row, 0 behind the rest; greedy rows at T = 1).
 
-    Logits of -inf have probability 0; a row with a NaN, a +inf or nothing but -inf ends its sequence with the token -1
-    and log probability NaN.  A draft outside ``[0, V)`` does not stay.  A sequence without rows: count 0, token -1; so all of
-    them where ``row_starts`` (of up to 65536 sequences) do not ascend within ``0 .. M``."""
+    Logits of -inf have probability 0; a row with a NaN, a +inf or nothing but -inf ends its sequence with the
+    token -1 and log probability NaN. A draft outside ``[0, V)`` does not stay. A sequence without rows: count
+    0, token -1; so all of them where ``row_starts`` (of up to 65536 sequences) do not ascend within ``0 ..
+    M``."""
     m, v, stride = _check_logits(logits)
     for n, t, dtype in (("row_starts", row_starts, torch.int32), ("tokens", tokens, torch.int32),
                         ("uniforms", uniforms, torch.float32)):
@@ -1582,12 +1585,14 @@ def verify_drafts(logits: torch.Tensor, row_starts: torch.Tensor, tokens: torch.
 class Adapters:
     """A pool of low-rank adapters of one projection: adapter i adds ``scales[i] * B_i (A_i x)`` to its output.
 
-    ``a`` bf16 ``[n, R, K]``, ``b`` bf16 ``[n, N, R]`` (n up to 511, R up to 256, K a multiple of 32, N of 16), ``scales``
-    fp32 ``[n]`` (1 by default).  Of a fused projection: ``a [n, slices, R, K]``, ``b``'s rows in the order of the fused columns, and either
-    ``widths`` (the columns of up to 4 projections beside each other, multiples of 128, as q|k|v) or ``paired=True`` (two
-    projections' columns in turn, as ``formats.interleave_gate_up``).  Smaller ranks among them: zeros in the last places.
+    ``a`` bf16 ``[n, R, K]``, ``b`` bf16 ``[n, N, R]`` (n up to 511, R up to 256, K a multiple of 32, N of
+    16), ``scales`` fp32 ``[n]`` (1 by default). Of a fused projection: ``a [n, slices, R, K]``, ``b``'s rows
+    in the order of the fused columns, and either ``widths`` (the columns of up to 4 projections beside each
+    other, multiples of 128, as q|k|v) or ``paired=True`` (two projections' columns in turn, as
+    ``formats.interleave_gate_up``). Smaller ranks among them: zeros in the last places.
 
-    The pool keeps its own copy, laid out once in the order of the kernels' operands; ``put`` replaces one adapter's values in place, so captured calls keep serving."""
+    The pool keeps its own copy, laid out once in the order of the kernels' operands; ``put`` replaces one
+    adapter's values in place, so captured calls keep serving."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scales: torch.Tensor | None = None, widths=None,
                  paired: bool = False):
