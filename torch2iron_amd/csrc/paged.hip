@@ -322,8 +322,9 @@ __device__ __forceinline__ void poison_item(const RaggedAttnParams& p, const Rag
 //     1000 to 4000 52 us (5.7 TB/s: shares of 9 blocks, whose first loads nothing hides), MFMA 12 % and VALU 14 % of a SIMD's cycles.
 //   1999 rows after 30001: 0.96-1.05 ms by the card, 0.97-1.05 PFLOP/s: MFMA 54 %, VALU 51 % at 1.7-1.9 GHz, as packed rows.
 //   two chunks with 24 tokens: 122 us, 2.8 TB/s and 0.52 PFLOP/s: the longest chains of loads beside the chunks' products.
-// Measured and dropped: wide tiles first; bins that carry their first tile's words; heavier shares where a CU has one
-// workgroup.
+// Measured and dropped: wide tiles first (two chunks with 24 tokens 130 -> 158 us), wide and narrow ones in turn, so that a CU
+// might run both (125-146 for 130-147 there, 16 chunks with 10 tokens 90 -> 92, in turns of four 94); bins that carry their
+// first tile's words; heavier shares where a CU has one workgroup.
 __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const RaggedAttnParams p, const PagedTables tab) {
   extern __shared__ __align__(256) uint16_t s_kv[];   // [buffer][K, V][key][dim]
   __shared__ uint32_t s_odd[RG_WAVES];                     // an item's pairs whose sums are not finite
