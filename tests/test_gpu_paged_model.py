@@ -294,3 +294,83 @@ def test_refusals(gpu, setup):
         with pytest.raises(ValueError):
             m.paged_step(**{**ok, **kw})
     assert all(torch.equal(a, b) for a, b in zip((cache.k, cache.v, cache.lens), before)), "a refused step wrote"
+
+
+def _used_before(cfg, m, gpu, n_pages):
+    """A cache of one sequence whose pages held another request's keys and values before."""
+    cache = gm.PagedCache(cfg, 1, n_pages, 6, gpu, page_slots=16)
+    g = torch.Generator().manual_seed(40)
+    cache.reserve(0, 96)
+    m.paged_step(cache, gm.PagedBatch([96], device=gpu), torch.randint(0, cfg.vocab, (96,), generator=g, dtype=torch.int32).to(gpu))
+    cache.release(0)
+    assert (cache.k[:, :6].float().abs().sum((0, 2, 3, 4)) > 0).all()
+    return cache
+
+
+@pytest.mark.parametrize("start,fed,drafts", [(32, 1, 0), (32, 1, 3), (30, 1, 3), (31, 30, 0)],
+                         ids=["token", "drafts", "drafts_over_the_border", "chunk"])
+@pytest.mark.parametrize("captured", [False, True], ids=["eager", "captured"])
+def test_a_step_without_room_can_be_made_again(gpu, setup, captured, start, fed, drafts):
+    """A step that runs past the end of its pages leaves the length as it was; after a reserve the same step, and the one
+    after it, have the bits of a run that had room from the start."""
+    cfg, _, _, _ = setup
+    m = _model(setup, gpu)
+    g = torch.Generator().manual_seed(41)
+    rnd = lambda n: torch.randint(0, cfg.vocab, (n,), generator=g, dtype=torch.int32).to(gpu)  # noqa: E731
+    prompt, tokens, after = rnd(start), rnd(fed + drafts), rnd(1)
+    batch, one = gm.PagedBatch([fed + drafts], [drafts], device=gpu), gm.PagedBatch([1], device=gpu)
+    u = torch.zeros(drafts + 1, device=gpu)                # every draft of any weight stays
+    runs = []
+    for slots in (96, 32):
+        cache = _used_before(cfg, m, gpu, 6)
+        cache.reserve(0, slots)
+        assert m.paged_step(cache, gm.PagedBatch([start], device=gpu), prompt).next_tokens[0] >= 0
+        step = lambda: m.paged_step(cache, batch, tokens, uniforms=u)  # noqa: E731
+        if captured:
+            if not runs:
+                step()                                     # the workspaces
+                cache.lens.fill_(start)
+            torch.cuda.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                got = step()
+
+            def step():
+                graph.replay()
+                return got
+
+        if slots == 32:
+            for _ in range(2):
+                got = step()
+                assert got.next_tokens.tolist() == [-1] and cache.lens.tolist() == [start]
+                torch.cuda.synchronize()
+            cache.reserve(0, 96)
+        first = [x.clone() for x in step()] + [cache.lens.clone()]
+        runs.append(first + list(m.paged_step(cache, one, after)) + [cache.lens.clone()])
+    assert runs[0][1].item() >= 0 and runs[0][4].item() == start + fed + runs[0][0].item()
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_a_step_past_the_table_can_be_made_smaller(gpu, setup):
+    """Too many tokens for a sequence's part of the table: the length stays, a smaller step fits, and the others go on."""
+    cfg, _, _, _ = setup
+    m = _model(setup, gpu)
+    g = torch.Generator().manual_seed(42)
+    tokens = torch.randint(0, cfg.vocab, (64,), generator=g, dtype=torch.int32).to(gpu)
+    runs = []
+    for too_many in (False, True):
+        cache = gm.PagedCache(cfg, 2, 8, 4, gpu, page_slots=16)
+        for s in range(2):
+            cache.reserve(s, 64)
+        m.paged_step(cache, gm.PagedBatch([60, 0], device=gpu), tokens[:60])
+        if too_many:
+            for n in (5, 70, 5):                           # (70 rows: more than the whole part)
+                before = cache.lens.clone()
+                many = torch.zeros(n + 1, dtype=torch.int32, device=gpu)
+                got = m.paged_step(cache, gm.PagedBatch([n, 1], device=gpu), many)
+                assert got.next_tokens[0] == -1 and got.next_tokens[1] >= 0
+                assert cache.lens.tolist() == [60, before[1].item() + 1]
+        got = m.paged_step(cache, gm.PagedBatch([4, 0], device=gpu), tokens[60:])
+        runs.append([got.next_tokens[:1], got.logits, cache.lens[:1]])
+        assert cache.lens[0] == 64 and got.next_tokens[0] >= 0
+    assert all(torch.equal(a, b) for a, b in zip(*runs))

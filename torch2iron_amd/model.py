@@ -372,7 +372,7 @@ class PagedStep(NamedTuple):
     """What ``Qwen3Model.paged_step`` says (device tensors)."""
 
     counts: torch.Tensor         # int32 [S] drafts that stay
-    next_tokens: torch.Tensor    # int32 [S] the token behind them (-1: a sequence without rows, or without a distribution)
+    next_tokens: torch.Tensor    # int32 [S] the token behind them (-1: a sequence without rows, room or a distribution; it stays)
     logprobs: torch.Tensor       # fp32 [head rows] of the token behind each of them, as ``ops.verify_drafts``
     logits: torch.Tensor         # fp32 [head rows, vocab]
 
@@ -921,8 +921,9 @@ class Qwen3Model:
 
         The pages must have room (``cache.reserve``): a token without a slot gives NaN logits, and the next token -1.
         ``cache.lens`` move on by the tokens that were fed and the drafts that stay (what a refused draft left in
-        the pages is written over by the next step).  Nothing is read back: the call can be captured once its
-        workspaces exist."""
+        the pages is written over by the next step).  A sequence whose next token is -1 stays where it was,
+        whatever its count: give it room and feed the same tokens again.  Nothing is read back: the call can be
+        captured once its workspaces exist."""
         c, ws = self.cfg, self.micro[0].buf.workspace
         ops._check_dev("tokens", tokens, torch.int32)
         if not isinstance(cache, PagedCache) or not isinstance(batch, PagedBatch) or batch.n_seqs != cache.n_seqs:
@@ -992,7 +993,8 @@ class Qwen3Model:
         ops.lm_head_argmax(xn, self.lm_head, keys, logits=logits)
         counts, nxt, lp = ops.verify_drafts(logits, batch.head_starts, tokens[batch.head_rows.long()], uniforms,
                                             draft_probs=draft_probs, temperatures=temperatures, workspace=ws)
-        cache.lens += batch.fed + counts
+        # (a row that is fed or stays without a slot is the last one's, or attended by it: its logits are NaN)
+        cache.lens += torch.where(nxt >= 0, batch.fed + counts, 0)
         return PagedStep(counts, nxt, lp, logits)
 
     # ---- graph-captured greedy generation ----
