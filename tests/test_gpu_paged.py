@@ -445,3 +445,21 @@ def test_wrapper_refusals(gpu):
         ops.paged_qk_rope_kv(qkv, c.plan, norm, norm, 1e-6, gm.rope_table(D, 16, 1e6, gpu), c.k, c.v)
     with pytest.raises(ValueError, match="qkv must be"):
         ops.paged_qk_rope_kv(qkv[:-1], c.plan, norm, norm, 1e-6, gm.rope_table(D, 1024, 1e6, gpu), c.k, c.v)
+
+
+@pytest.mark.parametrize("rows", [33, 40, 200])
+@pytest.mark.parametrize("hq,hkv", [(2, 2), (8, 2)])
+def test_more_rows_than_a_sequence_has_slots(gpu, hq, hkv, rows):
+    """Rows past everything that the table has: zero rows and sums, whatever the context; the others do not notice."""
+    c = Case(gpu, hq, hkv, 16, [3, rows, 1], [20, 0, 7])
+    ref, mag = c.reference()
+    table = c.table[:, :2].contiguous()                    # 32 slots a sequence
+    for ctx in (0, 5, -1):
+        c.ctx_dev[1] = ctx
+        plan = ops.PagedPlan(c.rows, c.row_starts, c.ctx_dev, table, hq, hkv, 16)
+        out = torch.full((c.rows, hq * D), 3.0, dtype=BF16, device=gpu)
+        sums = torch.full((hq, c.rows), 3.0, device=gpu)
+        ops.paged_attention(c.q, plan, c.k, c.v, out=out, out_sums=sums)
+        assert (out[3:-1] == 0).all() and (sums[:, 3:-1] == 0).all()
+        _check(out[:3], ref[:3], mag[:3])
+        _check(out[-1:], ref[-1:], mag[-1:])

@@ -343,9 +343,9 @@ __global__ __launch_bounds__(64 * RG_WAVES, 2) void paged_attention_kernel(const
     it.row0 = w[0]; it.rows = w[1]; it.start = w[2]; it.crow = w[3];
     it.j0 = w[4]; it.kb0 = at - w[5];
     const int units = w[6], take = min(units - it.kb0, end - at);
-    // a plan of other tensors is not followed
-    if (it.row0 < 0 || it.rows < 1 || it.row0 + (long long)it.rows > p.rows || it.start > p.cap - it.rows || it.crow < 0 ||
-        it.crow >= tab.B || it.j0 < 0 || it.kb0 < 0 || take < 1)
+    // a plan of other tensors is not followed (a start below 0 has no keys, however many its rows)
+    if (it.row0 < 0 || it.rows < 1 || it.row0 + (long long)it.rows > p.rows || (it.start >= 0 && it.start > p.cap - it.rows) ||
+        it.crow < 0 || it.crow >= tab.B || it.j0 < 0 || it.kb0 < 0 || take < 1)
       return;
     it.pairs = it.rows * p.G;
     if (it.j0 >= it.pairs) return;
