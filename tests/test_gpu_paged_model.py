@@ -374,3 +374,18 @@ def test_a_step_past_the_table_can_be_made_smaller(gpu, setup):
         runs.append([got.next_tokens[:1], got.logits, cache.lens[:1]])
         assert cache.lens[0] == 64 and got.next_tokens[0] >= 0
     assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_tokens_and_adapter_ids_of_another_shape(gpu, setup):
+    """As many values in more dimensions are refused, and nothing is written."""
+    cfg, _, _, pools = setup
+    m = _model(setup, gpu)
+    cache = gm.PagedCache(cfg, 2, 9, 4, gpu, page_slots=16)
+    batch, tokens, ids = gm.PagedBatch([2, 3], [0, 1], device=gpu), _i32(gpu, [1] * 5), _i32(gpu, [0, 1])
+    for s in range(2):
+        cache.reserve(s, 10)
+    for kw in (dict(tokens=tokens.view(1, 5)), dict(tokens=tokens.view(5, 1)), dict(adapters=pools, adapter_ids=ids.view(1, 2)),
+               dict(adapters=pools, adapter_ids=ids.view(2, 1))):
+        with pytest.raises(ValueError, match="must be"):
+            m.paged_step(cache, batch, **{**dict(tokens=tokens), **kw})
+    assert not cache.lens.any() and not cache.k.any() and not cache.v.any()

@@ -66,3 +66,20 @@ def test_lens_move_on_where_a_next_token_came_out(step):
     step.counts, step.next = _i32(0, 0, 3, 0), _i32(0, 31, 2, -1)
     step(cache, batch, torch.zeros(8, dtype=torch.int32))
     assert cache.lens.tolist() == [8 + 2, 17, 44, 7]
+
+
+def test_shapes_that_are_refused_before_the_pass(step):
+    """tokens and adapter_ids are indexed by row and by sequence: as many values in another shape would be looked up out
+    of range, behind the pages' writes."""
+    cache = gm.PagedCache(CFG, 2, 9, 4, "cpu", page_slots=16)
+    batch, tokens = gm.PagedBatch([2, 3], [0, 1], device="cpu"), torch.zeros(5, dtype=torch.int32)
+    none = [gm.LayerAdapters()] * CFG.n_layers
+    step.counts, step.next = _i32(0, 0), _i32(1, 1)
+    step(cache, batch, tokens, adapters=none, adapter_ids=_i32(0, 0))
+    assert step.passes == 1
+    for kw in (dict(tokens=tokens.view(1, 5)), dict(tokens=tokens.view(5, 1)), dict(tokens=tokens[:4]), dict(tokens=tokens.view(1, 5, 1)),
+               dict(adapters=none, adapter_ids=_i32(0, 0).view(1, 2)), dict(adapters=none, adapter_ids=_i32(0, 0).view(2, 1)),
+               dict(adapters=none, adapter_ids=_i32(0))):
+        with pytest.raises(ValueError, match="must hold|must be"):
+            step(cache, batch, **{**dict(tokens=tokens), **kw})
+    assert step.passes == 1

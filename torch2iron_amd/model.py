@@ -930,8 +930,8 @@ class Qwen3Model:
             raise ValueError("batch must be a PagedBatch of the cache's sequences")
         if cache.k.shape[0] != c.n_layers or tuple(cache.k.shape[2:]) != (c.n_kv_heads, cache.page_slots, c.head_dim):
             raise ValueError("the cache was made for another model")
-        if batch.rows < 1 or tokens.numel() != batch.rows:
-            raise ValueError(f"tokens must hold {batch.rows} ids, at least one")
+        if batch.rows < 1 or tuple(tokens.shape) != (batch.rows,):
+            raise ValueError(f"tokens must be [{batch.rows}], at least one id")
         if cache.max_pages * cache.page_slots > self.rope.shape[0]:
             raise ValueError(f"sequences of {cache.max_pages * cache.page_slots} slots exceed the model's "
                              f"{self.rope.shape[0]} positions")
@@ -969,8 +969,8 @@ class Qwen3Model:
                     if pool is not None and pool.device != tokens.device:
                         raise ValueError(f"adapters of {name} are on {pool.device}, not on {tokens.device}")
             pools = {p.n for a in adapters for p in a if p is not None}
-            if len(pools) > 1 or adapter_ids.numel() != batch.n_seqs:
-                raise ValueError(f"the pools must be of one size, and adapter_ids hold {batch.n_seqs} values")
+            if len(pools) > 1 or tuple(adapter_ids.shape) != (batch.n_seqs,):
+                raise ValueError(f"the pools must be of one size, and adapter_ids must be [{batch.n_seqs}]")
             plan = ops.AdapterPlan(adapter_ids[batch.row_seq], pools.pop()) if pools else None
         pages = ops.PagedPlan(batch.rows, batch.row_starts, cache.lens, cache.table, c.n_heads, c.n_kv_heads, cache.page_slots)
         past = cache.lens > cache.max_pages * cache.page_slots - batch.seq_rows   # their rows attend nothing
