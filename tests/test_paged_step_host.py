@@ -83,3 +83,15 @@ def test_shapes_that_are_refused_before_the_pass(step):
         with pytest.raises(ValueError, match="must hold|must be"):
             step(cache, batch, **{**dict(tokens=tokens), **kw})
     assert step.passes == 1
+
+
+def test_adapters_that_are_no_layer_adapters_are_refused_before_the_pass(step):
+    """A plain tuple has no projections by name, which came out in the layer that it was for, behind the writes of the others."""
+    cache = gm.PagedCache(CFG, 2, 9, 4, "cpu", page_slots=16)
+    batch, tokens = gm.PagedBatch([2, 3], device="cpu"), torch.zeros(5, dtype=torch.int32)
+    step.counts, step.next = _i32(0, 0), _i32(1, 1)
+    none = gm.LayerAdapters()
+    for bad in ([none, tuple(none)], [none, None], [none, none._replace(o=torch.zeros(1))], [none, none._replace(o="o")]):
+        with pytest.raises(ValueError, match="adapters"):
+            step(cache, batch, tokens, adapters=bad, adapter_ids=_i32(0, 0))
+    assert step.passes == 0

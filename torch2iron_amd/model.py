@@ -956,14 +956,16 @@ class Qwen3Model:
         ops._same_device(cache.table.device, tokens=tokens, row_starts=batch.row_starts, uniforms=uniforms,
                          temperatures=temperatures, draft_probs=draft_probs, adapter_ids=adapter_ids, rope=self.rope)
         if adapters is not None:
-            if len(adapters) != c.n_layers or adapter_ids is None:
+            if len(adapters) != c.n_layers or not all(isinstance(a, LayerAdapters) for a in adapters) or adapter_ids is None:
                 raise ValueError("adapters must hold a LayerAdapters for each layer, and adapter_ids each sequence's")
             ops._check_dev("adapter_ids", adapter_ids, torch.int32)
             q = c.n_heads * c.head_dim
             want = LayerAdapters((c.hidden, c.qkv_dim, False), (q, c.hidden, False), (c.hidden, 2 * c.intermediate, True),
                                  (c.intermediate, c.hidden, False))
             for a in adapters:
-                for name, pool, shape in zip(LayerAdapters._fields, LayerAdapters(*a), want):
+                for name, pool, shape in zip(LayerAdapters._fields, a, want):
+                    if pool is not None and not isinstance(pool, ops.Adapters):
+                        raise ValueError(f"adapters of {name} must be an Adapters, or None")
                     if pool is not None and (pool.K, pool.N, pool.paired) != shape:
                         raise ValueError(f"adapters of {name} must be [{shape[1]}, {shape[0]}]{', paired' if shape[2] else ''}")
                     if pool is not None and pool.device != tokens.device:
