@@ -274,3 +274,19 @@ def test_out_may_be_x(gpu):
         want = ops.adapter_add(y, x, pool, plan, out=torch.empty_like(y))
         got = ops.adapter_add(y, x, pool, plan, out=x)
         assert got is x and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("paired", [False, True])
+def test_rows_without_an_adapter_keep_their_bits(gpu, paired):
+    """Every bf16 pattern there is, negative zeros and NaN among them, into another tensor and in place."""
+    y = torch.arange(65536, device=gpu).to(torch.int16).view(BF16).view(256, 256)
+    g, a, b, scales, pool = _make(gpu, 64, [256] if paired else [128, 128], paired, 8, 2)
+    x = torch.randn(256, 64, device=gpu, generator=g).to(BF16)
+    ids = torch.full((256,), -1, dtype=torch.int32, device=gpu)
+    ids[200:203] = 1                                       # others among them
+    plan, none = ops.AdapterPlan(ids, 2), ids < 0
+    out = ops.adapter_add(y, x, pool, plan, out=torch.zeros_like(y))
+    assert torch.equal(out.view(torch.int16)[none], y.view(torch.int16)[none])
+    keep = y.clone()
+    ops.adapter_add(y, x, pool, plan)
+    assert torch.equal(y.view(torch.int16)[none], keep.view(torch.int16)[none])

@@ -266,6 +266,12 @@ __global__ __launch_bounds__(256) void adapter_expand_kernel(const AdapterParams
     row[i] = t.at(p, sub * 16 + 4 * g + i);
     y[i] = *reinterpret_cast<const u32x4*>(p.y + (size_t)row[i] * p.N + min(col, p.N - 8));
   }
+  if (t.adapter < 0 && !p.swiglu) {                        // their bits, where a sum with 0 makes 0 of -0
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col < p.N && sub * 16 + 4 * g + i < t.rows) *reinterpret_cast<u32x4*>(p.out + (size_t)row[i] * p.N + col) = y[i];
+    return;
+  }
   f32x4 acc[8];
 #pragma unroll
   for (int k = 0; k < 8; ++k) acc[k] = f32x4{0.f, 0.f, 0.f, 0.f};
