@@ -290,3 +290,11 @@ def test_rows_without_an_adapter_keep_their_bits(gpu, paired):
     keep = y.clone()
     ops.adapter_add(y, x, pool, plan)
     assert torch.equal(y.view(torch.int16)[none], keep.view(torch.int16)[none])
+
+
+def test_more_slices_than_four(gpu):
+    g = torch.Generator(device=gpu).manual_seed(6)
+    rnd = lambda *s: torch.randn(*s, device=gpu, generator=g).to(BF16)  # noqa: E731
+    ops.Adapters(rnd(1, 4, 8, 64), rnd(1, 512, 8), widths=[128] * 4)
+    with pytest.raises(ValueError, match="slices"):
+        ops.Adapters(rnd(1, 5, 8, 64), rnd(1, 640, 8), widths=[128] * 5)

@@ -333,3 +333,20 @@ def test_refusals(gpu):
     for kw in bad:
         with pytest.raises(ValueError):
             ops.verify_drafts(**{**good, **kw})
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,v", [([2] * 140, 30011), ([4] * 140, 30011), ([5, 1, 0, 3] * 7, 151936), ([2, 9] * 9, 300001)],
+                         ids=["140x2", "140x4", "28-151936", "18-300001"])
+def test_many_sequences_of_many_chunks(gpu, lens, v, dtype):
+    """Draft probabilities, the rest of a refused draft's row over several workgroups, and, for rows times chunks of 16384
+    and more, two chunks a wave of the rows' pass."""
+    args = _case(gpu, lens, v, TYPES[dtype], True, seed=v + len(lens))
+    chunks, drafted = -(-v // 1024), sum(n > 1 for n in lens)
+    assert len(lens) * -(-chunks // 16) > 256, "decided and summed in one launch"
+    got = ops.verify_drafts(*args[:4], draft_probs=args[4], temperatures=args[5])
+    again = ops.verify_drafts(*args[:4], draft_probs=args[4], temperatures=args[5], workspace=ops.Workspace())
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    _check(args, got)
+    refused = (got[0].cpu() < torch.tensor(lens) - 1) & (args[5].cpu() > 0)
+    assert int(refused.sum()) > drafted // 20, "hardly a draft was refused"
