@@ -90,9 +90,10 @@ __device__ __forceinline__ void plan_times(int pairs, float& alone, float& share
 // to a workgroup whole, longest first, or the units are cut into equal shares whose tiles' parts a second launch
 // joins, whichever the times say ends sooner; here the device decides, so that a captured step may
 // serve every later one.
-// A chain of scans and look-ups in one workgroup, bound by their latency: 32 single tokens 10.5 us, 16 x 5 drafts 8.3, 4997
-// rows of 16 prompts 15, once a step of all layers.  A thread finds its own share (one after the other took 13.2 us for the
-// 32 tokens), and shares are cut without 64-bit division.
+// A chain of scans and look-ups in one workgroup, bound by their latency: one token 6 us, 32 single tokens 10.5, 16 x 5
+// drafts 8.3, 4997 rows of 16 prompts 15 (from a graph; 12.0 for the 32 tokens behind an idle GPU), once a step of all
+// layers.  A thread finds its own share (one after the other took 13.2 us for the 32 tokens), and shares are cut without
+// 64-bit division.
 __global__ __launch_bounds__(PG_THREADS) void paged_plan_kernel(const PagedPlanParams p) {
   const int tid = threadIdx.x;
   int falls = 0;                             // row_starts that do not ascend: no row is anyone's
@@ -315,13 +316,15 @@ __device__ __forceinline__ void poison_item(const RaggedAttnParams& p, const Rag
 // A workgroup takes a bin's units for one kv head, tile by tile.  Sequences of one tile (single tokens, drafted
 // tokens, short chunks) multiply by weights of 16 bits: their products hide behind the loads.  Single tokens among the
 // tiles of long chunks, one workgroup each, are as slow as their own chain of loads: they take the form with more
-// of them on their way (two chunks of 509 and 701 rows with 24 tokens 146 -> 131 us).  Where they fill the chip themselves
+// of them on their way (two chunks of 509 and 701 rows with 24 tokens 146 -> 129 us).  Where they fill the chip themselves
 // that form has more barriers for nothing (32 tokens 56.9 -> 58.7 us, 64 after 4090 slots 170 -> 179).
 // What bounds it (16 / 8 and 32 / 8 heads, this launch alone):
 //   tokens and drafts: memory.  64 tokens after 4090 slots 6.3 TB/s, 8 after 30000 6.5, of the 6.85 that a bulk read reaches; 32 after
-//     1000 to 4000 52 us (5.7 TB/s: shares of 9 blocks, whose first loads nothing hides), MFMA 12 % and VALU 14 % of a SIMD's cycles.
-//   1999 rows after 30001: 0.96-1.05 ms by the card, 0.97-1.05 PFLOP/s: MFMA 54 %, VALU 51 % at 1.7-1.9 GHz, as packed rows.
-//   two chunks with 24 tokens: 122 us, 2.8 TB/s and 0.52 PFLOP/s: the longest chains of loads beside the chunks' products.
+//     409 to 4090 52 us (295 MB, 5.7 TB/s: shares of 9 blocks, whose first loads nothing hides), MFMA 12 % and VALU 15 % of
+//     a SIMD's cycles.
+//   1999 rows after 30001: 0.96-1.11 ms by the card, 0.91-1.06 PFLOP/s: MFMA 54 %, VALU 51 % at 1.7-1.9 GHz, as packed rows.
+//   two chunks with 24 tokens: 122 us of 116 to 137 by the card and by what ran before, 2.8 TB/s and 0.52 PFLOP/s: the longest
+//     chains of loads beside the chunks' products.
 // Measured and dropped: wide tiles first (two chunks with 24 tokens 130 -> 158 us), wide and narrow ones in turn, so that a CU
 // might run both (125-146 for 130-147 there, 16 chunks with 10 tokens 90 -> 92, in turns of four 94); bins that carry their
 // first tile's words; heavier shares where a CU has one workgroup.

@@ -751,7 +751,7 @@ class Qwen3Model:
                 adapt(a.qkv, qkv, xn)
             sums = attend(i, prep(i, qkv), ctx, xs_ctx)
             ops.linear(ctx, w.o, residual=x, out=x, x_sums=sums)
-            adapt(a.o, x, ctx)
+            adapt(a.o, x, ctx)          # (to the rounded residual rows: a rounding more than without an adapter)
             if r <= 64 and a.gate_up is None:
                 ops.rmsnorm_gate_up(x, w.ln2, c.eps, w.gate_up, swiglu=True, out=h)
             else:

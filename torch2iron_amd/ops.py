@@ -1490,7 +1490,8 @@ def paged_attention(q: torch.Tensor, plan: PagedPlan, k_pages: torch.Tensor, v_p
                     workspace: Workspace | None = None) -> torch.Tensor:
     """Causal GQA attention of the rows of ``plan`` (``q [rows, Hq, D]``) over the pages: row r of sequence s over its
     slots ``0 .. context_lens[s] + r``, whose k and v stand in the pages by then (``paged_qk_rope_kv``).
-    Returns bf16 ``[rows, Hq * D]``; ``out_sums`` (fp32 ``[Hq, rows]``) as ``prefill_attention``.
+    Returns bf16 ``[rows, Hq * D]``; ``out_sums`` (fp32 ``[Hq, rows]``) as ``prefill_attention``.  Softmax weights have 16
+    bits where a sequence's rows times Hq / Hkv are at most 128, and are rounded to bf16 in longer chunks.
 
     Slots that no row attends are never read.  Rows of a sequence without slots are zero, rows that are no
     sequence's are left as they are (unset without ``out``), and a page id outside the pool makes the rows that
